@@ -193,7 +193,8 @@ def _plain_loss(st):
 def _plain_int8(st):
     x = st["x"]
     sx = (x.abs().amax(1, keepdim=True).double() / 127.0).float()      # correctly rounded
-    q = torch.round(x.double() / sx.double())          # the quotient in 64 bits: values next to a border
+    # the quotient in 64 bits: values next to a border; a row of zeros stays zeros
+    q = torch.where(sx > 0, torch.round(x.double() / sx.double()), sx.double())
     y = (q @ st["wq"].double().t()).float() * sx * st["ws"]      # whole numbers past 2^24: exact in 64 bits
     if st["bias"] is not None:
         y = y + st["bias"]
@@ -312,7 +313,7 @@ def _exact_loss(st):
 def _exact_int8(st):
     x = st["x"].double()
     step = (x.abs().max(dim=1).values / 127.0).float().double()      # the scale is a 32-bit number
-    values = torch.round(x / step[:, None]) * step[:, None]
+    values = torch.where(step[:, None] == 0, x, torch.round(x / step[:, None]) * step[:, None])
     y = values @ (st["wq"].double() * st["ws"].double()[:, None]).T
     return {"y": y if st["bias"] is None else y + st["bias"].double()}
 
