@@ -3,6 +3,7 @@
 The library is the product path: there is no CPU or PyTorch fallback.  If the
 shared object is missing, or the device is not gfx950, every op raises.
 """
+import contextlib
 import ctypes
 import os
 
@@ -134,6 +135,18 @@ _SIGS = {
                         c_void_p, c_void_p, c_void_p],
     "po_maxpool2_bwd_box": [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int,
                             c_void_p, c_void_p, c_void_p, c_void_p],
+    "po_dropout": [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, ctypes.c_uint64, ctypes.c_uint64,
+                   c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p],
+    "po_linear_ce_fwd": [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                         c_float, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p],
+    "po_linear_ce_bwd": [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                         c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                         c_int64, c_void_p],
+    "po_linear_ce_workspace": [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_int, c_int,
+                               ctypes.POINTER(c_int64), ctypes.POINTER(c_int64)],
+    "po_quantize_rows": [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p],
+    "po_int8_matmul": [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                       c_void_p, c_int64, c_int, c_void_p],
     "po_nhwc_to_nchw": [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "po_nchw_to_nhwc": [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
 }
@@ -158,7 +171,10 @@ def load():
         raise ImportError("libadvpatch_hip.so has ABI %d, this package needs %d: rebuild it "
                           "(make -C csrc, or __graft_entry__.build())" % (got, PO_ABI_VERSION))
     for name, argtypes in _SIGS.items():
-        fn = getattr(lib, name)
+        fn = getattr(lib, name, None)
+        if fn is None:
+            raise ImportError("libadvpatch_hip.so has no %s: rebuild it (make -C csrc, or "
+                              "__graft_entry__.build())" % name)
         fn.argtypes = argtypes
         fn.restype = c_int
     lib.po_last_error.argtypes = []
@@ -218,6 +234,42 @@ def ptr(t, dtype=torch.float32):
     if not t.is_contiguous():
         raise ValueError("expected a contiguous tensor")
     return c_void_p(t.data_ptr())
+
+
+# Element types of the head's operators (include/advpatch.h: PO_F32, PO_F16, PO_BF16)
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+@contextlib.contextmanager
+def _other_device(device):
+    with torch.cuda.device(device):
+        yield
+
+
+def device_of(*tensors):
+    """Context of the tensors' device: launches and allocations inside go to it and
+    to its current stream, whatever device is current outside."""
+    t = tensors[0]
+    for u in tensors:
+        if not (isinstance(u, torch.Tensor) and u.is_cuda):
+            ensure_device(u)                 # raises
+        if u.device != t.device:
+            raise RuntimeError("advpatch HIP ops need their tensors on one device; got %s and %s" % (t.device, u.device))
+    if t.device.index == torch.cuda.current_device():
+        ensure_device(t)
+        return contextlib.nullcontext()
+    with torch.cuda.device(t.device):        # the check selects the device it looks at
+        ensure_device(t)
+    return _other_device(t.device)
+
+
+def rows2d(t):
+    """(matrix, row stride): t as [rows, cols] over its last dimension, a view where the
+    elements of a row are neighbours and rows do not overlap, else a copy."""
+    m = t.reshape(-1, t.shape[-1])
+    if (m.shape[1] > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < m.shape[1]):
+        m = m.contiguous()
+    return m, (m.stride(0) if m.shape[0] > 1 else m.shape[1])
 
 
 def ptr_array(ts):

@@ -1,0 +1,324 @@
+// The matrix-product core of the large-vocabulary head (vocab_loss.hip,
+// int8_linear.hip): C[m][n] = sum_k A[m][k] * B[n][k], both operands with k
+// contiguous, 16-bit floats or 8-bit integers, sums in 32 bits.
+//
+// One form only.  LDS reads with a transpose (ds_read_b64_tr_b16) run at 64 B
+// per clock and CU against 128 B for plain 16-byte reads (measured 41 against
+// 84 TB/s over the chip), and a product of two 256-row tiles already needs
+// three quarters of the latter; so operands that a product needs the other way
+// round are written that way once (a transpose, or the epilogue that makes
+// them), and every product runs this loop.
+//
+// A workgroup owns a BM x BN tile, its waves WM x WN rectangles of 32 x 32
+// MFMA blocks.  k advances in steps of KB bytes per row; STAGES LDS buffers are
+// filled ahead by 16-byte LDS-DMA.  Rows are KB bytes, their 16-byte chunks
+// XOR-swizzled by row (by the address each lane loads from: the DMA writes LDS
+// linearly), so 8 neighbouring lanes' fragment reads cover all banks.
+// Rows past the operand's end and k past its length read as zero (out-of-range
+// buffer offsets).
+#pragma once
+#include "common.h"
+#include <type_traits>
+
+namespace po {
+namespace mm {
+
+typedef int i4v __attribute__((ext_vector_type(4)));
+typedef int i16v __attribute__((ext_vector_type(16)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+
+enum Kind { BF16 = 0, F16 = 1, I8 = 2 };
+
+template <int KIND>
+struct Acc {
+  using type = f16v;
+};
+template <>
+struct Acc<I8> {
+  using type = i16v;
+};
+
+template <int KIND>
+__device__ __forceinline__ typename Acc<KIND>::type mfma(i4v a, i4v b, typename Acc<KIND>::type c) {
+  if constexpr (KIND == BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0, 0);
+  else if constexpr (KIND == F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+}
+
+// One operand: rows of k-contiguous elements, stride and length in bytes (both
+// multiples of 16 where they are read: the host pads or refuses others).
+struct Operand {
+  const char* p;
+  int64_t stride;   // bytes from row to row (256 rows stay under 2 GiB)
+  int64_t plane;    // bytes from plane to plane (operands split into planes)
+  int rows;
+};
+
+constexpr uint32_t kOOB = 0x80000000u;
+
+template <int KIND_, int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_>
+struct Cfg {
+  static constexpr int KIND = KIND_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = KB_, STAGES = STAGES_;
+  static constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  static constexpr int RPI = 1024 / KB;                                  // rows one wave's DMA instruction fills
+  static constexpr int NA = BM / RPI / NW, NB = BN / RPI / NW;           // instructions per wave and stage
+  static constexpr int STAGE_BYTES = (BM + BN) * KB, LDS = STAGES * STAGE_BYTES;
+  static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && NA * RPI * NW == BM && NB * RPI * NW == BN, "tile");
+};
+
+template <int KB>
+__device__ __forceinline__ int swz(int row) {
+  return KB == 128 ? (row & 7) : ((row >> 1) & 3);
+}
+
+template <class C>
+struct Loader {
+  __amdgpu_buffer_rsrc_t rs;
+  static __device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t rs, char* lds, uint32_t voff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16, voff, 0, 0, 0);
+  }
+};
+
+// acc += the tile's product over the k-steps [ks0, ks1) of the plane pairs.
+// Planes: an operand of wider numbers is stored as `planes` 16-bit matrices, and
+// the step index runs over pairs of them: pair q multiplies plane (pa >> 4q & 15)
+// of A with plane (pb >> 4q & 15) of B; steps [q * nk, (q + 1) * nk) are pair q's.
+// kbytes: length of a row; ends inside a step read as zero.
+template <class C>
+__device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM][C::TN], const Operand& A,
+                                        const Operand& B, int m0, int n0, int kbytes, int ks0, int ks1, int nk,
+                                        uint32_t pa, uint32_t pb, char* lds) {
+  constexpr int KB = C::KB, CPR = KB / 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / C::WN, wn = wave % C::WN;
+  const int lrow = lane / CPR;                               // row of this lane inside one DMA instruction
+  uint32_t oa[C::NA], ob[C::NB];
+#pragma unroll
+  for (int i = 0; i < C::NA; ++i) {
+    const int r = (i * C::NW + wave) * C::RPI + lrow;
+    const int ch = (lane % CPR) ^ swz<KB>(r);
+    oa[i] = m0 + r < A.rows ? (uint32_t)(r * (int)A.stride) + ch * 16 : kOOB;
+  }
+#pragma unroll
+  for (int i = 0; i < C::NB; ++i) {
+    const int r = (i * C::NW + wave) * C::RPI + lrow;
+    const int ch = (lane % CPR) ^ swz<KB>(r);
+    ob[i] = n0 + r < B.rows ? (uint32_t)(r * (int)B.stride) + ch * 16 : kOOB;
+  }
+  // the chunk of this lane inside a step is the same in every instruction: rows
+  // of one lane differ by multiples of RPI * NW, which the swizzle does not see
+  static_assert((C::RPI * C::NW) % 8 == 0, "swizzle period");
+  const uint32_t lch = ((lane % CPR) ^ swz<KB>(wave * C::RPI + lrow)) * 16;
+  const char* abase = A.p + (int64_t)m0 * A.stride;
+  const char* bbase = B.p + (int64_t)n0 * B.stride;
+  int q = ks0 / nk, kt = ks0 - q * nk;                       // plane pair and step of the next stage to load
+  auto issue = [&](int buf) {
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(abase + (int64_t)((pa >> (4 * q)) & 15) * A.plane), 0, 0x7fffffff, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(bbase + (int64_t)((pb >> (4 * q)) & 15) * B.plane), 0, 0x7fffffff, 0x00020000);
+    char* la = lds + buf * C::STAGE_BYTES;
+    char* lb = la + C::BM * KB;
+    const uint32_t k0 = (uint32_t)kt * KB;
+    // past the row's end: out of range by the sign bit (offsets stay below 2^31)
+    const uint32_t past = (int)(k0 + lch) < kbytes ? k0 : kOOB;
+#pragma unroll
+    for (int i = 0; i < C::NA; ++i)
+      Loader<C>::dma(ra, la + (i * C::NW + wave) * 1024, (oa[i] + (past & 0x7fffffffu)) | (past & kOOB) | (oa[i] & kOOB));
+#pragma unroll
+    for (int i = 0; i < C::NB; ++i)
+      Loader<C>::dma(rb, lb + (i * C::NW + wave) * 1024, (ob[i] + (past & 0x7fffffffu)) | (past & kOOB) | (ob[i] & kOOB));
+    if (++kt == nk) {
+      kt = 0;
+      ++q;
+    }
+  };
+  const int n = ks1 - ks0;
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s)
+    if (s < n) issue(s);
+  const int ar = wm * C::TM * 32 + (lane & 31), br = wn * C::TN * 32 + (lane & 31), h = lane >> 5;
+  int buf = 0;
+  for (int s = 0; s < n; ++s) {
+    // this step's loads have landed when at most the later stages' are in flight
+    if (C::STAGES > 2 && s + C::STAGES - 2 < n)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((C::STAGES - 2) * (C::NA + C::NB)) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();                            // ... every wave's, and the last step's reads are over
+    asm volatile("" ::: "memory");
+    if (s + C::STAGES - 1 < n) issue(buf == 0 ? C::STAGES - 1 : buf - 1);
+    const char* la = lds + buf * C::STAGE_BYTES;
+    const char* lb = la + C::BM * KB;
+#pragma unroll
+    for (int g = 0; g < KB / 32; ++g) {
+      i4v a[C::TM], b[C::TN];
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const int r = ar + i * 32;
+        a[i] = *reinterpret_cast<const i4v*>(la + r * KB + (((2 * g + h) ^ swz<KB>(r)) * 16));
+      }
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        const int r = br + j * 32;
+        b[j] = *reinterpret_cast<const i4v*>(lb + r * KB + (((2 * g + h) ^ swz<KB>(r)) * 16));
+      }
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) acc[i][j] = mfma<C::KIND>(a[i], b[j], acc[i][j]);
+    }
+    buf = buf + 1 == C::STAGES ? 0 : buf + 1;
+  }
+}
+
+// Element e of a 32 x 32 accumulator block lies in row (m) 8 * (e / 4) +
+// 4 * (lane / 32) + e % 4 and column (n) lane % 32: elements 4q .. 4q + 3 are
+// four consecutive rows of one column.  The kernels below take the operand whose
+// index is contiguous in the output (or is reduced over) as A.
+
+struct Args {
+  Operand A, B;
+  int tiles_m, tiles_n;
+  int kbytes, nk, pairs;      // bytes of a row, k-steps, plane pairs
+  uint32_t pa, pb;
+};
+
+template <class C>
+struct Tile {
+  typename Acc<C::KIND>::type acc[C::TM][C::TN];
+  int m0, n0;                 // first row of A and of B of this wave's rectangle
+  int tm, tn;
+  int lane, wave, wm, wn;
+  __device__ __forceinline__ int col(int j) const { return n0 + j * 32 + (lane & 31); }
+  __device__ __forceinline__ int row4(int i, int q) const { return m0 + i * 32 + 8 * q + 4 * (lane >> 5); }
+};
+
+// Workgroups of 8 tile rows by all tile columns in turn, an XCD's workgroups
+// next to each other: its L2 holds the k-window of the operands they share.
+// gridDim.y slices the k-steps.  Epi::run(tile, args, lds, slice) ends the tile.
+template <class C, class Epi>
+__global__ __launch_bounds__(C::NW * 64, 2) void product_k(const Args a, const typename Epi::Args e) {
+  __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+  const int id = xcd_remap();
+  constexpr int GM = 8;
+  const int grp = id / (GM * a.tiles_n), first = grp * GM, gm = min(GM, a.tiles_m - first);
+  const int r = id - grp * GM * a.tiles_n;
+  Tile<C> t;
+  t.tm = first + r % gm;
+  t.tn = r / gm;
+  t.lane = threadIdx.x & 63;
+  t.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  t.wm = t.wave / C::WN;
+  t.wn = t.wave % C::WN;
+  t.m0 = t.tm * C::BM + t.wm * C::TM * 32;
+  t.n0 = t.tn * C::BN + t.wn * C::TN * 32;
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) t.acc[i][j][k] = 0;
+  const int total = a.nk * a.pairs;
+  const int ks0 = (int)((int64_t)blockIdx.y * total / gridDim.y), ks1 = (int)((int64_t)(blockIdx.y + 1) * total / gridDim.y);
+  product<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, a.nk, a.pa, a.pb, lds);
+  Epi::template run<C>(t, e, lds, a);
+}
+
+template <class C, class Epi>
+inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipStream_t s, const char* what) {
+  a.tiles_m = ceil_div(a.A.rows, C::BM);
+  a.tiles_n = ceil_div(a.B.rows, C::BN);
+  a.nk = ceil_div(a.kbytes, C::KB);
+  if ((int64_t)a.tiles_m * a.tiles_n >= (1LL << 22) || slices > 65535 || (int64_t)a.nk * a.pairs >= (1LL << 31) ||
+      a.A.stride * C::BM >= (1LL << 31) || a.B.stride * C::BN >= (1LL << 31) || a.kbytes < 0) {
+    set_error("%s: operand too large", what);
+    return PO_EINVAL;
+  }
+  hipLaunchKernelGGL((product_k<C, Epi>), dim3(a.tiles_m * a.tiles_n, slices), dim3(C::NW * 64), 0, s, a, e);
+  return check_launch(what);
+}
+
+// ---- outputs -------------------------------------------------------------
+// A tile of 16-bit outputs passes through LDS as rows [n][m] and leaves as
+// 16-byte pieces of whole rows.  16-byte chunk c of row n lies at chunk
+// c ^ turn(n): the 8-byte writes of 32 columns, the 16-byte row reads and the
+// transposing reads of 4 rows x 32 bytes each touch every bank evenly.
+template <class C>
+__device__ __forceinline__ int turn(int n) {
+  constexpr int H = C::BM / 16;                 // half the chunks of a row
+  return ((n & (H - 1)) << 1) | ((n / H) & 1);
+}
+
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+
+template <class C>
+__device__ __forceinline__ void stage4(const Tile<C>& t, char* lds, int i, int j, int q, u2v four) {
+  const int n = t.wn * C::TN * 32 + j * 32 + (t.lane & 31);
+  const int c = t.wm * C::TM * 4 + i * 4 + q;   // 8 outputs to a chunk, this lane's 4 in one half
+  *reinterpret_cast<u2v*>(lds + n * (C::BM * 2) + ((c ^ turn<C>(n)) * 16) + 8 * (t.lane >> 5)) = four;
+}
+
+// rows [n][m] of the staged tile to out (16-bit, leading dimension ld), n < rows, m < cols
+template <class C>
+__device__ __forceinline__ void store_rows(const char* lds, uint16_t* out, int64_t ld, int n0, int m0, int rows,
+                                           int cols, bool wide) {
+  constexpr int NC = C::BM / 8;
+  for (int x = threadIdx.x; x < C::BN * NC; x += C::NW * 64) {
+    const int n = x / NC, c = x % NC, m = m0 + c * 8;
+    if (n0 + n >= rows || m >= cols) continue;
+    const i4v v = *reinterpret_cast<const i4v*>(lds + n * (C::BM * 2) + ((c ^ turn<C>(n)) * 16));
+    uint16_t* o = out + (int64_t)(n0 + n) * ld + m;
+    if (wide && m + 8 <= cols) {
+      *reinterpret_cast<i4v*>(o) = v;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (m + k < cols) o[k] = (uint16_t)((uint32_t)v[k >> 1] >> (16 * (k & 1)));
+    }
+  }
+}
+
+// the staged tile transposed, rows [m][n] of out: m < cols, n0 + n < rows (a multiple of 8)
+template <class C>
+__device__ __forceinline__ void store_columns(const char* lds, uint16_t* out, int64_t ld, int n0, int m0, int rows,
+                                              int cols) {
+  typedef short s4v __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  constexpr int MB = C::BM / 16, NB = C::BN / 32;
+  // a wave's step: 16 columns m by 32 rows n, 8 rows to a group of 16 lanes
+  for (int x = wave; x < MB * NB; x += C::NW) {
+    const int mb = x % MB, n = (x / MB) * 32 + g * 8;
+    u2v two[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int nr = n + 4 * k + (i >> 2);
+      const int c = mb * 2 + ((i >> 1) & 1);
+      const char* p = lds + nr * (C::BM * 2) + ((c ^ turn<C>(nr)) * 16) + 8 * (i & 1);
+      two[k] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (__attribute__((address_space(3))) s4v*)(const_cast<char*>(p))));
+    }
+    const int m = m0 + mb * 16 + i;
+    if (m < cols && n0 + n < rows)
+      *reinterpret_cast<i4v*>(out + (int64_t)m * ld + n0 + n) = i4v{(int)two[0][0], (int)two[0][1], (int)two[1][0], (int)two[1][1]};
+  }
+}
+
+typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+// two floats rounded to nearest even
+template <int KIND>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (KIND == F16)
+    return __builtin_bit_cast(uint32_t, h2v{(_Float16)x, (_Float16)y});
+  else
+    return __builtin_bit_cast(uint32_t, b2v{(__bf16)x, (__bf16)y});
+}
+
+}  // namespace mm
+}  // namespace po

@@ -1,0 +1,714 @@
+// Softmax cross entropy of a linear head over a large vocabulary, without its
+// logits in memory (po_linear_ce_fwd / _bwd).
+//
+//   l[n][v] = c * h[n] . w[v]        loss[n] = log sum_v exp l[n][v] - l[n][t_n]
+//   dl[n][v] = g_n (exp(l[n][v]) / sum_n - [v = t_n])
+//   dh = c * dl w                    dw = c * dl^T h
+//
+// Forward: one product over all of the vocabulary whose epilogue keeps, for
+// each tile of 256 vocabulary rows, the maximum and the sum of the exponentials
+// of a token (in 32 bits), and the target's logit.  A tile has the vocabulary as
+// its rows, so a token's values lie in one lane (and its neighbour 32 lanes on)
+// and the reduction stays in registers.  Backward: for one piece of the
+// vocabulary after the other, the logits again, dl in their place (16 bits, as
+// [n][v] and as [v][n]), then dh += dl w and the piece's rows of dw.  Every
+// product has k contiguous in both operands: w and h are transposed for that.
+//
+// Types.  16-bit inputs: exact products, sums in 32 bits; dl is rounded to the
+// inputs' type once, as an operand of the matrix cores: half a step against
+// each of a row's terms, below the rounding of the gradients themselves.  fp16 has
+// too little range for exp(l)/sum: its dl are kept relative to the largest |g_n|,
+// times 2^14 (at most 2^14, and normal down to 2^-28).  fp32 inputs: each number
+// is the sum of three bf16 (8 + 8 + 8 bits, nearest), and the six leading of the
+// nine products are summed in 32 bits; what is left out is below 2^-24 of a
+// product.  That is six bf16 products (about 200 TFLOP/s of fp32) where the fp32
+// matrix instructions end at 157.
+#include "mm_core.h"
+#include <math.h>
+
+namespace {
+using namespace po::mm;
+using po::ceil_div;
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kF16Lift = 16384.f;
+
+// tokens x vocabulary tiles: large, for up to 128 tokens, for up to 32
+template <int KIND>
+using Large = Cfg<KIND, 256, 256, 2, 4, 128, 2>;
+template <int KIND>
+using Mid = Cfg<KIND, 128, 128, 2, 2, 128, 2>;
+template <int KIND>
+using Few = Cfg<KIND, 128, 32, 4, 1, 128, 3>;
+
+__device__ __forceinline__ float xlane32_max(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
+__device__ __forceinline__ float xlane32_sum(float x) { return x + __shfl_xor(x, 32); }
+
+// ---- epilogues -----------------------------------------------------------
+
+// partial[tile][n] = {max of l * log2e, sum of 2^(l * log2e - max)} over the tile's vocabulary rows
+struct StatsEpi {
+  struct Args {
+    float2* partial;
+    float* tlogit;              // l / c of the target
+    const int64_t* target;
+    int64_t v0;                 // vocabulary row of A's first
+    int tile0;                  // first tile of this launch in partial
+    int N, V;                   // tokens, vocabulary rows of this launch
+    float k;                    // c * log2e > 0
+  };
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, char* lds, const po::mm::Args&) {
+    const bool edge = t.m0 + C::TM * 32 > e.V;
+    float2* mine = reinterpret_cast<float2*>(lds);          // [WM][BN]
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      const int n = t.col(j);
+      const int64_t tg = n < e.N ? e.target[n] - e.v0 - t.m0 : -1;
+      const bool has = tg >= 0 && tg < C::TM * 32 && ((tg >> 2) & 1) == (t.lane >> 5);
+      if (__any(has)) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if ((int)tg == i * 32 + 8 * (k >> 2) + 4 * (t.lane >> 5) + (k & 3)) x = t.acc[i][j][k];
+        if (has) e.tlogit[n] = x;
+      }
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (t.row4(i, k >> 2) + (k & 3) >= e.V) t.acc[i][j][k] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, t.acc[i][j][k]);
+      mx = xlane32_max(mx);
+      const float top = mx == -INFINITY ? 0.f : mx * e.k;    // nothing but -inf: no exponent of inf - inf
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) s += __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][k], e.k, -top));
+      s = xlane32_sum(s);
+      if (t.lane < 32) mine[t.wm * C::BN + t.wn * C::TN * 32 + j * 32 + t.lane] = make_float2(mx == -INFINITY ? -INFINITY : top, s);
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < C::BN; x += C::NW * 64) {
+      float2 r = mine[x];
+#pragma unroll
+      for (int w = 1; w < C::WM; ++w) {
+        const float2 o = mine[w * C::BN + x];
+        const float m = fmaxf(r.x, o.x), ref = m == -INFINITY ? 0.f : m;
+        r = make_float2(m, r.y * __builtin_amdgcn_exp2f(r.x - ref) + o.y * __builtin_amdgcn_exp2f(o.x - ref));
+      }
+      const int n = t.tn * C::BN + x;
+      if (n < e.N) e.partial[(int64_t)(e.tile0 + t.tm) * e.N + n] = r;
+    }
+  }
+};
+
+// dl of a piece of the vocabulary, as [n][v] and as [v][n]; PLANES = 3: as the three bf16 of each number
+template <int KIND, int PLANES>
+struct DlogitsEpi {
+  struct Args {
+    const float2* stat;         // {max * log2e, 1 / sum} of a token
+    const float* ratio;         // g_n over the largest |g|, times the lift of fp16; 0: the row takes no part
+    const int64_t* target;
+    int64_t v0;
+    int N, Np, V, Vp;           // tokens and vocabulary rows of the piece, and both as laid out
+    float k;
+    uint16_t *dl, *dlt;         // [N][ldl], [V][ldt]; planes behind each other
+    int64_t ldl, ldt, pl, pt;
+  };
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, char* lds, const po::mm::Args&) {
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      const int n = t.col(j);
+      const bool in = n < e.N;
+      const float2 st = in ? e.stat[n] : make_float2(0.f, 0.f);
+      const float r = in ? e.ratio[n] : 0.f, ir = st.y * r;
+      int64_t tg64 = in ? e.target[n] - e.v0 - t.m0 : -1;
+      const int tg = tg64 >= 0 && tg64 < C::TM * 32 ? (int)tg64 : -1;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const int m = i * 32 + 8 * (k >> 2) + 4 * (t.lane >> 5) + (k & 3);
+          float v = __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][k], e.k, -st.x)) * ir;
+          if (m == tg) v -= r;
+          // rows that take no part may hold anything, NaN too; vocabulary rows past the end
+          t.acc[i][j][k] = r != 0.f && t.m0 + m < e.V ? v : 0.f;
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) {
+      __syncthreads();                                       // the loop's (or the last plane's) reads are over
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            u2v w;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float x = t.acc[i][j][4 * q + 2 * k], y = t.acc[i][j][4 * q + 2 * k + 1];
+              w[k] = pack2<KIND>(x, y);
+              if constexpr (PLANES > 1) {                    // what this plane leaves to the next
+                t.acc[i][j][4 * q + 2 * k] = x - __uint_as_float(w[k] << 16);
+                t.acc[i][j][4 * q + 2 * k + 1] = y - __uint_as_float(w[k] & 0xffff0000u);
+              }
+            }
+            stage4(t, lds, i, j, q, w);
+          }
+      __syncthreads();
+      const int n0 = t.tn * C::BN, m0 = t.tm * C::BM;
+      if (e.dl) store_rows<C>(lds, e.dl + p * e.pl, e.ldl, n0, m0, e.N, e.Vp, true);
+      if (e.dlt) store_columns<C>(lds, e.dlt + p * e.pt, e.ldt, n0, m0, e.Np, e.V);
+    }
+  }
+};
+
+// slab[slice][n][m] (+)= acc in 32 bits: the sums of dh over slices of a piece's k and over the pieces
+struct SlabEpi {
+  struct Args {
+    float* slab;
+    int64_t ld, slice;          // ld a multiple of 4
+    int N, M, add;
+  };
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, char*, const po::mm::Args&) {
+    float* out = e.slab + blockIdx.y * e.slice;
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      const int n = t.col(j);
+      if (n >= e.N) continue;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int m = t.row4(i, q);
+          if (m >= e.ld) continue;
+          float4* o = reinterpret_cast<float4*>(out + (int64_t)n * e.ld + m);
+          float4 v = make_float4(t.acc[i][j][4 * q], t.acc[i][j][4 * q + 1], t.acc[i][j][4 * q + 2], t.acc[i][j][4 * q + 3]);
+          if (e.add) {
+            const float4 u = *o;
+            v = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
+          }
+          *o = v;
+        }
+    }
+  }
+};
+
+// out[n][m] = acc * *factor in the gradients' type (OUT: BF16, F16, or 3: fp32)
+template <int OUT>
+struct GradEpi {
+  struct Args {
+    void* out;
+    int64_t ld;
+    const float* factor;
+    int N, M, wide;             // wide: rows start on 16 bytes
+  };
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, char* lds, const po::mm::Args&) {
+    const float f = *e.factor;
+    if constexpr (OUT == 3) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        const int n = t.col(j);
+        if (n >= e.N) continue;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int m = t.row4(i, q);
+            float* o = static_cast<float*>(e.out) + (int64_t)n * e.ld + m;
+            if (e.wide && m + 4 <= e.M) {
+              *reinterpret_cast<float4*>(o) = make_float4(t.acc[i][j][4 * q] * f, t.acc[i][j][4 * q + 1] * f,
+                                                          t.acc[i][j][4 * q + 2] * f, t.acc[i][j][4 * q + 3] * f);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (m + k < e.M) o[k] = t.acc[i][j][4 * q + k] * f;
+            }
+          }
+      }
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            stage4(t, lds, i, j, q, u2v{pack2<OUT>(t.acc[i][j][4 * q] * f, t.acc[i][j][4 * q + 1] * f),
+                                        pack2<OUT>(t.acc[i][j][4 * q + 2] * f, t.acc[i][j][4 * q + 3] * f)});
+      __syncthreads();
+      store_rows<C>(lds, static_cast<uint16_t*>(e.out), e.ld, t.tn * C::BN, t.tm * C::BM, e.N, e.M, e.wide != 0);
+    }
+  }
+};
+
+// ---- the rows' kernels ---------------------------------------------------
+
+// Rows' statistics from the tiles': R rows to a workgroup, 256 / R lanes to a
+// row (many rows: neighbouring lanes read neighbouring rows; one row: all lanes
+// share its tiles).
+template <int R>
+__global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ partial, int parts, int N, int64_t V,
+                                                   const float* __restrict__ tlogit, const int64_t* __restrict__ target,
+                                                   int64_t ignore, float k, float2* __restrict__ stat,
+                                                   float* __restrict__ loss) {
+  __shared__ float2 red[256];
+  const int row = threadIdx.x % R, n = blockIdx.x * R + row;
+  float m = -INFINITY, s = 0.f;
+  if (n < N)
+    for (int p = threadIdx.x / R; p < parts; p += 256 / R) {
+      const float2 o = partial[(int64_t)p * N + n];
+      const float t = fmaxf(m, o.x), ref = t == -INFINITY ? 0.f : t;
+      s = s * __builtin_amdgcn_exp2f(m - ref) + o.y * __builtin_amdgcn_exp2f(o.x - ref);
+      m = t;
+    }
+  red[threadIdx.x] = make_float2(m, s);
+  __syncthreads();
+#pragma unroll
+  for (int w = 128; w >= R; w >>= 1) {
+    if (threadIdx.x < w) {
+      const float2 a = red[threadIdx.x], b = red[threadIdx.x + w];
+      const float t = fmaxf(a.x, b.x), ref = t == -INFINITY ? 0.f : t;
+      red[threadIdx.x] = make_float2(t, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x < R && n < N) {
+    const float2 r = red[threadIdx.x];
+    const int64_t t = target[n];
+    stat[n] = make_float2(r.x, 1.f / r.y);
+    // log(sum) - (l_t - max): the maximum leaves before anything is rounded to its size
+    loss[n] = t == ignore ? 0.f
+              : t < 0 || t >= V ? __uint_as_float(0x7fc00000u)
+                                : kLn2 * (__builtin_log2f(r.y) - __builtin_fmaf(tlogit[n], k, -r.x));
+  }
+}
+
+__device__ __forceinline__ double block_sum(double x) {
+  __shared__ double red[1024];
+  red[threadIdx.x] = x;
+  __syncthreads();
+  for (int w = 512; w; w >>= 1) {
+    if (threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+    __syncthreads();
+  }
+  const double r = red[0];
+  __syncthreads();
+  return r;
+}
+
+// *out = the sum (mean: over the rows that count) of the rows' losses; *count = those rows
+__global__ __launch_bounds__(1024) void total_loss_k(const float* __restrict__ loss, const int64_t* __restrict__ target,
+                                                     int N, int64_t ignore, int mean, float* __restrict__ out,
+                                                     float* __restrict__ count) {
+  double s = 0, c = 0;
+  for (int n = threadIdx.x; n < N; n += 1024) {
+    s += loss[n];
+    c += target[n] != ignore;
+  }
+  s = block_sum(s);
+  c = block_sum(c);
+  if (threadIdx.x == 0) {
+    *out = (float)(mean ? s / c : s);
+    *count = (float)c;
+  }
+}
+
+// ratio[n] = g_n / max |g| * lift (0: the row takes no part), *factor = max |g| / lift * c
+__global__ __launch_bounds__(1024) void grad_rows_k(const float* __restrict__ grad, int each, int mean,
+                                                    const float* __restrict__ count, const int64_t* __restrict__ target,
+                                                    int N, int64_t V, int64_t ignore, float lift, float c,
+                                                    float* __restrict__ ratio, float* __restrict__ factor) {
+  __shared__ float red[1024];
+  const float over = mean ? *count : 1.f;
+  float top = 0.f;
+  for (int n = threadIdx.x; n < N; n += 1024)
+    if (target[n] != ignore) top = fmaxf(top, fabsf(each ? grad[n] : *grad));
+  red[threadIdx.x] = top;
+  __syncthreads();
+  for (int w = 512; w; w >>= 1) {
+    if (threadIdx.x < w) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + w]);
+    __syncthreads();
+  }
+  top = red[0];
+  for (int n = threadIdx.x; n < N; n += 1024) {
+    const int64_t t = target[n];
+    const float g = each ? grad[n] : *grad;
+    ratio[n] = t == ignore ? 0.f : t < 0 || t >= V ? __uint_as_float(0x7fc00000u) : g == 0.f ? 0.f : g / top * lift;
+  }
+  if (threadIdx.x == 0) *factor = top > 0.f ? top / over / lift * c : 0.f;
+}
+
+// Rows laid out for the products: 16-bit rows padded with zeros to ldo, or fp32 as planes of three bf16.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_k(const T* __restrict__ x, int64_t ld, int64_t rows, int cols,
+                                              uint16_t* __restrict__ out, int ldo, int64_t plane) {
+  const int64_t total = rows * ldo;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / ldo;
+    const int c = (int)(i - r * ldo);
+    if constexpr (sizeof(T) == 4) {
+      float v = c < cols ? x[r * ld + c] : 0.f;
+      const bool finite = fabsf(v) < INFINITY;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        uint32_t b = pack2<BF16>(v, 0.f) & 0xffffu;
+        // a finite number next to the largest rounds to infinity: cut it off instead
+        if ((b & 0x7fffu) == 0x7f80u) b -= 1;
+        // infinity and NaN stand in the last plane alone: it meets the other operand's first plane only, so
+        // that infinity times a number is infinity (times a zero of its later planes it would be NaN)
+        if (!finite) b = p == 2 ? pack2<BF16>(v, 0.f) & 0xffffu : 0;
+        out[p * plane + i] = (uint16_t)b;
+        if (finite) v -= __uint_as_float(b << 16);
+      }
+    } else {
+      out[i] = c < cols ? x[r * ld + c] : (T)0;
+    }
+  }
+}
+
+// out[c][r] = x[r][c] (16 bits) for r < Rp: zero for r >= R and for rows whose ratio is 0 (they may hold
+// anything and multiply zeros only); blockIdx.z: plane
+__global__ __launch_bounds__(256) void transpose_k(const uint16_t* __restrict__ x, int64_t ld, int64_t plane, int R,
+                                                   int Cc, const float* __restrict__ ratio, uint16_t* __restrict__ out,
+                                                   int64_t ldo, int64_t oplane, int Rp) {
+  __shared__ uint16_t tile[64][66];
+  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  x += blockIdx.z * plane;
+  out += blockIdx.z * oplane;
+  for (int k = threadIdx.x; k < 64 * 64; k += 256) {
+    const int r = r0 + k / 64, c = c0 + k % 64;
+    const bool ok = r < R && c < Cc && (!ratio || ratio[r] != 0.f);
+    tile[k / 64][k % 64] = ok ? x[r * ld + c] : 0;
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < 64 * 64; k += 256) {
+    const int c = c0 + k / 64, r = r0 + k % 64;
+    if (c < Cc && r < Rp) out[c * ldo + r] = tile[k % 64][k / 64];
+  }
+}
+
+// dh[n][m] = factor * the slabs' sum, slab after slab
+template <int OUT>
+__global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab, int slices, int64_t slice, int64_t ld,
+                                                  int N, int M, const float* __restrict__ factor, void* __restrict__ out,
+                                                  int64_t ldo) {
+  const float f = *factor;
+  const int64_t total = (int64_t)N * M;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = i / M;
+    const int m = (int)(i - n * M);
+    float v = 0.f;
+    for (int s = 0; s < slices; ++s) v += slab[s * slice + n * ld + m];
+    v *= f;
+    if constexpr (OUT == 3)
+      static_cast<float*>(out)[n * ldo + m] = v;
+    else
+      static_cast<uint16_t*>(out)[n * ldo + m] = (uint16_t)pack2<OUT>(v, 0.f);
+  }
+}
+
+// ---- the plan ------------------------------------------------------------
+
+constexpr int64_t kPieceBytes = 512LL << 20;   // what a piece of the vocabulary may take of the workspace
+
+struct Shape {
+  int64_t N, V, D;
+  int dtype;
+  bool direct_h, direct_w;      // the caller's rows serve as they are
+  int planes() const { return dtype == PO_F32 ? 3 : 1; }
+  int Dp() const { return (int)((D + 7) / 8 * 8); }
+  int64_t Np() const { return (N + 31) / 32 * 32; }
+};
+
+inline int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
+
+// bytes of the workspace as it is laid out by both passes; p: pointers, or sizes from a null base
+struct Layout {
+  char* base;
+  int64_t at = 0;
+  explicit Layout(void* b) : base(static_cast<char*>(b)) {}
+  template <typename T>
+  T* take(int64_t n) {
+    T* r = reinterpret_cast<T*>(base + at);
+    at += up(n * (int64_t)sizeof(T));
+    return r;
+  }
+};
+
+// vocabulary rows of a piece: a multiple of 256, per_row bytes each
+inline int64_t piece_rows(int64_t V, int64_t per_row) {
+  int64_t p = kPieceBytes / (per_row > 0 ? per_row : 1) / 256 * 256;
+  p = std::min<int64_t>(std::max<int64_t>(p, 256), 1 << 20);
+  return p < V ? p : V;
+}
+
+struct FwdWs {
+  float2* partial;
+  float *tlogit, *rowloss;
+  uint16_t *hp, *wp;
+  int64_t piece, bytes;
+  int parts;
+  FwdWs(const Shape& s, void* b) {
+    Layout l(b);
+    const int64_t wrow = s.direct_w ? 0 : (int64_t)s.Dp() * 2 * s.planes();
+    piece = wrow ? piece_rows(s.V, wrow) : s.V;
+    parts = 0;
+    for (int64_t v = 0; v < s.V; v += piece) parts += ceil_div(std::min(piece, s.V - v), 128);
+    partial = l.take<float2>((int64_t)parts * s.N);
+    tlogit = l.take<float>(s.N);
+    rowloss = l.take<float>(s.N);
+    hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.Dp() * s.planes());
+    wp = l.take<uint16_t>(piece * wrow / 2);
+    bytes = l.at;
+  }
+};
+
+constexpr int kSlabSlices = 64;
+
+// slices of dh's k (a piece's vocabulary rows): few tiles are cut until the chip is filled
+inline int dh_slices(int64_t tiles, int64_t steps) {
+  int64_t s = tiles >= 256 ? 1 : 512 / tiles;
+  s = std::min<int64_t>(s, kSlabSlices);
+  return (int)std::max<int64_t>(1, std::min(s, steps / 4));
+}
+
+struct BwdWs {
+  float *ratio, *factor, *slab;
+  uint16_t *hp, *ht, *wp, *wt, *dl, *dlt;
+  int64_t piece, ldl, slab_ld, slab_slice, bytes;
+  int slices, bm, bn;
+  BwdWs(const Shape& s, bool dh, bool dw, void* b) {
+    Layout l(b);
+    const int P = s.planes();
+    const int64_t per = (s.direct_w ? 0 : (int64_t)s.Dp() * 2 * P) + (dh ? (s.N + s.D) * 2 * P : 0) + (dw ? s.Np() * 2 * P : 0);
+    piece = piece_rows(s.V, per);
+    ldl = (piece + 63) / 64 * 64;
+    ratio = l.take<float>(s.N);
+    factor = l.take<float>(1);
+    hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.Dp() * P);
+    ht = l.take<uint16_t>(dw ? s.D * s.Np() * P : 0);
+    wp = l.take<uint16_t>(s.direct_w ? 0 : piece * s.Dp() * P);
+    wt = l.take<uint16_t>(dh ? s.D * ldl * P : 0);
+    dl = l.take<uint16_t>(dh ? s.N * ldl * P : 0);
+    dlt = l.take<uint16_t>(dw ? piece * s.Np() * P : 0);
+    bm = s.N <= 32 ? 128 : 256;
+    bn = s.N <= 32 ? 32 : 256;
+    if (s.N > 32 && (int64_t)ceil_div(s.D, 256) * ceil_div(s.N, 256) < 128) bm = bn = 128;
+    slab_ld = (s.D + 3) / 4 * 4;
+    slab_slice = s.N * slab_ld;
+    slices = dh_slices((int64_t)ceil_div(s.D, bm) * ceil_div(s.N, bn), (int64_t)ceil_div(ldl * 2, 128) * (P == 3 ? 6 : 1));
+    slab = l.take<float>(dh ? slices * slab_slice : 0);
+    bytes = l.at;
+  }
+};
+
+// pairs of planes, the largest products first: 00 01 10 11 02 20
+inline void set_pairs(Args& a, int planes) {
+  a.pairs = planes == 3 ? 6 : 1;
+  a.pa = planes == 3 ? 0x201100u : 0u;
+  a.pb = planes == 3 ? 0x021010u : 0u;
+}
+
+template <typename T>
+inline void pack(const void* x, int64_t ld, int64_t rows, int cols, uint16_t* out, int ldo, hipStream_t s) {
+  const int64_t total = rows * ldo;
+  const int grid = (int)std::min<int64_t>((total + 255) / 256, 8192);
+  if (grid > 0)
+    hipLaunchKernelGGL((pack_k<T>), dim3(grid), dim3(256), 0, s, static_cast<const T*>(x), ld, rows, cols, out, ldo,
+                       rows * ldo);
+}
+
+// operand rows [r0, r0 + rows) of the caller's matrix, packed into buf where they do not serve as they are
+inline Operand rows_of(const Shape& s, bool direct, const void* x, int64_t ld, int64_t r0, int64_t rows, uint16_t* buf,
+                       hipStream_t st) {
+  const int es = s.dtype == PO_F32 ? 4 : 2;
+  const char* p = static_cast<const char*>(x) + r0 * ld * es;
+  if (direct) return Operand{p, ld * 2, 0, (int)rows};
+  if (s.dtype == PO_F32)
+    pack<float>(p, ld, rows, (int)s.D, buf, s.Dp(), st);
+  else
+    pack<uint16_t>(p, ld, rows, (int)s.D, buf, s.Dp(), st);
+  return Operand{reinterpret_cast<char*>(buf), (int64_t)s.Dp() * 2, rows * s.Dp() * 2, (int)rows};
+}
+
+inline bool serves(const void* x, int64_t ld, int dtype, int64_t D) {
+  return dtype != PO_F32 && D % 8 == 0 && ld % 8 == 0 && (uintptr_t)x % 16 == 0;
+}
+
+inline int check_shape(const char* what, int64_t N, int64_t V, int64_t D, int dtype, int64_t ldh, int64_t ldw) {
+  PO_REQUIRE(dtype == PO_F32 || dtype == PO_F16 || dtype == PO_BF16, "%s: unknown dtype %d", what, dtype);
+  PO_REQUIRE(N >= 1 && V >= 1 && D >= 1 && N <= (1 << 21) && V < (1LL << 31) - 256 && D <= (1 << 20),
+             "%s: bad sizes (N=%lld V=%lld D=%lld)", what, (long long)N, (long long)V, (long long)D);
+  PO_REQUIRE(ldh >= D && ldw >= D && ldh <= (1 << 21) && ldw <= (1 << 21), "%s: bad row strides", what);
+  return PO_OK;
+}
+
+template <int KIND, class Epi>
+inline int by_tokens(const Args& a, const typename Epi::Args& e, int64_t N, hipStream_t s, const char* what) {
+  if (N <= 32) return launch_product<Few<KIND>, Epi>(a, e, 1, s, what);
+  if (N <= 128) return launch_product<Mid<KIND>, Epi>(a, e, 1, s, what);
+  return launch_product<Large<KIND>, Epi>(a, e, 1, s, what);
+}
+
+inline int tile_rows(int64_t N) { return N <= 128 ? 128 : 256; }
+
+#define PO_TRY(x)             \
+  do {                        \
+    const int rc_ = (x);      \
+    if (rc_ != PO_OK) return rc_; \
+  } while (0)
+
+}  // namespace
+
+extern "C" int po_linear_ce_workspace(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N,
+                                      int64_t V, int64_t D, int dh, int dw, int64_t* fwd_bytes, int64_t* bwd_bytes) {
+  PO_TRY(check_shape("po_linear_ce_workspace", N, V, D, dtype, ldh, ldw));
+  const Shape s{N, V, D, dtype, serves(h, ldh, dtype, D), serves(w, ldw, dtype, D)};
+  if (fwd_bytes) *fwd_bytes = FwdWs(s, nullptr).bytes;
+  if (bwd_bytes) *bwd_bytes = BwdWs(s, dh != 0, dw != 0, nullptr).bytes;
+  return PO_OK;
+}
+
+extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V,
+                                int64_t D, const int64_t* target, int64_t ignore_index, float scale, int reduction,
+                                void* workspace, int64_t workspace_bytes, float* stat, float* loss, float* count,
+                                po_stream_t stream) {
+  PO_TRY(check_shape("po_linear_ce_fwd", N, V, D, dtype, ldh, ldw));
+  PO_REQUIRE(h && w && target && workspace && stat && loss && (reduction == 0 || count), "po_linear_ce_fwd: null pointer");
+  PO_REQUIRE(reduction >= 0 && reduction <= 2, "po_linear_ce_fwd: unknown reduction %d", reduction);
+  PO_REQUIRE(scale > 0.f && scale < INFINITY, "po_linear_ce_fwd: the scale must be positive and finite");
+  const Shape s{N, V, D, dtype, serves(h, ldh, dtype, D), serves(w, ldw, dtype, D)};
+  const FwdWs ws(s, workspace);
+  PO_REQUIRE(workspace_bytes >= ws.bytes, "po_linear_ce_fwd: workspace of %lld bytes, %lld needed",
+             (long long)workspace_bytes, (long long)ws.bytes);
+  const hipStream_t st = po::stream_of(stream);
+  Args a{};
+  set_pairs(a, s.planes());
+  a.kbytes = s.Dp() * 2;
+  a.B = rows_of(s, s.direct_h, h, ldh, 0, N, ws.hp, st);
+  StatsEpi::Args e{ws.partial, ws.tlogit, target, 0, 0, (int)N, 0, scale * kLog2e};
+  for (int64_t v = 0; v < V; v += ws.piece) {
+    const int64_t rows = std::min(ws.piece, V - v);
+    a.A = rows_of(s, s.direct_w, w, ldw, v, rows, ws.wp, st);
+    e.v0 = v;
+    e.V = (int)rows;
+    PO_TRY((dtype == PO_F16 ? by_tokens<F16, StatsEpi>(a, e, N, st, "po_linear_ce_fwd")
+                            : by_tokens<BF16, StatsEpi>(a, e, N, st, "po_linear_ce_fwd")));
+    e.tile0 += ceil_div(rows, tile_rows(N));
+  }
+  float* rows = reduction ? ws.rowloss : loss;
+  float2* stat2 = reinterpret_cast<float2*>(stat);
+  if (N >= 2048)
+    hipLaunchKernelGGL((row_stats_k<16>), dim3(ceil_div(N, 16)), dim3(256), 0, st, ws.partial, e.tile0, (int)N, V,
+                       ws.tlogit, target, ignore_index, e.k, stat2, rows);
+  else
+    hipLaunchKernelGGL((row_stats_k<1>), dim3((unsigned)N), dim3(256), 0, st, ws.partial, e.tile0, (int)N, V, ws.tlogit,
+                       target, ignore_index, e.k, stat2, rows);
+  if (reduction)
+    hipLaunchKernelGGL(total_loss_k, dim3(1), dim3(1024), 0, st, rows, target, (int)N, ignore_index, reduction == 2,
+                       loss, count);
+  return po::check_launch("po_linear_ce_fwd");
+}
+
+namespace {
+
+template <int KIND, int OUT>
+int backward(const Shape& s, const BwdWs& ws, const void* h, int64_t ldh, const void* w, int64_t ldw,
+             const int64_t* target, float scale, const float2* stat, void* dh, int64_t lddh, void* dw, int64_t lddw,
+             hipStream_t st) {
+  constexpr int P = OUT == 3 ? 3 : 1;
+  const char* what = "po_linear_ce_bwd";
+  const int N = (int)s.N, D = (int)s.D;
+  const Operand H = rows_of(s, s.direct_h, h, ldh, 0, N, ws.hp, st);
+  if (dw)
+    hipLaunchKernelGGL(transpose_k, dim3(ceil_div(s.Np(), 64), ceil_div(D, 64), P), dim3(256), 0, st,
+                       reinterpret_cast<const uint16_t*>(H.p), H.stride / 2, H.plane / 2, N, D, ws.ratio, ws.ht,
+                       s.Np(), D * s.Np(), (int)s.Np());
+  for (int64_t v = 0; v < s.V; v += ws.piece) {
+    const int rows = (int)std::min(ws.piece, s.V - v);
+    const int rp = (rows + 63) / 64 * 64;
+    const Operand W = rows_of(s, s.direct_w, w, ldw, v, rows, ws.wp, st);
+    Args a{};
+    set_pairs(a, P);
+    // dl of the piece
+    a.A = W;
+    a.B = H;
+    a.kbytes = s.Dp() * 2;
+    typename DlogitsEpi<KIND, P>::Args e{stat, ws.ratio, target, v, N, (int)s.Np(), rows, rp, scale * kLog2e,
+                                         dh ? ws.dl : nullptr, dw ? ws.dlt : nullptr, ws.ldl, s.Np(), N * ws.ldl,
+                                         ws.piece * s.Np()};
+    PO_TRY((by_tokens<KIND, DlogitsEpi<KIND, P>>(a, e, N, st, what)));
+    if (dh) {                                                // slab[n][d] += sum_v dl[n][v] w[v][d]
+      hipLaunchKernelGGL(transpose_k, dim3(ceil_div(rp, 64), ceil_div(D, 64), P), dim3(256), 0, st,
+                         reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, D,
+                         (const float*)nullptr, ws.wt, ws.ldl, D * ws.ldl, rp);
+      a.A = Operand{reinterpret_cast<char*>(ws.wt), ws.ldl * 2, D * ws.ldl * 2, D};
+      a.B = Operand{reinterpret_cast<char*>(ws.dl), ws.ldl * 2, N * ws.ldl * 2, N};
+      a.kbytes = rp * 2;
+      const SlabEpi::Args se{ws.slab, ws.slab_ld, ws.slab_slice, N, D, v > 0};
+      if (ws.bn == 32)
+        PO_TRY((launch_product<Few<KIND>, SlabEpi>(a, se, ws.slices, st, what)));
+      else if (ws.bn == 128)
+        PO_TRY((launch_product<Mid<KIND>, SlabEpi>(a, se, ws.slices, st, what)));
+      else
+        PO_TRY((launch_product<Large<KIND>, SlabEpi>(a, se, ws.slices, st, what)));
+    }
+    if (dw) {                                                // dw[v][d] = sum_n dl[n][v] h[n][d]
+      a.A = Operand{reinterpret_cast<char*>(ws.ht), s.Np() * 2, D * s.Np() * 2, D};
+      a.B = Operand{reinterpret_cast<char*>(ws.dlt), s.Np() * 2, ws.piece * s.Np() * 2, rows};
+      a.kbytes = (int)s.Np() * 2;
+      const int es = OUT == 3 ? 4 : 2;
+      char* out = static_cast<char*>(dw) + v * lddw * es;
+      const typename GradEpi<OUT>::Args ge{out, lddw, ws.factor, rows, D, (uintptr_t)out % 16 == 0 && lddw * es % 16 == 0};
+      PO_TRY((launch_product<Large<KIND>, GradEpi<OUT>>(a, ge, 1, st, what)));
+    }
+  }
+  if (dh) {
+    const int grid = (int)std::min<int64_t>(((int64_t)N * D + 255) / 256, 8192);
+    hipLaunchKernelGGL((slab_sum_k<OUT>), dim3(grid), dim3(256), 0, st, ws.slab, ws.slices, ws.slab_slice, ws.slab_ld,
+                       N, D, ws.factor, dh, lddh);
+  }
+  return po::check_launch(what);
+}
+
+}  // namespace
+
+extern "C" int po_linear_ce_bwd(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V,
+                                int64_t D, const int64_t* target, int64_t ignore_index, float scale, int reduction,
+                                const float* stat, const float* count, const float* grad, void* workspace,
+                                int64_t workspace_bytes, void* dh, int64_t lddh, void* dw, int64_t lddw,
+                                po_stream_t stream) {
+  PO_TRY(check_shape("po_linear_ce_bwd", N, V, D, dtype, ldh, ldw));
+  PO_REQUIRE(h && w && target && workspace && stat && grad && (reduction != 2 || count), "po_linear_ce_bwd: null pointer");
+  PO_REQUIRE(reduction >= 0 && reduction <= 2, "po_linear_ce_bwd: unknown reduction %d", reduction);
+  PO_REQUIRE(scale > 0.f && scale < INFINITY, "po_linear_ce_bwd: the scale must be positive and finite");
+  PO_REQUIRE((!dh || lddh >= D) && (!dw || lddw >= D), "po_linear_ce_bwd: bad row strides");
+  if (!dh && !dw) return PO_OK;
+  const Shape s{N, V, D, dtype, serves(h, ldh, dtype, D), serves(w, ldw, dtype, D)};
+  const BwdWs ws(s, dh != nullptr, dw != nullptr, workspace);
+  PO_REQUIRE(workspace_bytes >= ws.bytes, "po_linear_ce_bwd: workspace of %lld bytes, %lld needed",
+             (long long)workspace_bytes, (long long)ws.bytes);
+  const hipStream_t st = po::stream_of(stream);
+  hipLaunchKernelGGL(grad_rows_k, dim3(1), dim3(1024), 0, st, grad, reduction == 0, reduction == 2, count, target, (int)N,
+                     V, ignore_index, dtype == PO_F16 ? kF16Lift : 1.f, scale, ws.ratio, ws.factor);
+  const float2* st2 = reinterpret_cast<const float2*>(stat);
+  if (dtype == PO_F16) return backward<F16, F16>(s, ws, h, ldh, w, ldw, target, scale, st2, dh, lddh, dw, lddw, st);
+  if (dtype == PO_BF16) return backward<BF16, BF16>(s, ws, h, ldh, w, ldw, target, scale, st2, dh, lddh, dw, lddw, st);
+  return backward<BF16, 3>(s, ws, h, ldh, w, ldw, target, scale, st2, dh, lddh, dw, lddw, st);
+}

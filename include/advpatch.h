@@ -36,6 +36,11 @@ typedef void* po_stream_t;
 #define PO_ABI_VERSION 30
 #define PO_AMAX_SUB 64  /* sub-slots per max|x| slot (see po_conv_desc) */
 
+/* element types of the head's operators (po_dropout, po_linear_ce_*, po_quantize_rows, po_int8_matmul) */
+#define PO_F32 0
+#define PO_F16 1
+#define PO_BF16 2
+
 int po_abi_version(void);
 const char* po_last_error(void);
 /* Select the device and verify it is gfx950.  Returns PO_EDEVICE otherwise. */
@@ -716,6 +721,62 @@ int po_maxpool2_bwd_box(const float* d_dst, const int8_t* argmax, int B, int H, 
  * the drop-in Darknet.forward API). */
 int po_nhwc_to_nchw(const float* src, int B, int H, int W, int C, int Cp, float* dst, po_stream_t s);
 int po_nchw_to_nhwc(const float* src, int B, int H, int W, int C, int Cp, float* dst, po_stream_t s);
+
+/* ---------------- operators of a large-vocabulary head ---------------- */
+/* Matrices are [rows][cols] with a row stride (ld*) in elements; a row's
+ * elements are neighbours.  Types: PO_F32, PO_F16, PO_BF16. */
+
+/* Dropout whose mask is a function of a key, never stored:
+ *   y[r][c] = (u >= drop ? x[r][c] * 65536 / (65536 - drop) : 0) [+ residual[r][c]]
+ * u = 16 bits of Philox4x32-10, key {seed lo, seed hi ^ 0x64726F70}, counter
+ * {c / 8, row0 + r, step lo, step hi}: half c % 2 (low first) of word (c % 8) / 2.
+ * drop in [0, 65536] is the drop probability times 65536; a dropped element is 0
+ * whatever x holds.  residual may be NULL.  step_dev (may be NULL) overrides step
+ * with a number on the device (a replayed graph draws new masks); step_used (may
+ * be NULL) receives the step taken.  The backward pass is the same call on dy
+ * without a residual.  row0: global index of row 0 (shards of a batch draw the rows
+ * a single process draws); row0 + rows <= 2^32.  y may be x or residual. */
+int po_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, int dtype, int64_t rows, int64_t cols,
+               uint64_t seed, uint64_t step, const int64_t* step_dev, int64_t* step_used, int64_t row0, int drop,
+               void* y, int64_t ldy, po_stream_t s);
+
+/* Softmax cross entropy of a linear head, without its logits in memory:
+ *   l[n][v] = scale * h[n] . w[v]; loss[n] = log sum_v exp l[n][v] - l[n][target[n]]
+ * h [N][D], w [V][D], target [N]; rows with target == ignore_index take no part
+ * (loss 0, gradient 0, whatever h holds there); a target outside [0, V) that is
+ * not ignore_index makes its row's loss, and the gradients, NaN.  scale > 0.
+ * reduction 0: loss [N]; 1: their sum; 2: their mean over the rows that take part
+ * (NaN if there is none), with count [1] receiving the number of those rows
+ * (also for 1; may be NULL for 0).  loss is fp32.  stat [N][2] fp32 is what the
+ * backward pass needs of the forward's.  N <= 2^21, D <= 2^20. */
+int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V, int64_t D,
+                     const int64_t* target, int64_t ignore_index, float scale, int reduction, void* workspace,
+                     int64_t workspace_bytes, float* stat, float* loss, float* count, po_stream_t s);
+/* dh [N][D] and dw [V][D] (either may be NULL) of grad (fp32: [N] for reduction
+ * 0, else [1]).  Walks the vocabulary piece by piece: the logits once more, their
+ * gradient in 16 bits (fp32 inputs: in three planes of 16), the two products. */
+int po_linear_ce_bwd(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V, int64_t D,
+                     const int64_t* target, int64_t ignore_index, float scale, int reduction, const float* stat,
+                     const float* count, const float* grad, void* workspace, int64_t workspace_bytes, void* dh,
+                     int64_t lddh, void* dw, int64_t lddw, po_stream_t s);
+/* Bytes of the two workspaces (256-byte aligned, caller's) for these matrices
+ * (dh / dw: whether that gradient is wanted).  Matrices whose rows do not serve the
+ * matrix cores as they are (fp32, D or the stride no multiple of 8, rows off 16
+ * bytes) are laid out in them, w piece by piece. */
+int po_linear_ce_workspace(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V,
+                           int64_t D, int dh, int dw, int64_t* fwd_bytes, int64_t* bwd_bytes);
+
+/* scale[m] = max_k |x[m][k]| / 127; q[m][k] = x[m][k] / scale[m] rounded to the
+ * nearest (the exact quotient; ties to even), zeros up to the next multiple of 16
+ * columns.  A row of zeros gets scale 0; a row that holds NaN or an infinity gets
+ * scale NaN (and q 0).  ldq a multiple of 16, q on 16 bytes; K < 2^17. */
+int po_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale,
+                     po_stream_t s);
+/* y[m][n] = (sum_k q[m][k] * w[n][k]) * sx[m] * sw[n] [+ bias[n]]: whole-number
+ * sums in 32 bits, y in dtype.  Rows of q and w start on 16 bytes; q is zero (and
+ * w anything) from K up to the next multiple of 16.  K < 2^17. */
+int po_int8_matmul(const int8_t* q, int64_t ldq, const float* sx, const int8_t* w, int64_t ldw, const float* sw,
+                   const float* bias, int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int dtype, po_stream_t s);
 
 #ifdef __cplusplus
 }
