@@ -14,15 +14,35 @@ namespace {
 using namespace po::mm;
 using po::ceil_div;
 
-// Elements of the callers' types as fp32.
+// n <= 8 neighbouring elements as fp32, wherever they start (global loads need no alignment); 0 past n.
 template <int DT>
-__device__ __forceinline__ float load1(const void* p, int64_t i) {
-  if constexpr (DT == PO_F32)
-    return static_cast<const float*>(p)[i];
-  else if constexpr (DT == PO_F16)
-    return (float)static_cast<const _Float16*>(p)[i];
-  else
-    return __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
+struct Elem {
+  using type = uint16_t;
+  static __device__ __forceinline__ float f(uint16_t v) {
+    if constexpr (DT == PO_F16)
+      return (float)__builtin_bit_cast(_Float16, v);
+    else
+      return __uint_as_float((uint32_t)v << 16);
+  }
+};
+template <>
+struct Elem<PO_F32> {
+  using type = float;
+  static __device__ __forceinline__ float f(float v) { return v; }
+};
+template <int DT>
+__device__ __forceinline__ void load8(const void* x, int64_t at, int n, float* v) {
+  typedef typename Elem<DT>::type T;
+  typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  const T* p = static_cast<const T*>(x) + at;
+  if (n >= 8) {
+    const v8 r = *reinterpret_cast<const v8*>(p);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = Elem<DT>::f(r[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = k < n ? Elem<DT>::f(p[k]) : 0.f;
+  }
 }
 
 // The quotient x / s rounded to the nearest whole number, ties to even, from the
@@ -36,8 +56,10 @@ __device__ __forceinline__ int quotient(float x, float s, float inv) {
   return (int)q;
 }
 
-// One row to WPR waves.  A row that holds NaN or an infinity gets the scale NaN.
-template <int DT, int WPR>
+// One row to WPR waves, 8 elements to a lane and step; rows of up to STEPS steps stay
+// in registers between the maximum and the quotients, longer ones (STEPS = 0) are read
+// again.  A row that holds NaN or an infinity gets the scale NaN.
+template <int DT, int WPR, int STEPS>
 __global__ __launch_bounds__(256) void quantize_rows_k(const void* __restrict__ x, int64_t ldx, int64_t rows, int K,
                                                        int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
   __shared__ uint32_t tops[4];
@@ -45,9 +67,25 @@ __global__ __launch_bounds__(256) void quantize_rows_k(const void* __restrict__ 
   const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + threadIdx.x / T;
   const int t = threadIdx.x % T;
   const int64_t at = row * ldx;
+  const int mine = row < rows ? K : 0;
+  const int Kp = (K + 15) / 16 * 16;
+  float v[STEPS ? STEPS : 1][8];
   uint32_t top = 0;
-  if (row < rows)
-    for (int k = t; k < K; k += T) top = max(top, __float_as_uint(load1<DT>(x, at + k)) & 0x7fffffffu);
+  auto top8 = [&](const float* w) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(w[j]) & 0x7fffffffu);
+  };
+  if constexpr (STEPS > 0) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) load8<DT>(x, at + (i * T + t) * 8, mine - (i * T + t) * 8, v[i]);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) top8(v[i]);
+  } else {
+    for (int k = t * 8; k < mine; k += T * 8) {
+      load8<DT>(x, at + k, mine - k, v[0]);
+      top8(v[0]);
+    }
+  }
   top = po::wave_max_u32(top);
   if constexpr (WPR > 1) {
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
@@ -58,15 +96,27 @@ __global__ __launch_bounds__(256) void quantize_rows_k(const void* __restrict__ 
   const bool bad = top >= 0x7f800000u;                       // as bits NaN lies above infinity
   const float s = __uint_as_float(top) / 127.f, inv = 1.f / s;
   if (t == 0) scale[row] = bad ? __uint_as_float(0x7fc00000u) : s;
-  const int Kp = (K + 15) / 16 * 16;
-  for (int k = t; k < Kp; k += T) {
-    int v = 0;
-    if (k < K && !bad && s > 0.f) {
-      const float f = load1<DT>(x, at + k);
-      // 1 / s and half steps of s need normal numbers
-      v = s > 1e-30f ? quotient(f, s, inv) : (int)__builtin_rint((double)f / (double)s);
+  auto put8 = [&](int k, const float* w) {
+    if (k >= Kp) return;
+    uint32_t b[2] = {0, 0};
+    if (!bad && s > 0.f) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // 1 / s and half steps of s need normal numbers
+        const int n = s > 1e-30f ? quotient(w[j], s, inv) : (int)__builtin_rint((double)w[j] / (double)s);
+        b[j >> 2] |= (uint32_t)(n & 255) << (8 * (j & 3));
+      }
     }
-    q[row * ldq + k] = (int8_t)v;
+    *reinterpret_cast<uint2*>(q + row * ldq + k) = make_uint2(b[0], b[1]);
+  };
+  if constexpr (STEPS > 0) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) put8((i * T + t) * 8, v[i]);
+  } else {
+    for (int k = t * 8; k < Kp; k += T * 8) {
+      load8<DT>(x, at + k, mine - k, v[0]);
+      put8(k, v[0]);
+    }
   }
 }
 
@@ -79,45 +129,50 @@ struct ScaledEpi {
     int N, M, wide;             // tokens, outputs; wide: rows start on 16 bytes
   };
   template <class C>
-  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, char* lds, const po::mm::Args&) {
+  struct Pre {
     float sx[C::TN];
+    __device__ __forceinline__ void load(const Tile<C>& t, const Args& e) {
 #pragma unroll
-    for (int j = 0; j < C::TN; ++j) sx[j] = t.col(j) < e.N ? e.sx[t.col(j)] : 0.f;
-    __syncthreads();
+      for (int j = 0; j < C::TN; ++j) sx[j] = t.col(j) < e.N ? e.sx[t.col(j)] : 0.f;
+    }
+  };
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, const Pre<C>& pre, char* lds) {
+    float swv[C::TM][4], bv[C::TM][4];
 #pragma unroll
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int m = t.row4(i, q);
-        float sw[4], b[4];
+      for (int k = 0; k < 4; ++k) {
+        swv[i][k] = t.row(i) + k < e.M ? e.sw[t.row(i) + k] : 0.f;
+        bv[i][k] = e.bias && t.row(i) + k < e.M ? e.bias[t.row(i) + k] : 0.f;
+      }
+    __syncthreads();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          sw[k] = m + k < e.M ? e.sw[m + k] : 0.f;
-          b[k] = e.bias && m + k < e.M ? e.bias[m + k] : 0.f;
-        }
+    for (int i = 0; i < C::TM; ++i) {
+      const int m = t.row(i);
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) {
-          float v[4];
+      for (int j = 0; j < C::TN; ++j) {
+        float v[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = __builtin_fmaf((float)t.acc[i][j][4 * q + k] * sx[j], sw[k], b[k]);
-          if constexpr (DT == PO_F32) {
-            const int n = t.col(j);
-            if (n < e.N) {
-              float* o = static_cast<float*>(e.y) + (int64_t)n * e.ld + m;
-              if (e.wide && m + 4 <= e.M) {
-                *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-              } else {
+        for (int k = 0; k < 4; ++k) v[k] = __builtin_fmaf((float)t.acc[i][j][k] * pre.sx[j], swv[i][k], bv[i][k]);
+        if constexpr (DT == PO_F32) {
+          const int n = t.col(j);
+          if (n < e.N) {
+            float* o = static_cast<float*>(e.y) + (int64_t)n * e.ld + m;
+            if (e.wide && m + 4 <= e.M) {
+              *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  if (m + k < e.M) o[k] = v[k];
-              }
+              for (int k = 0; k < 4; ++k)
+                if (m + k < e.M) o[k] = v[k];
             }
-          } else {
-            constexpr int KIND = DT == PO_F16 ? F16 : BF16;
-            stage4(t, lds, i, j, q, u2v{pack2<KIND>(v[0], v[1]), pack2<KIND>(v[2], v[3])});
           }
+        } else {
+          constexpr int KIND = DT == PO_F16 ? F16 : BF16;
+          stage4(t, lds, i, j, u2v{pack2<KIND>(v[0], v[1]), pack2<KIND>(v[2], v[3])});
         }
       }
+    }
     if constexpr (DT != PO_F32) {
       __syncthreads();
       store_rows<C>(lds, static_cast<uint16_t*>(e.y), e.ld, t.tn * C::BN, t.tm * C::BM, e.N, e.M, e.wide != 0);
@@ -125,16 +180,17 @@ struct ScaledEpi {
   }
 };
 
-// Tile by the work: the largest that still gives most CUs one; few tokens: 32 columns.
 template <int DT>
 int product_of(const Args& a, const typename ScaledEpi<DT>::Args& e, hipStream_t s) {
   using E = ScaledEpi<DT>;
   const char* what = "po_int8_matmul";
-  const int64_t M = a.A.rows, N = a.B.rows;
-  if (N <= 32) return launch_product<Cfg<I8, 128, 32, 4, 1, 128, 3>, E>(a, e, 1, s, what);
-  if ((int64_t)ceil_div(M, 256) * ceil_div(N, 256) >= 192) return launch_product<Cfg<I8, 256, 256, 2, 4, 128, 2>, E>(a, e, 1, s, what);
-  if ((int64_t)ceil_div(M, 128) * ceil_div(N, 128) >= 192) return launch_product<Cfg<I8, 128, 128, 2, 2, 128, 2>, E>(a, e, 1, s, what);
-  return launch_product<Cfg<I8, 64, 64, 2, 2, 128, 3>, E>(a, e, 1, s, what);
+  const Plan p = plan_product(a.A.rows, a.B.rows, ceil_div(a.kbytes, 128));
+  if (p.tile == FEW) return launch_product<Cfg<I8, 128, 32, 4, 1, 128, 3>, E>(a, e, 1, s, what);
+  if (p.tile == LARGE) return launch_product<Cfg<I8, 256, 256, 2, 4, 128, 2>, E>(a, e, 1, s, what);
+  // 64 x 64 where tiles of 128 x 128 leave CUs without one
+  if ((int64_t)ceil_div(a.A.rows, 128) * ceil_div(a.B.rows, 128) < 256)
+    return launch_product<Cfg<I8, 64, 64, 2, 2, 128, 3>, E>(a, e, 1, s, what);
+  return launch_product<Cfg<I8, 128, 128, 2, 2, 128, 2>, E>(a, e, 1, s, what);
 }
 
 inline int element_bytes(int dtype) { return dtype == PO_F32 ? 4 : 2; }
@@ -151,20 +207,21 @@ extern "C" int po_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t M
   PO_REQUIRE(ldx >= K && ldq >= (K + 15) / 16 * 16 && ldq % 16 == 0 && (uintptr_t)q % 16 == 0,
              "po_quantize_rows: bad strides");
   const hipStream_t s = po::stream_of(stream);
-  const bool wave = K <= 1024;                               // a wave covers such a row in a few steps
-  const dim3 grid(wave ? ceil_div(M, 4) : (unsigned)M);
-#define PO_Q(DT)                                                                                                       \
-  if (wave)                                                                                                            \
-    hipLaunchKernelGGL((quantize_rows_k<DT, 1>), grid, dim3(256), 0, s, x, ldx, M, (int)K, q, ldq, scale);             \
-  else                                                                                                                 \
-    hipLaunchKernelGGL((quantize_rows_k<DT, 4>), grid, dim3(256), 0, s, x, ldx, M, (int)K, q, ldq, scale);
-  if (dtype == PO_F32) {
-    PO_Q(PO_F32)
-  } else if (dtype == PO_F16) {
-    PO_Q(PO_F16)
-  } else {
-    PO_Q(PO_BF16)
-  }
+  // a wave to a row of up to 2048, a workgroup (of 4) to a longer one
+#define PO_Q(DT, WPR, STEPS)                                                                                           \
+  hipLaunchKernelGGL((quantize_rows_k<DT, WPR, STEPS>), dim3(ceil_div(M, 4 / WPR)), dim3(256), 0, s, x, ldx, M, (int)K, q, \
+                     ldq, scale)
+#define PO_QT(DT)                          \
+  do {                                     \
+    if (K <= 512) PO_Q(DT, 1, 1);          \
+    else if (K <= 2048) PO_Q(DT, 1, 4);    \
+    else if (K <= 8192) PO_Q(DT, 4, 4);    \
+    else PO_Q(DT, 4, 0);                   \
+  } while (0)
+  if (dtype == PO_F32) PO_QT(PO_F32);
+  else if (dtype == PO_F16) PO_QT(PO_F16);
+  else PO_QT(PO_BF16);
+#undef PO_QT
 #undef PO_Q
   return po::check_launch("po_quantize_rows");
 }

@@ -9,13 +9,23 @@
 // round are written that way once (a transpose, or the epilogue that makes
 // them), and every product runs this loop.
 //
-// A workgroup owns a BM x BN tile, its waves WM x WN rectangles of 32 x 32
-// MFMA blocks.  k advances in steps of KB bytes per row; STAGES LDS buffers are
-// filled ahead by 16-byte LDS-DMA.  Rows are KB bytes, their 16-byte chunks
-// XOR-swizzled by row (by the address each lane loads from: the DMA writes LDS
-// linearly), so 8 neighbouring lanes' fragment reads cover all banks.
-// Rows past the operand's end and k past its length read as zero (out-of-range
-// buffer offsets).
+// A workgroup owns a BM x BN tile, its waves WM x WN rectangles of 16 x 16 MFMA
+// blocks (v_mfma 16x16x32 of 16-bit floats, 16x16x64 of bytes).  k advances in steps
+// of KB bytes per row; STAGES LDS buffers are filled ahead by 16-byte LDS-DMA.  Rows
+// are KB bytes, their 16-byte chunks XOR-swizzled by row (by the address each lane
+// loads from: the DMA writes LDS linearly), so 8 neighbouring lanes' fragment reads
+// cover all banks.  Rows past the operand's end and k past its length read as zero
+// (out-of-range buffer offsets).
+//
+// What bounds it is the chip's power: an 8192^3 bf16 product takes a quarter less time on
+// zeros than on random numbers (clock 1.9 to 2.1 GHz, matrix cores 55 % busy).  So the
+// form that moves least wins.  At that size, fp32 outputs: 8 waves of 128 x 64 in
+// 32x32x16 blocks 1.07 ms; in 16x16x32 blocks, which read and write accumulators half as
+// often, 0.91; 4 waves of 128 x 128 0.99 and 0.86 (a third less read from LDS), but a wave
+// alone on its SIMD leaves the epilogues uncovered: the losses' forward product of
+// 131072 x 8192 x 2048 takes 3.28 ms (1340 TFLOP/s) with 8 waves and 3.64 with 4.
+// Fragments are read one group ahead, a read behind every second MFMA (6 % over the
+// compiler's order).
 #pragma once
 #include "common.h"
 #include <type_traits>
@@ -24,8 +34,7 @@ namespace po {
 namespace mm {
 
 typedef int i4v __attribute__((ext_vector_type(4)));
-typedef int i16v __attribute__((ext_vector_type(16)));
-typedef float f16v __attribute__((ext_vector_type(16)));
+typedef float f4v __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 
@@ -33,21 +42,21 @@ enum Kind { BF16 = 0, F16 = 1, I8 = 2 };
 
 template <int KIND>
 struct Acc {
-  using type = f16v;
+  using type = f4v;
 };
 template <>
 struct Acc<I8> {
-  using type = i16v;
+  using type = i4v;
 };
 
 template <int KIND>
 __device__ __forceinline__ typename Acc<KIND>::type mfma(i4v a, i4v b, typename Acc<KIND>::type c) {
   if constexpr (KIND == BF16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0, 0);
   else if constexpr (KIND == F16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
   else
-    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
 // One operand: rows of k-contiguous elements, stride and length in bytes (both
@@ -64,11 +73,11 @@ constexpr uint32_t kOOB = 0x80000000u;
 template <int KIND_, int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_>
 struct Cfg {
   static constexpr int KIND = KIND_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = KB_, STAGES = STAGES_;
-  static constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  static constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   static constexpr int RPI = 1024 / KB;                                  // rows one wave's DMA instruction fills
   static constexpr int NA = BM / RPI / NW, NB = BN / RPI / NW;           // instructions per wave and stage
   static constexpr int STAGE_BYTES = (BM + BN) * KB, LDS = STAGES * STAGE_BYTES;
-  static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && NA * RPI * NW == BM && NB * RPI * NW == BN, "tile");
+  static_assert(KB % 64 == 0 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && NA * RPI * NW == BM && NB * RPI * NW == BN, "tile");
 };
 
 template <int KB>
@@ -88,7 +97,7 @@ struct Loader {
 // Planes: an operand of wider numbers is stored as `planes` 16-bit matrices, and
 // the step index runs over pairs of them: pair q multiplies plane (pa >> 4q & 15)
 // of A with plane (pb >> 4q & 15) of B; steps [q * nk, (q + 1) * nk) are pair q's.
-// kbytes: length of a row; ends inside a step read as zero.
+// kbytes: length of a row; ends inside a step read as zero.  ks1 > ks0.
 template <class C>
 __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM][C::TN], const Operand& A,
                                         const Operand& B, int m0, int n0, int kbytes, int ks0, int ks1, int nk,
@@ -142,45 +151,67 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
 #pragma unroll
   for (int s = 0; s < C::STAGES - 1; ++s)
     if (s < n) issue(s);
-  const int ar = wm * C::TM * 32 + (lane & 31), br = wn * C::TN * 32 + (lane & 31), h = lane >> 5;
-  int buf = 0;
-  for (int s = 0; s < n; ++s) {
-    // this step's loads have landed when at most the later stages' are in flight
+  const int ar = wm * C::TM * 16 + (lane & 15), br = wn * C::TN * 16 + (lane & 15), h = lane >> 4;
+  constexpr int G = KB / 64;                                 // groups of fragments in a step
+  i4v fa[2][C::TM], fb[2][C::TN];
+  auto fetch = [&](int buf, int g, i4v (&a)[C::TM], i4v (&b)[C::TN]) {
+    const char* la = lds + buf * C::STAGE_BYTES;
+    const char* lb = la + C::BM * KB;
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      const int r = br + j * 16;
+      b[j] = *reinterpret_cast<const i4v*>(lb + r * KB + (((4 * g + h) ^ swz<KB>(r)) * 16));
+    }
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+      const int r = ar + i * 16;
+      a[i] = *reinterpret_cast<const i4v*>(la + r * KB + (((4 * g + h) ^ swz<KB>(r)) * 16));
+    }
+  };
+  auto multiply = [&](const i4v (&a)[C::TM], const i4v (&b)[C::TN]) {
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) acc[i][j] = mfma<C::KIND>(a[i], b[j], acc[i][j]);
+    // the next group's reads between these MFMAs
+    constexpr int R = C::TM + C::TN, X = C::TM * C::TN, E = X >= 2 * R ? 2 : 1;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, E, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, X - E * R, 0);
+  };
+  static_assert(G == 2, "a step's two groups alternate between two sets of registers");
+  int buf = 0, s = 0;
+  auto step = [&](auto first) {
+    // this step's loads have landed when at most the later stages' are in flight; the
+    // fragments of the step before have left LDS
     if (C::STAGES > 2 && s + C::STAGES - 2 < n)
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((C::STAGES - 2) * (C::NA + C::NB)) : "memory");
     else
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();                            // ... every wave's, and the last step's reads are over
+    __builtin_amdgcn_s_barrier();                            // ... every wave's
     asm volatile("" ::: "memory");
     if (s + C::STAGES - 1 < n) issue(buf == 0 ? C::STAGES - 1 : buf - 1);
-    const char* la = lds + buf * C::STAGE_BYTES;
-    const char* lb = la + C::BM * KB;
-#pragma unroll
-    for (int g = 0; g < KB / 32; ++g) {
-      i4v a[C::TM], b[C::TN];
-#pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        const int r = ar + i * 32;
-        a[i] = *reinterpret_cast<const i4v*>(la + r * KB + (((2 * g + h) ^ swz<KB>(r)) * 16));
-      }
-#pragma unroll
-      for (int j = 0; j < C::TN; ++j) {
-        const int r = br + j * 32;
-        b[j] = *reinterpret_cast<const i4v*>(lb + r * KB + (((2 * g + h) ^ swz<KB>(r)) * 16));
-      }
-#pragma unroll
-      for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-        for (int j = 0; j < C::TN; ++j) acc[i][j] = mfma<C::KIND>(a[i], b[j], acc[i][j]);
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(buf, 0, fa[0], fb[0]);
+    if constexpr (!first) multiply(fa[1], fb[1]);            // the last group of the step before
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(buf, 1, fa[1], fb[1]);
+    multiply(fa[0], fb[0]);
+    __builtin_amdgcn_sched_barrier(0);
     buf = buf + 1 == C::STAGES ? 0 : buf + 1;
-  }
+  };
+  step(std::true_type{});
+  for (s = 1; s < n; ++s) step(std::false_type{});
+  multiply(fa[1], fb[1]);
+  __builtin_amdgcn_sched_barrier(0);
 }
 
-// Element e of a 32 x 32 accumulator block lies in row (m) 8 * (e / 4) +
-// 4 * (lane / 32) + e % 4 and column (n) lane % 32: elements 4q .. 4q + 3 are
-// four consecutive rows of one column.  The kernels below take the operand whose
-// index is contiguous in the output (or is reduced over) as A.
+// Element e of a 16 x 16 accumulator block lies in row (m) 4 * (lane / 16) + e and column
+// (n) lane % 16: a lane's four are consecutive rows of one column.  The kernels below take
+// the operand whose index is contiguous in the output (or is reduced over) as A.
 
 struct Args {
   Operand A, B;
@@ -195,15 +226,21 @@ struct Tile {
   int m0, n0;                 // first row of A and of B of this wave's rectangle
   int tm, tn;
   int lane, wave, wm, wn;
-  __device__ __forceinline__ int col(int j) const { return n0 + j * 32 + (lane & 31); }
-  __device__ __forceinline__ int row4(int i, int q) const { return m0 + i * 32 + 8 * q + 4 * (lane >> 5); }
+  __device__ __forceinline__ int col(int j) const { return n0 + j * 16 + (lane & 15); }
+  __device__ __forceinline__ int row(int i) const { return m0 + i * 16 + 4 * (lane >> 4); }   // of element 0
+};
+
+struct NoPre {
+  template <class T, class E>
+  __device__ __forceinline__ void load(const T&, const E&) {}
 };
 
 // Workgroups of 8 tile rows by all tile columns in turn, an XCD's workgroups
 // next to each other: its L2 holds the k-window of the operands they share.
-// gridDim.y slices the k-steps.  Epi::run(tile, args, lds, slice) ends the tile.
+// gridDim.y slices the k-steps.  Epi::run ends the tile; what it reads of a token it reads
+// before the loop (Pre): its waves have no others to wait behind.
 template <class C, class Epi>
-__global__ __launch_bounds__(C::NW * 64, 2) void product_k(const Args a, const typename Epi::Args e) {
+__global__ __launch_bounds__(C::NW * 64, C::LDS > 81920 ? 1 : 2) void product_k(const Args a, const typename Epi::Args e) {
   __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
   const int id = xcd_remap();
   constexpr int GM = 8;
@@ -216,18 +253,18 @@ __global__ __launch_bounds__(C::NW * 64, 2) void product_k(const Args a, const t
   t.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   t.wm = t.wave / C::WN;
   t.wn = t.wave % C::WN;
-  t.m0 = t.tm * C::BM + t.wm * C::TM * 32;
-  t.n0 = t.tn * C::BN + t.wn * C::TN * 32;
+  t.m0 = t.tm * C::BM + t.wm * C::TM * 16;
+  t.n0 = t.tn * C::BN + t.wn * C::TN * 16;
 #pragma unroll
   for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-    for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-      for (int k = 0; k < 16; ++k) t.acc[i][j][k] = 0;
+    for (int j = 0; j < C::TN; ++j) t.acc[i][j] = typename Acc<C::KIND>::type{0, 0, 0, 0};
+  typename Epi::template Pre<C> pre;
+  pre.load(t, e);
   const int total = a.nk * a.pairs;
   const int ks0 = (int)((int64_t)blockIdx.y * total / gridDim.y), ks1 = (int)((int64_t)(blockIdx.y + 1) * total / gridDim.y);
   product<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, a.nk, a.pa, a.pb, lds);
-  Epi::template run<C>(t, e, lds, a);
+  Epi::template run<C>(t, e, pre, lds);
 }
 
 template <class C, class Epi>
@@ -235,7 +272,7 @@ inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipSt
   a.tiles_m = ceil_div(a.A.rows, C::BM);
   a.tiles_n = ceil_div(a.B.rows, C::BN);
   a.nk = ceil_div(a.kbytes, C::KB);
-  if ((int64_t)a.tiles_m * a.tiles_n >= (1LL << 22) || slices > 65535 || (int64_t)a.nk * a.pairs >= (1LL << 31) ||
+  if ((int64_t)a.tiles_m * a.tiles_n >= (1LL << 22) || slices > 65535 || (int64_t)a.nk * a.pairs >= (1LL << 31) || slices > (int64_t)a.nk * a.pairs ||
       a.A.stride * C::BM >= (1LL << 31) || a.B.stride * C::BN >= (1LL << 31) || a.kbytes < 0) {
     set_error("%s: operand too large", what);
     return PO_EINVAL;
@@ -244,10 +281,42 @@ inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipSt
   return check_launch(what);
 }
 
+// ---- which tile ----------------------------------------------------------
+// Three tiles: LARGE 256 x 256 (one workgroup of 8 waves to a CU), MID 128 x 128
+// (two of 4 waves), FEW 128 x 32 for up to 32 columns.  What a step of k takes a
+// workgroup and what its start and end take, in us, measured on 8192-row products
+// (16-bit: LARGE 1300 TFLOP/s in the loop, MID 0.72 of it); the choice is the
+// shorter total over the rounds in which the chip takes the tiles.  slices > 1 cuts k
+// between workgroups, each slice's sums then cost sum_us.
+enum TileId { FEW, MID, LARGE };
+struct Plan {
+  TileId tile;
+  int slices;
+};
+inline Plan plan_product(int64_t M, int64_t N, int64_t steps, int max_slices = 1, double sum_us = 0) {
+  struct {
+    TileId id;
+    int bm, bn, slots;
+    double step, ends;
+  } const kinds[] = {{FEW, 128, 32, 512, 0.6, 5}, {MID, 128, 128, 512, 1.15, 5}, {LARGE, 256, 256, 256, 1.65, 8}};
+  Plan best{LARGE, 1};
+  double least = 1e300;
+  for (auto& k : kinds) {
+    if ((k.id == FEW) != (N <= 32)) continue;
+    const int64_t tiles = ((M + k.bm - 1) / k.bm) * ((N + k.bn - 1) / k.bn);
+    for (int s = 1; s <= max_slices && (s == 1 || steps / s >= 4); ++s) {
+      const int64_t rounds = (tiles * s + k.slots - 1) / k.slots;
+      const double t = rounds * ((double)((steps + s - 1) / s) * k.step + k.ends) + s * sum_us;
+      if (t < least) least = t, best = Plan{k.id, s};
+    }
+  }
+  return best;
+}
+
 // ---- outputs -------------------------------------------------------------
 // A tile of 16-bit outputs passes through LDS as rows [n][m] and leaves as
 // 16-byte pieces of whole rows.  16-byte chunk c of row n lies at chunk
-// c ^ turn(n): the 8-byte writes of 32 columns, the 16-byte row reads and the
+// c ^ turn(n): the 8-byte writes of 16 columns, the 16-byte row reads and the
 // transposing reads of 4 rows x 32 bytes each touch every bank evenly.
 template <class C>
 __device__ __forceinline__ int turn(int n) {
@@ -258,28 +327,39 @@ __device__ __forceinline__ int turn(int n) {
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 
 template <class C>
-__device__ __forceinline__ void stage4(const Tile<C>& t, char* lds, int i, int j, int q, u2v four) {
-  const int n = t.wn * C::TN * 32 + j * 32 + (t.lane & 31);
-  const int c = t.wm * C::TM * 4 + i * 4 + q;   // 8 outputs to a chunk, this lane's 4 in one half
-  *reinterpret_cast<u2v*>(lds + n * (C::BM * 2) + ((c ^ turn<C>(n)) * 16) + 8 * (t.lane >> 5)) = four;
+__device__ __forceinline__ void stage4(const Tile<C>& t, char* lds, int i, int j, u2v four) {
+  const int n = t.wn * C::TN * 16 + j * 16 + (t.lane & 15);
+  const int c = t.wm * C::TM * 2 + i * 2 + (t.lane >> 5);   // 8 outputs to a chunk, this lane's 4 in one half
+  *reinterpret_cast<u2v*>(lds + n * (C::BM * 2) + ((c ^ turn<C>(n)) * 16) + 8 * ((t.lane >> 4) & 1)) = four;
 }
 
 // rows [n][m] of the staged tile to out (16-bit, leading dimension ld), n < rows, m < cols
 template <class C>
 __device__ __forceinline__ void store_rows(const char* lds, uint16_t* out, int64_t ld, int n0, int m0, int rows,
                                            int cols, bool wide) {
-  constexpr int NC = C::BM / 8;
-  for (int x = threadIdx.x; x < C::BN * NC; x += C::NW * 64) {
-    const int n = x / NC, c = x % NC, m = m0 + c * 8;
-    if (n0 + n >= rows || m >= cols) continue;
-    const i4v v = *reinterpret_cast<const i4v*>(lds + n * (C::BM * 2) + ((c ^ turn<C>(n)) * 16));
-    uint16_t* o = out + (int64_t)(n0 + n) * ld + m;
-    if (wide && m + 8 <= cols) {
-      *reinterpret_cast<i4v*>(o) = v;
-    } else {
+  constexpr int NC = C::BM / 8, STEPS = C::BN * NC / (C::NW * 64), U = STEPS % 8 == 0 ? 8 : STEPS;
+  static_assert(STEPS * C::NW * 64 == C::BN * NC, "whole steps");
+  // a thread's chunk is the same in every step, its row advances
+  constexpr int ROWS = C::NW * 64 / NC;
+  const int c = threadIdx.x % NC, n = threadIdx.x / NC, m = m0 + c * 8;
+  uint16_t* o = out + (int64_t)(n0 + n) * ld + m;
+  for (int s = 0; s < STEPS; s += U) {
+    i4v v[U];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (m + k < cols) o[k] = (uint16_t)((uint32_t)v[k >> 1] >> (16 * (k & 1)));
+    for (int u = 0; u < U; ++u) {
+      const int r = n + (s + u) * ROWS;
+      v[u] = *reinterpret_cast<const i4v*>(lds + r * (C::BM * 2) + ((c ^ turn<C>(r)) * 16));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u, o += ROWS * ld) {
+      if (n0 + n + (s + u) * ROWS >= rows || m >= cols) continue;
+      if (wide && m + 8 <= cols) {
+        *reinterpret_cast<i4v*>(o) = v[u];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (m + k < cols) o[k] = (uint16_t)((uint32_t)v[u][k >> 1] >> (16 * (k & 1)));
+      }
     }
   }
 }
@@ -290,22 +370,30 @@ __device__ __forceinline__ void store_columns(const char* lds, uint16_t* out, in
                                               int cols) {
   typedef short s4v __attribute__((ext_vector_type(4)));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
-  constexpr int MB = C::BM / 16, NB = C::BN / 32;
   // a wave's step: 16 columns m by 32 rows n, 8 rows to a group of 16 lanes
-  for (int x = wave; x < MB * NB; x += C::NW) {
-    const int mb = x % MB, n = (x / MB) * 32 + g * 8;
-    u2v two[2];
+  constexpr int MB = C::BM / 16, STEPS = MB * (C::BN / 32) / C::NW, U = STEPS % 4 == 0 ? 4 : STEPS;
+  static_assert(STEPS * C::NW == MB * (C::BN / 32), "whole steps");
+  for (int s = 0; s < STEPS; s += U) {
+    u2v two[U][2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int nr = n + 4 * k + (i >> 2);
-      const int c = mb * 2 + ((i >> 1) & 1);
-      const char* p = lds + nr * (C::BM * 2) + ((c ^ turn<C>(nr)) * 16) + 8 * (i & 1);
-      two[k] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                           (__attribute__((address_space(3))) s4v*)(const_cast<char*>(p))));
+    for (int u = 0; u < U; ++u) {
+      const int x = (s + u) * C::NW + wave;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int nr = (x / MB) * 32 + g * 8 + 4 * k + (i >> 2);
+        const int c = (x % MB) * 2 + ((i >> 1) & 1);
+        const char* p = lds + nr * (C::BM * 2) + ((c ^ turn<C>(nr)) * 16) + 8 * (i & 1);
+        two[u][k] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                (__attribute__((address_space(3))) s4v*)(const_cast<char*>(p))));
+      }
     }
-    const int m = m0 + mb * 16 + i;
-    if (m < cols && n0 + n < rows)
-      *reinterpret_cast<i4v*>(out + (int64_t)m * ld + n0 + n) = i4v{(int)two[0][0], (int)two[0][1], (int)two[1][0], (int)two[1][1]};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int x = (s + u) * C::NW + wave, m = m0 + (x % MB) * 16 + i, n = n0 + (x / MB) * 32 + g * 8;
+      if (m < cols && n < rows)
+        *reinterpret_cast<i4v*>(out + (int64_t)m * ld + n) =
+            i4v{(int)two[u][0][0], (int)two[u][0][1], (int)two[u][1][0], (int)two[u][1][1]};
+    }
   }
 }
 

@@ -29,6 +29,9 @@
 namespace {
 using namespace po::mm;
 using po::ceil_div;
+#ifndef PIECE_MB
+#define PIECE_MB 640
+#endif
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kF16Lift = 16384.f;
@@ -41,8 +44,15 @@ using Mid = Cfg<KIND, 128, 128, 2, 2, 128, 2>;
 template <int KIND>
 using Few = Cfg<KIND, 128, 32, 4, 1, 128, 3>;
 
-__device__ __forceinline__ float xlane32_max(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
-__device__ __forceinline__ float xlane32_sum(float x) { return x + __shfl_xor(x, 32); }
+// over the four lanes that hold a column
+__device__ __forceinline__ float column_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float column_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
 
 // ---- epilogues -----------------------------------------------------------
 
@@ -58,45 +68,75 @@ struct StatsEpi {
     float k;                    // c * log2e > 0
   };
   template <class C>
-  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, char* lds, const po::mm::Args&) {
-    const bool edge = t.m0 + C::TM * 32 > e.V;
+  struct Pre {
+    int at[C::TN];              // the target's row within this wave's, or none of them
+    __device__ __forceinline__ void load(const Tile<C>& t, const Args& e) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        const int64_t r = (t.col(j) < e.N ? e.target[t.col(j)] : -1) - e.v0 - t.m0;
+        at[j] = r >= 0 && r < C::TM * 16 ? (int)r : -1;
+      }
+    }
+  };
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, const Pre<C>& pre, char* lds) {
     float2* mine = reinterpret_cast<float2*>(lds);          // [WM][BN]
+    const int quad = t.lane >> 4;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
-      const int n = t.col(j);
-      const int64_t tg = n < e.N ? e.target[n] - e.v0 - t.m0 : -1;
-      const bool has = tg >= 0 && tg < C::TM * 32 && ((tg >> 2) & 1) == (t.lane >> 5);
+      const bool has = pre.at[j] >= 0 && ((pre.at[j] >> 2) & 3) == quad;
       if (__any(has)) {
         float x = 0.f;
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-          for (int k = 0; k < 16; ++k)
-            if ((int)tg == i * 32 + 8 * (k >> 2) + 4 * (t.lane >> 5) + (k & 3)) x = t.acc[i][j][k];
-        if (has) e.tlogit[n] = x;
+          for (int k = 0; k < 4; ++k)
+            if (pre.at[j] == i * 16 + 4 * quad + k) x = t.acc[i][j][k];
+        if (has) e.tlogit[t.col(j)] = x;
       }
-      if (edge) {
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-          for (int k = 0; k < 16; ++k)
-            if (t.row4(i, k >> 2) + (k & 3) >= e.V) t.acc[i][j][k] = -INFINITY;
-      }
-      float mx = -INFINITY;
+    }
+    if (t.m0 + C::TM * 16 > e.V) {
 #pragma unroll
       for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, t.acc[i][j][k]);
-      mx = xlane32_max(mx);
-      const float top = mx == -INFINITY ? 0.f : mx * e.k;    // nothing but -inf: no exponent of inf - inf
-      float s = 0.f;
+        for (int k = 0; k < 4; ++k)
+          if (t.row(i) + k >= e.V) {
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j) t.acc[i][j][k] = -INFINITY;
+          }
+    }
+    // all columns' maxima, then all their sums: the exchanges between lanes overlap
+    float mx[C::TN], top[C::TN], s[C::TN];
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+      mx[j] = -INFINITY;
 #pragma unroll
       for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) s += __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][k], e.k, -top));
-      s = xlane32_sum(s);
-      if (t.lane < 32) mine[t.wm * C::BN + t.wn * C::TN * 32 + j * 32 + t.lane] = make_float2(mx == -INFINITY ? -INFINITY : top, s);
+        for (int k = 0; k < 4; ++k) mx[j] = fmaxf(mx[j], t.acc[i][j][k]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) mx[j] = column_max(mx[j]);
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+      top[j] = mx[j] == -INFINITY ? 0.f : mx[j] * e.k;       // nothing but -inf: no exponent of inf - inf
+      s[j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[j] += __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][k], e.k, -top[j]));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) s[j] = column_sum(s[j]);
+    if (t.lane < 16) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+        mine[t.wm * C::BN + t.wn * C::TN * 16 + j * 16 + t.lane] = make_float2(mx[j] == -INFINITY ? -INFINITY : top[j], s[j]);
     }
     __syncthreads();
     for (int x = threadIdx.x; x < C::BN; x += C::NW * 64) {
@@ -127,47 +167,76 @@ struct DlogitsEpi {
     int64_t ldl, ldt, pl, pt;
   };
   template <class C>
-  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, char* lds, const po::mm::Args&) {
+  struct Pre {
+    float2 stat[C::TN];
+    float ratio[C::TN];
+    int at[C::TN];
+    __device__ __forceinline__ void load(const Tile<C>& t, const Args& e) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        const int n = t.col(j);
+        const bool in = n < e.N;
+        stat[j] = in ? e.stat[n] : make_float2(0.f, 0.f);
+        ratio[j] = in ? e.ratio[n] : 0.f;
+        const int64_t r = (in ? e.target[n] : -1) - e.v0 - t.m0;
+        at[j] = r >= 0 && r < C::TM * 16 ? (int)r : -1;
+      }
+    }
+  };
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, const Pre<C>& pre, char* lds) {
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
-      const int n = t.col(j);
-      const bool in = n < e.N;
-      const float2 st = in ? e.stat[n] : make_float2(0.f, 0.f);
-      const float r = in ? e.ratio[n] : 0.f, ir = st.y * r;
-      int64_t tg64 = in ? e.target[n] - e.v0 - t.m0 : -1;
-      const int tg = tg64 >= 0 && tg64 < C::TM * 32 ? (int)tg64 : -1;
+      __builtin_amdgcn_sched_barrier(0);                     // a column block at a time: the accumulators fill the registers
+      const float2 st = pre.stat[j];
+      const float r = pre.ratio[j], ir = st.y * r;
+      const bool live = r != 0.f;                            // rows that take no part may hold anything, NaN too
 #pragma unroll
       for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const int m = i * 32 + 8 * (k >> 2) + 4 * (t.lane >> 5) + (k & 3);
-          float v = __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][k], e.k, -st.x)) * ir;
-          if (m == tg) v -= r;
-          // rows that take no part may hold anything, NaN too; vocabulary rows past the end
-          t.acc[i][j][k] = r != 0.f && t.m0 + m < e.V ? v : 0.f;
+        for (int k = 0; k < 4; ++k) {
+          const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][k], e.k, -st.x)) * ir;
+          t.acc[i][j][k] = live ? v : 0.f;
         }
+      if (__any(pre.at[j] >= 0)) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (pre.at[j] == i * 16 + 4 * (t.lane >> 4) + k) t.acc[i][j][k] -= r;
+      }
+    }
+    if (t.m0 + C::TM * 16 > e.V) {                           // vocabulary rows past the end
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (t.row(i) + k >= e.V) {
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j) t.acc[i][j][k] = 0.f;
+          }
     }
 #pragma unroll
     for (int p = 0; p < PLANES; ++p) {
       __syncthreads();                                       // the loop's (or the last plane's) reads are over
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j)
+      for (int j = 0; j < C::TN; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i)
+        for (int i = 0; i < C::TM; ++i) {
+          u2v w;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            u2v w;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float x = t.acc[i][j][4 * q + 2 * k], y = t.acc[i][j][4 * q + 2 * k + 1];
-              w[k] = pack2<KIND>(x, y);
-              if constexpr (PLANES > 1) {                    // what this plane leaves to the next
-                t.acc[i][j][4 * q + 2 * k] = x - __uint_as_float(w[k] << 16);
-                t.acc[i][j][4 * q + 2 * k + 1] = y - __uint_as_float(w[k] & 0xffff0000u);
-              }
+          for (int k = 0; k < 2; ++k) {
+            const float x = t.acc[i][j][2 * k], y = t.acc[i][j][2 * k + 1];
+            w[k] = pack2<KIND>(x, y);
+            if constexpr (PLANES > 1) {                      // what this plane leaves to the next
+              t.acc[i][j][2 * k] = x - __uint_as_float(w[k] << 16);
+              t.acc[i][j][2 * k + 1] = y - __uint_as_float(w[k] & 0xffff0000u);
             }
-            stage4(t, lds, i, j, q, w);
           }
+          stage4(t, lds, i, j, w);
+        }
+      }
       __syncthreads();
       const int n0 = t.tn * C::BN, m0 = t.tm * C::BM;
       if (e.dl) store_rows<C>(lds, e.dl + p * e.pl, e.ldl, n0, m0, e.N, e.Vp, true);
@@ -184,26 +253,22 @@ struct SlabEpi {
     int N, M, add;
   };
   template <class C>
-  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, char*, const po::mm::Args&) {
+  using Pre = NoPre;
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, const Pre<C>&, char*) {
     float* out = e.slab + blockIdx.y * e.slice;
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
+      __builtin_amdgcn_sched_barrier(0);                     // a column block at a time: the accumulators fill the registers
       const int n = t.col(j);
       if (n >= e.N) continue;
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int m = t.row4(i, q);
-          if (m >= e.ld) continue;
-          float4* o = reinterpret_cast<float4*>(out + (int64_t)n * e.ld + m);
-          float4 v = make_float4(t.acc[i][j][4 * q], t.acc[i][j][4 * q + 1], t.acc[i][j][4 * q + 2], t.acc[i][j][4 * q + 3]);
-          if (e.add) {
-            const float4 u = *o;
-            v = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
-          }
-          *o = v;
-        }
+      for (int i = 0; i < C::TM; ++i) {
+        const int m = t.row(i);
+        if (m >= e.ld) continue;
+        f4v* o = reinterpret_cast<f4v*>(out + (int64_t)n * e.ld + m);
+        *o = e.add ? *o + t.acc[i][j] : t.acc[i][j];
+      }
     }
   }
 };
@@ -218,7 +283,9 @@ struct GradEpi {
     int N, M, wide;             // wide: rows start on 16 bytes
   };
   template <class C>
-  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, char* lds, const po::mm::Args&) {
+  using Pre = NoPre;
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, const Pre<C>& pre, char* lds) {
     const float f = *e.factor;
     if constexpr (OUT == 3) {
 #pragma unroll
@@ -226,31 +293,28 @@ struct GradEpi {
         const int n = t.col(j);
         if (n >= e.N) continue;
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i)
+        for (int i = 0; i < C::TM; ++i) {
+          const int m = t.row(i);
+          float* o = static_cast<float*>(e.out) + (int64_t)n * e.ld + m;
+          if (e.wide && m + 4 <= e.M) {
+            *reinterpret_cast<f4v*>(o) = t.acc[i][j] * f;
+          } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int m = t.row4(i, q);
-            float* o = static_cast<float*>(e.out) + (int64_t)n * e.ld + m;
-            if (e.wide && m + 4 <= e.M) {
-              *reinterpret_cast<float4*>(o) = make_float4(t.acc[i][j][4 * q] * f, t.acc[i][j][4 * q + 1] * f,
-                                                          t.acc[i][j][4 * q + 2] * f, t.acc[i][j][4 * q + 3] * f);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (m + k < e.M) o[k] = t.acc[i][j][4 * q + k] * f;
-            }
+            for (int k = 0; k < 4; ++k)
+              if (m + k < e.M) o[k] = t.acc[i][j][k] * f;
           }
+        }
       }
     } else {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j)
+      for (int j = 0; j < C::TN; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            stage4(t, lds, i, j, q, u2v{pack2<OUT>(t.acc[i][j][4 * q] * f, t.acc[i][j][4 * q + 1] * f),
-                                        pack2<OUT>(t.acc[i][j][4 * q + 2] * f, t.acc[i][j][4 * q + 3] * f)});
+          stage4(t, lds, i, j, u2v{pack2<OUT>(t.acc[i][j][0] * f, t.acc[i][j][1] * f),
+                                   pack2<OUT>(t.acc[i][j][2] * f, t.acc[i][j][3] * f)});
+      }
       __syncthreads();
       store_rows<C>(lds, static_cast<uint16_t*>(e.out), e.ld, t.tn * C::BN, t.tm * C::BM, e.N, e.M, e.wide != 0);
     }
@@ -425,7 +489,16 @@ __global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab
 
 // ---- the plan ------------------------------------------------------------
 
-constexpr int64_t kPieceBytes = 512LL << 20;   // what a piece of the vocabulary may take of the workspace
+constexpr int64_t kPieceBytes = (PIECE_MB) * (1LL << 20);   // what a piece of the vocabulary may take of the workspace
+
+// Rows of the operands made here: a multiple of 128 bytes, and long ones no multiple of 512:
+// 256 rows a power of two apart fall on few memory channels (dh of a 16384-row piece
+// 473 us with rows of 32768 bytes, 430 us with 384 bytes more; 490 us with 320 more, rows
+// that start within a 128-byte line).
+inline int64_t padded(int64_t n) {
+  const int64_t p = (n + 63) / 64 * 64;
+  return p >= 1024 && p % 256 == 0 ? p + 192 : p;
+}
 
 struct Shape {
   int64_t N, V, D;
@@ -434,6 +507,7 @@ struct Shape {
   int planes() const { return dtype == PO_F32 ? 3 : 1; }
   int Dp() const { return (int)((D + 7) / 8 * 8); }
   int64_t Np() const { return (N + 31) / 32 * 32; }
+  int64_t ldn() const { return padded(Np()); }
 };
 
 inline int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
@@ -451,11 +525,12 @@ struct Layout {
   }
 };
 
-// vocabulary rows of a piece: a multiple of 256, per_row bytes each
+// Vocabulary rows of a piece, per_row bytes each: pieces of one size, a multiple of
+// 256 rows, as few as kPieceBytes allows.
 inline int64_t piece_rows(int64_t V, int64_t per_row) {
-  int64_t p = kPieceBytes / (per_row > 0 ? per_row : 1) / 256 * 256;
-  p = std::min<int64_t>(std::max<int64_t>(p, 256), 1 << 20);
-  return p < V ? p : V;
+  const int64_t most = std::min<int64_t>(std::max<int64_t>(kPieceBytes / (per_row > 0 ? per_row : 1) / 256 * 256, 256), 1 << 20);
+  const int64_t pieces = (V + most - 1) / most, each = (V + pieces - 1) / pieces;
+  return std::min(V, (each + 255) / 256 * 256);
 }
 
 struct FwdWs {
@@ -481,39 +556,30 @@ struct FwdWs {
 
 constexpr int kSlabSlices = 64;
 
-// slices of dh's k (a piece's vocabulary rows): few tiles are cut until the chip is filled
-inline int dh_slices(int64_t tiles, int64_t steps) {
-  int64_t s = tiles >= 256 ? 1 : 512 / tiles;
-  s = std::min<int64_t>(s, kSlabSlices);
-  return (int)std::max<int64_t>(1, std::min(s, steps / 4));
-}
-
 struct BwdWs {
   float *ratio, *factor, *slab;
   uint16_t *hp, *ht, *wp, *wt, *dl, *dlt;
   int64_t piece, ldl, slab_ld, slab_slice, bytes;
-  int slices, bm, bn;
+  Plan dh_plan;
   BwdWs(const Shape& s, bool dh, bool dw, void* b) {
     Layout l(b);
     const int P = s.planes();
     const int64_t per = (s.direct_w ? 0 : (int64_t)s.Dp() * 2 * P) + (dh ? (s.N + s.D) * 2 * P : 0) + (dw ? s.Np() * 2 * P : 0);
     piece = piece_rows(s.V, per);
-    ldl = (piece + 63) / 64 * 64;
+    ldl = padded(piece);
     ratio = l.take<float>(s.N);
     factor = l.take<float>(1);
     hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.Dp() * P);
-    ht = l.take<uint16_t>(dw ? s.D * s.Np() * P : 0);
+    ht = l.take<uint16_t>(dw ? s.D * s.ldn() * P : 0);
     wp = l.take<uint16_t>(s.direct_w ? 0 : piece * s.Dp() * P);
     wt = l.take<uint16_t>(dh ? s.D * ldl * P : 0);
     dl = l.take<uint16_t>(dh ? s.N * ldl * P : 0);
-    dlt = l.take<uint16_t>(dw ? piece * s.Np() * P : 0);
-    bm = s.N <= 32 ? 128 : 256;
-    bn = s.N <= 32 ? 32 : 256;
-    if (s.N > 32 && (int64_t)ceil_div(s.D, 256) * ceil_div(s.N, 256) < 128) bm = bn = 128;
+    dlt = l.take<uint16_t>(dw ? piece * s.ldn() * P : 0);
     slab_ld = (s.D + 3) / 4 * 4;
     slab_slice = s.N * slab_ld;
-    slices = dh_slices((int64_t)ceil_div(s.D, bm) * ceil_div(s.N, bn), (int64_t)ceil_div(ldl * 2, 128) * (P == 3 ? 6 : 1));
-    slab = l.take<float>(dh ? slices * slab_slice : 0);
+    // a slice's sums are written and read once: 8 bytes of each at about 4 TB/s
+    dh_plan = plan_product(s.D, s.N, (int64_t)ceil_div(ldl * 2, 128) * (P == 3 ? 6 : 1), kSlabSlices, slab_slice * 8 / 4e6);
+    slab = l.take<float>(dh ? dh_plan.slices * slab_slice : 0);
     bytes = l.at;
   }
 };
@@ -560,13 +626,15 @@ inline int check_shape(const char* what, int64_t N, int64_t V, int64_t D, int dt
 }
 
 template <int KIND, class Epi>
-inline int by_tokens(const Args& a, const typename Epi::Args& e, int64_t N, hipStream_t s, const char* what) {
-  if (N <= 32) return launch_product<Few<KIND>, Epi>(a, e, 1, s, what);
-  if (N <= 128) return launch_product<Mid<KIND>, Epi>(a, e, 1, s, what);
-  return launch_product<Large<KIND>, Epi>(a, e, 1, s, what);
+inline int launch_planned(const Args& a, const typename Epi::Args& e, Plan p, hipStream_t s, const char* what) {
+  if (p.tile == FEW) return launch_product<Few<KIND>, Epi>(a, e, p.slices, s, what);
+  if (p.tile == MID) return launch_product<Mid<KIND>, Epi>(a, e, p.slices, s, what);
+  return launch_product<Large<KIND>, Epi>(a, e, p.slices, s, what);
 }
 
-inline int tile_rows(int64_t N) { return N <= 128 ? 128 : 256; }
+inline Plan plan_of(const Args& a) {
+  return plan_product(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs);
+}
 
 #define PO_TRY(x)             \
   do {                        \
@@ -608,9 +676,10 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
     a.A = rows_of(s, s.direct_w, w, ldw, v, rows, ws.wp, st);
     e.v0 = v;
     e.V = (int)rows;
-    PO_TRY((dtype == PO_F16 ? by_tokens<F16, StatsEpi>(a, e, N, st, "po_linear_ce_fwd")
-                            : by_tokens<BF16, StatsEpi>(a, e, N, st, "po_linear_ce_fwd")));
-    e.tile0 += ceil_div(rows, tile_rows(N));
+    const Plan p = plan_of(a);
+    PO_TRY((dtype == PO_F16 ? launch_planned<F16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
+                            : launch_planned<BF16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")));
+    e.tile0 += ceil_div(rows, p.tile == LARGE ? 256 : 128);
   }
   float* rows = reduction ? ws.rowloss : loss;
   float2* stat2 = reinterpret_cast<float2*>(stat);
@@ -639,7 +708,7 @@ int backward(const Shape& s, const BwdWs& ws, const void* h, int64_t ldh, const 
   if (dw)
     hipLaunchKernelGGL(transpose_k, dim3(ceil_div(s.Np(), 64), ceil_div(D, 64), P), dim3(256), 0, st,
                        reinterpret_cast<const uint16_t*>(H.p), H.stride / 2, H.plane / 2, N, D, ws.ratio, ws.ht,
-                       s.Np(), D * s.Np(), (int)s.Np());
+                       s.ldn(), D * s.ldn(), (int)s.Np());
   for (int64_t v = 0; v < s.V; v += ws.piece) {
     const int rows = (int)std::min(ws.piece, s.V - v);
     const int rp = (rows + 63) / 64 * 64;
@@ -651,9 +720,9 @@ int backward(const Shape& s, const BwdWs& ws, const void* h, int64_t ldh, const 
     a.B = H;
     a.kbytes = s.Dp() * 2;
     typename DlogitsEpi<KIND, P>::Args e{stat, ws.ratio, target, v, N, (int)s.Np(), rows, rp, scale * kLog2e,
-                                         dh ? ws.dl : nullptr, dw ? ws.dlt : nullptr, ws.ldl, s.Np(), N * ws.ldl,
-                                         ws.piece * s.Np()};
-    PO_TRY((by_tokens<KIND, DlogitsEpi<KIND, P>>(a, e, N, st, what)));
+                                         dh ? ws.dl : nullptr, dw ? ws.dlt : nullptr, ws.ldl, s.ldn(), N * ws.ldl,
+                                         ws.piece * s.ldn()};
+    PO_TRY((launch_planned<KIND, DlogitsEpi<KIND, P>>(a, e, plan_of(a), st, what)));
     if (dh) {                                                // slab[n][d] += sum_v dl[n][v] w[v][d]
       hipLaunchKernelGGL(transpose_k, dim3(ceil_div(rp, 64), ceil_div(D, 64), P), dim3(256), 0, st,
                          reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, D,
@@ -662,26 +731,23 @@ int backward(const Shape& s, const BwdWs& ws, const void* h, int64_t ldh, const 
       a.B = Operand{reinterpret_cast<char*>(ws.dl), ws.ldl * 2, N * ws.ldl * 2, N};
       a.kbytes = rp * 2;
       const SlabEpi::Args se{ws.slab, ws.slab_ld, ws.slab_slice, N, D, v > 0};
-      if (ws.bn == 32)
-        PO_TRY((launch_product<Few<KIND>, SlabEpi>(a, se, ws.slices, st, what)));
-      else if (ws.bn == 128)
-        PO_TRY((launch_product<Mid<KIND>, SlabEpi>(a, se, ws.slices, st, what)));
-      else
-        PO_TRY((launch_product<Large<KIND>, SlabEpi>(a, se, ws.slices, st, what)));
+      // the last piece may have fewer steps than slices: the other slabs keep their sums
+      const Plan p{ws.dh_plan.tile, std::min(ws.dh_plan.slices, ceil_div(a.kbytes, 128) * a.pairs)};
+      PO_TRY((launch_planned<KIND, SlabEpi>(a, se, p, st, what)));
     }
     if (dw) {                                                // dw[v][d] = sum_n dl[n][v] h[n][d]
-      a.A = Operand{reinterpret_cast<char*>(ws.ht), s.Np() * 2, D * s.Np() * 2, D};
-      a.B = Operand{reinterpret_cast<char*>(ws.dlt), s.Np() * 2, ws.piece * s.Np() * 2, rows};
+      a.A = Operand{reinterpret_cast<char*>(ws.ht), s.ldn() * 2, D * s.ldn() * 2, D};
+      a.B = Operand{reinterpret_cast<char*>(ws.dlt), s.ldn() * 2, ws.piece * s.ldn() * 2, rows};
       a.kbytes = (int)s.Np() * 2;
       const int es = OUT == 3 ? 4 : 2;
       char* out = static_cast<char*>(dw) + v * lddw * es;
       const typename GradEpi<OUT>::Args ge{out, lddw, ws.factor, rows, D, (uintptr_t)out % 16 == 0 && lddw * es % 16 == 0};
-      PO_TRY((launch_product<Large<KIND>, GradEpi<OUT>>(a, ge, 1, st, what)));
+      PO_TRY((launch_planned<KIND, GradEpi<OUT>>(a, ge, plan_of(a), st, what)));
     }
   }
   if (dh) {
     const int grid = (int)std::min<int64_t>(((int64_t)N * D + 255) / 256, 8192);
-    hipLaunchKernelGGL((slab_sum_k<OUT>), dim3(grid), dim3(256), 0, st, ws.slab, ws.slices, ws.slab_slice, ws.slab_ld,
+    hipLaunchKernelGGL((slab_sum_k<OUT>), dim3(grid), dim3(256), 0, st, ws.slab, ws.dh_plan.slices, ws.slab_slice, ws.slab_ld,
                        N, D, ws.factor, dh, lddh);
   }
   return po::check_launch(what);
