@@ -184,7 +184,7 @@ template <int DT>
 int product_of(const Args& a, const typename ScaledEpi<DT>::Args& e, hipStream_t s) {
   using E = ScaledEpi<DT>;
   const char* what = "po_int8_matmul";
-  const Plan p = plan_product(a.A.rows, a.B.rows, ceil_div(a.kbytes, 128));
+  const Plan p = plan_product(a.A.rows, a.B.rows, ceil_div(a.kbytes, 128), 6, 10);
   if (p.tile == FEW) return launch_product<Cfg<I8, 128, 32, 4, 1, 128, 3>, E>(a, e, 1, s, what);
   if (p.tile == LARGE) return launch_product<Cfg<I8, 256, 256, 2, 4, 128, 2>, E>(a, e, 1, s, what);
   // 64 x 64 where tiles of 128 x 128 leave CUs without one

@@ -283,22 +283,26 @@ inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipSt
 
 // ---- which tile ----------------------------------------------------------
 // Three tiles: LARGE 256 x 256 (one workgroup of 8 waves to a CU), MID 128 x 128
-// (two of 4 waves), FEW 128 x 32 for up to 32 columns.  What a step of k takes a
-// workgroup and what its start and end take, in us, measured on 8192-row products
-// (16-bit: LARGE 1300 TFLOP/s in the loop, MID 0.72 of it); the choice is the
-// shorter total over the rounds in which the chip takes the tiles.  slices > 1 cuts k
-// between workgroups, each slice's sums then cost sum_us.
+// (two of 4 waves), FEW 128 x 32 for up to 32 columns.  The choice is the least time over
+// the rounds in which the chip takes the tiles, from what a step of k takes a workgroup
+// (us, measured: LARGE 1.7, MID 1.08 with two on the CU) and what its start and its
+// epilogue take (the epilogue's; MID's are covered by the other workgroup).  So LARGE is
+// taken for long k or cheap epilogues, MID for few tiles and short k: the losses' forward
+// product of 32768 x 2048 x 512 78 against 95 us; the gradient of the logits there 117
+// against 112 us, at k = 128 73 against 63.  slices > 1 cuts k between workgroups, each
+// slice's sums then cost sum_us.
 enum TileId { FEW, MID, LARGE };
 struct Plan {
   TileId tile;
   int slices;
 };
-inline Plan plan_product(int64_t M, int64_t N, int64_t steps, int max_slices = 1, double sum_us = 0) {
+inline Plan plan_product(int64_t M, int64_t N, int64_t steps, double ends_mid, double ends_large, int max_slices = 1,
+                         double sum_us = 0) {
   struct {
     TileId id;
     int bm, bn, slots;
     double step, ends;
-  } const kinds[] = {{FEW, 128, 32, 512, 0.6, 5}, {MID, 128, 128, 512, 1.15, 5}, {LARGE, 256, 256, 256, 1.65, 8}};
+  } const kinds[] = {{FEW, 128, 32, 512, 0.45, 5}, {MID, 128, 128, 512, 1.08, ends_mid}, {LARGE, 256, 256, 256, 1.7, ends_large}};
   Plan best{LARGE, 1};
   double least = 1e300;
   for (auto& k : kinds) {

@@ -58,6 +58,7 @@ __device__ __forceinline__ float column_sum(float x) {
 
 // partial[tile][n] = {max of l * log2e, sum of 2^(l * log2e - max)} over the tile's vocabulary rows
 struct StatsEpi {
+  static constexpr double kMid = 3, kLarge = 5.5;            // us, see plan_product
   struct Args {
     float2* partial;
     float* tlogit;              // l / c of the target
@@ -156,6 +157,7 @@ struct StatsEpi {
 // dl of a piece of the vocabulary, as [n][v] and as [v][n]; PLANES = 3: as the three bf16 of each number
 template <int KIND, int PLANES>
 struct DlogitsEpi {
+  static constexpr double kMid = 6 * PLANES, kLarge = 15 * PLANES;
   struct Args {
     const float2* stat;         // {max * log2e, 1 / sum} of a token
     const float* ratio;         // g_n over the largest |g|, times the lift of fp16; 0: the row takes no part
@@ -247,6 +249,7 @@ struct DlogitsEpi {
 
 // slab[slice][n][m] (+)= acc in 32 bits: the sums of dh over slices of a piece's k and over the pieces
 struct SlabEpi {
+  static constexpr double kMid = 8, kLarge = 12;
   struct Args {
     float* slab;
     int64_t ld, slice;          // ld a multiple of 4
@@ -276,6 +279,7 @@ struct SlabEpi {
 // out[n][m] = acc * *factor in the gradients' type (OUT: BF16, F16, or 3: fp32)
 template <int OUT>
 struct GradEpi {
+  static constexpr double kMid = 9, kLarge = 14;
   struct Args {
     void* out;
     int64_t ld;
@@ -418,72 +422,119 @@ __global__ __launch_bounds__(1024) void grad_rows_k(const float* __restrict__ gr
   if (threadIdx.x == 0) *factor = top > 0.f ? top / over / lift * c : 0.f;
 }
 
-// Rows laid out for the products: 16-bit rows padded with zeros to ldo, or fp32 as planes of three bf16.
+// Rows laid out for the products: 16-bit rows padded with zeros to ldo (a multiple of 8), or
+// fp32 as planes of three bf16.  A thread makes 8 columns.
 template <typename T>
 __global__ __launch_bounds__(256) void pack_k(const T* __restrict__ x, int64_t ld, int64_t rows, int cols,
                                               uint16_t* __restrict__ out, int ldo, int64_t plane) {
-  const int64_t total = rows * ldo;
+  typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  const int per = ldo / 8;
+  const int64_t total = rows * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / ldo;
-    const int c = (int)(i - r * ldo);
-    if constexpr (sizeof(T) == 4) {
-      float v = c < cols ? x[r * ld + c] : 0.f;
-      const bool finite = fabsf(v) < INFINITY;
-#pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        uint32_t b = pack2<BF16>(v, 0.f) & 0xffffu;
-        // a finite number next to the largest rounds to infinity: cut it off instead
-        if ((b & 0x7fffu) == 0x7f80u) b -= 1;
-        // infinity and NaN stand in the last plane alone: it meets the other operand's first plane only, so
-        // that infinity times a number is infinity (times a zero of its later planes it would be NaN)
-        if (!finite) b = p == 2 ? pack2<BF16>(v, 0.f) & 0xffffu : 0;
-        out[p * plane + i] = (uint16_t)b;
-        if (finite) v -= __uint_as_float(b << 16);
-      }
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * 8;
+    const T* p = x + r * ld + c;
+    v8 v;
+    if (c + 8 <= cols) {
+      v = *reinterpret_cast<const v8*>(p);
     } else {
-      out[i] = c < cols ? x[r * ld + c] : (T)0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? p[k] : (T)0;
+    }
+    uint16_t* o = out + r * ldo + c;
+    if constexpr (sizeof(T) == 4) {
+      uint32_t b[3][4] = {};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float f = v[k];
+        const bool finite = fabsf(f) < INFINITY;
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          uint32_t h = pack2<BF16>(f, 0.f) & 0xffffu;
+          // a finite number next to the largest rounds to infinity: cut it off instead
+          if ((h & 0x7fffu) == 0x7f80u) h -= 1;
+          // infinity and NaN stand in the last plane alone: it meets the other operand's first plane only, so
+          // that infinity times a number is infinity (times a zero of its later planes it would be NaN)
+          if (!finite) h = q == 2 ? pack2<BF16>(f, 0.f) & 0xffffu : 0;
+          b[q][k >> 1] |= h << (16 * (k & 1));
+          if (finite) f -= __uint_as_float(h << 16);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(o + q * plane) = make_uint4(b[q][0], b[q][1], b[q][2], b[q][3]);
+    } else {
+      typedef T w8 __attribute__((ext_vector_type(8)));
+      *reinterpret_cast<w8*>(o) = v;
     }
   }
 }
 
-// out[c][r] = x[r][c] (16 bits) for r < Rp: zero for r >= R and for rows whose ratio is 0 (they may hold
-// anything and multiply zeros only); blockIdx.z: plane
+// out[c][r] = x[r][c] (16 bits) for r < Rp (a multiple of 8): zero for r >= R and for rows whose ratio is 0
+// (they may hold anything and multiply zeros only).  x: rows on 16 bytes, readable to the next multiple of 8
+// columns.  64 rows x 256 columns to a workgroup, through LDS as a product's outputs; blockIdx.z: plane.
+struct Pane {
+  static constexpr int BM = 256, BN = 64, NW = 4;
+};
 __global__ __launch_bounds__(256) void transpose_k(const uint16_t* __restrict__ x, int64_t ld, int64_t plane, int R,
                                                    int Cc, const float* __restrict__ ratio, uint16_t* __restrict__ out,
                                                    int64_t ldo, int64_t oplane, int Rp) {
-  __shared__ uint16_t tile[64][66];
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  __shared__ __attribute__((aligned(16))) char lds[Pane::BM * Pane::BN * 2];
+  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 256;
   x += blockIdx.z * plane;
   out += blockIdx.z * oplane;
-  for (int k = threadIdx.x; k < 64 * 64; k += 256) {
-    const int r = r0 + k / 64, c = c0 + k % 64;
-    const bool ok = r < R && c < Cc && (!ratio || ratio[r] != 0.f);
-    tile[k / 64][k % 64] = ok ? x[r * ld + c] : 0;
+  const int c = threadIdx.x % 32, cc = c0 + c * 8;
+  i4v v[8];
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    const int r = r0 + threadIdx.x / 32 + s * 8;
+    const bool ok = r < R && cc < Cc && (!ratio || ratio[r] != 0.f);
+    v[s] = ok ? *reinterpret_cast<const i4v*>(x + r * ld + cc) : i4v{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    const int n = threadIdx.x / 32 + s * 8;
+    *reinterpret_cast<i4v*>(lds + n * 512 + ((c ^ turn<Pane>(n)) * 16)) = v[s];
   }
   __syncthreads();
-  for (int k = threadIdx.x; k < 64 * 64; k += 256) {
-    const int c = c0 + k / 64, r = r0 + k % 64;
-    if (c < Cc && r < Rp) out[c * ldo + r] = tile[k % 64][k / 64];
-  }
+  store_columns<Pane>(lds, out, ldo, r0, c0, Rp, Cc);
 }
 
-// dh[n][m] = factor * the slabs' sum, slab after slab
+// dh[n][m] = factor * the slabs' sum, slab after slab; a thread makes 4 columns
 template <int OUT>
 __global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab, int slices, int64_t slice, int64_t ld,
                                                   int N, int M, const float* __restrict__ factor, void* __restrict__ out,
-                                                  int64_t ldo) {
+                                                  int64_t ldo, int wide) {
   const float f = *factor;
-  const int64_t total = (int64_t)N * M;
+  const int per = (int)(ld / 4);
+  const int64_t total = (int64_t)N * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t n = i / M;
-    const int m = (int)(i - n * M);
-    float v = 0.f;
-    for (int s = 0; s < slices; ++s) v += slab[s * slice + n * ld + m];
+    const int64_t n = i / per;
+    const int m = (int)(i - n * per) * 4;
+    const float* p = slab + n * ld + m;
+    f4v v = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const f4v*>(p + s * slice);
     v *= f;
-    if constexpr (OUT == 3)
-      static_cast<float*>(out)[n * ldo + m] = v;
-    else
-      static_cast<uint16_t*>(out)[n * ldo + m] = (uint16_t)pack2<OUT>(v, 0.f);
+    if constexpr (OUT == 3) {
+      float* o = static_cast<float*>(out) + n * ldo + m;
+      if (wide && m + 4 <= M) {
+        *reinterpret_cast<f4v*>(o) = v;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (m + k < M) o[k] = v[k];
+      }
+    } else {
+      const u2v w = {pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
+      uint16_t* o = static_cast<uint16_t*>(out) + n * ldo + m;
+      if (wide && m + 4 <= M) {
+        *reinterpret_cast<u2v*>(o) = w;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (m + k < M) o[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+      }
+    }
   }
 }
 
@@ -578,7 +629,8 @@ struct BwdWs {
     slab_ld = (s.D + 3) / 4 * 4;
     slab_slice = s.N * slab_ld;
     // a slice's sums are written and read once: 8 bytes of each at about 4 TB/s
-    dh_plan = plan_product(s.D, s.N, (int64_t)ceil_div(ldl * 2, 128) * (P == 3 ? 6 : 1), kSlabSlices, slab_slice * 8 / 4e6);
+    dh_plan = plan_product(s.D, s.N, (int64_t)ceil_div(ldl * 2, 128) * (P == 3 ? 6 : 1),
+                           SlabEpi::kMid, SlabEpi::kLarge, kSlabSlices, slab_slice * 8 / 4e6);
     slab = l.take<float>(dh ? dh_plan.slices * slab_slice : 0);
     bytes = l.at;
   }
@@ -593,8 +645,7 @@ inline void set_pairs(Args& a, int planes) {
 
 template <typename T>
 inline void pack(const void* x, int64_t ld, int64_t rows, int cols, uint16_t* out, int ldo, hipStream_t s) {
-  const int64_t total = rows * ldo;
-  const int grid = (int)std::min<int64_t>((total + 255) / 256, 8192);
+  const int grid = (int)std::min<int64_t>((rows * (ldo / 8) + 255) / 256, 8192);
   if (grid > 0)
     hipLaunchKernelGGL((pack_k<T>), dim3(grid), dim3(256), 0, s, static_cast<const T*>(x), ld, rows, cols, out, ldo,
                        rows * ldo);
@@ -632,8 +683,9 @@ inline int launch_planned(const Args& a, const typename Epi::Args& e, Plan p, hi
   return launch_product<Large<KIND>, Epi>(a, e, p.slices, s, what);
 }
 
+template <class Epi>
 inline Plan plan_of(const Args& a) {
-  return plan_product(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs);
+  return plan_product(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs, Epi::kMid, Epi::kLarge);
 }
 
 #define PO_TRY(x)             \
@@ -676,7 +728,7 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
     a.A = rows_of(s, s.direct_w, w, ldw, v, rows, ws.wp, st);
     e.v0 = v;
     e.V = (int)rows;
-    const Plan p = plan_of(a);
+    const Plan p = plan_of<StatsEpi>(a);
     PO_TRY((dtype == PO_F16 ? launch_planned<F16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
                             : launch_planned<BF16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")));
     e.tile0 += ceil_div(rows, p.tile == LARGE ? 256 : 128);
@@ -706,7 +758,7 @@ int backward(const Shape& s, const BwdWs& ws, const void* h, int64_t ldh, const 
   const int N = (int)s.N, D = (int)s.D;
   const Operand H = rows_of(s, s.direct_h, h, ldh, 0, N, ws.hp, st);
   if (dw)
-    hipLaunchKernelGGL(transpose_k, dim3(ceil_div(s.Np(), 64), ceil_div(D, 64), P), dim3(256), 0, st,
+    hipLaunchKernelGGL(transpose_k, dim3(ceil_div(s.Np(), 64), ceil_div(D, 256), P), dim3(256), 0, st,
                        reinterpret_cast<const uint16_t*>(H.p), H.stride / 2, H.plane / 2, N, D, ws.ratio, ws.ht,
                        s.ldn(), D * s.ldn(), (int)s.Np());
   for (int64_t v = 0; v < s.V; v += ws.piece) {
@@ -722,9 +774,9 @@ int backward(const Shape& s, const BwdWs& ws, const void* h, int64_t ldh, const 
     typename DlogitsEpi<KIND, P>::Args e{stat, ws.ratio, target, v, N, (int)s.Np(), rows, rp, scale * kLog2e,
                                          dh ? ws.dl : nullptr, dw ? ws.dlt : nullptr, ws.ldl, s.ldn(), N * ws.ldl,
                                          ws.piece * s.ldn()};
-    PO_TRY((launch_planned<KIND, DlogitsEpi<KIND, P>>(a, e, plan_of(a), st, what)));
+    PO_TRY((launch_planned<KIND, DlogitsEpi<KIND, P>>(a, e, plan_of<DlogitsEpi<KIND, P>>(a), st, what)));
     if (dh) {                                                // slab[n][d] += sum_v dl[n][v] w[v][d]
-      hipLaunchKernelGGL(transpose_k, dim3(ceil_div(rp, 64), ceil_div(D, 64), P), dim3(256), 0, st,
+      hipLaunchKernelGGL(transpose_k, dim3(ceil_div(rp, 64), ceil_div(D, 256), P), dim3(256), 0, st,
                          reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, D,
                          (const float*)nullptr, ws.wt, ws.ldl, D * ws.ldl, rp);
       a.A = Operand{reinterpret_cast<char*>(ws.wt), ws.ldl * 2, D * ws.ldl * 2, D};
@@ -742,13 +794,14 @@ int backward(const Shape& s, const BwdWs& ws, const void* h, int64_t ldh, const 
       const int es = OUT == 3 ? 4 : 2;
       char* out = static_cast<char*>(dw) + v * lddw * es;
       const typename GradEpi<OUT>::Args ge{out, lddw, ws.factor, rows, D, (uintptr_t)out % 16 == 0 && lddw * es % 16 == 0};
-      PO_TRY((launch_planned<KIND, GradEpi<OUT>>(a, ge, plan_of(a), st, what)));
+      PO_TRY((launch_planned<KIND, GradEpi<OUT>>(a, ge, plan_of<GradEpi<OUT>>(a), st, what)));
     }
   }
   if (dh) {
-    const int grid = (int)std::min<int64_t>(((int64_t)N * D + 255) / 256, 8192);
+    const int grid = (int)std::min<int64_t>((N * (ws.slab_ld / 4) + 255) / 256, 8192);
+    const int es = OUT == 3 ? 4 : 2, wide = (uintptr_t)dh % 16 == 0 && lddh * es % 16 == 0;
     hipLaunchKernelGGL((slab_sum_k<OUT>), dim3(grid), dim3(256), 0, st, ws.slab, ws.dh_plan.slices, ws.slab_slice, ws.slab_ld,
-                       N, D, ws.factor, dh, lddh);
+                       N, D, ws.factor, dh, lddh, wide);
   }
   return po::check_launch(what);
 }
