@@ -147,6 +147,8 @@ _SIGS = {
     "po_quantize_rows": [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p],
     "po_int8_matmul": [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                        c_void_p, c_int64, c_int, c_void_p],
+    "po_int8_linear": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                       c_void_p, c_int64, c_int, c_void_p],
     "po_nhwc_to_nchw": [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "po_nchw_to_nhwc": [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
 }
@@ -240,33 +242,38 @@ def ptr(t, dtype=torch.float32):
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-@contextlib.contextmanager
-def _other_device(device):
-    with torch.cuda.device(device):
-        yield
+_HERE_ALREADY = contextlib.nullcontext()
 
 
 def device_of(*tensors):
     """Context of the tensors' device: launches and allocations inside go to it and
     to its current stream, whatever device is current outside."""
-    t = tensors[0]
-    for u in tensors:
-        if not (isinstance(u, torch.Tensor) and u.is_cuda):
-            ensure_device(u)                 # raises
-        if u.device != t.device:
-            raise RuntimeError("advpatch HIP ops need their tensors on one device; got %s and %s" % (t.device, u.device))
-    if t.device.index == torch.cuda.current_device():
-        ensure_device(t)
-        return contextlib.nullcontext()
-    with torch.cuda.device(t.device):        # the check selects the device it looks at
-        ensure_device(t)
-    return _other_device(t.device)
+    device = tensors[0].device
+    for t in tensors:
+        if not t.is_cuda:
+            ensure_device(t)                 # raises
+        if t.device != device:
+            raise RuntimeError("advpatch HIP ops need their tensors on one device; got %s and %s" % (device, t.device))
+    if device.index == torch._C._cuda_getDevice():
+        if device.index not in _checked_devices:
+            ensure_device(tensors[0])
+        return _HERE_ALREADY
+    with torch.cuda.device(device):          # the check selects the device it looks at
+        ensure_device(tensors[0])
+    return torch.cuda.device(device)
+
+
+def raw_stream(t):
+    """The current stream of t's device, as a number for a po_stream_t argument."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def rows2d(t):
     """(matrix, row stride): t as [rows, cols] over its last dimension, a view where the
     elements of a row are neighbours and rows do not overlap, else a copy."""
-    m = t.reshape(-1, t.shape[-1])
+    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if m.is_contiguous():
+        return m, m.shape[1]
     if (m.shape[1] > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < m.shape[1]):
         m = m.contiguous()
     return m, (m.stride(0) if m.shape[0] > 1 else m.shape[1])

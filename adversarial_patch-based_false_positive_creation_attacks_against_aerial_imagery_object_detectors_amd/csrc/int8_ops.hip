@@ -56,6 +56,26 @@ __device__ __forceinline__ int quotient(float x, float s, float inv) {
   return (int)q;
 }
 
+// A row's scale, from the bits of its largest |x|, and the 8-bit numbers under it.
+struct RowScale {
+  float s, inv;
+  bool bad;                                                  // the row holds NaN or an infinity: as bits they lie on top
+  __device__ __forceinline__ explicit RowScale(uint32_t top) : s(__uint_as_float(top) / 127.f), inv(1.f / s), bad(top >= 0x7f800000u) {}
+  __device__ __forceinline__ float stored() const { return bad ? __uint_as_float(0x7fc00000u) : s; }
+  __device__ __forceinline__ uint2 quotients(const float* v) const {
+    uint32_t b[2] = {0, 0};
+    if (!bad && s > 0.f) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // 1 / s and half steps of s need normal numbers
+        const int n = s > 1e-30f ? quotient(v[j], s, inv) : (int)__builtin_rint((double)v[j] / (double)s);
+        b[j >> 2] |= (uint32_t)(n & 255) << (8 * (j & 3));
+      }
+    }
+    return make_uint2(b[0], b[1]);
+  }
+};
+
 // One row to WPR waves, 8 elements to a lane and step; rows of up to STEPS steps stay
 // in registers between the maximum and the quotients, longer ones (STEPS = 0) are read
 // again.  A row that holds NaN or an infinity gets the scale NaN.
@@ -93,21 +113,10 @@ __global__ __launch_bounds__(256) void quantize_rows_k(const void* __restrict__ 
     top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
   }
   if (row >= rows) return;
-  const bool bad = top >= 0x7f800000u;                       // as bits NaN lies above infinity
-  const float s = __uint_as_float(top) / 127.f, inv = 1.f / s;
-  if (t == 0) scale[row] = bad ? __uint_as_float(0x7fc00000u) : s;
+  const RowScale r(top);
+  if (t == 0) scale[row] = r.stored();
   auto put8 = [&](int k, const float* w) {
-    if (k >= Kp) return;
-    uint32_t b[2] = {0, 0};
-    if (!bad && s > 0.f) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // 1 / s and half steps of s need normal numbers
-        const int n = s > 1e-30f ? quotient(w[j], s, inv) : (int)__builtin_rint((double)w[j] / (double)s);
-        b[j >> 2] |= (uint32_t)(n & 255) << (8 * (j & 3));
-      }
-    }
-    *reinterpret_cast<uint2*>(q + row * ldq + k) = make_uint2(b[0], b[1]);
+    if (k < Kp) *reinterpret_cast<uint2*>(q + row * ldq + k) = r.quotients(w);
   };
   if constexpr (STEPS > 0) {
 #pragma unroll
@@ -116,6 +125,115 @@ __global__ __launch_bounds__(256) void quantize_rows_k(const void* __restrict__ 
     for (int k = t * 8; k < Kp; k += T * 8) {
       load8<DT>(x, at + k, mine - k, v[0]);
       put8(k, v[0]);
+    }
+  }
+}
+
+// ---- few tokens ----------------------------------------------------------
+// Up to 32 tokens: the weights' bytes are the work (16.8 MB of 4096 x 4096 take 3.3 us at
+// 5.2 TB/s).  A workgroup owns 16 weight rows, its waves slices of k of 1024 bytes: a lane's
+// 16 loads of 16 bytes (row lane % 16, 64 bytes of a row to a load) are all in flight at once,
+// and go into the matrix cores as they are.  The waves' sums meet in LDS.  FUSED (a few
+// tokens): the workgroup quantises the tokens itself, into LDS, behind its weights' loads:
+// one launch, where the quantisation alone takes 4 us.
+constexpr int kFewSlice = 1024, kFewLds = 56 << 10;         // with the sums below 64 KB
+
+// token t's row of 8-bit numbers in LDS and its scale, made by the whole workgroup
+template <int DT>
+__device__ __forceinline__ void quantize_to_lds(const void* x, int64_t at, int K, int Kp, int8_t* q, uint32_t* tops,
+                                                float* scale) {
+  uint32_t top = 0;
+  float v[8];
+  for (int k = threadIdx.x * 8; k < K; k += 256 * 8) {
+    load8<DT>(x, at + k, K - k, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+  }
+  top = po::wave_max_u32(top);
+  __syncthreads();                                           // the last token's maxima are read
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+  const RowScale r(top);
+  if (threadIdx.x == 0) *scale = r.stored();
+  for (int k = threadIdx.x * 8; k < Kp; k += 256 * 8) {
+    load8<DT>(x, at + k, K - k, v);
+    *reinterpret_cast<uint2*>(q + k) = r.quotients(v);
+  }
+}
+
+template <int DT, int TB, bool FUSED>
+__global__ __launch_bounds__(256) void few_tokens_k(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict__ q,
+                                                    int64_t ldq, const float* __restrict__ sx, const int8_t* __restrict__ w,
+                                                    int64_t ldw, const float* __restrict__ sw,
+                                                    const float* __restrict__ bias, int M, int N, int K,
+                                                    void* __restrict__ y, int64_t ldy) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ i4v sums[4][TB][64];
+  __shared__ uint32_t tops[4];
+  __shared__ float scales[32];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16, Kp = (K + 15) / 16 * 16;
+  const int row = n0 + (lane & 15), quad = lane >> 4;
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(w + (int64_t)n0 * ldw), 0,
+                                                                     0x7fffffff, 0x00020000);
+  const uint32_t wat = row < N ? (uint32_t)((lane & 15) * (int)ldw) : kOOB;
+  i4v a[16];
+  auto weights = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int k = k0 + j * 64 + quad * 16;
+      a[j] = __builtin_bit_cast(i4v, __builtin_amdgcn_raw_buffer_load_b128(rw, k < Kp ? wat + (uint32_t)k : kOOB, 0, 0));
+    }
+  };
+  weights(wave * kFewSlice);
+  if constexpr (FUSED) {
+    __builtin_amdgcn_sched_barrier(0);
+    for (int t = 0; t < M; ++t)
+      quantize_to_lds<DT>(x, t * ldx, K, Kp, reinterpret_cast<int8_t*>(lds) + t * Kp, tops, scales + t);
+    __syncthreads();
+  } else if (threadIdx.x < 32) {
+    scales[threadIdx.x] = threadIdx.x < M ? sx[threadIdx.x] : 0.f;
+  }
+  i4v acc[TB];
+#pragma unroll
+  for (int b = 0; b < TB; ++b) acc[b] = i4v{0, 0, 0, 0};
+  const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(q), 0, 0x7fffffff, 0x00020000);
+  for (int k0 = wave * kFewSlice; k0 < Kp; k0 += 4 * kFewSlice) {
+    if (k0 != wave * kFewSlice) weights(k0);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int k = k0 + j * 64 + quad * 16;
+#pragma unroll
+      for (int b = 0; b < TB; ++b) {
+        const int t = b * 16 + (lane & 15);
+        i4v v = {0, 0, 0, 0};
+        if constexpr (FUSED) {
+          if (t < M && k < Kp) v = *reinterpret_cast<const i4v*>(lds + t * Kp + k);
+        } else {
+          v = __builtin_bit_cast(i4v, __builtin_amdgcn_raw_buffer_load_b128(
+                                          rq, t < M && k < Kp ? (uint32_t)(t * (int)ldq + k) : kOOB, 0, 0));
+        }
+        acc[b] = mfma<I8>(a[j], v, acc[b]);
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < TB; ++b) sums[wave][b][lane] = acc[b];
+  __syncthreads();
+  if (wave < TB) {
+    const i4v s = sums[0][wave][lane] + sums[1][wave][lane] + sums[2][wave][lane] + sums[3][wave][lane];
+    const int t = wave * 16 + (lane & 15), n = n0 + quad * 4;
+    if (t < M) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (n + k < N) {
+          const float v = __builtin_fmaf((float)s[k] * scales[t], sw[n + k], bias ? bias[n + k] : 0.f);
+          if constexpr (DT == PO_F32)
+            static_cast<float*>(y)[(int64_t)t * ldy + n + k] = v;
+          else
+            static_cast<uint16_t*>(y)[(int64_t)t * ldy + n + k] = (uint16_t)pack2<DT == PO_F16 ? F16 : BF16>(v, 0.f);
+        }
     }
   }
 }
@@ -185,12 +303,32 @@ int product_of(const Args& a, const typename ScaledEpi<DT>::Args& e, hipStream_t
   using E = ScaledEpi<DT>;
   const char* what = "po_int8_matmul";
   const Plan p = plan_product(a.A.rows, a.B.rows, ceil_div(a.kbytes, 128), 6, 10);
-  if (p.tile == FEW) return launch_product<Cfg<I8, 128, 32, 4, 1, 128, 3>, E>(a, e, 1, s, what);
   if (p.tile == LARGE) return launch_product<Cfg<I8, 256, 256, 2, 4, 128, 2>, E>(a, e, 1, s, what);
   // 64 x 64 where tiles of 128 x 128 leave CUs without one
   if ((int64_t)ceil_div(a.A.rows, 128) * ceil_div(a.B.rows, 128) < 256)
     return launch_product<Cfg<I8, 64, 64, 2, 2, 128, 3>, E>(a, e, 1, s, what);
   return launch_product<Cfg<I8, 128, 128, 2, 2, 128, 2>, E>(a, e, 1, s, what);
+}
+
+constexpr int kFewTokens = 32;
+
+// Tokens that a workgroup of few_tokens_k quantises itself.
+inline bool fuses(int64_t M, int64_t K) { return M <= 4 && M * ((K + 15) / 16 * 16) <= kFewLds; }
+
+template <int DT>
+int few_tokens(bool fused, const void* x, int64_t ldx, const int8_t* q, int64_t ldq, const float* sx, const int8_t* w,
+               int64_t ldw, const float* sw, const float* bias, int M, int N, int K, void* y, int64_t ldy, hipStream_t s) {
+  const dim3 grid(ceil_div(N, 16));
+  if (fused)
+    hipLaunchKernelGGL((few_tokens_k<DT, 1, true>), grid, dim3(256), M * ((K + 15) / 16 * 16), s, x, ldx, q, ldq, sx, w, ldw,
+                       sw, bias, M, N, K, y, ldy);
+  else if (M <= 16)
+    hipLaunchKernelGGL((few_tokens_k<DT, 1, false>), grid, dim3(256), 0, s, x, ldx, q, ldq, sx, w, ldw, sw, bias, M, N, K, y,
+                       ldy);
+  else
+    hipLaunchKernelGGL((few_tokens_k<DT, 2, false>), grid, dim3(256), 0, s, x, ldx, q, ldq, sx, w, ldw, sw, bias, M, N, K, y,
+                       ldy);
+  return po::check_launch("po_int8_matmul");
 }
 
 inline int element_bytes(int dtype) { return dtype == PO_F32 ? 4 : 2; }
@@ -226,26 +364,70 @@ extern "C" int po_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t M
   return po::check_launch("po_quantize_rows");
 }
 
+namespace {
+
+int check_matmul(const char* what, const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, int64_t M, int64_t N, int64_t K,
+                 int64_t ldy, int dtype) {
+  PO_REQUIRE(known(dtype), "%s: unknown dtype %d", what, dtype);
+  PO_REQUIRE(M >= 1 && N >= 1 && K >= 1 && M <= (1 << 21) && N <= (1 << 24) && K < (1 << 17),
+             "%s: bad sizes (M=%lld N=%lld K=%lld)", what, (long long)M, (long long)N, (long long)K);
+  const int64_t Kp = (K + 15) / 16 * 16;
+  PO_REQUIRE(ldq >= Kp && ldq % 16 == 0 && (uintptr_t)q % 16 == 0 && ldw >= Kp && ldw % 16 == 0 && (uintptr_t)w % 16 == 0 &&
+                 ldq <= (1 << 22) && ldw <= (1 << 22) && ldy >= N,
+             "%s: rows must start on 16 bytes and be laid out to a multiple of 16", what);
+  return PO_OK;
+}
+
+int matmul(const int8_t* q, int64_t ldq, const float* sx, const int8_t* w, int64_t ldw, const float* sw, const float* bias,
+           int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int dtype, hipStream_t s) {
+  if (M <= kFewTokens) {
+#define PO_FEW(DT) few_tokens<DT>(false, nullptr, 0, q, ldq, sx, w, ldw, sw, bias, (int)M, (int)N, (int)K, y, ldy, s)
+    return dtype == PO_F32 ? PO_FEW(PO_F32) : dtype == PO_F16 ? PO_FEW(PO_F16) : PO_FEW(PO_BF16);
+#undef PO_FEW
+  }
+  Args a{};
+  a.A = Operand{reinterpret_cast<const char*>(w), ldw, 0, (int)N};
+  a.B = Operand{reinterpret_cast<const char*>(q), ldq, 0, (int)M};
+  a.kbytes = (int)((K + 15) / 16 * 16);
+  a.pairs = 1;
+  const int wide = (uintptr_t)y % 16 == 0 && ldy * element_bytes(dtype) % 16 == 0;
+  if (dtype == PO_F32) return product_of<PO_F32>(a, {y, ldy, sx, sw, bias, (int)M, (int)N, wide}, s);
+  if (dtype == PO_F16) return product_of<PO_F16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N, wide}, s);
+  return product_of<PO_BF16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N, wide}, s);
+}
+
+// workspace of po_int8_linear: the tokens' 8-bit rows, then their scales
+inline int64_t linear_ldq(int64_t K) { return (K + 63) / 64 * 64; }
+
+}  // namespace
+
 extern "C" int po_int8_matmul(const int8_t* q, int64_t ldq, const float* sx, const int8_t* w, int64_t ldw,
                               const float* sw, const float* bias, int64_t M, int64_t N, int64_t K, void* y, int64_t ldy,
                               int dtype, po_stream_t stream) {
   PO_REQUIRE(q && sx && w && sw && y, "po_int8_matmul: null pointer");
-  PO_REQUIRE(known(dtype), "po_int8_matmul: unknown dtype %d", dtype);
-  PO_REQUIRE(M >= 1 && N >= 1 && K >= 1 && M <= (1 << 21) && N <= (1 << 24) && K < (1 << 17),
-             "po_int8_matmul: bad sizes (M=%lld N=%lld K=%lld)", (long long)M, (long long)N, (long long)K);
-  const int64_t Kp = (K + 15) / 16 * 16;
-  PO_REQUIRE(ldq >= Kp && ldq % 16 == 0 && (uintptr_t)q % 16 == 0 && ldw >= Kp && ldw % 16 == 0 && (uintptr_t)w % 16 == 0 &&
-                 ldq <= (1 << 22) && ldw <= (1 << 22) && ldy >= N,
-             "po_int8_matmul: rows must start on 16 bytes and be laid out to a multiple of 16");
-  Args a{};
-  a.A = Operand{reinterpret_cast<const char*>(w), ldw, 0, (int)N};
-  a.B = Operand{reinterpret_cast<const char*>(q), ldq, 0, (int)M};
-  a.kbytes = (int)Kp;
-  a.pairs = 1;
-  const int es = element_bytes(dtype);
-  const int wide = (uintptr_t)y % 16 == 0 && ldy * es % 16 == 0;
-  const hipStream_t s = po::stream_of(stream);
-  if (dtype == PO_F32) return product_of<PO_F32>(a, {y, ldy, sx, sw, bias, (int)M, (int)N, wide}, s);
-  if (dtype == PO_F16) return product_of<PO_F16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N, wide}, s);
-  return product_of<PO_BF16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N, wide}, s);
+  const int rc = check_matmul("po_int8_matmul", q, ldq, w, ldw, M, N, K, ldy, dtype);
+  if (rc != PO_OK) return rc;
+  return matmul(q, ldq, sx, w, ldw, sw, bias, M, N, K, y, ldy, dtype, po::stream_of(stream));
+}
+
+extern "C" int po_int8_linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const float* sw, const float* bias,
+                              int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* y,
+                              int64_t ldy, int dtype, po_stream_t stream) {
+  PO_REQUIRE(x && w && sw && y && workspace, "po_int8_linear: null pointer");
+  const int64_t ldq = linear_ldq(K);
+  const int rc = check_matmul("po_int8_linear", static_cast<int8_t*>(workspace), ldq, w, ldw, M, N, K, ldy, dtype);
+  if (rc != PO_OK) return rc;
+  PO_REQUIRE(ldx >= K, "po_int8_linear: bad strides");
+  PO_REQUIRE(workspace_bytes >= M * (ldq + 4), "po_int8_linear: workspace of %lld bytes, %lld needed",
+             (long long)workspace_bytes, (long long)(M * (ldq + 4)));
+  int8_t* q = static_cast<int8_t*>(workspace);
+  float* sx = reinterpret_cast<float*>(q + M * ldq);
+  if (fuses(M, K)) {
+#define PO_FEW(DT) few_tokens<DT>(true, x, ldx, nullptr, 0, nullptr, w, ldw, sw, bias, (int)M, (int)N, (int)K, y, ldy, po::stream_of(stream))
+    return dtype == PO_F32 ? PO_FEW(PO_F32) : dtype == PO_F16 ? PO_FEW(PO_F16) : PO_FEW(PO_BF16);
+#undef PO_FEW
+  }
+  const int rq = po_quantize_rows(x, ldx, dtype, M, K, q, ldq, sx, stream);
+  if (rq != PO_OK) return rq;
+  return matmul(q, ldq, sx, w, ldw, sw, bias, M, N, K, y, ldy, dtype, po::stream_of(stream));
 }

@@ -31,7 +31,7 @@ def _quantize(x):
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     if rows:
         nat.call("po_quantize_rows", m.data_ptr(), ld, nat.DTYPES[x.dtype], rows, K, q.data_ptr(), q.stride(0),
-                 scale.data_ptr(), nat.stream())
+                 scale.data_ptr(), nat.raw_stream(x))
     return q, scale
 
 
@@ -51,7 +51,7 @@ def _matmul(q, sx, rows, K, wq, wscale, bias, dtype):
         w, ldw = _weights(wq)
         nat.call("po_int8_matmul", q.data_ptr(), q.stride(0), sx.data_ptr(), w.data_ptr(), ldw, wscale.data_ptr(),
                  None if bias is None else bias.data_ptr(), rows, wq.shape[0], K, y.data_ptr(), wq.shape[0],
-                 nat.DTYPES[dtype], nat.stream())
+                 nat.DTYPES[dtype], nat.raw_stream(q))
     return y
 
 
@@ -120,10 +120,19 @@ def int8_linear(x, wq, wscale, bias=None):
     _check_inner("int8_linear", K)
     _no_grad("int8_linear", x, wscale, bias)
     _check_weights("int8_linear", K, wq, wscale, bias)
-    with nat.device_of(*(t for t in (x, wq, wscale, bias) if t is not None)):
-        q, scale = _quantize(x)
-        y = _matmul(q, scale, q.shape[0], K, wq, wscale.contiguous(), None if bias is None else bias.contiguous(), x.dtype)
-    return y.view(x.shape[:-1] + (wq.shape[0],))
+    with nat.device_of(*((x, wq, wscale) if bias is None else (x, wq, wscale, bias))):
+        m, ldx = nat.rows2d(x)
+        M, N = m.shape[0], wq.shape[0]
+        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+        if M:
+            w, ldw = _weights(wq)
+            ws = torch.empty(M * ((K + 63) // 64 * 64 + 4), dtype=torch.uint8, device=x.device)
+            wscale = wscale.contiguous()
+            bias = None if bias is None else bias.contiguous()
+            nat.call("po_int8_linear", m.data_ptr(), ldx, w.data_ptr(), ldw, wscale.data_ptr(),
+                     None if bias is None else bias.data_ptr(), M, N, K, ws.data_ptr(), ws.numel(), y.data_ptr(), N,
+                     nat.DTYPES[x.dtype], nat.raw_stream(x))
+    return y
 
 
 class Int8Linear(nn.Module):

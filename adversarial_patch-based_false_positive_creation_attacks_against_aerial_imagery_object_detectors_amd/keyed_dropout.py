@@ -27,15 +27,19 @@ def _launch(x, residual, drop, seed, step, row0):
     rows, cols = xm.shape
     nat.call("po_dropout", xm.data_ptr(), ldx, None if rm is None else rm.data_ptr(), ldr, nat.DTYPES[x.dtype], rows, cols,
              seed, 0 if on_device else step, step.data_ptr() if on_device else None,
-             used.data_ptr() if on_device else None, row0, drop, y.data_ptr(), cols, nat.stream())
+             used.data_ptr() if on_device else None, row0, drop, y.data_ptr(), cols, nat.raw_stream(x))
     return y, used
+
+
+def _run(x, residual, drop, seed, step, row0):
+    with nat.device_of(*(t for t in (x, residual, step) if isinstance(t, torch.Tensor))):
+        return _launch(x, residual, drop, seed, step, row0)
 
 
 class _KeyedDropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, drop, seed, step, row0):
-        with nat.device_of(*(t for t in (x, residual, step) if isinstance(t, torch.Tensor))):
-            y, used = _launch(x, residual, drop, seed, step, row0)
+        y, used = _run(x, residual, drop, seed, step, row0)
         ctx.key = (drop, seed, step if used is None else None, row0)
         if used is not None:
             ctx.save_for_backward(used)      # the caller may move its step on before the backward pass
@@ -46,8 +50,13 @@ class _KeyedDropout(torch.autograd.Function):
         drop, seed, step, row0 = ctx.key
         if step is None:
             (step,) = ctx.saved_tensors
-        # the same linear map: differentiable again
-        dx = _KeyedDropout.apply(dy, None, drop, seed, step, row0) if ctx.needs_input_grad[0] else None
+        dx = None
+        if ctx.needs_input_grad[0]:
+            # the same linear map; through apply where it has to be differentiable again
+            if torch.is_grad_enabled():
+                dx = _KeyedDropout.apply(dy, None, drop, seed, step, row0)
+            else:
+                dx = _run(dy, None, drop, seed, step, row0)[0]
         return dx, (dy if ctx.needs_input_grad[1] else None), None, None, None, None
 
 
@@ -82,8 +91,10 @@ def keyed_dropout(x, p, seed, step=0, row0=0, residual=None):
     rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
     if int(row0) < 0 or int(row0) + rows > 1 << 32:
         raise ValueError("keyed_dropout: rows row0 .. row0 + rows must stay within 2^32")
-    return _KeyedDropout.apply(x, residual, round(p * 65536), int(seed), step if isinstance(step, torch.Tensor) else int(step),
-                               int(row0))
+    args = (x, residual, round(p * 65536), int(seed), step if isinstance(step, torch.Tensor) else int(step), int(row0))
+    if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad):
+        return _KeyedDropout.apply(*args)
+    return _run(*args)[0]
 
 
 class KeyedDropout(nn.Module):

@@ -8,6 +8,7 @@ are thousands of embeddings.  With a frozen vocabulary only the embeddings'
 gradient is computed.
 """
 import ctypes
+import functools
 
 import torch
 import torch.nn as nn
@@ -24,40 +25,52 @@ def _matrix(t):
     return (m, ld) if ld <= _MAX_STRIDE else (m.contiguous(), m.shape[1])
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(h_at, ldh, w_at, ldw, dtype, N, V, D, dh, dw):
+    """(forward, backward) bytes: a function of the sizes and of whether rows start on 16 bytes."""
+    fwd, bwd = ctypes.c_int64(), ctypes.c_int64()
+    nat.call("po_linear_ce_workspace", h_at, ldh, w_at, ldw, dtype, N, V, D, dh, dw, ctypes.byref(fwd), ctypes.byref(bwd))
+    return fwd.value, bwd.value
+
+
 def _workspace(h, ldh, w, ldw, dh, dw, backward):
-    byts = ctypes.c_int64()
-    out = (None, ctypes.byref(byts)) if backward else (ctypes.byref(byts), None)
-    nat.call("po_linear_ce_workspace", h.data_ptr(), ldh, w.data_ptr(), ldw, nat.DTYPES[h.dtype], h.shape[0], w.shape[0],
-             h.shape[1], int(dh), int(dw), *out)
-    return torch.empty(byts.value, dtype=torch.uint8, device=h.device)
+    # 256 + the offset into 16 bytes stands for the address
+    byts = _workspace_bytes(256 + h.data_ptr() % 16, ldh, 256 + w.data_ptr() % 16, ldw, nat.DTYPES[h.dtype], h.shape[0],
+                            w.shape[0], h.shape[1], int(dh), int(dw))[backward]
+    return torch.empty(byts, dtype=torch.uint8, device=h.device)
+
+
+def _forward(hidden, weight, target, ignore_index, reduction, scale):
+    """(loss, what the backward pass needs: target as a vector, statistics [N][2] and the count behind them)."""
+    with nat.device_of(hidden, weight, target):
+        h, ldh = _matrix(hidden)
+        w, ldw = _matrix(weight)
+        t = target.reshape(-1).contiguous()
+        N, D = h.shape
+        loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=h.device)
+        stat = torch.empty(2 * N + 1, dtype=torch.float32, device=h.device)
+        if N:
+            ws = _workspace(h, ldh, w, ldw, False, False, False)
+            nat.call("po_linear_ce_fwd", h.data_ptr(), ldh, w.data_ptr(), ldw, nat.DTYPES[h.dtype], N, w.shape[0], D,
+                     t.data_ptr(), ignore_index, scale, reduction, ws.data_ptr(), ws.numel(), stat.data_ptr(),
+                     loss.data_ptr(), stat.data_ptr() + 8 * N, nat.raw_stream(h))
+        elif reduction:
+            loss.fill_(float("nan") if reduction == 2 else 0.0)
+    return loss, t, stat
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction, scale):
-        with nat.device_of(hidden, weight, target):
-            h, ldh = _matrix(hidden)
-            w, ldw = _matrix(weight)
-            t = target.reshape(-1).contiguous()
-            N = h.shape[0]
-            loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=h.device)
-            stat = torch.empty(N, 2, dtype=torch.float32, device=h.device)
-            count = torch.empty(1, dtype=torch.float32, device=h.device)
-            if N:
-                ws = _workspace(h, ldh, w, ldw, False, False, False)
-                nat.call("po_linear_ce_fwd", h.data_ptr(), ldh, w.data_ptr(), ldw, nat.DTYPES[h.dtype], N, w.shape[0],
-                         h.shape[1], t.data_ptr(), ignore_index, scale, reduction, ws.data_ptr(), ws.numel(),
-                         stat.data_ptr(), loss.data_ptr(), count.data_ptr(), nat.stream())
-            elif reduction:
-                loss.fill_(float("nan") if reduction == 2 else 0.0)
-        ctx.save_for_backward(hidden, weight, t, stat, count)
+        loss, t, stat = _forward(hidden, weight, target, ignore_index, reduction, scale)
+        ctx.save_for_backward(hidden, weight, t, stat)
         ctx.meta = (ignore_index, reduction, scale)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        hidden, weight, t, stat, count = ctx.saved_tensors
+        hidden, weight, t, stat = ctx.saved_tensors
         ignore_index, reduction, scale = ctx.meta
         need_h, need_w = ctx.needs_input_grad[:2]
         with nat.device_of(hidden, weight, grad):
@@ -72,9 +85,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
             dw = torch.empty(V, D, dtype=w.dtype, device=w.device) if need_w else None
             ws = _workspace(h, ldh, w, ldw, need_h, need_w, True)
             nat.call("po_linear_ce_bwd", h.data_ptr(), ldh, w.data_ptr(), ldw, nat.DTYPES[h.dtype], N, V, D,
-                     t.data_ptr(), ignore_index, scale, reduction, stat.data_ptr(), count.data_ptr(), g.data_ptr(),
+                     t.data_ptr(), ignore_index, scale, reduction, stat.data_ptr(), stat.data_ptr() + 8 * N, g.data_ptr(),
                      ws.data_ptr(), ws.numel(), None if dh is None else dh.data_ptr(), D,
-                     None if dw is None else dw.data_ptr(), D, nat.stream())
+                     None if dw is None else dw.data_ptr(), D, nat.raw_stream(h))
         return (None if dh is None else dh.view(hidden.shape)), dw, None, None, None, None
 
 
@@ -105,7 +118,10 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
         raise ValueError("linear_cross_entropy: reduction must be one of %s" % ", ".join(REDUCTIONS))
     if not 0.0 < float(scale) < float("inf"):
         raise ValueError("linear_cross_entropy: scale must be positive and finite, got %r" % (scale,))
-    return _LinearCrossEntropy.apply(hidden, weight, target, int(ignore_index), REDUCTIONS[reduction], float(scale))
+    args = (hidden, weight, target, int(ignore_index), REDUCTIONS[reduction], float(scale))
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _LinearCrossEntropy.apply(*args)
+    return _forward(*args)[0]
 
 
 class LinearCrossEntropy(nn.Module):

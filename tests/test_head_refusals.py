@@ -214,8 +214,9 @@ def test_workspace_sizes_follow_the_work():
     N, V, D = 8192, 131072, 2048
     f, g = sizes(N, V, D, 2, D, 1, 1)
     assert f < N * V * 4 // 50 and g < N * V * 4 // 4
-    # a frozen vocabulary, or frozen embeddings, need less; unpadded rows more
-    assert sizes(N, V, D, 2, D, 1, 0)[1] < g and sizes(N, V, D, 2, D, 0, 1)[1] < g + 1
+    # nor with one side frozen (pieces grow to the same bound); a small head needs little; unpadded rows more
+    assert max(sizes(N, V, D, 2, D, 1, 0)[1], sizes(N, V, D, 2, D, 0, 1)[1]) < N * V * 4 // 4
+    assert sizes(32, 4096, 256, 2, 256, 1, 1)[1] < 64 << 20
     assert sizes(N, V, D, 2, D + 1, 1, 1)[0] > f
     assert sizes(N, V, D, 0, D, 1, 1)[0] > f
 
