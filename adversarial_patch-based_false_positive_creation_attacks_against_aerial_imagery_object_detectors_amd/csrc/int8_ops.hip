@@ -306,7 +306,7 @@ int product_of(const Args& a, const typename ScaledEpi<DT>::Args& e, hipStream_t
   if (p.tile == LARGE) return launch_product<Cfg<I8, 256, 256, 2, 4, 128, 2>, E>(a, e, 1, s, what);
   // 64 x 64 where tiles of 128 x 128 leave CUs without one
   if ((int64_t)ceil_div(a.A.rows, 128) * ceil_div(a.B.rows, 128) < 256)
-    return launch_product<Cfg<I8, 64, 64, 2, 2, 128, 3>, E>(a, e, 1, s, what);
+    return launch_product<Cfg<I8, 64, 64, 2, 2, 256, 2>, E>(a, e, 1, s, what);
   return launch_product<Cfg<I8, 128, 128, 2, 2, 128, 2>, E>(a, e, 1, s, what);
 }
 

@@ -82,7 +82,7 @@ struct Cfg {
 
 template <int KB>
 __device__ __forceinline__ int swz(int row) {
-  return KB == 128 ? (row & 7) : ((row >> 1) & 3);
+  return KB == 256 ? (row & 15) : (row & 7);
 }
 
 template <class C>
@@ -121,7 +121,7 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
   }
   // the chunk of this lane inside a step is the same in every instruction: rows
   // of one lane differ by multiples of RPI * NW, which the swizzle does not see
-  static_assert((C::RPI * C::NW) % 8 == 0, "swizzle period");
+  static_assert((C::RPI * C::NW) % (KB == 256 ? 16 : 8) == 0 && (KB == 128 || KB == 256), "swizzle period");
   const uint32_t lch = ((lane % CPR) ^ swz<KB>(wave * C::RPI + lrow)) * 16;
   const char* abase = A.p + (int64_t)m0 * A.stride;
   const char* bbase = B.p + (int64_t)n0 * B.stride;
@@ -182,7 +182,7 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
     }
     __builtin_amdgcn_sched_group_barrier(0x008, X - E * R, 0);
   };
-  static_assert(G == 2, "a step's two groups alternate between two sets of registers");
+  static_assert(G % 2 == 0, "a step's groups alternate between two sets of registers");
   int buf = 0, s = 0;
   auto step = [&](auto first) {
     // this step's loads have landed when at most the later stages' are in flight; the
@@ -197,9 +197,12 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
     __builtin_amdgcn_sched_barrier(0);
     fetch(buf, 0, fa[0], fb[0]);
     if constexpr (!first) multiply(fa[1], fb[1]);            // the last group of the step before
-    __builtin_amdgcn_sched_barrier(0);
-    fetch(buf, 1, fa[1], fb[1]);
-    multiply(fa[0], fb[0]);
+#pragma unroll
+    for (int g = 1; g < G; ++g) {
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(buf, g, fa[g & 1], fb[g & 1]);
+      multiply(fa[(g & 1) ^ 1], fb[(g & 1) ^ 1]);
+    }
     __builtin_amdgcn_sched_barrier(0);
     buf = buf + 1 == C::STAGES ? 0 : buf + 1;
   };
@@ -358,7 +361,8 @@ __device__ __forceinline__ void store_rows(const char* lds, uint16_t* out, int64
     for (int u = 0; u < U; ++u, o += ROWS * ld) {
       if (n0 + n + (s + u) * ROWS >= rows || m >= cols) continue;
       if (wide && m + 8 <= cols) {
-        *reinterpret_cast<i4v*>(o) = v[u];
+        // past the caches' keeping: the next product's operands stay (dh of 4096x32768x1024 233 -> 219 us)
+        __builtin_nontemporal_store(v[u], reinterpret_cast<i4v*>(o));
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -374,18 +378,18 @@ __device__ __forceinline__ void store_columns(const char* lds, uint16_t* out, in
                                               int cols) {
   typedef short s4v __attribute__((ext_vector_type(4)));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
-  // a wave's step: 16 columns m by 32 rows n, 8 rows to a group of 16 lanes
-  constexpr int MB = C::BM / 16, STEPS = MB * (C::BN / 32) / C::NW, U = STEPS % 4 == 0 ? 4 : STEPS;
-  static_assert(STEPS * C::NW == MB * (C::BN / 32), "whole steps");
+  // a wave's step: 16 columns m by 32 rows n, 8 rows to a group of 16 lanes; its steps go along n
+  constexpr int MB = C::BM / 16, NB = C::BN / 32, STEPS = MB * NB / C::NW, U = STEPS % 4 == 0 ? 4 : STEPS;
+  static_assert(STEPS * C::NW == MB * NB, "whole steps");
   for (int s = 0; s < STEPS; s += U) {
     u2v two[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int x = (s + u) * C::NW + wave;
+      const int x = wave * STEPS + s + u;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int nr = (x / MB) * 32 + g * 8 + 4 * k + (i >> 2);
-        const int c = (x % MB) * 2 + ((i >> 1) & 1);
+        const int nr = (x % NB) * 32 + g * 8 + 4 * k + (i >> 2);
+        const int c = (x / NB) * 2 + ((i >> 1) & 1);
         const char* p = lds + nr * (C::BM * 2) + ((c ^ turn<C>(nr)) * 16) + 8 * (i & 1);
         two[u][k] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                 (__attribute__((address_space(3))) s4v*)(const_cast<char*>(p))));
@@ -393,7 +397,7 @@ __device__ __forceinline__ void store_columns(const char* lds, uint16_t* out, in
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int x = (s + u) * C::NW + wave, m = m0 + (x % MB) * 16 + i, n = n0 + (x / MB) * 32 + g * 8;
+      const int x = wave * STEPS + s + u, m = m0 + (x / NB) * 16 + i, n = n0 + (x % NB) * 32 + g * 8;
       if (m < cols && n < rows)
         *reinterpret_cast<i4v*>(out + (int64_t)m * ld + n) =
             i4v{(int)two[u][0][0], (int)two[u][0][1], (int)two[u][1][0], (int)two[u][1][1]};

@@ -144,6 +144,30 @@ def test_several_pieces_of_the_vocabulary(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_long_rows_of_many_tokens(dtype):
+    """Sizes at which every product takes its largest tile, ragged on all sides."""
+    N, V, D = 4090, 8190, 2052
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w, t = inputs(N, V, D, dtype)
+    h.requires_grad_()
+    w.requires_grad_()
+    g = (torch.rand(N, device=DEV) + 0.5) * (64 if dtype == torch.float16 else 1)
+    ref = reference(h.detach(), w.detach(), t, g)
+    b = bounds(ref, dtype, N, V, D)
+    loss = lce(h, w, t, reduction="none")
+    within(loss.detach(), ref["loss"], b["loss"], "loss")
+    dh, dw = torch.autograd.grad(loss, (h, w), g)
+    within(dh, ref["dh"], b["dh"], "dh")
+    within(dw, ref["dw"], b["dw"], "dw")
+    # the elementwise bounds are worst cases of 2052 terms; in the mean the roundings are random: a gradient's
+    # norm is off by its two roundings to 16 bits (dl's and its own), each eps / 2 / sqrt(3) rms at most, fp32's by
+    # the sums' (a walk of 2^-24 steps over up to 8190 terms: 6e-6)
+    tol = 6e-6 if dtype == torch.float32 else 2 * torch.finfo(dtype).eps / 2 / 3 ** 0.5
+    for got, want in ((dh, ref["dh"]), (dw, ref["dw"])):
+        assert float((got.double() - want).norm() / want.norm()) < tol
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_ignored_rows_may_hold_anything(dtype):
     N, V, D = 70, 300, 64
     lce = pkg_mod("vocab_loss").linear_cross_entropy
