@@ -185,6 +185,25 @@ def load():
     return lib
 
 
+_head = None
+
+
+def head():
+    """The compiled binding of the large-vocabulary head's operators (csrc/head_binding.cpp),
+    calling the library that load() loaded."""
+    global _head
+    if _head is None:
+        load()
+        try:
+            from . import _head as m
+        except ImportError as e:
+            raise ImportError("_head.so is not built for this torch (%s); run `python -c 'import __graft_entry__ "
+                              "as g; g.build()'` or `make -C csrc`" % e)
+        m.bind(LIB_PATH)
+        _head = m
+    return _head
+
+
 def symbols():
     return sorted(list(_SIGS) + ["po_last_error"])
 

@@ -114,25 +114,7 @@ def int8_matmul(q, scale, wq, wscale, bias=None, dtype=torch.bfloat16):
 
 def int8_linear(x, wq, wscale, bias=None):
     """A linear layer in 8 bits: x [..., K] quantised row by row, times wq [out, K], in x's type."""
-    if not isinstance(x, torch.Tensor) or x.dtype not in nat.DTYPES or x.dim() < 1:
-        raise TypeError("int8_linear: x must be a float32, float16 or bfloat16 tensor of rows")
-    K = x.shape[-1]
-    _check_inner("int8_linear", K)
-    _no_grad("int8_linear", x, wscale, bias)
-    _check_weights("int8_linear", K, wq, wscale, bias)
-    with nat.device_of(*((x, wq, wscale) if bias is None else (x, wq, wscale, bias))):
-        m, ldx = nat.rows2d(x)
-        M, N = m.shape[0], wq.shape[0]
-        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
-        if M:
-            w, ldw = _weights(wq)
-            ws = torch.empty(M * ((K + 63) // 64 * 64 + 4), dtype=torch.uint8, device=x.device)
-            wscale = wscale.contiguous()
-            bias = None if bias is None else bias.contiguous()
-            nat.call("po_int8_linear", m.data_ptr(), ldx, w.data_ptr(), ldw, wscale.data_ptr(),
-                     None if bias is None else bias.data_ptr(), M, N, K, ws.data_ptr(), ws.numel(), y.data_ptr(), N,
-                     nat.DTYPES[x.dtype], nat.raw_stream(x))
-    return y
+    return nat.head().int8_linear(x, wq, wscale, bias)
 
 
 class Int8Linear(nn.Module):

@@ -294,6 +294,17 @@ def test_infinite_logits_are_what_the_formula_says():
     assert torch.isnan(lce(h, torch.full_like(w, -float("inf")), t, reduction="none")).all()
 
 
+def test_gradients_of_second_order_are_refused():
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w, t = inputs(9, 30, 16, torch.float32)
+    h.requires_grad_()
+    first = torch.autograd.grad(lce(h, w, t), h)[0]
+    (dh,) = torch.autograd.grad(lce(h, w, t), h, create_graph=True)
+    assert torch.equal(dh, first)               # the first order itself is there
+    with pytest.raises(RuntimeError, match="second order"):
+        torch.autograd.grad(dh.sum(), h)
+
+
 @pytest.mark.parametrize("N", [7, 200])
 def test_gradient_against_differences(N):
     """(L(h + e u) - L(h - e u)) / 2e = dh . u + e^2 / 6 L'''; with a = max |w . u| the third cumulant is
