@@ -286,7 +286,7 @@ inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipSt
 
 // ---- which tile ----------------------------------------------------------
 // Three tiles: LARGE 256 x 256 (one workgroup of 8 waves to a CU), MID 128 x 128
-// (two of 4 waves), FEW 128 x 32 for up to 32 columns.  The choice is the least time over
+// (two of 4 waves), FEW 128 x 32 for few columns or few tiles (two of 4 waves).  The choice is the least time over
 // the rounds in which the chip takes the tiles, from what a step of k takes a workgroup
 // (us, measured: LARGE 1.7, MID 1.08 with two on the CU) and what its start and its
 // epilogue take (the epilogue's; MID's are covered by the other workgroup).  So LARGE is
@@ -309,11 +309,11 @@ inline Plan plan_product(int64_t M, int64_t N, int64_t steps, double ends_mid, d
   Plan best{LARGE, 1};
   double least = 1e300;
   for (auto& k : kinds) {
-    if ((k.id == FEW) != (N <= 32)) continue;
     const int64_t tiles = ((M + k.bm - 1) / k.bm) * ((N + k.bn - 1) / k.bn);
     for (int s = 1; s <= max_slices && (s == 1 || steps / s >= 4); ++s) {
       const int64_t rounds = (tiles * s + k.slots - 1) / k.slots;
-      const double t = rounds * ((double)((steps + s - 1) / s) * k.step + k.ends) + s * sum_us;
+      const double step = k.id != LARGE && tiles * s <= 256 ? 0.65 * k.step : k.step;   // one to a CU
+      const double t = rounds * ((double)((steps + s - 1) / s) * step + k.ends) + s * sum_us;
       if (t < least) least = t, best = Plan{k.id, s};
     }
   }

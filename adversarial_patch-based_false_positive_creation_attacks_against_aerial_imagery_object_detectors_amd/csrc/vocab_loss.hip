@@ -54,6 +54,29 @@ __device__ __forceinline__ float column_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+// The rows' upstream gradients.  Of a sum or a mean there is one, and what the rows need of it
+// is made where it is used; of single losses (each) grad_rows_k makes ratio and factor.
+struct GradOf {
+  const float *grad, *count;
+  const int64_t* target;
+  int64_t ignore, V;
+  int each, mean;
+  float lift, c;
+  const float *ratio, *factor;
+  // g_n over the largest |g|, times the lift of fp16; 0: the row takes no part; NaN: its target is none
+  __device__ __forceinline__ float of_row(int n) const {
+    if (each) return ratio[n];
+    const int64_t t = target[n];
+    const float g = *grad;
+    return t == ignore || g == 0.f ? 0.f : t < 0 || t >= V || g != g ? __uint_as_float(0x7fc00000u) : copysignf(lift, g);
+  }
+  __device__ __forceinline__ bool live(int n) const { return each ? ratio[n] != 0.f : target[n] != ignore && *grad != 0.f; }
+  // what the products' sums are multiplied with in the end
+  __device__ __forceinline__ float end() const {
+    return each ? *factor : fabsf(*grad) / (mean ? fmaxf(*count, 1.f) : 1.f) / lift * c;
+  }
+};
+
 // ---- epilogues -----------------------------------------------------------
 
 // partial[tile][n] = {max of l * log2e, sum of 2^(l * log2e - max)} over the tile's vocabulary rows
@@ -61,6 +84,7 @@ struct StatsEpi {
   static constexpr double kMid = 3, kLarge = 5.5;            // us, see plan_product
   struct Args {
     float2* partial;
+    uint32_t* arrived;          // of row_stats_k, which follows: set to 0
     float* tlogit;              // l / c of the target
     const int64_t* target;
     int64_t v0;                 // vocabulary row of A's first
@@ -83,6 +107,7 @@ struct StatsEpi {
   static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, const Pre<C>& pre, char* lds) {
     float2* mine = reinterpret_cast<float2*>(lds);          // [WM][BN]
     const int quad = t.lane >> 4;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *e.arrived = 0;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
@@ -160,8 +185,7 @@ struct DlogitsEpi {
   static constexpr double kMid = 6 * PLANES, kLarge = 15 * PLANES;
   struct Args {
     const float2* stat;         // {max * log2e, 1 / sum} of a token
-    const float* ratio;         // g_n over the largest |g|, times the lift of fp16; 0: the row takes no part
-    const int64_t* target;
+    GradOf g;
     int64_t v0;
     int N, Np, V, Vp;           // tokens and vocabulary rows of the piece, and both as laid out
     float k;
@@ -179,8 +203,8 @@ struct DlogitsEpi {
         const int n = t.col(j);
         const bool in = n < e.N;
         stat[j] = in ? e.stat[n] : make_float2(0.f, 0.f);
-        ratio[j] = in ? e.ratio[n] : 0.f;
-        const int64_t r = (in ? e.target[n] : -1) - e.v0 - t.m0;
+        ratio[j] = in ? e.g.of_row(n) : 0.f;
+        const int64_t r = (in ? e.g.target[n] : -1) - e.v0 - t.m0;
         at[j] = r >= 0 && r < C::TM * 16 ? (int)r : -1;
       }
     }
@@ -276,21 +300,21 @@ struct SlabEpi {
   }
 };
 
-// out[n][m] = acc * *factor in the gradients' type (OUT: BF16, F16, or 3: fp32)
+// out[n][m] = acc * g.end() in the gradients' type (OUT: BF16, F16, or 3: fp32)
 template <int OUT>
 struct GradEpi {
   static constexpr double kMid = 9, kLarge = 14;
   struct Args {
     void* out;
     int64_t ld;
-    const float* factor;
+    GradOf g;
     int N, M, wide;             // wide: rows start on 16 bytes
   };
   template <class C>
   using Pre = NoPre;
   template <class C>
   static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, const Pre<C>& pre, char* lds) {
-    const float f = *e.factor;
+    const float f = e.g.end();
     if constexpr (OUT == 3) {
 #pragma unroll
       for (int j = 0; j < C::TN; ++j) {
@@ -327,15 +351,34 @@ struct GradEpi {
 
 // ---- the rows' kernels ---------------------------------------------------
 
-// Rows' statistics from the tiles': R rows to a workgroup, 256 / R lanes to a
-// row (many rows: neighbouring lanes read neighbouring rows; one row: all lanes
-// share its tiles).
+__device__ __forceinline__ double block_sum(double x, double* red) {
+  red[threadIdx.x] = x;
+  __syncthreads();
+#pragma unroll
+  for (int w = 128; w; w >>= 1) {
+    if (threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+    __syncthreads();
+  }
+  const double r = red[0];
+  __syncthreads();
+  return r;
+}
+
+// Rows' statistics and losses from the tiles': R rows to a workgroup, 256 / R lanes to a row
+// (many rows: neighbouring lanes read neighbouring rows; one row: all lanes share its tiles).
+// total: also the sum (mean: over the rows that count) of the losses, and those rows' number.
+// Each workgroup publishes its rows' sum past its XCD's cache (agent-scope stores, drained
+// before it counts itself in); the one that arrives last adds them up in order.  A launch of
+// its own for that took 3 us.
 template <int R>
 __global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ partial, int parts, int N, int64_t V,
                                                    const float* __restrict__ tlogit, const int64_t* __restrict__ target,
                                                    int64_t ignore, float k, float2* __restrict__ stat,
-                                                   float* __restrict__ loss) {
+                                                   float* __restrict__ loss, double* sums, uint32_t* arrived, int mean,
+                                                   float* __restrict__ total, float* __restrict__ count) {
   __shared__ float2 red[256];
+  __shared__ double dred[256];
+  __shared__ uint32_t order;
   const int row = threadIdx.x % R, n = blockIdx.x * R + row;
   float m = -INFINITY, s = 0.f;
   if (n < N)
@@ -356,57 +399,48 @@ __global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ pa
     }
     __syncthreads();
   }
+  float l = 0.f;
+  bool counts = false;
   if (threadIdx.x < R && n < N) {
     const float2 r = red[threadIdx.x];
     const int64_t t = target[n];
+    counts = t != ignore;
     stat[n] = make_float2(r.x, 1.f / r.y);
     // log(sum) - (l_t - max): the maximum leaves before anything is rounded to its size
-    loss[n] = t == ignore ? 0.f
-              : t < 0 || t >= V ? __uint_as_float(0x7fc00000u)
-                                : kLn2 * (__builtin_log2f(r.y) - __builtin_fmaf(tlogit[n], k, -r.x));
+    l = !counts ? 0.f
+        : t < 0 || t >= V ? __uint_as_float(0x7fc00000u)
+                          : kLn2 * (__builtin_log2f(r.y) - __builtin_fmaf(tlogit[n], k, -r.x));
+    if (loss) loss[n] = l;
   }
-}
-
-__device__ __forceinline__ double block_sum(double x) {
-  __shared__ double red[1024];
-  red[threadIdx.x] = x;
-  __syncthreads();
-  for (int w = 512; w; w >>= 1) {
-    if (threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
-    __syncthreads();
-  }
-  const double r = red[0];
-  __syncthreads();
-  return r;
-}
-
-// *out = the sum (mean: over the rows that count) of the rows' losses; *count = those rows
-__global__ __launch_bounds__(1024) void total_loss_k(const float* __restrict__ loss, const int64_t* __restrict__ target,
-                                                     int N, int64_t ignore, int mean, float* __restrict__ out,
-                                                     float* __restrict__ count) {
-  double s = 0, c = 0;
-  for (int n = threadIdx.x; n < N; n += 1024) {
-    s += loss[n];
-    c += target[n] != ignore;
-  }
-  s = block_sum(s);
-  c = block_sum(c);
+  if (!total) return;
+  const double sum = block_sum(l, dred), num = block_sum(counts, dred);
   if (threadIdx.x == 0) {
-    *out = (float)(mean ? s / c : s);
+    __hip_atomic_store(sums + 2 * blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(sums + 2 * blockIdx.x + 1, num, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    order = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (order != gridDim.x - 1) return;
+  double a = 0, c = 0;
+  for (int b = threadIdx.x; b < gridDim.x; b += 256) {
+    a += __hip_atomic_load(sums + 2 * b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    c += __hip_atomic_load(sums + 2 * b + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  a = block_sum(a, dred);
+  c = block_sum(c, dred);
+  if (threadIdx.x == 0) {
+    *total = (float)(mean ? a / c : a);
     *count = (float)c;
   }
 }
 
-// ratio[n] = g_n / max |g| * lift (0: the row takes no part), *factor = max |g| / lift * c
-__global__ __launch_bounds__(1024) void grad_rows_k(const float* __restrict__ grad, int each, int mean,
-                                                    const float* __restrict__ count, const int64_t* __restrict__ target,
-                                                    int N, int64_t V, int64_t ignore, float lift, float c,
-                                                    float* __restrict__ ratio, float* __restrict__ factor) {
+// ratio[n] and *factor (GradOf) of single losses' gradients: relative to the largest |g|
+__global__ __launch_bounds__(1024) void grad_rows_k(const GradOf g, int N, float* __restrict__ ratio, float* __restrict__ factor) {
   __shared__ float red[1024];
-  const float over = mean ? *count : 1.f;
   float top = 0.f;
   for (int n = threadIdx.x; n < N; n += 1024)
-    if (target[n] != ignore) top = fmaxf(top, fabsf(each ? grad[n] : *grad));
+    if (g.target[n] != g.ignore) top = fmaxf(top, fabsf(g.grad[n]));
   red[threadIdx.x] = top;
   __syncthreads();
   for (int w = 512; w; w >>= 1) {
@@ -415,25 +449,33 @@ __global__ __launch_bounds__(1024) void grad_rows_k(const float* __restrict__ gr
   }
   top = red[0];
   for (int n = threadIdx.x; n < N; n += 1024) {
-    const int64_t t = target[n];
-    const float g = each ? grad[n] : *grad;
-    ratio[n] = t == ignore ? 0.f : t < 0 || t >= V ? __uint_as_float(0x7fc00000u) : g == 0.f ? 0.f : g / top * lift;
+    const int64_t t = g.target[n];
+    const float x = g.grad[n];
+    ratio[n] = t == g.ignore ? 0.f : t < 0 || t >= g.V ? __uint_as_float(0x7fc00000u) : x == 0.f ? 0.f : x / top * g.lift;
   }
-  if (threadIdx.x == 0) *factor = top > 0.f ? top / over / lift * c : 0.f;
+  if (threadIdx.x == 0) *factor = top > 0.f ? top / g.lift * g.c : 0.f;
 }
 
 // Rows laid out for the products: 16-bit rows padded with zeros to ldo (a multiple of 8), or
-// fp32 as planes of three bf16.  A thread makes 8 columns.
+// fp32 as planes of three bf16.  A thread makes 8 columns.  Two matrices in one launch.
+struct PackJob {
+  const void* x;
+  int64_t ld, rows, plane;
+  uint16_t* out;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void pack_k(const T* __restrict__ x, int64_t ld, int64_t rows, int cols,
-                                              uint16_t* __restrict__ out, int ldo, int64_t plane) {
+__global__ __launch_bounds__(256) void pack_k(const PackJob j0, const PackJob j1, int cols, int ldo) {
   typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
   const int per = ldo / 8;
-  const int64_t total = rows * per;
+  const int64_t total = (j0.rows + j1.rows) * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per;
+    int64_t r = i / per;
     const int c = (int)(i - r * per) * 8;
-    const T* p = x + r * ld + c;
+    const bool second = r >= j0.rows;
+    if (second) r -= j0.rows;
+    const int64_t plane = second ? j1.plane : j0.plane;
+    const T* p = static_cast<const T*>(second ? j1.x : j0.x) + r * (second ? j1.ld : j0.ld) + c;
+    uint16_t* const out = second ? j1.out : j0.out;
     v8 v;
     if (c + 8 <= cols) {
       v = *reinterpret_cast<const v8*>(p);
@@ -469,26 +511,33 @@ __global__ __launch_bounds__(256) void pack_k(const T* __restrict__ x, int64_t l
   }
 }
 
-// out[c][r] = x[r][c] (16 bits) for r < Rp (a multiple of 8): zero for r >= R and for rows whose ratio is 0
-// (they may hold anything and multiply zeros only).  x: rows on 16 bytes, readable to the next multiple of 8
+// out[c][r] = x[r][c] (16 bits) for r < Rp (a multiple of 8): zero for r >= R and, masked, for rows that take
+// no part (they may hold anything and multiply zeros only).  Two matrices of one width in one launch.  x: rows on 16 bytes, readable to the next multiple of 8
 // columns.  64 rows x 256 columns to a workgroup, through LDS as a product's outputs; blockIdx.z: plane.
 struct Pane {
   static constexpr int BM = 256, BN = 64, NW = 4;
 };
-__global__ __launch_bounds__(256) void transpose_k(const uint16_t* __restrict__ x, int64_t ld, int64_t plane, int R,
-                                                   int Cc, const float* __restrict__ ratio, uint16_t* __restrict__ out,
-                                                   int64_t ldo, int64_t oplane, int Rp) {
+struct TransposeJob {
+  const uint16_t* x;
+  int64_t ld, plane;
+  int R, Rp, masked;            // masked: rows that take no part are zero
+  uint16_t* out;
+  int64_t ldo, oplane;
+};
+__global__ __launch_bounds__(256) void transpose_k(const TransposeJob j0, const TransposeJob j1, int blocks0, int Cc,
+                                                   const GradOf g) {
   __shared__ __attribute__((aligned(16))) char lds[Pane::BM * Pane::BN * 2];
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 256;
-  x += blockIdx.z * plane;
-  out += blockIdx.z * oplane;
+  const bool second = (int)blockIdx.x >= blocks0;
+  const TransposeJob& j = second ? j1 : j0;
+  const int r0 = ((int)blockIdx.x - (second ? blocks0 : 0)) * 64, c0 = blockIdx.y * 256;
+  const uint16_t* x = j.x + blockIdx.z * j.plane;
   const int c = threadIdx.x % 32, cc = c0 + c * 8;
   i4v v[8];
 #pragma unroll
   for (int s = 0; s < 8; ++s) {
     const int r = r0 + threadIdx.x / 32 + s * 8;
-    const bool ok = r < R && cc < Cc && (!ratio || ratio[r] != 0.f);
-    v[s] = ok ? *reinterpret_cast<const i4v*>(x + r * ld + cc) : i4v{0, 0, 0, 0};
+    const bool ok = r < j.R && cc < Cc && (!j.masked || g.live(r));
+    v[s] = ok ? *reinterpret_cast<const i4v*>(x + r * j.ld + cc) : i4v{0, 0, 0, 0};
   }
 #pragma unroll
   for (int s = 0; s < 8; ++s) {
@@ -496,15 +545,14 @@ __global__ __launch_bounds__(256) void transpose_k(const uint16_t* __restrict__ 
     *reinterpret_cast<i4v*>(lds + n * 512 + ((c ^ turn<Pane>(n)) * 16)) = v[s];
   }
   __syncthreads();
-  store_columns<Pane>(lds, out, ldo, r0, c0, Rp, Cc);
+  store_columns<Pane>(lds, j.out + blockIdx.z * j.oplane, j.ldo, r0, c0, j.Rp, Cc);
 }
 
-// dh[n][m] = factor * the slabs' sum, slab after slab; a thread makes 4 columns
+// dh[n][m] = g.end() * the slabs' sum, slab after slab; a thread makes 4 columns
 template <int OUT>
 __global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab, int slices, int64_t slice, int64_t ld,
-                                                  int N, int M, const float* __restrict__ factor, void* __restrict__ out,
-                                                  int64_t ldo, int wide) {
-  const float f = *factor;
+                                                  int N, int M, const GradOf g, void* __restrict__ out, int64_t ldo, int wide) {
+  const float f = g.end();
   const int per = (int)(ld / 4);
   const int64_t total = (int64_t)N * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
@@ -586,7 +634,9 @@ inline int64_t piece_rows(int64_t V, int64_t per_row) {
 
 struct FwdWs {
   float2* partial;
-  float *tlogit, *rowloss;
+  double* sums;
+  uint32_t* arrived;
+  float* tlogit;
   uint16_t *hp, *wp;
   int64_t piece, bytes;
   int parts;
@@ -598,7 +648,8 @@ struct FwdWs {
     for (int64_t v = 0; v < s.V; v += piece) parts += ceil_div(std::min(piece, s.V - v), 128);
     partial = l.take<float2>((int64_t)parts * s.N);
     tlogit = l.take<float>(s.N);
-    rowloss = l.take<float>(s.N);
+    sums = l.take<double>(2 * s.N);
+    arrived = l.take<uint32_t>(1);
     hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.Dp() * s.planes());
     wp = l.take<uint16_t>(piece * wrow / 2);
     bytes = l.at;
@@ -612,6 +663,7 @@ struct BwdWs {
   uint16_t *hp, *ht, *wp, *wt, *dl, *dlt;
   int64_t piece, ldl, slab_ld, slab_slice, bytes;
   Plan dh_plan;
+  bool direct_dh;               // one piece in one slice: dh leaves the product as it is wanted
   BwdWs(const Shape& s, bool dh, bool dw, void* b) {
     Layout l(b);
     const int P = s.planes();
@@ -631,7 +683,8 @@ struct BwdWs {
     // a slice's sums are written and read once: 8 bytes of each at about 4 TB/s
     dh_plan = plan_product(s.D, s.N, (int64_t)ceil_div(ldl * 2, 128) * (P == 3 ? 6 : 1),
                            SlabEpi::kMid, SlabEpi::kLarge, kSlabSlices, slab_slice * 8 / 4e6);
-    slab = l.take<float>(dh ? dh_plan.slices * slab_slice : 0);
+    direct_dh = piece >= s.V && dh_plan.slices == 1;
+    slab = l.take<float>(dh && !direct_dh ? dh_plan.slices * slab_slice : 0);
     bytes = l.at;
   }
 };
@@ -643,25 +696,32 @@ inline void set_pairs(Args& a, int planes) {
   a.pb = planes == 3 ? 0x021010u : 0u;
 }
 
-template <typename T>
-inline void pack(const void* x, int64_t ld, int64_t rows, int cols, uint16_t* out, int ldo, hipStream_t s) {
-  const int grid = (int)std::min<int64_t>((rows * (ldo / 8) + 255) / 256, 8192);
-  if (grid > 0)
-    hipLaunchKernelGGL((pack_k<T>), dim3(grid), dim3(256), 0, s, static_cast<const T*>(x), ld, rows, cols, out, ldo,
-                       rows * ldo);
+// operand rows [r0, r0 + rows) of the caller's matrix, or of buf where they do not serve as they are
+struct Side {
+  const void* x;
+  int64_t ld;
+  bool direct;
+  uint16_t* buf;
+};
+inline Operand rows_of(const Shape& s, const Side& m, int64_t r0, int64_t rows) {
+  if (m.direct) return Operand{static_cast<const char*>(m.x) + r0 * m.ld * 2, m.ld * 2, 0, (int)rows};
+  return Operand{reinterpret_cast<char*>(m.buf), (int64_t)s.Dp() * 2, rows * s.Dp() * 2, (int)rows};
 }
-
-// operand rows [r0, r0 + rows) of the caller's matrix, packed into buf where they do not serve as they are
-inline Operand rows_of(const Shape& s, bool direct, const void* x, int64_t ld, int64_t r0, int64_t rows, uint16_t* buf,
-                       hipStream_t st) {
+// lays them out there, h's rows (0: not this time) and w's in one launch
+inline void pack(const Shape& s, const Side& h, int64_t hrows, const Side& w, int64_t w0, int64_t wrows, hipStream_t st) {
   const int es = s.dtype == PO_F32 ? 4 : 2;
-  const char* p = static_cast<const char*>(x) + r0 * ld * es;
-  if (direct) return Operand{p, ld * 2, 0, (int)rows};
+  auto job = [&](const Side& m, int64_t r0, int64_t rows) {
+    if (m.direct) rows = 0;
+    return PackJob{static_cast<const char*>(m.x) + r0 * m.ld * es, m.ld, rows, rows * s.Dp(), m.buf};
+  };
+  const PackJob a = job(h, 0, hrows), b = job(w, w0, wrows);
+  const int64_t items = (a.rows + b.rows) * (s.Dp() / 8);
+  if (!items) return;
+  const dim3 grid((unsigned)std::min<int64_t>((items + 255) / 256, 8192));
   if (s.dtype == PO_F32)
-    pack<float>(p, ld, rows, (int)s.D, buf, s.Dp(), st);
+    hipLaunchKernelGGL((pack_k<float>), grid, dim3(256), 0, st, a, b, (int)s.D, s.Dp());
   else
-    pack<uint16_t>(p, ld, rows, (int)s.D, buf, s.Dp(), st);
-  return Operand{reinterpret_cast<char*>(buf), (int64_t)s.Dp() * 2, rows * s.Dp() * 2, (int)rows};
+    hipLaunchKernelGGL((pack_k<uint16_t>), grid, dim3(256), 0, st, a, b, (int)s.D, s.Dp());
 }
 
 inline bool serves(const void* x, int64_t ld, int dtype, int64_t D) {
@@ -721,11 +781,13 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
   Args a{};
   set_pairs(a, s.planes());
   a.kbytes = s.Dp() * 2;
-  a.B = rows_of(s, s.direct_h, h, ldh, 0, N, ws.hp, st);
-  StatsEpi::Args e{ws.partial, ws.tlogit, target, 0, 0, (int)N, 0, scale * kLog2e};
+  const Side hs{h, ldh, s.direct_h, ws.hp}, wside{w, ldw, s.direct_w, ws.wp};
+  a.B = rows_of(s, hs, 0, N);
+  StatsEpi::Args e{ws.partial, ws.arrived, ws.tlogit, target, 0, 0, (int)N, 0, scale * kLog2e};
   for (int64_t v = 0; v < V; v += ws.piece) {
     const int64_t rows = std::min(ws.piece, V - v);
-    a.A = rows_of(s, s.direct_w, w, ldw, v, rows, ws.wp, st);
+    pack(s, hs, v ? 0 : N, wside, v, rows, st);
+    a.A = rows_of(s, wside, v, rows);
     e.v0 = v;
     e.V = (int)rows;
     const Plan p = plan_of<StatsEpi>(a);
@@ -733,75 +795,70 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
                             : launch_planned<BF16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")));
     e.tile0 += ceil_div(rows, p.tile == LARGE ? 256 : 128);
   }
-  float* rows = reduction ? ws.rowloss : loss;
-  float2* stat2 = reinterpret_cast<float2*>(stat);
-  if (N >= 2048)
-    hipLaunchKernelGGL((row_stats_k<16>), dim3(ceil_div(N, 16)), dim3(256), 0, st, ws.partial, e.tile0, (int)N, V,
-                       ws.tlogit, target, ignore_index, e.k, stat2, rows);
-  else
-    hipLaunchKernelGGL((row_stats_k<1>), dim3((unsigned)N), dim3(256), 0, st, ws.partial, e.tile0, (int)N, V, ws.tlogit,
-                       target, ignore_index, e.k, stat2, rows);
-  if (reduction)
-    hipLaunchKernelGGL(total_loss_k, dim3(1), dim3(1024), 0, st, rows, target, (int)N, ignore_index, reduction == 2,
-                       loss, count);
+  const bool many = N >= 2048;
+  hipLaunchKernelGGL((many ? row_stats_k<16> : row_stats_k<1>), dim3(many ? ceil_div(N, 16) : (unsigned)N), dim3(256), 0, st,
+                     ws.partial, e.tile0, (int)N, V, ws.tlogit, target, ignore_index, e.k, reinterpret_cast<float2*>(stat),
+                     reduction ? nullptr : loss, ws.sums, ws.arrived, reduction == 2, reduction ? loss : nullptr, count);
   return po::check_launch("po_linear_ce_fwd");
 }
 
 namespace {
 
 template <int KIND, int OUT>
-int backward(const Shape& s, const BwdWs& ws, const void* h, int64_t ldh, const void* w, int64_t ldw,
-             const int64_t* target, float scale, const float2* stat, void* dh, int64_t lddh, void* dw, int64_t lddw,
-             hipStream_t st) {
-  constexpr int P = OUT == 3 ? 3 : 1;
+int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, const GradOf& g, float scale,
+             const float2* stat, void* dh, int64_t lddh, void* dw, int64_t lddw, hipStream_t st) {
+  constexpr int P = OUT == 3 ? 3 : 1, es = OUT == 3 ? 4 : 2;
   const char* what = "po_linear_ce_bwd";
   const int N = (int)s.N, D = (int)s.D;
-  const Operand H = rows_of(s, s.direct_h, h, ldh, 0, N, ws.hp, st);
-  if (dw)
-    hipLaunchKernelGGL(transpose_k, dim3(ceil_div(s.Np(), 64), ceil_div(D, 256), P), dim3(256), 0, st,
-                       reinterpret_cast<const uint16_t*>(H.p), H.stride / 2, H.plane / 2, N, D, ws.ratio, ws.ht,
-                       s.ldn(), D * s.ldn(), (int)s.Np());
+  const Operand H = rows_of(s, h, 0, N);
   for (int64_t v = 0; v < s.V; v += ws.piece) {
     const int rows = (int)std::min(ws.piece, s.V - v);
     const int rp = (rows + 63) / 64 * 64;
-    const Operand W = rows_of(s, s.direct_w, w, ldw, v, rows, ws.wp, st);
+    const Operand W = rows_of(s, w, v, rows);
+    pack(s, h, v ? 0 : N, w, v, rows, st);
     Args a{};
     set_pairs(a, P);
     // dl of the piece
     a.A = W;
     a.B = H;
     a.kbytes = s.Dp() * 2;
-    typename DlogitsEpi<KIND, P>::Args e{stat, ws.ratio, target, v, N, (int)s.Np(), rows, rp, scale * kLog2e,
-                                         dh ? ws.dl : nullptr, dw ? ws.dlt : nullptr, ws.ldl, s.ldn(), N * ws.ldl,
-                                         ws.piece * s.ldn()};
+    typename DlogitsEpi<KIND, P>::Args e{stat, g, v, N, (int)s.Np(), rows, rp, scale * kLog2e, dh ? ws.dl : nullptr,
+                                         dw ? ws.dlt : nullptr, ws.ldl, s.ldn(), N * ws.ldl, ws.piece * s.ldn()};
     PO_TRY((launch_planned<KIND, DlogitsEpi<KIND, P>>(a, e, plan_of<DlogitsEpi<KIND, P>>(a), st, what)));
-    if (dh) {                                                // slab[n][d] += sum_v dl[n][v] w[v][d]
-      hipLaunchKernelGGL(transpose_k, dim3(ceil_div(rp, 64), ceil_div(D, 256), P), dim3(256), 0, st,
-                         reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, D,
-                         (const float*)nullptr, ws.wt, ws.ldl, D * ws.ldl, rp);
+    // the piece's w, and once h, the other way round
+    const TransposeJob tw{reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, rp, 0, ws.wt, ws.ldl, D * ws.ldl};
+    const TransposeJob th{reinterpret_cast<const uint16_t*>(H.p), H.stride / 2, H.plane / 2, N, (int)s.Np(), 1, ws.ht, s.ldn(), D * s.ldn()};
+    const int bw = dh ? ceil_div(rp, 64) : 0, bh = dw && !v ? ceil_div(s.Np(), 64) : 0;
+    if (bw + bh)
+      hipLaunchKernelGGL(transpose_k, dim3(bw + bh, ceil_div(D, 256), P), dim3(256), 0, st, tw, th, bw, D, g);
+    if (dh) {                                                // sums over v of dl[n][v] w[v][d]
       a.A = Operand{reinterpret_cast<char*>(ws.wt), ws.ldl * 2, D * ws.ldl * 2, D};
       a.B = Operand{reinterpret_cast<char*>(ws.dl), ws.ldl * 2, N * ws.ldl * 2, N};
       a.kbytes = rp * 2;
-      const SlabEpi::Args se{ws.slab, ws.slab_ld, ws.slab_slice, N, D, v > 0};
       // the last piece may have fewer steps than slices: the other slabs keep their sums
       const Plan p{ws.dh_plan.tile, std::min(ws.dh_plan.slices, ceil_div(a.kbytes, 128) * a.pairs)};
-      PO_TRY((launch_planned<KIND, SlabEpi>(a, se, p, st, what)));
+      if (ws.direct_dh) {
+        const typename GradEpi<OUT>::Args ge{dh, lddh, g, N, D, (uintptr_t)dh % 16 == 0 && lddh * es % 16 == 0};
+        PO_TRY((launch_planned<KIND, GradEpi<OUT>>(a, ge, p, st, what)));
+      } else {
+        const SlabEpi::Args se{ws.slab, ws.slab_ld, ws.slab_slice, N, D, v > 0};
+        PO_TRY((launch_planned<KIND, SlabEpi>(a, se, p, st, what)));
+      }
     }
     if (dw) {                                                // dw[v][d] = sum_n dl[n][v] h[n][d]
       a.A = Operand{reinterpret_cast<char*>(ws.ht), s.ldn() * 2, D * s.ldn() * 2, D};
       a.B = Operand{reinterpret_cast<char*>(ws.dlt), s.ldn() * 2, ws.piece * s.ldn() * 2, rows};
       a.kbytes = (int)s.Np() * 2;
-      const int es = OUT == 3 ? 4 : 2;
       char* out = static_cast<char*>(dw) + v * lddw * es;
-      const typename GradEpi<OUT>::Args ge{out, lddw, ws.factor, rows, D, (uintptr_t)out % 16 == 0 && lddw * es % 16 == 0};
+      const typename GradEpi<OUT>::Args ge{out, lddw, g, rows, D, (uintptr_t)out % 16 == 0 && lddw * es % 16 == 0};
       PO_TRY((launch_planned<KIND, GradEpi<OUT>>(a, ge, plan_of<GradEpi<OUT>>(a), st, what)));
     }
   }
-  if (dh) {
+  if (dh && !ws.direct_dh) {
     const int grid = (int)std::min<int64_t>((N * (ws.slab_ld / 4) + 255) / 256, 8192);
-    const int es = OUT == 3 ? 4 : 2, wide = (uintptr_t)dh % 16 == 0 && lddh * es % 16 == 0;
+    const int wide = (uintptr_t)dh % 16 == 0 && lddh * es % 16 == 0;
     hipLaunchKernelGGL((slab_sum_k<OUT>), dim3(grid), dim3(256), 0, st, ws.slab, ws.dh_plan.slices, ws.slab_slice, ws.slab_ld,
-                       N, D, ws.factor, dh, lddh, wide);
+                       N, D, g, dh, lddh, wide);
   }
   return po::check_launch(what);
 }
@@ -824,10 +881,12 @@ extern "C" int po_linear_ce_bwd(const void* h, int64_t ldh, const void* w, int64
   PO_REQUIRE(workspace_bytes >= ws.bytes, "po_linear_ce_bwd: workspace of %lld bytes, %lld needed",
              (long long)workspace_bytes, (long long)ws.bytes);
   const hipStream_t st = po::stream_of(stream);
-  hipLaunchKernelGGL(grad_rows_k, dim3(1), dim3(1024), 0, st, grad, reduction == 0, reduction == 2, count, target, (int)N,
-                     V, ignore_index, dtype == PO_F16 ? kF16Lift : 1.f, scale, ws.ratio, ws.factor);
+  const GradOf g{grad, count, target, ignore_index, V, reduction == 0, reduction == 2, dtype == PO_F16 ? kF16Lift : 1.f, scale,
+                 ws.ratio, ws.factor};
+  if (g.each) hipLaunchKernelGGL(grad_rows_k, dim3(1), dim3(1024), 0, st, g, (int)N, ws.ratio, ws.factor);
   const float2* st2 = reinterpret_cast<const float2*>(stat);
-  if (dtype == PO_F16) return backward<F16, F16>(s, ws, h, ldh, w, ldw, target, scale, st2, dh, lddh, dw, lddw, st);
-  if (dtype == PO_BF16) return backward<BF16, BF16>(s, ws, h, ldh, w, ldw, target, scale, st2, dh, lddh, dw, lddw, st);
-  return backward<BF16, 3>(s, ws, h, ldh, w, ldw, target, scale, st2, dh, lddh, dw, lddw, st);
+  const Side hs{h, ldh, s.direct_h, ws.hp}, wside{w, ldw, s.direct_w, ws.wp};
+  if (dtype == PO_F16) return backward<F16, F16>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
+  if (dtype == PO_BF16) return backward<BF16, BF16>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
+  return backward<BF16, 3>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
 }
