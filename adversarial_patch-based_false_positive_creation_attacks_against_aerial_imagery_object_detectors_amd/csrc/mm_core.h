@@ -66,6 +66,7 @@ struct Operand {
   int64_t stride;   // bytes from row to row (256 rows stay under 2 GiB)
   int64_t plane;    // bytes from plane to plane (operands split into planes)
   int rows;
+  Operand from(int64_t r) const { return Operand{p + r * stride, stride, plane, (int)(rows - r)}; }
 };
 
 constexpr uint32_t kOOB = 0x80000000u;
@@ -298,6 +299,7 @@ enum TileId { FEW, MID, LARGE };
 struct Plan {
   TileId tile;
   int slices;
+  double us;
 };
 inline Plan plan_product(int64_t M, int64_t N, int64_t steps, double ends_mid, double ends_large, int max_slices = 1,
                          double sum_us = 0) {
@@ -306,18 +308,29 @@ inline Plan plan_product(int64_t M, int64_t N, int64_t steps, double ends_mid, d
     int bm, bn, slots;
     double step, ends;
   } const kinds[] = {{FEW, 128, 32, 512, 0.45, 5}, {MID, 128, 128, 512, 1.08, ends_mid}, {LARGE, 256, 256, 256, 1.7, ends_large}};
-  Plan best{LARGE, 1};
-  double least = 1e300;
+  Plan best{LARGE, 1, 1e300};
   for (auto& k : kinds) {
     const int64_t tiles = ((M + k.bm - 1) / k.bm) * ((N + k.bn - 1) / k.bn);
     for (int s = 1; s <= max_slices && (s == 1 || steps / s >= 4); ++s) {
       const int64_t rounds = (tiles * s + k.slots - 1) / k.slots;
       const double step = k.id != LARGE && tiles * s <= 256 ? 0.65 * k.step : k.step;   // one to a CU
       const double t = rounds * ((double)((steps + s - 1) / s) * step + k.ends) + s * sum_us;
-      if (t < least) least = t, best = Plan{k.id, s};
+      if (t < best.us) best = Plan{k.id, s, t};
     }
   }
   return best;
+}
+
+// Rows of A (of M) to take first: those of whole rounds of LARGE tiles, where the rest is quicker
+// with tiles of its own than as one more round (the losses of 50001 x 2047 x 1000: 6.1 rounds).
+inline int64_t whole_rounds(int64_t M, int64_t N, int64_t steps, double ends_mid, double ends_large) {
+  const int64_t tn = (N + 255) / 256, full = (M + 255) / 256 * tn / 256, first = full * 256 / tn * 256;
+  if (first <= 0 || first >= M) return M;
+  const double gap = 3;                                      // from one launch to the next
+  return plan_product(first, N, steps, ends_mid, ends_large).us + plan_product(M - first, N, steps, ends_mid, ends_large).us + gap <
+                 plan_product(M, N, steps, ends_mid, ends_large).us
+             ? first
+             : M;
 }
 
 // ---- outputs -------------------------------------------------------------

@@ -182,7 +182,7 @@ struct StatsEpi {
 // dl of a piece of the vocabulary, as [n][v] and as [v][n]; PLANES = 3: as the three bf16 of each number
 template <int KIND, int PLANES>
 struct DlogitsEpi {
-  static constexpr double kMid = 6 * PLANES, kLarge = 15 * PLANES;
+  static constexpr double kMid = 6 * PLANES, kLarge = PLANES > 1 ? 70 : 15;
   struct Args {
     const float2* stat;         // {max * log2e, 1 / sum} of a token
     GradOf g;
@@ -264,9 +264,12 @@ struct DlogitsEpi {
         }
       }
       __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
       const int n0 = t.tn * C::BN, m0 = t.tm * C::BM;
       if (e.dl) store_rows<C>(lds, e.dl + p * e.pl, e.ldl, n0, m0, e.N, e.Vp, true);
+      __builtin_amdgcn_sched_barrier(0);
       if (e.dlt) store_columns<C>(lds, e.dlt + p * e.pt, e.ldt, n0, m0, e.Np, e.V);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -748,6 +751,11 @@ inline Plan plan_of(const Args& a) {
   return plan_product(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs, Epi::kMid, Epi::kLarge);
 }
 
+template <class Epi>
+inline int64_t first_part(const Args& a) {
+  return whole_rounds(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs, Epi::kMid, Epi::kLarge);
+}
+
 #define PO_TRY(x)             \
   do {                        \
     const int rc_ = (x);      \
@@ -787,17 +795,23 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
   for (int64_t v = 0; v < V; v += ws.piece) {
     const int64_t rows = std::min(ws.piece, V - v);
     pack(s, hs, v ? 0 : N, wside, v, rows, st);
-    a.A = rows_of(s, wside, v, rows);
-    e.v0 = v;
-    e.V = (int)rows;
-    const Plan p = plan_of<StatsEpi>(a);
-    PO_TRY((dtype == PO_F16 ? launch_planned<F16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
-                            : launch_planned<BF16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")));
-    e.tile0 += ceil_div(rows, p.tile == LARGE ? 256 : 128);
+    const Operand W = rows_of(s, wside, v, rows);
+    for (int64_t r = 0, part; r < rows; r += part) {
+      a.A = W.from(r);
+      part = first_part<StatsEpi>(a);
+      a.A.rows = (int)part;
+      e.v0 = v + r;
+      e.V = (int)part;
+      const Plan p = plan_of<StatsEpi>(a);
+      PO_TRY((dtype == PO_F16 ? launch_planned<F16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
+                              : launch_planned<BF16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")));
+      e.tile0 += ceil_div(part, p.tile == LARGE ? 256 : 128);
+    }
   }
-  const bool many = N >= 2048;
-  hipLaunchKernelGGL((many ? row_stats_k<16> : row_stats_k<1>), dim3(many ? ceil_div(N, 16) : (unsigned)N), dim3(256), 0, st,
-                     ws.partial, e.tile0, (int)N, V, ws.tlogit, target, ignore_index, e.k, reinterpret_cast<float2*>(stat),
+  // total: few workgroups, since each counts itself in (1000 of them: 20 us, 63: 6)
+  const int R = reduction ? (N <= 64 ? 1 : N <= 512 ? 4 : 16) : N < 2048 ? 1 : 16;
+  hipLaunchKernelGGL((R == 1 ? row_stats_k<1> : R == 4 ? row_stats_k<4> : row_stats_k<16>), dim3(ceil_div(N, R)), dim3(256), 0,
+                     st, ws.partial, e.tile0, (int)N, V, ws.tlogit, target, ignore_index, e.k, reinterpret_cast<float2*>(stat),
                      reduction ? nullptr : loss, ws.sums, ws.arrived, reduction == 2, reduction ? loss : nullptr, count);
   return po::check_launch("po_linear_ce_fwd");
 }
@@ -819,12 +833,18 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
     Args a{};
     set_pairs(a, P);
     // dl of the piece
-    a.A = W;
     a.B = H;
     a.kbytes = s.Dp() * 2;
-    typename DlogitsEpi<KIND, P>::Args e{stat, g, v, N, (int)s.Np(), rows, rp, scale * kLog2e, dh ? ws.dl : nullptr,
-                                         dw ? ws.dlt : nullptr, ws.ldl, s.ldn(), N * ws.ldl, ws.piece * s.ldn()};
-    PO_TRY((launch_planned<KIND, DlogitsEpi<KIND, P>>(a, e, plan_of<DlogitsEpi<KIND, P>>(a), st, what)));
+    for (int64_t r = 0, part; r < rows; r += part) {
+      using E = DlogitsEpi<KIND, P>;
+      a.A = W.from(r);
+      part = first_part<E>(a);
+      a.A.rows = (int)part;
+      const typename E::Args e{stat, g, v + r, N, (int)s.Np(), (int)part, (int)(r + part < rows ? part : rp - r), scale * kLog2e,
+                               dh ? ws.dl + r : nullptr, dw ? ws.dlt + r * s.ldn() : nullptr, ws.ldl, s.ldn(), N * ws.ldl,
+                               ws.piece * s.ldn()};
+      PO_TRY((launch_planned<KIND, E>(a, e, plan_of<E>(a), st, what)));
+    }
     // the piece's w, and once h, the other way round
     const TransposeJob tw{reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, rp, 0, ws.wt, ws.ldl, D * ws.ldl};
     const TransposeJob th{reinterpret_cast<const uint16_t*>(H.p), H.stride / 2, H.plane / 2, N, (int)s.Np(), 1, ws.ht, s.ldn(), D * s.ldn()};
@@ -836,7 +856,7 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
       a.B = Operand{reinterpret_cast<char*>(ws.dl), ws.ldl * 2, N * ws.ldl * 2, N};
       a.kbytes = rp * 2;
       // the last piece may have fewer steps than slices: the other slabs keep their sums
-      const Plan p{ws.dh_plan.tile, std::min(ws.dh_plan.slices, ceil_div(a.kbytes, 128) * a.pairs)};
+      const Plan p{ws.dh_plan.tile, std::min(ws.dh_plan.slices, ceil_div(a.kbytes, 128) * a.pairs), 0};
       if (ws.direct_dh) {
         const typename GradEpi<OUT>::Args ge{dh, lddh, g, N, D, (uintptr_t)dh % 16 == 0 && lddh * es % 16 == 0};
         PO_TRY((launch_planned<KIND, GradEpi<OUT>>(a, ge, p, st, what)));
