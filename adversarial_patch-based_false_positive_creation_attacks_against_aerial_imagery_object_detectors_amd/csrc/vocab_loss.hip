@@ -6,10 +6,10 @@
 //   dh = c * dl w                    dw = c * dl^T h
 //
 // Forward: one product over all of the vocabulary whose epilogue keeps, for
-// each tile of 256 vocabulary rows, the maximum and the sum of the exponentials
+// each tile of vocabulary rows, the maximum and the sum of the exponentials
 // of a token (in 32 bits), and the target's logit.  A tile has the vocabulary as
-// its rows, so a token's values lie in one lane (and its neighbour 32 lanes on)
-// and the reduction stays in registers.  Backward: for one piece of the
+// its rows, so a token's values lie in four lanes, and the reduction stays in
+// registers but for two exchanges.  Backward: for one piece of the
 // vocabulary after the other, the logits again, dl in their place (16 bits, as
 // [n][v] and as [v][n]), then dh += dl w and the piece's rows of dw.  Every
 // product has k contiguous in both operands: w and h are transposed for that.
@@ -21,22 +21,19 @@
 // times 2^14 (at most 2^14, and normal down to 2^-28).  fp32 inputs: each number
 // is the sum of three bf16 (8 + 8 + 8 bits, nearest), and the six leading of the
 // nine products are summed in 32 bits; what is left out is below 2^-24 of a
-// product.  That is six bf16 products (about 200 TFLOP/s of fp32) where the fp32
-// matrix instructions end at 157.
+// product.  That is six bf16 products (220 TFLOP/s of fp32 in the loop) where the
+// fp32 matrix instructions end at 157.
 #include "mm_core.h"
 #include <math.h>
 
 namespace {
 using namespace po::mm;
 using po::ceil_div;
-#ifndef PIECE_MB
-#define PIECE_MB 640
-#endif
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kF16Lift = 16384.f;
 
-// tokens x vocabulary tiles: large, for up to 128 tokens, for up to 32
+// plan_product's tiles
 template <int KIND>
 using Large = Cfg<KIND, 256, 256, 2, 4, 128, 2>;
 template <int KIND>
@@ -459,17 +456,17 @@ __global__ __launch_bounds__(1024) void grad_rows_k(const GradOf g, int N, float
   if (threadIdx.x == 0) *factor = top > 0.f ? top / g.lift * g.c : 0.f;
 }
 
-// Rows laid out for the products: 16-bit rows padded with zeros to ldo (a multiple of 8), or
-// fp32 as planes of three bf16.  A thread makes 8 columns.  Two matrices in one launch.
+// Rows laid out for the products, cols padded with zeros to a multiple of 8, rows ldo apart: 16-bit
+// numbers, or fp32 as planes of three bf16.  A thread makes 8 columns.  Two matrices in one launch.
 struct PackJob {
   const void* x;
   int64_t ld, rows, plane;
   uint16_t* out;
 };
 template <typename T>
-__global__ __launch_bounds__(256) void pack_k(const PackJob j0, const PackJob j1, int cols, int ldo) {
+__global__ __launch_bounds__(256) void pack_k(const PackJob j0, const PackJob j1, int cols, int64_t ldo) {
   typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  const int per = ldo / 8;
+  const int per = (cols + 7) / 8;
   const int64_t total = (j0.rows + j1.rows) * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     int64_t r = i / per;
@@ -515,8 +512,8 @@ __global__ __launch_bounds__(256) void pack_k(const PackJob j0, const PackJob j1
 }
 
 // out[c][r] = x[r][c] (16 bits) for r < Rp (a multiple of 8): zero for r >= R and, masked, for rows that take
-// no part (they may hold anything and multiply zeros only).  Two matrices of one width in one launch.  x: rows on 16 bytes, readable to the next multiple of 8
-// columns.  64 rows x 256 columns to a workgroup, through LDS as a product's outputs; blockIdx.z: plane.
+// no part (they may hold anything and multiply zeros only).  Two matrices of one width in one launch.  x: rows
+// on 16 bytes, readable to the next multiple of 8 columns.  64 rows x 256 columns to a workgroup, through LDS as a product's outputs; blockIdx.z: plane.
 struct Pane {
   static constexpr int BM = 256, BN = 64, NW = 4;
 };
@@ -591,7 +588,10 @@ __global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab
 
 // ---- the plan ------------------------------------------------------------
 
-constexpr int64_t kPieceBytes = (PIECE_MB) * (1LL << 20);   // what a piece of the vocabulary may take of the workspace
+// What a piece of the vocabulary may take of the workspace: 16384 rows of 8192 tokens.  Pieces of
+// 8192, whose gradients would stay in the last-level cache, cost dh more (twice the sums read and
+// written: 486 against 430 us for 16384 rows) than they save elsewhere.
+constexpr int64_t kPieceBytes = 640LL << 20;
 
 // Rows of the operands made here: a multiple of 128 bytes, and long ones no multiple of 512:
 // 256 rows a power of two apart fall on few memory channels (dh of a 16384-row piece
@@ -607,14 +607,15 @@ struct Shape {
   int dtype;
   bool direct_h, direct_w;      // the caller's rows serve as they are
   int planes() const { return dtype == PO_F32 ? 3 : 1; }
-  int Dp() const { return (int)((D + 7) / 8 * 8); }
+  int Dp() const { return (int)((D + 7) / 8 * 8); }     // columns of rows laid out here, zeros past D
+  int64_t ldp() const { return padded(Dp()); }
   int64_t Np() const { return (N + 31) / 32 * 32; }
   int64_t ldn() const { return padded(Np()); }
 };
 
 inline int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 
-// bytes of the workspace as it is laid out by both passes; p: pointers, or sizes from a null base
+// A workspace laid out from its base; from a null base only its size is of use.
 struct Layout {
   char* base;
   int64_t at = 0;
@@ -645,7 +646,7 @@ struct FwdWs {
   int parts;
   FwdWs(const Shape& s, void* b) {
     Layout l(b);
-    const int64_t wrow = s.direct_w ? 0 : (int64_t)s.Dp() * 2 * s.planes();
+    const int64_t wrow = s.direct_w ? 0 : s.ldp() * 2 * s.planes();
     piece = wrow ? piece_rows(s.V, wrow) : s.V;
     parts = 0;
     for (int64_t v = 0; v < s.V; v += piece) parts += ceil_div(std::min(piece, s.V - v), 128);
@@ -653,7 +654,7 @@ struct FwdWs {
     tlogit = l.take<float>(s.N);
     sums = l.take<double>(2 * s.N);
     arrived = l.take<uint32_t>(1);
-    hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.Dp() * s.planes());
+    hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.ldp() * s.planes());
     wp = l.take<uint16_t>(piece * wrow / 2);
     bytes = l.at;
   }
@@ -670,14 +671,14 @@ struct BwdWs {
   BwdWs(const Shape& s, bool dh, bool dw, void* b) {
     Layout l(b);
     const int P = s.planes();
-    const int64_t per = (s.direct_w ? 0 : (int64_t)s.Dp() * 2 * P) + (dh ? (s.N + s.D) * 2 * P : 0) + (dw ? s.Np() * 2 * P : 0);
+    const int64_t per = (s.direct_w ? 0 : s.ldp() * 2 * P) + (dh ? (s.N + s.D) * 2 * P : 0) + (dw ? s.Np() * 2 * P : 0);
     piece = piece_rows(s.V, per);
     ldl = padded(piece);
     ratio = l.take<float>(s.N);
     factor = l.take<float>(1);
-    hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.Dp() * P);
+    hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.ldp() * P);
     ht = l.take<uint16_t>(dw ? s.D * s.ldn() * P : 0);
-    wp = l.take<uint16_t>(s.direct_w ? 0 : piece * s.Dp() * P);
+    wp = l.take<uint16_t>(s.direct_w ? 0 : piece * s.ldp() * P);
     wt = l.take<uint16_t>(dh ? s.D * ldl * P : 0);
     dl = l.take<uint16_t>(dh ? s.N * ldl * P : 0);
     dlt = l.take<uint16_t>(dw ? piece * s.ldn() * P : 0);
@@ -708,23 +709,23 @@ struct Side {
 };
 inline Operand rows_of(const Shape& s, const Side& m, int64_t r0, int64_t rows) {
   if (m.direct) return Operand{static_cast<const char*>(m.x) + r0 * m.ld * 2, m.ld * 2, 0, (int)rows};
-  return Operand{reinterpret_cast<char*>(m.buf), (int64_t)s.Dp() * 2, rows * s.Dp() * 2, (int)rows};
+  return Operand{reinterpret_cast<char*>(m.buf), s.ldp() * 2, rows * s.ldp() * 2, (int)rows};
 }
 // lays them out there, h's rows (0: not this time) and w's in one launch
 inline void pack(const Shape& s, const Side& h, int64_t hrows, const Side& w, int64_t w0, int64_t wrows, hipStream_t st) {
   const int es = s.dtype == PO_F32 ? 4 : 2;
   auto job = [&](const Side& m, int64_t r0, int64_t rows) {
     if (m.direct) rows = 0;
-    return PackJob{static_cast<const char*>(m.x) + r0 * m.ld * es, m.ld, rows, rows * s.Dp(), m.buf};
+    return PackJob{static_cast<const char*>(m.x) + r0 * m.ld * es, m.ld, rows, rows * s.ldp(), m.buf};
   };
   const PackJob a = job(h, 0, hrows), b = job(w, w0, wrows);
   const int64_t items = (a.rows + b.rows) * (s.Dp() / 8);
   if (!items) return;
   const dim3 grid((unsigned)std::min<int64_t>((items + 255) / 256, 8192));
   if (s.dtype == PO_F32)
-    hipLaunchKernelGGL((pack_k<float>), grid, dim3(256), 0, st, a, b, (int)s.D, s.Dp());
+    hipLaunchKernelGGL((pack_k<float>), grid, dim3(256), 0, st, a, b, (int)s.D, s.ldp());
   else
-    hipLaunchKernelGGL((pack_k<uint16_t>), grid, dim3(256), 0, st, a, b, (int)s.D, s.Dp());
+    hipLaunchKernelGGL((pack_k<uint16_t>), grid, dim3(256), 0, st, a, b, (int)s.D, s.ldp());
 }
 
 inline bool serves(const void* x, int64_t ld, int dtype, int64_t D) {
