@@ -28,6 +28,7 @@
 // compiler's order).
 #pragma once
 #include "common.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace po {
@@ -71,14 +72,16 @@ struct Operand {
 
 constexpr uint32_t kOOB = 0x80000000u;
 
-template <int KIND_, int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_>
+template <int KIND_, int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_, int KG_ = 1>
 struct Cfg {
+  static constexpr int KG = KG_;                                         // groups of waves that take k-steps in turn
   static constexpr int KIND = KIND_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = KB_, STAGES = STAGES_;
   static constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   static constexpr int RPI = 1024 / KB;                                  // rows one wave's DMA instruction fills
   static constexpr int NA = BM / RPI / NW, NB = BN / RPI / NW;           // instructions per wave and stage
-  static constexpr int STAGE_BYTES = (BM + BN) * KB, LDS = STAGES * STAGE_BYTES;
+  static constexpr int STAGE_BYTES = (BM + BN) * KB, LDS = KG * STAGES * STAGE_BYTES;
   static_assert(KB % 64 == 0 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && NA * RPI * NW == BM && NB * RPI * NW == BN, "tile");
+  static_assert((KG - 1) * BM * BN * 4 <= LDS, "the groups' sums pass through LDS");
 };
 
 template <int KB>
@@ -104,7 +107,9 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
                                         const Operand& B, int m0, int n0, int kbytes, int ks0, int ks1, int nk,
                                         uint32_t pa, uint32_t pb, char* lds) {
   constexpr int KB = C::KB, CPR = KB / 16;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = wid % C::NW, kg = wid / C::NW;
+  lds += kg * C::STAGES * C::STAGE_BYTES;
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int lrow = lane / CPR;                               // row of this lane inside one DMA instruction
   uint32_t oa[C::NA], ob[C::NB];
@@ -126,7 +131,7 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
   const uint32_t lch = ((lane % CPR) ^ swz<KB>(wave * C::RPI + lrow)) * 16;
   const char* abase = A.p + (int64_t)m0 * A.stride;
   const char* bbase = B.p + (int64_t)n0 * B.stride;
-  int q = ks0 / nk, kt = ks0 - q * nk;                       // plane pair and step of the next stage to load
+  int next = ks0 + kg, q = next / nk, kt = next - q * nk;    // the next stage's step, its plane pair and place in it
   auto issue = [&](int buf) {
     const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<char*>(abase + (int64_t)((pa >> (4 * q)) & 15) * A.plane), 0, 0x7fffffff, 0x00020000);
@@ -136,19 +141,21 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
     char* lb = la + C::BM * KB;
     const uint32_t k0 = (uint32_t)kt * KB;
     // past the row's end: out of range by the sign bit (offsets stay below 2^31)
-    const uint32_t past = (int)(k0 + lch) < kbytes ? k0 : kOOB;
+    const uint32_t past = (int)(k0 + lch) < kbytes && (C::KG == 1 || next < ks1) ? k0 : kOOB;
 #pragma unroll
     for (int i = 0; i < C::NA; ++i)
       Loader<C>::dma(ra, la + (i * C::NW + wave) * 1024, (oa[i] + (past & 0x7fffffffu)) | (past & kOOB) | (oa[i] & kOOB));
 #pragma unroll
     for (int i = 0; i < C::NB; ++i)
       Loader<C>::dma(rb, lb + (i * C::NW + wave) * 1024, (ob[i] + (past & 0x7fffffffu)) | (past & kOOB) | (ob[i] & kOOB));
-    if (++kt == nk) {
-      kt = 0;
+    next += C::KG;
+    kt += C::KG;
+    while (kt >= nk) {
+      kt -= nk;
       ++q;
     }
   };
-  const int n = ks1 - ks0;
+  const int n = (ks1 - ks0 + C::KG - 1) / C::KG;             // of every group: a last step past the end adds zeros
 #pragma unroll
   for (int s = 0; s < C::STAGES - 1; ++s)
     if (s < n) issue(s);
@@ -211,6 +218,26 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
   for (s = 1; s < n; ++s) step(std::false_type{});
   multiply(fa[1], fb[1]);
   __builtin_amdgcn_sched_barrier(0);
+  if constexpr (C::KG > 1) {                                 // the groups' sums, in order, in the first one's registers
+    lds -= kg * C::STAGES * C::STAGE_BYTES;
+    using V = typename Acc<C::KIND>::type;
+    __syncthreads();
+    V* sums = reinterpret_cast<V*>(lds) + wave * C::TM * C::TN * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+        if (kg > 0) sums[(kg - 1) * (C::BM * C::BN / 4) + (i * C::TN + j) * 64] = acc[i][j];
+    __syncthreads();
+    if (kg == 0) {
+#pragma unroll
+      for (int g = 0; g < C::KG - 1; ++g)
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j) acc[i][j] += sums[g * (C::BM * C::BN / 4) + (i * C::TN + j) * 64];
+    }
+  }
 }
 
 // Element e of a 16 x 16 accumulator block lies in row (m) 4 * (lane / 16) + e and column
@@ -244,7 +271,7 @@ struct NoPre {
 // gridDim.y slices the k-steps.  Epi::run ends the tile; what it reads of a token it reads
 // before the loop (Pre): its waves have no others to wait behind.
 template <class C, class Epi>
-__global__ __launch_bounds__(C::NW * 64, C::LDS > 81920 ? 1 : 2) void product_k(const Args a, const typename Epi::Args e) {
+__global__ __launch_bounds__(C::NW * C::KG * 64, C::LDS > 81920 ? 1 : 2) void product_k(const Args a, const typename Epi::Args e) {
   __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
   const int id = xcd_remap();
   constexpr int GM = 8;
@@ -255,7 +282,7 @@ __global__ __launch_bounds__(C::NW * 64, C::LDS > 81920 ? 1 : 2) void product_k(
   t.tn = r / gm;
   t.lane = threadIdx.x & 63;
   t.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  t.wm = t.wave / C::WN;
+  t.wm = t.wave % C::NW / C::WN;
   t.wn = t.wave % C::WN;
   t.m0 = t.tm * C::BM + t.wm * C::TM * 16;
   t.n0 = t.tn * C::BN + t.wn * C::TN * 16;
@@ -268,6 +295,8 @@ __global__ __launch_bounds__(C::NW * 64, C::LDS > 81920 ? 1 : 2) void product_k(
   const int total = a.nk * a.pairs;
   const int ks0 = (int)((int64_t)blockIdx.y * total / gridDim.y), ks1 = (int)((int64_t)(blockIdx.y + 1) * total / gridDim.y);
   product<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, a.nk, a.pa, a.pb, lds);
+  // waves of the other groups end here; barriers below wait for the ones that remain
+  if (C::KG > 1 && t.wave >= C::NW) return;
   Epi::template run<C>(t, e, pre, lds);
 }
 
@@ -281,7 +310,7 @@ inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipSt
     set_error("%s: operand too large", what);
     return PO_EINVAL;
   }
-  hipLaunchKernelGGL((product_k<C, Epi>), dim3(a.tiles_m * a.tiles_n, slices), dim3(C::NW * 64), 0, s, a, e);
+  hipLaunchKernelGGL((product_k<C, Epi>), dim3(a.tiles_m * a.tiles_n, slices), dim3(C::NW * C::KG * 64), 0, s, a, e);
   return check_launch(what);
 }
 
@@ -311,11 +340,15 @@ inline Plan plan_product(int64_t M, int64_t N, int64_t steps, double ends_mid, d
   Plan best{LARGE, 1, 1e300};
   for (auto& k : kinds) {
     const int64_t tiles = ((M + k.bm - 1) / k.bm) * ((N + k.bn - 1) / k.bn);
-    for (int s = 1; s <= max_slices && (s == 1 || steps / s >= 4); ++s) {
-      const int64_t rounds = (tiles * s + k.slots - 1) / k.slots;
-      const double step = k.id != LARGE && tiles * s <= 256 ? 0.65 * k.step : k.step;   // one to a CU
-      const double t = rounds * ((double)((steps + s - 1) / s) * step + k.ends) + s * sum_us;
-      if (t < best.us) best = Plan{k.id, s, t};
+    // one slice, or as many as fill the chip half, once or twice
+    for (int64_t fill : {(int64_t)1, k.slots / 2 / tiles, k.slots / tiles, 2 * k.slots / tiles}) {
+      const int s = (int)std::min<int64_t>(fill, std::min<int64_t>(max_slices, steps / 4));
+      if (s < 1 && fill != 1) continue;
+      const int n = std::max(s, 1);
+      const int64_t rounds = (tiles * n + k.slots - 1) / k.slots;
+      const double step = k.id != LARGE && tiles * n <= 256 ? 0.65 * k.step : k.step;   // one to a CU
+      const double t = rounds * ((double)((steps + n - 1) / n) * step + k.ends) + n * sum_us;
+      if (t < best.us) best = Plan{k.id, n, t};
     }
   }
   return best;

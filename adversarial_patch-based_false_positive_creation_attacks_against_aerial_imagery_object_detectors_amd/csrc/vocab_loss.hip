@@ -40,6 +40,10 @@ template <int KIND>
 using Mid = Cfg<KIND, 128, 128, 2, 2, 128, 2>;
 template <int KIND>
 using Few = Cfg<KIND, 128, 32, 4, 1, 128, 3>;
+// few of them: two groups of waves take the steps of k in turn (fp32 losses of 81 x 7855 x 1032, 186 tiles
+// of 102 steps: 39 -> 30 us; where tiles fill the chip twice the groups stand in each other's way: 10 -> 14)
+template <int KIND>
+using Fewer = Cfg<KIND, 128, 32, 4, 1, 128, 3, 2>;
 
 // over the four lanes that hold a column
 __device__ __forceinline__ float column_max(float x) {
@@ -742,7 +746,12 @@ inline int check_shape(const char* what, int64_t N, int64_t V, int64_t D, int dt
 
 template <int KIND, class Epi>
 inline int launch_planned(const Args& a, const typename Epi::Args& e, Plan p, hipStream_t s, const char* what) {
-  if (p.tile == FEW) return launch_product<Few<KIND>, Epi>(a, e, p.slices, s, what);
+  if (p.tile == FEW) {
+    const int64_t tiles = (int64_t)ceil_div(a.A.rows, 128) * ceil_div(a.B.rows, 32) * p.slices;
+    if (tiles <= 256 && (int64_t)ceil_div(a.kbytes, 128) * a.pairs >= 8 * p.slices)
+      return launch_product<Fewer<KIND>, Epi>(a, e, p.slices, s, what);
+    return launch_product<Few<KIND>, Epi>(a, e, p.slices, s, what);
+  }
   if (p.tile == MID) return launch_product<Mid<KIND>, Epi>(a, e, p.slices, s, what);
   return launch_product<Large<KIND>, Epi>(a, e, p.slices, s, what);
 }
