@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -134,6 +135,25 @@ bool wants_grad(const Tensor& a, const Tensor& b) {
   return at::GradMode::is_enabled() && (a.requires_grad() || (b.defined() && b.requires_grad()));
 }
 
+// A captured backward pass ends at the leaves' gradient accumulators.  One that an eager graph
+// of the same leaf keeps alive belongs to that graph's stream: the engine makes that stream wait
+// for the captured one, which ends the process where it is the default stream.  Refused here,
+// before anything is captured.
+void check_capture(const char* what, std::initializer_list<const Tensor*> leaves) {
+  const Tensor& first = **leaves.begin();
+  if (!first.is_cuda()) return;                               // refused later
+  const c10::OptionalDeviceGuard guard(first.device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto now = c10::hip::getCurrentHIPStream(first.device().index()).id();
+  for (const Tensor* t : leaves) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!stream || stream->id() == now, what,
+                ": a graph made outside this capture still holds one of its leaves (free that graph's outputs before capturing)");
+  }
+}
+
 // ---- dropout ---------------------------------------------------------------
 
 struct DropoutKey {
@@ -218,7 +238,10 @@ Tensor keyed_dropout(const py::object& x_, double p, const py::object& seed_, co
                     "keyed_dropout: rows row0 .. row0 + rows must stay within 2^32");
   k.row0 = (int64_t)row0;
   py::gil_scoped_release free;
-  if (wants_grad(x, residual)) return Dropout::apply(x, some(residual), some(step), k.drop, k.seed, k.step, k.row0);
+  if (wants_grad(x, residual)) {
+    check_capture("keyed_dropout", {&x, &residual});
+    return Dropout::apply(x, some(residual), some(step), k.drop, k.seed, k.step, k.row0);
+  }
   Tensor used;
   return dropout_run(x, residual, k, step, &used);
 }
@@ -332,7 +355,10 @@ Tensor linear_cross_entropy(const py::object& hidden_, const py::object& weight_
   TORCH_CHECK_VALUE(scale > 0.0 && std::isfinite(scale), "linear_cross_entropy: scale must be positive and finite, got ", scale);
   const Tensor& target = tensor_of(target_);
   py::gil_scoped_release free;
-  if (wants_grad(hidden, weight)) return LinearCe::apply(hidden, weight, target, ignore, red, scale);
+  if (wants_grad(hidden, weight)) {
+    check_capture("linear_cross_entropy", {&hidden, &weight});
+    return LinearCe::apply(hidden, weight, target, ignore, red, scale);
+  }
   return ce_forward(hidden, weight, target, ignore, red, scale).loss;
 }
 

@@ -135,25 +135,27 @@ __global__ __launch_bounds__(256) void quantize_rows_k(const void* __restrict__ 
 // loads of 16 bytes (row lane % 16, 64 bytes of a row to a load) are in flight together, and
 // go into the matrix cores as they are.  The waves' sums meet in LDS.  FUSED (up to 4
 // tokens): the workgroup quantises the tokens itself, into LDS, behind its weights' loads: one
-// launch, where the quantisation alone takes 4 us.  One token of 4096 x 4096 takes 7.0 us,
-// 8192 x 8192 15.6; with 4 waves and four times the loads 8.4 and 18.6; streaming
-// (non-temporal) loads 6.9 and 17.6.
+// launch, where the quantisation alone takes 4 us.  One token of 4096 x 4096 takes 6.2 us,
+// 8192 x 8192 15; with 4 waves and four times the loads 1.4 and 2.2 us more; with streaming
+// (non-temporal) loads 8192 x 8192 1 us more.
 constexpr int kFewWaves = 16, kFewLoads = 4, kFewSlice = kFewLoads * 64;
 constexpr int kFewLds = 44 << 10;                            // of the 8-bit tokens; with the sums below 64 KB
 
-// token t's row of 8-bit numbers in LDS and its scale, made by the whole workgroup
+// A token's row of 8-bit numbers in LDS and its scale, made by the whole workgroup.  A row of
+// up to 8192 stays in registers between the maximum and the quotients.  tops: the waves'
+// maxima, of every second token the same (one barrier a token).
 template <int DT>
 __device__ __forceinline__ void quantize_to_lds(const void* x, int64_t at, int K, int Kp, int8_t* q, uint32_t* tops,
                                                 float* scale) {
+  constexpr int T = kFewWaves * 64;
   uint32_t top = 0;
   float v[8];
-  for (int k = threadIdx.x * 8; k < K; k += kFewWaves * 64 * 8) {
+  for (int k = threadIdx.x * 8; k < K; k += T * 8) {
     load8<DT>(x, at + k, K - k, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
   }
   top = po::wave_max_u32(top);
-  __syncthreads();                                           // the last token's maxima are read
   if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
   top = 0;
@@ -161,8 +163,8 @@ __device__ __forceinline__ void quantize_to_lds(const void* x, int64_t at, int K
   for (int w = 0; w < kFewWaves; ++w) top = max(top, tops[w]);
   const RowScale r(top);
   if (threadIdx.x == 0) *scale = r.stored();
-  for (int k = threadIdx.x * 8; k < Kp; k += kFewWaves * 64 * 8) {
-    load8<DT>(x, at + k, K - k, v);
+  for (int k = threadIdx.x * 8; k < Kp; k += T * 8) {
+    if (K > T * 8 || k >= K) load8<DT>(x, at + k, K - k, v);
     *reinterpret_cast<uint2*>(q + k) = r.quotients(v);
   }
 }
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_tokens_k(const void* __res
                                                     void* __restrict__ y, int64_t ldy) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ i4v sums[kFewWaves][TB][64];
-  __shared__ uint32_t tops[kFewWaves];
+  __shared__ uint32_t tops[2][kFewWaves];
   __shared__ float scales[32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * 16, Kp = (K + 15) / 16 * 16;
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_tokens_k(const void* __res
   if constexpr (FUSED) {
     __builtin_amdgcn_sched_barrier(0);
     for (int t = 0; t < M; ++t)
-      quantize_to_lds<DT>(x, t * ldx, K, Kp, reinterpret_cast<int8_t*>(lds) + t * Kp, tops, scales + t);
+      quantize_to_lds<DT>(x, t * ldx, K, Kp, reinterpret_cast<int8_t*>(lds) + t * Kp, tops[t & 1], scales + t);
     __syncthreads();
   } else if (threadIdx.x < 32) {
     scales[threadIdx.x] = threadIdx.x < M ? sx[threadIdx.x] : 0.f;

@@ -138,6 +138,24 @@ def test_gradient_of_a_broadcast_input_and_of_second_order():
     assert abs(float(num - (gx.double() * d.double()).sum())) < 50 * 64 * 2.0 ** -21 * 16
 
 
+def test_gradient_of_the_residual_alone_and_inference_mode():
+    kd = pkg_mod("keyed_dropout").keyed_dropout
+    x, r, dy = (torch.randn(20, 33, device=DEV) for _ in range(3))
+    r.requires_grad_()
+    y = kd(x, 0.5, 2, 3, residual=r)
+    y.backward(dy)
+    assert torch.equal(r.grad, dy)
+    with torch.inference_mode():
+        assert torch.equal(kd(x, 0.5, 2, 3, residual=r), y)
+    assert not kd(x, 0.5, 2, 3).requires_grad
+    step = torch.tensor([3], device=DEV)
+    xx = x.clone().requires_grad_()
+    z = kd(xx, 0.5, 2, step, residual=r)
+    step += 1
+    (dx,) = torch.autograd.grad(z, xx, dy)
+    check(dx, dy, keep_ref(20, 33, 0.5, 2, 3), 0.5)
+
+
 def test_step_on_the_device_in_a_replayed_graph():
     kd = pkg_mod("keyed_dropout").keyed_dropout
     x = torch.randn(33, 65, device=DEV, requires_grad=True)

@@ -5,6 +5,8 @@ the values the exact quotients' nearest).  A product's sum is exact; it then tak
 a conversion, two products and a sum in 32 bits (4 * 2^-24 of |sum| s sw plus 2^-24
 of the result) and one rounding to its type (eps / 2, half of fp16's smallest
 number)."""
+import copy
+
 import pytest
 import torch
 
@@ -187,4 +189,7 @@ def test_module_of_a_linear_and_its_moves():
     other = m.Int8Linear(torch.randn(37, 100, device=DEV), torch.zeros(37, device=DEV))
     other.load_state_dict(layer.state_dict())
     assert torch.equal(other(x), y)
-    assert not y.requires_grad
+    assert torch.equal(copy.deepcopy(layer)(x), y)
+    assert not y.requires_grad and not layer(x.requires_grad_()).requires_grad
+    with pytest.raises(RuntimeError, match="no gradient"):
+        m.int8_linear(x, layer.wq, layer.wscale)

@@ -368,6 +368,31 @@ def test_forward_and_backward_in_a_replayed_graph():
                 assert torch.equal(a.detach(), b)
 
 
+def test_a_capture_while_an_eager_graph_holds_the_leaves_is_refused():
+    """The eager graph's accumulators belong to its stream; capturing a backward pass into them would end the
+    process.  The call raises inside the capture, and both go on after it."""
+    lce, kd = pkg_mod("vocab_loss").linear_cross_entropy, pkg_mod("keyed_dropout").keyed_dropout
+    h, w, t = inputs(60, 400, 40, torch.float32)
+    h.requires_grad_()
+    w.requires_grad_()
+    want = torch.autograd.grad(lce(h, w, t), (h, w))
+    eager = lce(h, w, t)
+    for call in (lambda: lce(h, w, t), lambda: lce(h.detach(), w, t), lambda: kd(h, 0.5, 1), lambda: kd(h.detach(), 0.5, 1, residual=h)):
+        with pytest.raises(RuntimeError, match="outside this capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    late = torch.autograd.grad(eager, (h, w))
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(lce(h, w, t), (h, w))
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b, c in zip(got, late, want):
+            assert torch.equal(a, c) and torch.equal(b, c)
+
+
 def test_two_streams_at_once_and_repeats_are_equal():
     lce = pkg_mod("vocab_loss").linear_cross_entropy
     sets = [inputs(260, 3000, 128, torch.bfloat16, seed=k) for k in range(2)]
