@@ -119,6 +119,16 @@ def test_strides_offsets_and_shapes():
         assert kd(torch.zeros(shape, device=DEV), 0.25, 1, 1).shape == shape
 
 
+def test_offsets_past_32_bits():
+    kd = pkg_mod("keyed_dropout").keyed_dropout
+    rows, cols = 65540, 32777                      # 2.15e9 elements, rows on odd places
+    x = torch.ones(rows, cols, dtype=torch.bfloat16, device=DEV)
+    y = kd(x, 0.5, 6, 7)
+    for r in (0, 32767, 65534):
+        check(y[r:r + 4], x[r:r + 4], keep_ref(4, cols, 0.5, 6, 7, row0=r), 0.5)
+    assert y.view(-1)[2 ** 31 - 5:2 ** 31 + 5].float().max() <= 2.0
+
+
 def test_gradient_of_a_broadcast_input_and_of_second_order():
     kd = pkg_mod("keyed_dropout").keyed_dropout
     keep = keep_ref(50, 64, 0.5, 8, 9)

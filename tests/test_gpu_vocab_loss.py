@@ -280,6 +280,36 @@ def test_large_logits_stay_finite(dtype):
     assert torch.isfinite(dh).all() and torch.isfinite(dw).all()
 
 
+@pytest.mark.parametrize("N,frozen", [(3, False), (140, True)])
+def test_a_vocabulary_past_4_gib(N, frozen):
+    """2.2e9 weights; the reference walks them in 64 bits, piece by piece."""
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    V, D = 2_150_000, 1032
+    g = torch.Generator(device=DEV).manual_seed(N)
+    w = (torch.randn(V, D, generator=g, device=DEV, dtype=torch.bfloat16) / 32).requires_grad_(not frozen)
+    h = torch.randn(N, D, generator=g, device=DEV).bfloat16().requires_grad_()
+    t = torch.randint(0, V, (N,), generator=g, device=DEV)
+    t[0], t[-1] = V - 1, 2_100_000
+    parts = [(a, min(V, a + 250_000)) for a in range(0, V, 250_000)]
+    w64 = lambda a, b: w.detach()[a:b].double()          # noqa: E731
+    h64 = h.detach().double()
+    lse = torch.logsumexp(torch.stack([torch.logsumexp(h64 @ w64(a, b).t(), 1) for a, b in parts]), 0)
+    loss = lce(h, w, t, reduction="none")
+    want = lse - (h64 * w.detach()[t].double()).sum(1)
+    within(loss.detach(), want, 2 * (D + 4) * 2.0 ** -23 * 60 + 4e-5, "loss")     # sums of |h w| up to 60
+    grads = torch.autograd.grad(loss.sum(), [h] if frozen else [h, w])
+    dh = -w.detach()[t].double()
+    for a, b in parts:
+        dh += torch.exp(h64 @ w64(a, b).t() - lse[:, None]) @ w64(a, b)
+    # the target's embedding dominates; roundings of 2^-8 to it and to each of the terms
+    assert float((grads[0].double() - dh).norm() / dh.norm()) < 2.0 ** -8
+    if not frozen:
+        for v in (0, 1_040_000, int(t[-1]), int(t[0])):
+            p = torch.exp(h64 @ w.detach()[v].double() - lse) - (t == v).double()
+            ref = p @ h64
+            assert float((grads[1][v].double() - ref).norm() / ref.norm()) < 2.0 ** -7
+
+
 def test_infinite_logits_are_what_the_formula_says():
     lce = pkg_mod("vocab_loss").linear_cross_entropy
     h = torch.ones(3, 8, device=DEV)
