@@ -62,15 +62,24 @@ struct RowScale {
   bool bad;                                                  // the row holds NaN or an infinity: as bits they lie on top
   __device__ __forceinline__ explicit RowScale(uint32_t top) : s(__uint_as_float(top) / 127.f), inv(1.f / s), bad(top >= 0x7f800000u) {}
   __device__ __forceinline__ float stored() const { return bad ? __uint_as_float(0x7fc00000u) : s; }
+  // 8 bits each, of eight
   __device__ __forceinline__ uint2 quotients(const float* v) const {
     uint32_t b[2] = {0, 0};
-    if (!bad && s > 0.f) {
+    if (!bad && s > 1e-30f) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // 1 / s and half steps of s need normal numbers
-        const int n = s > 1e-30f ? quotient(v[j], s, inv) : (int)__builtin_rint((double)v[j] / (double)s);
-        b[j >> 2] |= (uint32_t)(n & 255) << (8 * (j & 3));
-      }
+      for (int j = 0; j < 8; ++j) b[j >> 2] |= (uint32_t)(quotient(v[j], s, inv) & 255) << (8 * (j & 3));
+    } else if (!bad && s > 0.f) {                            // 1 / s and half steps of s need normal numbers
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+        for (int j = 3; j >= 0; --j) {
+          float x = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x = i == h * 4 + j ? v[i] : x;
+          const uint32_t n = (uint32_t)((int)__builtin_rint((double)x / (double)s) & 255);
+          if (h) b[1] = b[1] << 8 | n;
+          else b[0] = b[0] << 8 | n;
+        }
     }
     return make_uint2(b[0], b[1]);
   }
@@ -313,11 +322,13 @@ int product_of(const Args& a, const typename ScaledEpi<DT>::Args& e, hipStream_t
   const char* what = "po_int8_matmul";
   const Plan p = plan_product(a.A.rows, a.B.rows, ceil_div(a.kbytes, 128), 6, 10);
   if (p.tile == LARGE) return launch_product<Cfg<I8, 256, 256, 2, 4, 128, 2>, E>(a, e, 1, s, what);
-  // 64 x 64 where tiles of 128 x 128 leave CUs without one; where even these do, two groups of
-  // waves take the steps in turn (200 x 2000 x 1500 9.7 -> 8.4 us; 1111 x 4001 x 1000, 288 tiles, 16 -> 21)
+  // 64 x 64 where tiles of 128 x 128 leave CUs without one; where even these do, two groups of waves
+  // take the steps in turn (200 x 2000 x 1500 9.7 -> 8.4 us).  64 x 96 where that makes one round of
+  // more (1111 x 4001 x 1000, 288 tiles or 192: 15.9 -> 14.3 us)
   if ((int64_t)ceil_div(a.A.rows, 128) * ceil_div(a.B.rows, 128) < 256) {
-    if ((int64_t)ceil_div(a.A.rows, 64) * ceil_div(a.B.rows, 64) <= 256)
-      return launch_product<Cfg<I8, 64, 64, 2, 2, 128, 3, 2>, E>(a, e, 1, s, what);
+    const int64_t tm = ceil_div(a.A.rows, 64);
+    if (tm * ceil_div(a.B.rows, 64) <= 256) return launch_product<Cfg<I8, 64, 64, 2, 2, 128, 3, 2>, E>(a, e, 1, s, what);
+    if (tm * ceil_div(a.B.rows, 96) <= 256) return launch_product<Cfg<I8, 64, 96, 2, 2, 128, 3, 2>, E>(a, e, 1, s, what);
     return launch_product<Cfg<I8, 64, 64, 2, 2, 256, 2>, E>(a, e, 1, s, what);
   }
   return launch_product<Cfg<I8, 128, 128, 2, 2, 128, 2>, E>(a, e, 1, s, what);

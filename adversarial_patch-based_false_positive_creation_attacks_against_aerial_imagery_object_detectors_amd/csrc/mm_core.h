@@ -188,7 +188,7 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x008, E, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, X - E * R, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, X > E * R ? X - E * R : 0, 0);
   };
   static_assert(G % 2 == 0, "a step's groups alternate between two sets of registers");
   int buf = 0, s = 0;
