@@ -355,17 +355,10 @@ struct GradEpi {
 
 // ---- the rows' kernels ---------------------------------------------------
 
-__device__ __forceinline__ double block_sum(double x, double* red) {
-  red[threadIdx.x] = x;
-  __syncthreads();
+__device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
-  for (int w = 128; w; w >>= 1) {
-    if (threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
-    __syncthreads();
-  }
-  const double r = red[0];
-  __syncthreads();
-  return r;
+  for (int w = 32; w; w >>= 1) x += __shfl_xor(x, w);
+  return x;
 }
 
 // Rows' statistics and losses from the tiles': R rows to a workgroup, 256 / R lanes to a row
@@ -381,15 +374,23 @@ __global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ pa
                                                    float* __restrict__ loss, double* sums, uint32_t* arrived, int mean,
                                                    float* __restrict__ total, float* __restrict__ count) {
   __shared__ float2 red[256];
-  __shared__ double dred[256];
-  __shared__ uint32_t order;
   const int row = threadIdx.x % R, n = blockIdx.x * R + row;
   float m = -INFINITY, s = 0.f;
   if (n < N)
-    for (int p = threadIdx.x / R; p < parts; p += 256 / R) {
-      const float2 o = partial[(int64_t)p * N + n];
-      const float t = fmaxf(m, o.x), ref = t == -INFINITY ? 0.f : t;
-      s = s * __builtin_amdgcn_exp2f(m - ref) + o.y * __builtin_amdgcn_exp2f(o.x - ref);
+    for (int p = threadIdx.x / R; p < parts; p += 8 * (256 / R)) {
+      float2 o[8];                                           // loads in flight together: they come from other XCDs
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int at = p + u * (256 / R);
+        o[u] = at < parts ? partial[(int64_t)at * N + n] : make_float2(-INFINITY, 0.f);
+      }
+      float t = m;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) t = fmaxf(t, o[u].x);
+      const float ref = t == -INFINITY ? 0.f : t;
+      s *= __builtin_amdgcn_exp2f(m - ref);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += o[u].y * __builtin_amdgcn_exp2f(o[u].x - ref);
       m = t;
     }
   red[threadIdx.x] = make_float2(m, s);
@@ -416,23 +417,25 @@ __global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ pa
                           : kLn2 * (__builtin_log2f(r.y) - __builtin_fmaf(tlogit[n], k, -r.x));
     if (loss) loss[n] = l;
   }
-  if (!total) return;
-  const double sum = block_sum(l, dred), num = block_sum(counts, dred);
+  if (!total || threadIdx.x >= 64) return;
+  static_assert(R <= 64, "a workgroup's rows in its first wave");
+  const double sum = wave_sum(l), num = wave_sum(counts);
+  uint32_t order = 0;
   if (threadIdx.x == 0) {
     __hip_atomic_store(sums + 2 * blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __hip_atomic_store(sums + 2 * blockIdx.x + 1, num, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     order = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  __syncthreads();
-  if (order != gridDim.x - 1) return;
+  if (__builtin_amdgcn_readfirstlane(order) != gridDim.x - 1) return;
   double a = 0, c = 0;
-  for (int b = threadIdx.x; b < gridDim.x; b += 256) {
+#pragma unroll 4
+  for (int b = threadIdx.x; b < gridDim.x; b += 64) {
     a += __hip_atomic_load(sums + 2 * b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     c += __hip_atomic_load(sums + 2 * b + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  a = block_sum(a, dred);
-  c = block_sum(c, dred);
+  a = wave_sum(a);
+  c = wave_sum(c);
   if (threadIdx.x == 0) {
     *total = (float)(mean ? a / c : a);
     *count = (float)c;
@@ -819,7 +822,7 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
     }
   }
   // total: few workgroups, since each counts itself in (1000 of them: 20 us, 63: 6)
-  const int R = reduction ? (N <= 64 ? 1 : N <= 512 ? 4 : 16) : N < 2048 ? 1 : 16;
+  const int R = reduction ? (N <= 64 ? 1 : N <= 512 ? 4 : 16) : N <= 256 ? 1 : N <= 2048 ? 4 : 16;
   hipLaunchKernelGGL((R == 1 ? row_stats_k<1> : R == 4 ? row_stats_k<4> : row_stats_k<16>), dim3(ceil_div(N, R)), dim3(256), 0,
                      st, ws.partial, e.tile0, (int)N, V, ws.tlogit, target, ignore_index, e.k, reinterpret_cast<float2*>(stat),
                      reduction ? nullptr : loss, ws.sums, ws.arrived, reduction == 2, reduction ? loss : nullptr, count);
