@@ -320,7 +320,7 @@ template <int DT>
 int product_of(const Args& a, const typename ScaledEpi<DT>::Args& e, hipStream_t s) {
   using E = ScaledEpi<DT>;
   const char* what = "po_int8_matmul";
-  const Plan p = plan_product(a.A.rows, a.B.rows, ceil_div(a.kbytes, 128), 6, 10);
+  const Plan p = plan_product(a.A.rows, a.B.rows, ceil_div(a.kbytes, 128), Ends{6, 10, false});
   if (p.tile == LARGE) return launch_product<Cfg<I8, 256, 256, 2, 4, 128, 2>, E>(a, e, 1, s, what);
   // 64 x 64 where tiles of 128 x 128 leave CUs without one; where even these do, two groups of waves
   // take the steps in turn (200 x 2000 x 1500 9.7 -> 8.4 us).  64 x 96 where that makes one round of

@@ -72,15 +72,17 @@ struct Operand {
 
 constexpr uint32_t kOOB = 0x80000000u;
 
-template <int KIND_, int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_, int KG_ = 1>
+template <int KIND_, int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_, int KG_ = 1, int PLANES_ = 1>
 struct Cfg {
   static constexpr int KG = KG_;                                         // groups of waves that take k-steps in turn
+  static constexpr int PLANES = PLANES_;                                 // 3: a step holds both operands' three (product3)
   static constexpr int KIND = KIND_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = KB_, STAGES = STAGES_;
   static constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   static constexpr int RPI = 1024 / KB;                                  // rows one wave's DMA instruction fills
-  static constexpr int NA = BM / RPI / NW, NB = BN / RPI / NW;           // instructions per wave and stage
-  static constexpr int STAGE_BYTES = (BM + BN) * KB, LDS = KG * STAGES * STAGE_BYTES;
-  static_assert(KB % 64 == 0 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && NA * RPI * NW == BM && NB * RPI * NW == BN, "tile");
+  static constexpr int NA = (BM / RPI + NW - 1) / NW, NB = BN / RPI / NW;   // instructions per wave and stage
+  static constexpr int STAGE_BYTES = (BM + BN) * KB * PLANES, LDS = KG * STAGES * STAGE_BYTES;
+  static_assert(KB % 64 == 0 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && BM % RPI == 0 && NB * RPI * NW == BN, "tile");
+  static_assert(PLANES == 3 || NA * RPI * NW == BM, "every wave loads as much");
   static_assert((KG - 1) * BM * BN * 4 <= LDS, "the groups' sums pass through LDS");
 };
 
@@ -240,6 +242,113 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
   }
 }
 
+// The same of operands in three planes: acc += A0 B0 + A0 B1 + A1 B0 + A1 B1 + A0 B2 + A2 B0.
+// A step holds 32 k of all six planes: what product() loads and reads for each of the six
+// products is loaded once, and read once into registers (a 64 x 64 wave takes 24 fragments for 96
+// MFMAs where the pairs in turn take 36; fp32 head of 3000 x 5000 x 1500, trained: the four
+// products 1100 -> 980 us, of 512 x 8192 x 256 126 -> 100).  Rows are 64 bytes, four chunks, turned every four rows,
+// so that 8 neighbouring lanes' reads cover all banks.
+template <class C>
+__device__ __forceinline__ void product3(f4v (&acc)[C::TM][C::TN], const Operand& A, const Operand& B, int m0, int n0,
+                                         int kbytes, int ks0, int ks1, char* lds) {
+  static_assert(C::KB == 64 && C::PLANES == 3 && C::KG == 1 && C::STAGES == 2, "form");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / C::WN, wn = wave % C::WN, lrow = lane / 4;
+  // rows of one lane differ by multiples of 16, which the turn does not see
+  const uint32_t lch = (uint32_t)((lane & 3) ^ ((lrow >> 2) & 3)) * 16;
+  uint32_t oa[C::NA], ob[C::NB];
+#pragma unroll
+  for (int i = 0; i < C::NA; ++i) {
+    const int r = (i * C::NW + wave) * C::RPI + lrow;
+    oa[i] = m0 + r < A.rows ? (uint32_t)(r * (int)A.stride) + lch : kOOB;
+  }
+#pragma unroll
+  for (int i = 0; i < C::NB; ++i) {
+    const int r = (i * C::NW + wave) * C::RPI + lrow;
+    ob[i] = n0 + r < B.rows ? (uint32_t)(r * (int)B.stride) + lch : kOOB;
+  }
+  const char* abase = A.p + (int64_t)m0 * A.stride;
+  const char* bbase = B.p + (int64_t)n0 * B.stride;
+  constexpr int PA = C::BM * 64, PB = C::BN * 64;            // bytes of a plane of a stage
+  auto issue = [&](int buf, int step) {
+    const uint32_t k0 = (uint32_t)step * 64;
+    const uint32_t past = (int)(k0 + lch) < kbytes ? k0 : kOOB;
+    char* la = lds + buf * C::STAGE_BYTES;
+    char* lb = la + 3 * PA;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const __amdgpu_buffer_rsrc_t ra =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(abase + p * A.plane), 0, 0x7fffffff, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rb =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(bbase + p * B.plane), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < C::NA; ++i)
+        if (C::NA * C::NW * C::RPI == C::BM || i * C::NW + wave < C::BM / C::RPI)
+          Loader<C>::dma(ra, la + p * PA + (i * C::NW + wave) * 1024, (oa[i] + (past & 0x7fffffffu)) | (past & kOOB) | (oa[i] & kOOB));
+#pragma unroll
+      for (int i = 0; i < C::NB; ++i)
+        Loader<C>::dma(rb, lb + p * PB + (i * C::NW + wave) * 1024, (ob[i] + (past & 0x7fffffffu)) | (past & kOOB) | (ob[i] & kOOB));
+    }
+  };
+  const int h = lane >> 4, r16 = lane & 15, turned = (h ^ ((r16 >> 2) & 3)) * 16 + r16 * 64;
+  i4v a0[C::TM], a1[C::TM], a2[C::TM], b0[C::TN], b1[C::TN], b2[C::TN];
+  auto fetch_a = [&](int buf, int p, i4v (&a)[C::TM]) {
+    const char* la = lds + buf * C::STAGE_BYTES + p * PA + wm * C::TM * 1024 + turned;
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) a[i] = *reinterpret_cast<const i4v*>(la + i * 1024);
+  };
+  auto fetch_b = [&](int buf, int p, i4v (&b)[C::TN]) {
+    const char* lb = lds + buf * C::STAGE_BYTES + 3 * PA + p * PB + wn * C::TN * 1024 + turned;
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) b[j] = *reinterpret_cast<const i4v*>(lb + j * 1024);
+  };
+  // a product, the next ones' `reads` reads between its MFMAs
+  auto multiply = [&](const i4v (&a)[C::TM], const i4v (&b)[C::TN], auto reads) {
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) acc[i][j] = mfma<C::KIND>(a[i], b[j], acc[i][j]);
+    constexpr int R = decltype(reads)::value, X = C::TM * C::TN, E = R ? (X / R > 1 ? X / R / 2 * 2 : 1) : 1;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, E, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, X > E * R ? X - E * R : 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  using RA = std::integral_constant<int, C::TM>;
+  using RB = std::integral_constant<int, C::TN>;
+  using RAB = std::integral_constant<int, C::TM + C::TN>;
+  using R0 = std::integral_constant<int, 0>;
+  issue(0, ks0);
+  int buf = 0, s = ks0;
+  auto step = [&](auto first) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // this step's loads; the last one's fragments are out
+    __builtin_amdgcn_s_barrier();                                 // ... every wave's
+    asm volatile("" ::: "memory");
+    if (s + 1 < ks1) issue(buf ^ 1, s + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_a(buf, 0, a0);
+    fetch_b(buf, 0, b0);
+    if constexpr (!first) multiply(a1, b1, RAB{});                // the last product of the step before
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_b(buf, 2, b2);
+    multiply(a0, b0, RB{});
+    fetch_a(buf, 2, a2);
+    multiply(a0, b2, RA{});
+    fetch_b(buf, 1, b1);
+    multiply(a2, b0, RB{});
+    fetch_a(buf, 1, a1);
+    multiply(a0, b1, RA{});
+    multiply(a1, b0, R0{});
+    buf ^= 1;
+  };
+  step(std::true_type{});
+  for (s = ks0 + 1; s < ks1; ++s) step(std::false_type{});
+  multiply(a1, b1, R0{});
+}
+
 // Element e of a 16 x 16 accumulator block lies in row (m) 4 * (lane / 16) + e and column
 // (n) lane % 16: a lane's four are consecutive rows of one column.  The kernels below take
 // the operand whose index is contiguous in the output (or is reduced over) as A.
@@ -294,7 +403,10 @@ __global__ __launch_bounds__(C::NW * C::KG * 64, C::LDS > 81920 ? 1 : 2) void pr
   pre.load(t, e);
   const int total = a.nk * a.pairs;
   const int ks0 = (int)((int64_t)blockIdx.y * total / gridDim.y), ks1 = (int)((int64_t)(blockIdx.y + 1) * total / gridDim.y);
-  product<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, a.nk, a.pa, a.pb, lds);
+  if constexpr (C::PLANES == 3)
+    product3<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, lds);
+  else
+    product<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, a.nk, a.pa, a.pb, lds);
   // waves of the other groups end here; barriers below wait for the ones that remain
   if (C::KG > 1 && t.wave >= C::NW) return;
   Epi::template run<C>(t, e, pre, lds);
@@ -305,6 +417,7 @@ inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipSt
   a.tiles_m = ceil_div(a.A.rows, C::BM);
   a.tiles_n = ceil_div(a.B.rows, C::BN);
   a.nk = ceil_div(a.kbytes, C::KB);
+  if (C::PLANES == 3) a.pairs = 1;                           // six in a step
   if ((int64_t)a.tiles_m * a.tiles_n >= (1LL << 22) || slices > 65535 || (int64_t)a.nk * a.pairs >= (1LL << 31) || slices > (int64_t)a.nk * a.pairs ||
       a.A.stride * C::BM >= (1LL << 31) || a.B.stride * C::BN >= (1LL << 31) || a.kbytes < 0) {
     set_error("%s: operand too large", what);
@@ -323,31 +436,44 @@ inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipSt
 // taken for long k or cheap epilogues, MID for few tiles and short k: the losses' forward
 // product of 32768 x 2048 x 512 78 against 95 us; the gradient of the logits there 117
 // against 112 us, at k = 128 73 against 63.  slices > 1 cuts k between workgroups, each
-// slice's sums then cost sum_us.
-enum TileId { FEW, MID, LARGE };
+// slice's sums then cost sum_us.  Products of three planes: LARGE 256 x 128, MID 128 x 64, and TALL
+// 192 x 128 for widths that fill 256 badly (the gradients of 20011 x 1000 x 513: 172 and 152 us in
+// 768 rows of LARGE tiles, 157 and 141 in 576 of TALL).
+enum TileId { FEW, MID, LARGE, TALL };
 struct Plan {
   TileId tile;
   int slices;
   double us;
 };
-inline Plan plan_product(int64_t M, int64_t N, int64_t steps, double ends_mid, double ends_large, int max_slices = 1,
-                         double sum_us = 0) {
-  struct {
-    TileId id;
-    int bm, bn, slots;
-    double step, ends;
-  } const kinds[] = {{FEW, 128, 32, 512, 0.45, 5}, {MID, 128, 128, 512, 1.08, ends_mid}, {LARGE, 256, 256, 256, 1.7, ends_large}};
+struct TileKind {
+  TileId id;
+  int bm, bn, slots;
+  double step, ends;            // ends: share of the epilogue's time
+};
+// of products of single planes, and of three (a step: 64 k of one of the six products)
+constexpr TileKind kTiles[2][4] = {
+    {{FEW, 128, 32, 512, 0.45, 0}, {MID, 128, 128, 512, 1.08, 1}, {LARGE, 256, 256, 256, 1.7, 1}, {}},
+    {{FEW, 128, 32, 512, 0.45, 0}, {MID, 128, 64, 512, 0.45, 0.5}, {LARGE, 256, 128, 256, 0.73, 0.5}, {TALL, 192, 128, 256, 0.57, 0.4}}};
+// What the plan has to know of a product's epilogue: us, and whether its tiles may be TALL
+struct Ends {
+  double mid, large;
+  bool tall;
+};
+inline Plan plan_product(int64_t M, int64_t N, int64_t steps, Ends ends, bool triple = false, int max_slices = 1, double sum_us = 0) {
   Plan best{LARGE, 1, 1e300};
-  for (auto& k : kinds) {
+  for (auto& k : kTiles[triple]) {
+    if (k.id == TALL && !ends.tall) continue;
+    if (!k.bm) continue;
     const int64_t tiles = ((M + k.bm - 1) / k.bm) * ((N + k.bn - 1) / k.bn);
+    const double end = k.id == FEW ? 5 : k.ends * (k.id == MID ? ends.mid : ends.large);
     // one slice, or as many as fill the chip half, once or twice
     for (int64_t fill : {(int64_t)1, k.slots / 2 / tiles, k.slots / tiles, 2 * k.slots / tiles}) {
       const int s = (int)std::min<int64_t>(fill, std::min<int64_t>(max_slices, steps / 4));
       if (s < 1 && fill != 1) continue;
       const int n = std::max(s, 1);
       const int64_t rounds = (tiles * n + k.slots - 1) / k.slots;
-      const double step = k.id != LARGE && tiles * n <= 256 ? 0.65 * k.step : k.step;   // one to a CU
-      const double t = rounds * ((double)((steps + n - 1) / n) * step + k.ends) + n * sum_us;
+      const double step = k.slots == 512 && tiles * n <= 256 ? 0.65 * k.step : k.step;   // one to a CU
+      const double t = rounds * ((double)((steps + n - 1) / n) * step + end) + n * sum_us;
       if (t < best.us) best = Plan{k.id, n, t};
     }
   }
@@ -356,14 +482,13 @@ inline Plan plan_product(int64_t M, int64_t N, int64_t steps, double ends_mid, d
 
 // Rows of A (of M) to take first: those of whole rounds of LARGE tiles, where the rest is quicker
 // with tiles of its own than as one more round (the losses of 50001 x 2047 x 1000: 6.1 rounds).
-inline int64_t whole_rounds(int64_t M, int64_t N, int64_t steps, double ends_mid, double ends_large) {
-  const int64_t tn = (N + 255) / 256, full = (M + 255) / 256 * tn / 256, first = full * 256 / tn * 256;
+inline int64_t whole_rounds(int64_t M, int64_t N, int64_t steps, Ends ends, bool triple = false) {
+  const int bm = kTiles[triple][2].bm, bn = kTiles[triple][2].bn;
+  const int64_t tn = (N + bn - 1) / bn, full = (M + bm - 1) / bm * tn / 256, first = full * 256 / tn * bm;
   if (first <= 0 || first >= M) return M;
   const double gap = 3;                                      // from one launch to the next
-  return plan_product(first, N, steps, ends_mid, ends_large).us + plan_product(M - first, N, steps, ends_mid, ends_large).us + gap <
-                 plan_product(M, N, steps, ends_mid, ends_large).us
-             ? first
-             : M;
+  auto us = [&](int64_t m) { return plan_product(m, N, steps, ends, triple).us; };
+  return us(first) + us(M - first) + gap < us(M) ? first : M;
 }
 
 // ---- outputs -------------------------------------------------------------

@@ -33,11 +33,13 @@ using po::ceil_div;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kF16Lift = 16384.f;
 
-// plan_product's tiles
+// plan_product's tiles, of one plane and of three
+template <int KIND, int P>
+using Large = std::conditional_t<P == 3, Cfg<KIND, 256, 128, 4, 2, 64, 2, 1, 3>, Cfg<KIND, 256, 256, 2, 4, 128, 2>>;
+template <int KIND, int P>
+using Mid = std::conditional_t<P == 3, Cfg<KIND, 128, 64, 2, 2, 64, 2, 1, 3>, Cfg<KIND, 128, 128, 2, 2, 128, 2>>;
 template <int KIND>
-using Large = Cfg<KIND, 256, 256, 2, 4, 128, 2>;
-template <int KIND>
-using Mid = Cfg<KIND, 128, 128, 2, 2, 128, 2>;
+using Tall = Cfg<KIND, 192, 128, 4, 2, 64, 2, 1, 3>;         // of three planes only
 template <int KIND>
 using Few = Cfg<KIND, 128, 32, 4, 1, 128, 3>;
 // few of them: two groups of waves take the steps of k in turn (fp32 losses of 81 x 7855 x 1032, 186 tiles
@@ -82,7 +84,7 @@ struct GradOf {
 
 // partial[tile][n] = {max of l * log2e, sum of 2^(l * log2e - max)} over the tile's vocabulary rows
 struct StatsEpi {
-  static constexpr double kMid = 3, kLarge = 5.5;            // us, see plan_product
+  static constexpr Ends kEnds{3, 5.5, false};                // us, see plan_product
   struct Args {
     float2* partial;
     uint32_t* arrived;          // of row_stats_k, which follows: set to 0
@@ -183,7 +185,7 @@ struct StatsEpi {
 // dl of a piece of the vocabulary, as [n][v] and as [v][n]; PLANES = 3: as the three bf16 of each number
 template <int KIND, int PLANES>
 struct DlogitsEpi {
-  static constexpr double kMid = 6 * PLANES, kLarge = PLANES > 1 ? 70 : 15;
+  static constexpr Ends kEnds{6. * PLANES, PLANES > 1 ? 36. : 15., false};
   struct Args {
     const float2* stat;         // {max * log2e, 1 / sum} of a token
     GradOf g;
@@ -277,7 +279,7 @@ struct DlogitsEpi {
 
 // slab[slice][n][m] (+)= acc in 32 bits: the sums of dh over slices of a piece's k and over the pieces
 struct SlabEpi {
-  static constexpr double kMid = 8, kLarge = 12;
+  static constexpr Ends kEnds{8, 12, true};
   struct Args {
     float* slab;
     int64_t ld, slice;          // ld a multiple of 4
@@ -307,7 +309,7 @@ struct SlabEpi {
 // out[n][m] = acc * g.end() in the gradients' type (OUT: BF16, F16, or 3: fp32)
 template <int OUT>
 struct GradEpi {
-  static constexpr double kMid = 9, kLarge = 14;
+  static constexpr Ends kEnds{9, 14, OUT == 3};
   struct Args {
     void* out;
     int64_t ld;
@@ -693,7 +695,7 @@ struct BwdWs {
     slab_slice = s.N * slab_ld;
     // a slice's sums are written and read once: 8 bytes of each at about 4 TB/s
     dh_plan = plan_product(s.D, s.N, (int64_t)ceil_div(ldl * 2, 128) * (P == 3 ? 6 : 1),
-                           SlabEpi::kMid, SlabEpi::kLarge, kSlabSlices, slab_slice * 8 / 4e6);
+                           SlabEpi::kEnds, P == 3, kSlabSlices, slab_slice * 8 / 4e6);
     direct_dh = piece >= s.V && dh_plan.slices == 1;
     slab = l.take<float>(dh && !direct_dh ? dh_plan.slices * slab_slice : 0);
     bytes = l.at;
@@ -747,7 +749,7 @@ inline int check_shape(const char* what, int64_t N, int64_t V, int64_t D, int dt
   return PO_OK;
 }
 
-template <int KIND, class Epi>
+template <int KIND, int P, class Epi>
 inline int launch_planned(const Args& a, const typename Epi::Args& e, Plan p, hipStream_t s, const char* what) {
   if (p.tile == FEW) {
     const int64_t tiles = (int64_t)ceil_div(a.A.rows, 128) * ceil_div(a.B.rows, 32) * p.slices;
@@ -755,18 +757,20 @@ inline int launch_planned(const Args& a, const typename Epi::Args& e, Plan p, hi
       return launch_product<Fewer<KIND>, Epi>(a, e, p.slices, s, what);
     return launch_product<Few<KIND>, Epi>(a, e, p.slices, s, what);
   }
-  if (p.tile == MID) return launch_product<Mid<KIND>, Epi>(a, e, p.slices, s, what);
-  return launch_product<Large<KIND>, Epi>(a, e, p.slices, s, what);
+  if constexpr (P == 3 && Epi::kEnds.tall)
+    if (p.tile == TALL) return launch_product<Tall<KIND>, Epi>(a, e, p.slices, s, what);
+  if (p.tile == MID) return launch_product<Mid<KIND, P>, Epi>(a, e, p.slices, s, what);
+  return launch_product<Large<KIND, P>, Epi>(a, e, p.slices, s, what);
 }
 
 template <class Epi>
 inline Plan plan_of(const Args& a) {
-  return plan_product(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs, Epi::kMid, Epi::kLarge);
+  return plan_product(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs, Epi::kEnds, a.pairs > 1);
 }
 
 template <class Epi>
 inline int64_t first_part(const Args& a) {
-  return whole_rounds(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs, Epi::kMid, Epi::kLarge);
+  return whole_rounds(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs, Epi::kEnds, a.pairs > 1);
 }
 
 #define PO_TRY(x)             \
@@ -816,8 +820,9 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
       e.v0 = v + r;
       e.V = (int)part;
       const Plan p = plan_of<StatsEpi>(a);
-      PO_TRY((dtype == PO_F16 ? launch_planned<F16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
-                              : launch_planned<BF16, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")));
+      PO_TRY((dtype == PO_F16    ? launch_planned<F16, 1, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
+               : dtype == PO_BF16 ? launch_planned<BF16, 1, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
+                                  : launch_planned<BF16, 3, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")));
       e.tile0 += ceil_div(part, p.tile == LARGE ? 256 : 128);
     }
   }
@@ -856,7 +861,7 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
       const typename E::Args e{stat, g, v + r, N, (int)s.Np(), (int)part, (int)(r + part < rows ? part : rp - r), scale * kLog2e,
                                dh ? ws.dl + r : nullptr, dw ? ws.dlt + r * s.ldn() : nullptr, ws.ldl, s.ldn(), N * ws.ldl,
                                ws.piece * s.ldn()};
-      PO_TRY((launch_planned<KIND, E>(a, e, plan_of<E>(a), st, what)));
+      PO_TRY((launch_planned<KIND, P, E>(a, e, plan_of<E>(a), st, what)));
     }
     // the piece's w, and once h, the other way round
     const TransposeJob tw{reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, rp, 0, ws.wt, ws.ldl, D * ws.ldl};
@@ -869,13 +874,13 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
       a.B = Operand{reinterpret_cast<char*>(ws.dl), ws.ldl * 2, N * ws.ldl * 2, N};
       a.kbytes = rp * 2;
       // the last piece may have fewer steps than slices: the other slabs keep their sums
-      const Plan p{ws.dh_plan.tile, std::min(ws.dh_plan.slices, ceil_div(a.kbytes, 128) * a.pairs), 0};
+      const Plan p{ws.dh_plan.tile, std::min(ws.dh_plan.slices, ceil_div(a.kbytes, P == 3 ? 64 : 128)), 0};
       if (ws.direct_dh) {
         const typename GradEpi<OUT>::Args ge{dh, lddh, g, N, D, (uintptr_t)dh % 16 == 0 && lddh * es % 16 == 0};
-        PO_TRY((launch_planned<KIND, GradEpi<OUT>>(a, ge, p, st, what)));
+        PO_TRY((launch_planned<KIND, P, GradEpi<OUT>>(a, ge, p, st, what)));
       } else {
         const SlabEpi::Args se{ws.slab, ws.slab_ld, ws.slab_slice, N, D, v > 0};
-        PO_TRY((launch_planned<KIND, SlabEpi>(a, se, p, st, what)));
+        PO_TRY((launch_planned<KIND, P, SlabEpi>(a, se, p, st, what)));
       }
     }
     if (dw) {                                                // dw[v][d] = sum_n dl[n][v] h[n][d]
@@ -884,7 +889,7 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
       a.kbytes = (int)s.Np() * 2;
       char* out = static_cast<char*>(dw) + v * lddw * es;
       const typename GradEpi<OUT>::Args ge{out, lddw, g, rows, D, (uintptr_t)out % 16 == 0 && lddw * es % 16 == 0};
-      PO_TRY((launch_planned<KIND, GradEpi<OUT>>(a, ge, plan_of<GradEpi<OUT>>(a), st, what)));
+      PO_TRY((launch_planned<KIND, P, GradEpi<OUT>>(a, ge, plan_of<GradEpi<OUT>>(a), st, what)));
     }
   }
   if (dh && !ws.direct_dh) {
