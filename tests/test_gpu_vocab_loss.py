@@ -98,6 +98,24 @@ def test_losses_and_gradients(N, V, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", [(1100, 9001, 513), (2050, 16001, 385), (700, 33001, 520), (300, 20000, 1030)])
+def test_large_tiles(N, V, D, dtype):
+    """Sizes of whole rounds of the largest tiles with ragged ends, the rest in smaller ones, k cut in slices."""
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w, t = inputs(N, V, D, dtype)
+    h.requires_grad_()
+    w.requires_grad_()
+    g = (64.0 if dtype == torch.float16 else 1.0) * (0.5 + torch.arange(N, device=DEV) % 7 / 7)
+    loss = lce(h, w, t, reduction="none")
+    dh, dw = torch.autograd.grad(loss, (h, w), g)
+    ref = reference(h.detach(), w.detach(), t, g)
+    b = bounds(ref, dtype, N, V, D)
+    within(loss.detach(), ref["loss"], b["loss"], "loss")
+    within(dh, ref["dh"], b["dh"], "dh")
+    within(dw, ref["dw"], b["dw"], "dw")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("reduction", ["sum", "mean"])
 @pytest.mark.parametrize("frozen,N", [("", 150), ("hidden", 150), ("weight", 150), ("", 1), ("", 40), ("weight", 640), ("", 2500)])
 def test_reductions_and_frozen_sides(dtype, reduction, frozen, N):
