@@ -144,6 +144,12 @@ _SIGS = {
                          c_int64, c_void_p],
     "po_linear_ce_workspace": [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_int, c_int,
                                ctypes.POINTER(c_int64), ctypes.POINTER(c_int64)],
+    "po_linear_ce_frozen_workspace": [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64,
+                                      ctypes.POINTER(c_int64)],
+    "po_linear_ce_frozen_fwd": [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                                c_float, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p],
+    "po_linear_ce_frozen_bwd": [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p,
+                                c_int64, c_void_p],
     "po_quantize_rows": [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p],
     "po_int8_matmul": [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                        c_void_p, c_int64, c_int, c_void_p],

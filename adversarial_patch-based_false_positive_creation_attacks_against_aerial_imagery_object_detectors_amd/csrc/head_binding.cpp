@@ -39,6 +39,9 @@ struct Entries {
   decltype(&po_linear_ce_fwd) ce_fwd;
   decltype(&po_linear_ce_bwd) ce_bwd;
   decltype(&po_linear_ce_workspace) ce_workspace;
+  decltype(&po_linear_ce_frozen_fwd) ce_frozen_fwd;
+  decltype(&po_linear_ce_frozen_bwd) ce_frozen_bwd;
+  decltype(&po_linear_ce_frozen_workspace) ce_frozen_workspace;
   decltype(&po_int8_linear) int8_linear;
 } lib{};
 
@@ -57,6 +60,9 @@ void bind(const std::string& path) {
   take(e.ce_fwd, "po_linear_ce_fwd");
   take(e.ce_bwd, "po_linear_ce_bwd");
   take(e.ce_workspace, "po_linear_ce_workspace");
+  take(e.ce_frozen_fwd, "po_linear_ce_frozen_fwd");
+  take(e.ce_frozen_bwd, "po_linear_ce_frozen_bwd");
+  take(e.ce_frozen_workspace, "po_linear_ce_frozen_workspace");
   take(e.int8_linear, "po_int8_linear");
   lib = e;
 }
@@ -252,23 +258,35 @@ constexpr int64_t kMostStride = 1 << 21;
 
 struct CeForward {
   Tensor loss, target, stat;                                  // stat: [N][2] statistics, then the count
+  Tensor dhu;                                                 // frozen: the embeddings' gradient, [N][D up to a multiple of 4]
 };
 
 CeForward ce_forward(const Tensor& hidden, const Tensor& weight, const Tensor& target, int64_t ignore, int64_t reduction,
-                     double scale) {
+                     double scale, bool frozen = false) {
   On on({&hidden, &weight, &target});
   const Rows h(hidden, kMostStride), w(weight, kMostStride);
   const auto f32 = hidden.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
   CeForward r;
   r.target = target.reshape({-1}).contiguous();
   r.loss = reduction == 0 ? at::empty(target.sizes(), f32) : at::empty({}, f32);
-  r.stat = at::empty({2 * h.rows + 1}, f32);
+  r.stat = at::empty({frozen ? 1 : 2 * h.rows + 1}, f32);
+  if (frozen) r.dhu = at::empty({h.rows, (h.cols + 3) / 4 * 4}, f32);
   if (h.rows == 0) {
     if (reduction) r.loss.fill_(reduction == 2 ? std::numeric_limits<double>::quiet_NaN() : 0.0);
     return r;
   }
   int64_t bytes = 0;
   const int dt = dtype_of(hidden);
+  if (frozen) {
+    check(lib.ce_frozen_workspace(h.t.data_ptr(), h.ld, w.t.data_ptr(), w.ld, dt, h.rows, w.rows, h.cols, &bytes),
+          "po_linear_ce_frozen_workspace");
+    const Tensor ws = at::empty({bytes}, f32.dtype(at::kByte));
+    check(lib.ce_frozen_fwd(h.t.data_ptr(), h.ld, w.t.data_ptr(), w.ld, dt, h.rows, w.rows, h.cols,
+                            r.target.const_data_ptr<int64_t>(), ignore, (float)scale, (int)reduction, ws.data_ptr(), bytes,
+                            r.loss.data_ptr<float>(), r.stat.data_ptr<float>(), r.dhu.data_ptr<float>(), on.stream),
+          "po_linear_ce_frozen_fwd");
+    return r;
+  }
   check(lib.ce_workspace(h.t.data_ptr(), h.ld, w.t.data_ptr(), w.ld, dt, h.rows, w.rows, h.cols, 0, 0, &bytes, nullptr),
         "po_linear_ce_workspace");
   const Tensor ws = at::empty({bytes}, f32.dtype(at::kByte));
@@ -283,8 +301,8 @@ CeForward ce_forward(const Tensor& hidden, const Tensor& weight, const Tensor& t
 struct LinearCe : torch::autograd::Function<LinearCe> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& target,
                         int64_t ignore, int64_t reduction, double scale) {
-    CeForward r = ce_forward(hidden, weight, target, ignore, reduction, scale);
-    ctx->save_for_backward({hidden, weight, r.target, r.stat});
+    CeForward r = ce_forward(hidden, weight, target, ignore, reduction, scale, !weight.requires_grad());
+    ctx->save_for_backward({hidden, weight, r.target, r.stat, r.dhu});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["scale"] = scale;
@@ -299,8 +317,12 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
     const bool again = wants_grad(grads[0], hidden) || wants_grad(weight, Tensor());
     {
       at::AutoGradMode off(false);
-      run(hidden, weight, target, stat, grads[0], ctx->saved_data["ignore"].toInt(), ctx->saved_data["reduction"].toInt(),
-          ctx->saved_data["scale"].toDouble(), need_h ? &out[0] : nullptr, need_w ? &out[1] : nullptr);
+      const int64_t ignore = ctx->saved_data["ignore"].toInt(), reduction = ctx->saved_data["reduction"].toInt();
+      if (saved[4].defined())
+        out[0] = scaled(hidden, saved[4], target, stat, grads[0], ignore, reduction);
+      else
+        run(hidden, weight, target, stat, grads[0], ignore, reduction, ctx->saved_data["scale"].toDouble(),
+            need_h ? &out[0] : nullptr, need_w ? &out[1] : nullptr);
     }
     if (again) {                                              // gradients of second order: refused where they are asked for
       auto no = std::make_shared<torch::autograd::DelayedError>("linear_cross_entropy has no gradient of second order", 4);
@@ -309,6 +331,19 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
       out[1] = marked[1];
     }
     return out;
+  }
+  // a frozen vocabulary's gradient of the embeddings: made in the forward pass
+  static Tensor scaled(const Tensor& hidden, const Tensor& dhu, const Tensor& target, const Tensor& count, const Tensor& grad,
+                       int64_t ignore, int64_t reduction) {
+    On on({&hidden, &dhu, &grad});
+    Tensor dh = at::empty(hidden.sizes(), hidden.options().memory_format(at::MemoryFormat::Contiguous));
+    if (target.numel() == 0) return dh;
+    const Tensor g = grad.reshape({-1}).contiguous();
+    const int64_t D = hidden.size(-1);
+    check(lib.ce_frozen_bwd(dhu.data_ptr<float>(), dtype_of(hidden), target.numel(), D, target.const_data_ptr<int64_t>(), ignore,
+                            (int)reduction, count.data_ptr<float>(), g.const_data_ptr<float>(), dh.data_ptr(), D, on.stream),
+          "po_linear_ce_frozen_bwd");
+    return dh;
   }
   static void run(const Tensor& hidden, const Tensor& weight, const Tensor& target, const Tensor& stat, const Tensor& grad,
                   int64_t ignore, int64_t reduction, double scale, Tensor* dh, Tensor* dw) {

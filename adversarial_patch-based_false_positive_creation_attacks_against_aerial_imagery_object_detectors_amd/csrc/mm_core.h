@@ -99,15 +99,91 @@ struct Loader {
   }
 };
 
+// B may hold, in place of numbers, their multiples by powers of two that differ from one 128 of k to the
+// next (a block): those of block b in row n are 2^-r times the numbers, r = ref[b][n] a whole number
+// (-infinity: all zero).  Refs keeps the sums of a column as multiples of 2^-(the last block's r): where r
+// changes the sums are multiplied by 2^(old - new), exactly.  A block whose r lies 48 below
+// the column's largest so far is left out: its numbers are below 2^-48 of that block's largest
+// one, and sums that followed r downwards without end would overflow.  A tile's references
+// come to LDS by the loads that bring its operands.
+struct NoRefs {
+  static constexpr bool on = false;
+};
+template <class C>
+struct Refs {
+  static constexpr bool on = true;
+  static constexpr int SLOTS = 4, COLS = C::TN * 16;         // four: blocks of single steps, two steps ahead
+  static constexpr int LDS = SLOTS * 1024 + C::NW * COLS * 8;
+  static_assert(C::KG == 1 && C::BN <= 256, "one group's sums, a tile's references in one load");
+  const char* p;                                             // of block 0 and the tile's first column
+  int64_t ld;                                                // bytes from block to block
+  int cols;                                                  // columns there
+  char* lds;
+  int wave, wn, lane;
+  int issued = 0, taken = 0;
+  uint32_t left_out = 0;                                     // bit j: this lane's column j of the block
+  bool any = false;                                          // some lane's
+  // this wave's columns: r of the sums, then the largest so far (in LDS: LARGE has no registers left)
+  __device__ __forceinline__ float* state() const { return reinterpret_cast<float*>(lds + SLOTS * 1024) + wave * COLS * 2; }
+  __device__ __forceinline__ float last(int j) const { return state()[j * 16 + (lane & 15)]; }
+  __device__ __forceinline__ void start() {
+    for (int i = lane; i < COLS * 2; i += 64) state()[i] = -INFINITY;
+  }
+  __device__ __forceinline__ void load(int block) {
+    if (wave == 0) {
+      const __amdgpu_buffer_rsrc_t rs =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p + block * ld), 0, 0x7fffffff, 0x00020000);
+      Loader<C>::dma(rs, lds + (issued % SLOTS) * 1024, lane * 4 < C::BN && lane * 4 < cols ? (uint32_t)lane * 16 : kOOB);
+    }
+    ++issued;
+  }
+  static __device__ __forceinline__ float pow2(float d) { return __builtin_amdgcn_ldexpf(1.f, (int)fmaxf(d, -300.f)); }
+  __device__ __forceinline__ void take(f4v (&acc)[C::TM][C::TN]) {
+    const float* slot = reinterpret_cast<const float*>(lds + (taken % SLOTS) * 1024) + wn * COLS;
+    float* st = state();
+    ++taken;
+    float by[C::TN];
+    bool change = false;
+    left_out = 0;
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      const int c = j * 16 + (lane & 15);
+      const float r = slot[c], old = st[c], top = st[COLS + c];
+      const bool out = r == -INFINITY || r < top - 48.f;
+      left_out |= (uint32_t)out << j;
+      by[j] = out || old == -INFINITY ? 1.f : pow2(old - r);
+      change |= by[j] != 1.f;
+      if (!out && lane < 16) {
+        st[c] = r;
+        st[COLS + c] = fmaxf(top, r);
+      }
+    }
+    any = __any(left_out != 0);
+    if (__any(change)) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) acc[i][j] *= by[j];
+    }
+  }
+  __device__ __forceinline__ void mask(i4v (&b)[C::TN]) const {
+    if (any) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+        if (left_out >> j & 1) b[j] = i4v{0, 0, 0, 0};
+    }
+  }
+};
+
 // acc += the tile's product over the k-steps [ks0, ks1) of the plane pairs.
 // Planes: an operand of wider numbers is stored as `planes` 16-bit matrices, and
 // the step index runs over pairs of them: pair q multiplies plane (pa >> 4q & 15)
 // of A with plane (pb >> 4q & 15) of B; steps [q * nk, (q + 1) * nk) are pair q's.
 // kbytes: length of a row; ends inside a step read as zero.  ks1 > ks0.
-template <class C>
+template <class C, class RefsT>
 __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM][C::TN], const Operand& A,
                                         const Operand& B, int m0, int n0, int kbytes, int ks0, int ks1, int nk,
-                                        uint32_t pa, uint32_t pb, char* lds) {
+                                        uint32_t pa, uint32_t pb, char* lds, RefsT& refs) {
   constexpr int KB = C::KB, CPR = KB / 16;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = wid % C::NW, kg = wid / C::NW;
@@ -134,7 +210,12 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
   const char* abase = A.p + (int64_t)m0 * A.stride;
   const char* bbase = B.p + (int64_t)n0 * B.stride;
   int next = ks0 + kg, q = next / nk, kt = next - q * nk;    // the next stage's step, its plane pair and place in it
+  int place = kt;                                            // of the step that is multiplied (one group)
+  constexpr int PER = 256 / KB;                              // steps of a block of references
+  if constexpr (RefsT::on) refs.start();
   auto issue = [&](int buf) {
+    if constexpr (RefsT::on)
+      if (kt % PER == 0 || next == ks0) refs.load(kt / PER);  // ahead of the operands: the waits below count them
     const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<char*>(abase + (int64_t)((pa >> (4 * q)) & 15) * A.plane), 0, 0x7fffffff, 0x00020000);
     const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
@@ -207,13 +288,22 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
     __builtin_amdgcn_sched_barrier(0);
     fetch(buf, 0, fa[0], fb[0]);
     if constexpr (!first) multiply(fa[1], fb[1]);            // the last group of the step before
+    if constexpr (RefsT::on) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (first || place % PER == 0) refs.take(acc);
+      refs.mask(fb[0]);
+      place = place + 1 == nk ? 0 : place + 1;
+    }
 #pragma unroll
     for (int g = 1; g < G; ++g) {
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (RefsT::on)
+        if (g > 1) refs.mask(fb[(g & 1) ^ 1]);
       fetch(buf, g, fa[g & 1], fb[g & 1]);
       multiply(fa[(g & 1) ^ 1], fb[(g & 1) ^ 1]);
     }
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (RefsT::on) refs.mask(fb[1]);
     buf = buf + 1 == C::STAGES ? 0 : buf + 1;
   };
   step(std::true_type{});
@@ -248,9 +338,9 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
 // MFMAs where the pairs in turn take 36; fp32 head of 3000 x 5000 x 1500, trained: the four
 // products 1100 -> 980 us, of 512 x 8192 x 256 126 -> 100).  Rows are 64 bytes, four chunks, turned every four rows,
 // so that 8 neighbouring lanes' reads cover all banks.
-template <class C>
+template <class C, class RefsT>
 __device__ __forceinline__ void product3(f4v (&acc)[C::TM][C::TN], const Operand& A, const Operand& B, int m0, int n0,
-                                         int kbytes, int ks0, int ks1, char* lds) {
+                                         int kbytes, int ks0, int ks1, char* lds, RefsT& refs) {
   static_assert(C::KB == 64 && C::PLANES == 3 && C::KG == 1 && C::STAGES == 2, "form");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN, lrow = lane / 4;
@@ -270,7 +360,10 @@ __device__ __forceinline__ void product3(f4v (&acc)[C::TM][C::TN], const Operand
   const char* abase = A.p + (int64_t)m0 * A.stride;
   const char* bbase = B.p + (int64_t)n0 * B.stride;
   constexpr int PA = C::BM * 64, PB = C::BN * 64;            // bytes of a plane of a stage
+  if constexpr (RefsT::on) refs.start();
   auto issue = [&](int buf, int step) {
+    if constexpr (RefsT::on)
+      if (step % 4 == 0 || step == ks0) refs.load(step / 4);
     const uint32_t k0 = (uint32_t)step * 64;
     const uint32_t past = (int)(k0 + lch) < kbytes ? k0 : kOOB;
     char* la = lds + buf * C::STAGE_BYTES;
@@ -333,12 +426,18 @@ __device__ __forceinline__ void product3(f4v (&acc)[C::TM][C::TN], const Operand
     fetch_b(buf, 0, b0);
     if constexpr (!first) multiply(a1, b1, RAB{});                // the last product of the step before
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (RefsT::on) {
+      if (first || s % 4 == 0) refs.take(acc);
+      refs.mask(b0);
+    }
     fetch_b(buf, 2, b2);
     multiply(a0, b0, RB{});
+    if constexpr (RefsT::on) refs.mask(b2);
     fetch_a(buf, 2, a2);
     multiply(a0, b2, RA{});
     fetch_b(buf, 1, b1);
     multiply(a2, b0, RB{});
+    if constexpr (RefsT::on) refs.mask(b1);
     fetch_a(buf, 1, a1);
     multiply(a0, b1, RA{});
     multiply(a1, b0, R0{});
@@ -369,6 +468,13 @@ struct Tile {
   __device__ __forceinline__ int col(int j) const { return n0 + j * 16 + (lane & 15); }
   __device__ __forceinline__ int row(int i) const { return m0 + i * 16 + 4 * (lane >> 4); }   // of element 0
 };
+
+// Epilogues of products whose B has references (Refs) hold kRefs, and say of a tile's columns whether
+// they have any but base.
+template <class Epi, class = void>
+struct HasRefs : std::false_type {};
+template <class Epi>
+struct HasRefs<Epi, std::void_t<decltype(Epi::kRefs)>> : std::true_type {};
 
 struct NoPre {
   template <class T, class E>
@@ -403,13 +509,37 @@ __global__ __launch_bounds__(C::NW * C::KG * 64, C::LDS > 81920 ? 1 : 2) void pr
   pre.load(t, e);
   const int total = a.nk * a.pairs;
   const int ks0 = (int)((int64_t)blockIdx.y * total / gridDim.y), ks1 = (int)((int64_t)(blockIdx.y + 1) * total / gridDim.y);
-  if constexpr (C::PLANES == 3)
-    product3<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, lds);
-  else
-    product<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, a.nk, a.pa, a.pb, lds);
+  auto multiply = [&](auto& refs) {
+    if constexpr (C::PLANES == 3)
+      product3<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, lds, refs);
+    else
+      product<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, a.nk, a.pa, a.pb, lds, refs);
+  };
+  if constexpr (HasRefs<Epi>::value) {
+    // tokens of one r in all of these blocks: an ordinary product
+    float last[C::TN];
+    if (Epi::template plain<C>(t, e)) {
+      NoRefs none;
+      multiply(none);
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) last[j] = t.col(j) < e.N ? e.base[t.col(j)] : 0.f;
+    } else {
+      __shared__ __attribute__((aligned(1024))) char ref_lds[Refs<C>::LDS];
+      const int first_col = t.tn * C::BN;
+      Refs<C> refs{reinterpret_cast<const char*>(e.refs + first_col), e.ldr * 4, (int)e.ldr - first_col, ref_lds, t.wave, t.wn, t.lane};
+      multiply(refs);
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) last[j] = refs.last(j);
+    }
+    Epi::template run<C>(t, e, pre, last);
+    return;
+  } else {
+    NoRefs none;
+    multiply(none);
+  }
   // waves of the other groups end here; barriers below wait for the ones that remain
   if (C::KG > 1 && t.wave >= C::NW) return;
-  Epi::template run<C>(t, e, pre, lds);
+  if constexpr (!HasRefs<Epi>::value) Epi::template run<C>(t, e, pre, lds);
 }
 
 template <class C, class Epi>

@@ -1,5 +1,5 @@
 // Softmax cross entropy of a linear head over a large vocabulary, without its
-// logits in memory (po_linear_ce_fwd / _bwd).
+// logits in memory (po_linear_ce_fwd / _bwd, po_linear_ce_frozen_fwd / _bwd).
 //
 //   l[n][v] = c * h[n] . w[v]        loss[n] = log sum_v exp l[n][v] - l[n][t_n]
 //   dl[n][v] = g_n (exp(l[n][v]) / sum_n - [v = t_n])
@@ -13,6 +13,14 @@
 // vocabulary after the other, the logits again, dl in their place (16 bits, as
 // [n][v] and as [v][n]), then dh += dl w and the piece's rows of dw.  Every
 // product has k contiguous in both operands: w and h are transposed for that.
+//
+// Against a frozen vocabulary dh alone is wanted, and the forward pass can have it: dh_n = c (sum_v
+// exp(l) w - ...) / sum_n needs the exponentials up to a factor of the row.  So a piece's are
+// stored in 16 bits, as multiples of powers of two, and multiplied with its rows at once
+// (KeepEpi, RefSlabEpi); what is left to the backward pass is a scaling.  Two products instead of
+// three: bf16 4096 x 32768 x 1024 784 -> 592 us, 8192 x 100000 x 2048 8.2 -> 5.7 ms,
+// fp32 4096 x 32768 x 1024 3.84 -> 2.80.  With dw this gains nothing: dw's terms need
+// the rows' whole sums first.
 //
 // Types.  16-bit inputs: exact products, sums in 32 bits; dl is rounded to the
 // inputs' type once, as an operand of the matrix cores: half a step against
@@ -273,6 +281,225 @@ struct DlogitsEpi {
       __builtin_amdgcn_sched_barrier(0);
       if (e.dlt) store_columns<C>(lds, e.dlt + p * e.pt, e.ldt, n0, m0, e.Np, e.V);
       __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
+// The forward pass of a frozen vocabulary: StatsEpi's statistics, and the exponentials themselves, of
+// a piece, as [n][v]: exp(l) = 2^r E, E <= 1.  r is the tile's largest l * log2e of a token, rounded up; bf16
+// has the range for one r in most tiles, base, with which the next product is an ordinary one
+// (4096 x 32768 x 1024: 221 us, 272 with every tile's own): 2^40 over the target's exponential, which
+// is one of the row's, so that what E loses below 2^-126 is below 2^-86 of the row's sum.
+// fp16: 2^15 E, normal from 2^-29 on.  The target's E is left out: its part of
+// the gradient, p_t - 1, is made in 32 bits.  refs[v / 128][n] = r (-infinity where all E are 0); other[v / 128][n / 32]: there is
+// one beside base among those.
+template <int KIND, int PLANES>
+struct KeepEpi {
+  static constexpr Ends kEnds{6. * PLANES, PLANES > 1 ? 30. : 15., false};
+  static constexpr float kLift = KIND == F16 ? 15.f : 0.f;
+  // a tile's r, from its largest l * log2e; base: frozen_base_k's
+  static __device__ __forceinline__ float reference(float top, float base) {
+    return base == INFINITY ? 0.f : top <= base ? base : __builtin_ceilf(top);
+  }
+  struct Args {
+    StatsEpi::Args s;
+    const float* base;          // frozen_base_k's of the tokens; null: a tile's own r
+    float* refs;                // of this launch's first 128 vocabulary rows
+    uint8_t* other;
+    int64_t ldr, ldo;
+    int Vp;                     // vocabulary rows of the launch as laid out
+    uint16_t* kept;             // [N][ld]; planes behind each other
+    int64_t ld, plane;
+  };
+  template <class C>
+  using Pre = NoPre;
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& a, const NoPre&, char* lds) {
+    float(*const mine)[C::BN] = reinterpret_cast<float(*)[C::BN]>(lds);                // [WM]: maxima, then [WM]: sums
+    const StatsEpi::Args& e = a.s;
+    typename StatsEpi::Pre<C> pre;                           // read here: LARGE has no registers for it in the loop
+    pre.load(t, e);
+    float base[C::TN];
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) base[j] = a.base && t.col(j) < e.N ? a.base[t.col(j)] : __uint_as_float(0x7fc00000u);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *e.arrived = 0;
+    if (t.m0 + C::TM * 16 > e.V) {
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (t.row(i) + k >= e.V) {
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j) t.acc[i][j][k] = -INFINITY;
+          }
+    }
+    float mx[C::TN];
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+      mx[j] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[j] = fmaxf(mx[j], t.acc[i][j][k]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) mx[j] = column_max(mx[j]);
+    __syncthreads();                                         // the loop's reads are over
+    const int c0 = t.wn * C::TN * 16 + (t.lane & 15);
+    if (t.lane < 16) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) mine[t.wm][c0 + j * 16] = mx[j];
+    }
+    __syncthreads();
+    float s[C::TN];
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      __builtin_amdgcn_sched_barrier(0);
+      float top = mine[0][c0 + j * 16];
+#pragma unroll
+      for (int w = 1; w < C::WM; ++w) top = fmaxf(top, mine[w][c0 + j * 16]);
+      top = reference(top * e.k, base[j]);
+      const bool none = base[j] == INFINITY;  // the row takes no part
+      const float ref = (top == -INFINITY ? 0.f : top) - kLift;
+      const bool has = pre.at[j] >= 0 && ((pre.at[j] >> 2) & 3) == t.lane >> 4;
+      if (__any(has)) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (pre.at[j] == i * 16 + 4 * (t.lane >> 4) + k) x = t.acc[i][j][k];
+        if (has) e.tlogit[t.col(j)] = x;
+      }
+      s[j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][k], e.k, -ref));
+          t.acc[i][j][k] = none ? 0.f : x;
+          s[j] += t.acc[i][j][k];
+        }
+      if (__any(has)) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (pre.at[j] == i * 16 + 4 * (t.lane >> 4) + k) t.acc[i][j][k] = 0.f;
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) s[j] = column_sum(s[j]);
+    if (t.lane < 16) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) mine[C::WM + t.wm][c0 + j * 16] = s[j];
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < C::BN; x += C::NW * 64) {
+      float top = mine[0][x], sum = mine[C::WM][x];
+#pragma unroll
+      for (int w = 1; w < C::WM; ++w) {
+        top = fmaxf(top, mine[w][x]);
+        sum += mine[C::WM + w][x];
+      }
+      const int n = t.tn * C::BN + x;
+      bool is_other = false;
+      if (n < e.N) {
+        const float base = a.base ? a.base[n] : __uint_as_float(0x7fc00000u);
+        top = reference(top * e.k, base);
+        is_other = top != base && base != INFINITY;
+        e.partial[(int64_t)(e.tile0 + t.tm) * e.N + n] = make_float2(top, sum * (kLift ? 0x1p-15f : 1.f));
+        // an infinite maximum: E is NaN, and the sums with it, whatever they are multiples of
+#pragma unroll
+        for (int b = 0; b < C::BM / 128; ++b)
+          a.refs[(int64_t)(t.tm * (C::BM / 128) + b) * a.ldr + n] = top == INFINITY ? 0.f : top;
+      }
+      const uint64_t others = __ballot(is_other);
+      if (t.lane % 32 == 0 && n < e.N) {
+#pragma unroll
+        for (int b = 0; b < C::BM / 128; ++b)
+          a.other[(int64_t)(t.tm * (C::BM / 128) + b) * a.ldo + n / 32] = (uint8_t)((uint32_t)(others >> t.lane) != 0);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < PLANES; ++q) {
+      __syncthreads();                                       // the loop's (or the last plane's) reads are over
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) {
+          u2v w;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float x = t.acc[i][j][2 * k], y = t.acc[i][j][2 * k + 1];
+            w[k] = pack2<KIND>(x, y);
+            if constexpr (PLANES > 1) {                      // what this plane leaves to the next
+              t.acc[i][j][2 * k] = x - __uint_as_float(w[k] << 16);
+              t.acc[i][j][2 * k + 1] = y - __uint_as_float(w[k] & 0xffff0000u);
+            }
+          }
+          stage4(t, lds, i, j, w);
+        }
+      }
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+      store_rows<C>(lds, a.kept + q * a.plane, a.ld, t.tn * C::BN, t.tm * C::BM, e.N, a.Vp, true);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
+// The sums of a product with references: slab[slice][n][m] (+)= acc, with the power of two of a slice's
+// row in out_refs[slice][n] (in_refs: of what the slab holds).
+struct RefSlabEpi {
+  static constexpr Ends kEnds{8, 12, true};
+  static constexpr bool kRefs = true;
+  struct Args {
+    const float *refs, *base;   // [k / 128][ldr], [N]
+    const uint8_t* other;       // [k / 128][ldo]
+    int64_t ldr, ldo;
+    int blocks;
+    float* slab;
+    int64_t ld, slice;          // ld a multiple of 4
+    int N, M;
+    const float* in_refs;       // [slices][ldr], null: the slab holds nothing
+    float* out_refs;
+  };
+  template <class C>
+  using Pre = NoPre;
+  template <class C>
+  static __device__ __forceinline__ bool plain(const Tile<C>& t, const Args& e) {
+    constexpr int PER = C::BN / 32;
+    const int first = t.tn * PER, here = min(PER, (int)e.ldo - first);
+    int other = 0;
+    for (int i = threadIdx.x; i < e.blocks * PER; i += C::NW * 64)
+      if (i % PER < here) other |= e.other[(int64_t)(i / PER) * e.ldo + first + i % PER];
+    return !__syncthreads_or(other);
+  }
+  template <class C>
+  static __device__ __forceinline__ void run(Tile<C>& t, const Args& e, const Pre<C>&, const float (&last)[C::TN]) {
+    float* out = e.slab + blockIdx.y * e.slice;
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      __builtin_amdgcn_sched_barrier(0);                     // a column block at a time: the accumulators fill the registers
+      const int n = t.col(j);
+      if (n >= e.N) continue;
+      const float mine = last[j], held = e.in_refs ? e.in_refs[blockIdx.y * e.ldr + n] : -INFINITY;
+      const float r = fmaxf(mine, held);
+      // sums of nothing but zeros have no power of two
+      const float fm = mine == -INFINITY ? 0.f : Refs<C>::pow2(mine - r), fh = held == -INFINITY ? 0.f : Refs<C>::pow2(held - r);
+      if (t.tm == 0 && t.wm == 0 && t.lane < 16) e.out_refs[blockIdx.y * e.ldr + n] = r;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const int m = t.row(i);
+        if (m >= e.ld) continue;
+        f4v* o = reinterpret_cast<f4v*>(out + (int64_t)n * e.ld + m);
+        *o = e.in_refs ? *o * fh + t.acc[i][j] * fm : t.acc[i][j];
+      }
     }
   }
 };
@@ -557,6 +784,31 @@ __global__ __launch_bounds__(256) void transpose_k(const TransposeJob j0, const 
   store_columns<Pane>(lds, j.out + blockIdx.z * j.oplane, j.ldo, r0, c0, j.Rp, Cc);
 }
 
+// four neighbours in the gradients' type (OUT: BF16, F16, or 3: fp32), those below cols
+template <int OUT>
+__device__ __forceinline__ void put4(void* out, int64_t at, int cols, int wide, f4v v) {
+  if constexpr (OUT == 3) {
+    float* o = static_cast<float*>(out) + at;
+    if (wide && cols >= 4) {
+      *reinterpret_cast<f4v*>(o) = v;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < cols) o[k] = v[k];
+    }
+  } else {
+    const u2v w = {pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
+    uint16_t* o = static_cast<uint16_t*>(out) + at;
+    if (wide && cols >= 4) {
+      *reinterpret_cast<u2v*>(o) = w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < cols) o[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+    }
+  }
+}
+
 // dh[n][m] = g.end() * the slabs' sum, slab after slab; a thread makes 4 columns
 template <int OUT>
 __global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab, int slices, int64_t slice, int64_t ld,
@@ -572,26 +824,105 @@ __global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab
 #pragma unroll 4
     for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const f4v*>(p + s * slice);
     v *= f;
-    if constexpr (OUT == 3) {
-      float* o = static_cast<float*>(out) + n * ldo + m;
-      if (wide && m + 4 <= M) {
-        *reinterpret_cast<f4v*>(o) = v;
-      } else {
+    put4<OUT>(out, n * ldo + m, M - m, wide, v);
+  }
+}
+
+// base[n] = the target's l * log2e, rounded, and 40 (KeepEpi); infinity: the row takes no part; NaN: that
+// logit is no number that exponents can be taken against.  A wave to a row.
+template <typename T>
+__global__ __launch_bounds__(256) void frozen_base_k(const T* __restrict__ h, int64_t ldh, const T* __restrict__ w, int64_t ldw,
+                                                     int N, int64_t V, int D, const int64_t* __restrict__ target,
+                                                     int64_t ignore, float k, float* __restrict__ base) {
+  const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (n >= N) return;
+  const int64_t t = target[n];
+  const bool in = t != ignore && t >= 0 && t < V;
+  auto number = [](T x) {
+    if constexpr (sizeof(T) == 4) return x;
+    else return __uint_as_float((uint32_t)x << 16);
+  };
+  float sum = 0.f;
+  if (in) {
+    typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    const T *p = h + n * ldh, *q = w + t * ldw;
+    for (int d = lane * 8; d < D; d += 512) {
+      if (d + 8 <= D) {
+        const v8 x = *reinterpret_cast<const v8*>(p + d), y = *reinterpret_cast<const v8*>(q + d);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (m + k < M) o[k] = v[k];
-      }
-    } else {
-      const u2v w = {pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
-      uint16_t* o = static_cast<uint16_t*>(out) + n * ldo + m;
-      if (wide && m + 4 <= M) {
-        *reinterpret_cast<u2v*>(o) = w;
+        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(number(x[i]), number(y[i]), sum);
       } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (m + k < M) o[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+        for (int i = d; i < D; ++i) sum = __builtin_fmaf(number(p[i]), number(q[i]), sum);
       }
     }
+  }
+#pragma unroll
+  for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+  sum = __builtin_rintf(sum * k);
+  if (lane == 0) base[n] = !in ? INFINITY : fabsf(sum) < INFINITY ? sum + 40.f : __uint_as_float(0x7fc00000u);
+}
+
+// A frozen vocabulary's gradient of the embeddings, of an upstream gradient of 1, in fp32:
+// dhu[n][m] = c (sum over the slabs of 2^(r - M) / S - (1 - p_t) w[t][m]), with S 2^M the row's
+// sum of exponentials; rows that take no part 0, rows whose target is none NaN.  A thread makes 4 columns.
+template <typename T, bool HALF>
+__global__ __launch_bounds__(256) void frozen_dh_k(const float* __restrict__ slab, int slices, int last_slices, int64_t slice,
+                                                   int64_t ld, int N, int M, const float* __restrict__ refs,
+                                                   const float* __restrict__ refs_before, int64_t ldr, float lift,
+                                                   const float2* __restrict__ stat, const float* __restrict__ tlogit,
+                                                   const int64_t* __restrict__ target, int64_t ignore, int64_t V, float k, float c,
+                                                   const T* __restrict__ w, int64_t ldw, float* dhu) {
+  const int per = (int)(ld / 4);
+  const int64_t total = (int64_t)N * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = i / per;
+    const int m = (int)(i - n * per) * 4;
+    const int64_t t = target[n];
+    f4v v = {0, 0, 0, 0};
+    if (t != ignore) {
+      const float2 st = stat[n];
+      const float* p = slab + n * ld + m;
+#pragma unroll 4
+      for (int s = 0; s < slices; ++s) {
+        // the last piece of the vocabulary may have reached fewer slabs
+        const float r = (s < last_slices ? refs : refs_before)[s * ldr + n];
+        const float f = r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - st.x) * lift;
+        v += *reinterpret_cast<const f4v*>(p + s * slice) * f;
+      }
+      const bool in = t >= 0 && t < V;
+      const float rest = in ? 1.f - __builtin_amdgcn_exp2f(__builtin_fmaf(tlogit[n], k, -st.x)) * st.y : __uint_as_float(0x7fc00000u);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float x = 0.f;
+        if (in && m + q < M) {
+          const T b = w[t * ldw + m + q];
+          if constexpr (sizeof(T) == 4) x = b;
+          else if constexpr (HALF) x = (float)__builtin_bit_cast(_Float16, b);
+          else x = __uint_as_float((uint32_t)b << 16);
+        }
+        v[q] = c * (v[q] * st.y - rest * x);
+      }
+    }
+    *reinterpret_cast<f4v*>(dhu + n * ld + m) = v;
+  }
+}
+
+// dh[n][m] = g_n dhu[n][m] (GradOf's rules of rows that take no part)
+template <int OUT>
+__global__ __launch_bounds__(256) void frozen_scale_k(const float* __restrict__ dhu, int64_t ld, int N, int M,
+                                                      const int64_t* __restrict__ target, int64_t ignore,
+                                                      const float* __restrict__ grad, int each, const float* __restrict__ count,
+                                                      void* __restrict__ out, int64_t ldo, int wide) {
+  const int per = (int)(ld / 4);
+  const int64_t total = (int64_t)N * per;
+  const float over = count ? fmaxf(*count, 1.f) : 1.f;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = i / per;
+    const int m = (int)(i - n * per) * 4;
+    const float g = grad[each ? n : 0] / over;
+    f4v v = *reinterpret_cast<const f4v*>(dhu + n * ld + m) * g;
+    if (target[n] == ignore || g == 0.f) v = f4v{0, 0, 0, 0};
+    put4<OUT>(out, n * ldo + m, M - m, wide, v);
   }
 }
 
@@ -702,6 +1033,46 @@ struct BwdWs {
   }
 };
 
+struct FrozenWs {
+  float2 *partial, *stat;
+  double* sums;
+  uint32_t* arrived;
+  float *tlogit, *base, *refs, *slab_refs, *slab;
+  uint8_t* other;
+  uint16_t *hp, *wp, *wt, *kept;
+  int64_t piece, ldk, ldr, ldo, slab_ld, slab_slice, bytes;
+  Plan plan;
+  FrozenWs(const Shape& s, void* b) {
+    Layout l(b);
+    const int P = s.planes();
+    piece = piece_rows(s.V, (s.direct_w ? 0 : s.ldp() * 2 * P) + (s.N + s.D) * 2 * P);
+    ldk = padded(piece);
+    ldr = (s.N + 3) / 4 * 4;
+    int64_t parts = 0;
+    for (int64_t v = 0; v < s.V; v += piece) parts += ceil_div(std::min(piece, s.V - v), 128);
+    partial = l.take<float2>(parts * s.N);
+    stat = l.take<float2>(s.N);
+    tlogit = l.take<float>(s.N);
+    sums = l.take<double>(2 * s.N);
+    arrived = l.take<uint32_t>(1);
+    base = l.take<float>(s.N);
+    refs = l.take<float>(ceil_div(piece, 256) * 2 * ldr);
+    ldo = ceil_div(s.N, 32);
+    other = l.take<uint8_t>(ceil_div(piece, 256) * 2 * ldo);
+    hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.ldp() * P);
+    wp = l.take<uint16_t>(s.direct_w ? 0 : piece * s.ldp() * P);
+    wt = l.take<uint16_t>(s.D * ldk * P);
+    kept = l.take<uint16_t>(s.N * ldk * P);
+    slab_ld = (s.D + 3) / 4 * 4;
+    slab_slice = s.N * slab_ld;
+    plan = plan_product(s.D, s.N, (int64_t)ceil_div(ldk * 2, 128) * (P == 3 ? 6 : 1), RefSlabEpi::kEnds, P == 3, kSlabSlices,
+                        slab_slice * 8 / 4e6);
+    slab_refs = l.take<float>(2 * plan.slices * ldr);
+    slab = l.take<float>(plan.slices > 1 ? plan.slices * slab_slice : 0);       // one: the gradient's own place
+    bytes = l.at;
+  }
+};
+
 // pairs of planes, the largest products first: 00 01 10 11 02 20
 inline void set_pairs(Args& a, int planes) {
   a.pairs = planes == 3 ? 6 : 1;
@@ -752,9 +1123,11 @@ inline int check_shape(const char* what, int64_t N, int64_t V, int64_t D, int dt
 template <int KIND, int P, class Epi>
 inline int launch_planned(const Args& a, const typename Epi::Args& e, Plan p, hipStream_t s, const char* what) {
   if (p.tile == FEW) {
-    const int64_t tiles = (int64_t)ceil_div(a.A.rows, 128) * ceil_div(a.B.rows, 32) * p.slices;
-    if (tiles <= 256 && (int64_t)ceil_div(a.kbytes, 128) * a.pairs >= 8 * p.slices)
-      return launch_product<Fewer<KIND>, Epi>(a, e, p.slices, s, what);
+    if constexpr (!HasRefs<Epi>::value) {
+      const int64_t tiles = (int64_t)ceil_div(a.A.rows, 128) * ceil_div(a.B.rows, 32) * p.slices;
+      if (tiles <= 256 && (int64_t)ceil_div(a.kbytes, 128) * a.pairs >= 8 * p.slices)
+        return launch_product<Fewer<KIND>, Epi>(a, e, p.slices, s, what);
+    }
     return launch_product<Few<KIND>, Epi>(a, e, p.slices, s, what);
   }
   if constexpr (P == 3 && Epi::kEnds.tall)
@@ -771,6 +1144,16 @@ inline Plan plan_of(const Args& a) {
 template <class Epi>
 inline int64_t first_part(const Args& a) {
   return whole_rounds(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs, Epi::kEnds, a.pairs > 1);
+}
+
+inline void row_stats(const float2* partial, int parts, const Shape& s, const float* tlogit, const int64_t* target, int64_t ignore,
+                      float k, float2* stat, double* sums, uint32_t* arrived, int reduction, float* loss, float* count,
+                      hipStream_t st) {
+  // total: few workgroups, since each counts itself in (1000 of them: 20 us, 63: 6)
+  const int N = (int)s.N, R = reduction ? (N <= 64 ? 1 : N <= 512 ? 4 : 16) : N <= 256 ? 1 : N <= 2048 ? 4 : 16;
+  hipLaunchKernelGGL((R == 1 ? row_stats_k<1> : R == 4 ? row_stats_k<4> : row_stats_k<16>), dim3(ceil_div(N, R)), dim3(256), 0, st,
+                     partial, parts, N, s.V, tlogit, target, ignore, k, stat, reduction ? nullptr : loss, sums, arrived,
+                     reduction == 2, reduction ? loss : nullptr, count);
 }
 
 #define PO_TRY(x)             \
@@ -826,11 +1209,8 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
       e.tile0 += ceil_div(part, p.tile == LARGE ? 256 : 128);
     }
   }
-  // total: few workgroups, since each counts itself in (1000 of them: 20 us, 63: 6)
-  const int R = reduction ? (N <= 64 ? 1 : N <= 512 ? 4 : 16) : N <= 256 ? 1 : N <= 2048 ? 4 : 16;
-  hipLaunchKernelGGL((R == 1 ? row_stats_k<1> : R == 4 ? row_stats_k<4> : row_stats_k<16>), dim3(ceil_div(N, R)), dim3(256), 0,
-                     st, ws.partial, e.tile0, (int)N, V, ws.tlogit, target, ignore_index, e.k, reinterpret_cast<float2*>(stat),
-                     reduction ? nullptr : loss, ws.sums, ws.arrived, reduction == 2, reduction ? loss : nullptr, count);
+  row_stats(ws.partial, e.tile0, s, ws.tlogit, target, ignore_index, e.k, reinterpret_cast<float2*>(stat), ws.sums, ws.arrived,
+            reduction, loss, count, st);
   return po::check_launch("po_linear_ce_fwd");
 }
 
@@ -927,4 +1307,128 @@ extern "C" int po_linear_ce_bwd(const void* h, int64_t ldh, const void* w, int64
   if (dtype == PO_F16) return backward<F16, F16>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
   if (dtype == PO_BF16) return backward<BF16, BF16>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
   return backward<BF16, 3>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
+}
+
+namespace {
+
+template <int KIND, int P>
+int frozen_forward(const Shape& s, const FrozenWs& ws, const Side& h, const Side& w, const int64_t* target, float k, const float* base,
+                   float* slab, int* parts, int* last_slices, int* pieces, hipStream_t st) {
+  const char* what = "po_linear_ce_frozen_fwd";
+  const int N = (int)s.N, D = (int)s.D;
+  StatsEpi::Args e{ws.partial, ws.arrived, ws.tlogit, target, 0, 0, N, 0, k};
+  *pieces = 0;
+  for (int64_t v = 0; v < s.V; v += ws.piece, ++*pieces) {
+    const int rows = (int)std::min(ws.piece, s.V - v), rp = (rows + 63) / 64 * 64;
+    pack(s, h, v ? 0 : N, w, v, rows, st);
+    const Operand W = rows_of(s, w, v, rows);
+    Args a{};
+    set_pairs(a, P);
+    a.B = rows_of(s, h, 0, N);
+    a.kbytes = s.Dp() * 2;
+    for (int64_t r = 0, part; r < rows; r += part) {
+      using E = KeepEpi<KIND, P>;
+      a.A = W.from(r);
+      part = first_part<E>(a);
+      a.A.rows = (int)part;
+      e.v0 = v + r;
+      e.V = (int)part;
+      const Plan p = plan_of<E>(a);
+      const typename E::Args ke{e, base, ws.refs + r / 128 * ws.ldr, ws.other + r / 128 * ws.ldo, ws.ldr, ws.ldo,
+                                (int)(r + part < rows ? part : rp - r), ws.kept + r, ws.ldk, N * ws.ldk};
+      PO_TRY((launch_planned<KIND, P, E>(a, ke, p, st, what)));
+      e.tile0 += ceil_div(part, p.tile == LARGE ? 256 : 128);
+    }
+    const TransposeJob tw{reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, rp, 0, ws.wt, ws.ldk, D * ws.ldk};
+    const int blocks = ceil_div(rp, 64);
+    hipLaunchKernelGGL(transpose_k, dim3(blocks, ceil_div(D, 256), P), dim3(256), 0, st, tw, tw, blocks, D, GradOf{});
+    a.A = Operand{reinterpret_cast<char*>(ws.wt), ws.ldk * 2, D * ws.ldk * 2, D};
+    a.B = Operand{reinterpret_cast<char*>(ws.kept), ws.ldk * 2, N * ws.ldk * 2, N};
+    a.kbytes = rp * 2;
+    const int64_t half = ws.plan.slices * ws.ldr;
+    const Plan p{ws.plan.tile, std::min(ws.plan.slices, ceil_div(a.kbytes, P == 3 ? 64 : 128)), 0};
+    const RefSlabEpi::Args se{ws.refs, base, ws.other, ws.ldr, ws.ldo, ceil_div(rp, 128), slab, ws.slab_ld, ws.slab_slice, N, D, v ? ws.slab_refs + (*pieces + 1) % 2 * half : nullptr,
+                              ws.slab_refs + *pieces % 2 * half};
+    PO_TRY((launch_planned<KIND, P, RefSlabEpi>(a, se, p, st, what)));
+    *last_slices = p.slices;
+  }
+  *parts = e.tile0;
+  return PO_OK;
+}
+
+}  // namespace
+
+extern "C" int po_linear_ce_frozen_workspace(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N,
+                                             int64_t V, int64_t D, int64_t* bytes) {
+  PO_TRY(check_shape("po_linear_ce_frozen_workspace", N, V, D, dtype, ldh, ldw));
+  PO_REQUIRE(bytes, "po_linear_ce_frozen_workspace: null pointer");
+  *bytes = FrozenWs(Shape{N, V, D, dtype, serves(h, ldh, dtype, D), serves(w, ldw, dtype, D)}, nullptr).bytes;
+  return PO_OK;
+}
+
+extern "C" int po_linear_ce_frozen_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V,
+                                       int64_t D, const int64_t* target, int64_t ignore_index, float scale, int reduction,
+                                       void* workspace, int64_t workspace_bytes, float* loss, float* count, float* dhu,
+                                       po_stream_t stream) {
+  PO_TRY(check_shape("po_linear_ce_frozen_fwd", N, V, D, dtype, ldh, ldw));
+  PO_REQUIRE(h && w && target && workspace && loss && dhu && (reduction == 0 || count), "po_linear_ce_frozen_fwd: null pointer");
+  PO_REQUIRE((uintptr_t)dhu % 16 == 0, "po_linear_ce_frozen_fwd: dhu must start on 16 bytes");
+  PO_REQUIRE(reduction >= 0 && reduction <= 2, "po_linear_ce_frozen_fwd: unknown reduction %d", reduction);
+  PO_REQUIRE(scale > 0.f && scale < INFINITY, "po_linear_ce_frozen_fwd: the scale must be positive and finite");
+  const Shape s{N, V, D, dtype, serves(h, ldh, dtype, D), serves(w, ldw, dtype, D)};
+  const FrozenWs ws(s, workspace);
+  PO_REQUIRE(workspace_bytes >= ws.bytes, "po_linear_ce_frozen_fwd: workspace of %lld bytes, %lld needed",
+             (long long)workspace_bytes, (long long)ws.bytes);
+  const hipStream_t st = po::stream_of(stream);
+  const Side hs{h, ldh, s.direct_h, ws.hp}, wside{w, ldw, s.direct_w, ws.wp};
+  const float k = scale * kLog2e;
+  float* slab = ws.plan.slices > 1 ? ws.slab : dhu;
+  // Its launch costs the host 3 us (500 x 8000 x 384, all the call 72 us or 75) and spares a fifth of
+  // the second product's time: from some 25 us of that on.
+  const float* base = dtype != PO_F16 && (double)N * V * D * (s.planes() == 3 ? 6 : 1) >= 0x1p34 ? ws.base : nullptr;
+  const dim3 rows4(ceil_div(N, 4));
+  if (base && dtype == PO_BF16)
+    hipLaunchKernelGGL((frozen_base_k<uint16_t>), rows4, dim3(256), 0, st, static_cast<const uint16_t*>(h), ldh,
+                       static_cast<const uint16_t*>(w), ldw, (int)N, V, (int)D, target, ignore_index, k, ws.base);
+  if (base && dtype == PO_F32)
+    hipLaunchKernelGGL((frozen_base_k<float>), rows4, dim3(256), 0, st, static_cast<const float*>(h), ldh,
+                       static_cast<const float*>(w), ldw, (int)N, V, (int)D, target, ignore_index, k, ws.base);
+  int parts = 0, last = 0, pieces = 0;
+  PO_TRY((dtype == PO_F16    ? frozen_forward<F16, 1>(s, ws, hs, wside, target, k, base, slab, &parts, &last, &pieces, st)
+          : dtype == PO_BF16 ? frozen_forward<BF16, 1>(s, ws, hs, wside, target, k, base, slab, &parts, &last, &pieces, st)
+                             : frozen_forward<BF16, 3>(s, ws, hs, wside, target, k, base, slab, &parts, &last, &pieces, st)));
+  row_stats(ws.partial, parts, s, ws.tlogit, target, ignore_index, k, ws.stat, ws.sums, ws.arrived, reduction, loss, count, st);
+  const int64_t half = ws.plan.slices * ws.ldr;
+  const float *refs = ws.slab_refs + (pieces - 1) % 2 * half, *before = ws.slab_refs + pieces % 2 * half;
+  const int grid = (int)std::min<int64_t>((N * (ws.slab_ld / 4) + 255) / 256, 8192);
+  const float lift = dtype == PO_F16 ? 0x1p-15f : 1.f;
+#define PO_DH(T, HALF)                                                                                                     \
+  hipLaunchKernelGGL((frozen_dh_k<T, HALF>), dim3(grid), dim3(256), 0, st, slab, ws.plan.slices, last, ws.slab_slice, ws.slab_ld, \
+                     (int)N, (int)D, refs, before, ws.ldr, lift, ws.stat, ws.tlogit, target, ignore_index, V, k, scale,     \
+                     static_cast<const T*>(w), ldw, dhu)
+  if (dtype == PO_F32) PO_DH(float, false);
+  else if (dtype == PO_F16) PO_DH(uint16_t, true);
+  else PO_DH(uint16_t, false);
+#undef PO_DH
+  return po::check_launch("po_linear_ce_frozen_fwd");
+}
+
+extern "C" int po_linear_ce_frozen_bwd(const float* dhu, int dtype, int64_t N, int64_t D, const int64_t* target,
+                                       int64_t ignore_index, int reduction, const float* count, const float* grad, void* dh,
+                                       int64_t lddh, po_stream_t stream) {
+  PO_TRY(check_shape("po_linear_ce_frozen_bwd", N, 1, D, dtype, D, D));
+  PO_REQUIRE(dhu && target && grad && dh && (reduction != 2 || count), "po_linear_ce_frozen_bwd: null pointer");
+  PO_REQUIRE((uintptr_t)dhu % 16 == 0, "po_linear_ce_frozen_bwd: dhu must start on 16 bytes");
+  PO_REQUIRE(reduction >= 0 && reduction <= 2, "po_linear_ce_frozen_bwd: unknown reduction %d", reduction);
+  PO_REQUIRE(lddh >= D, "po_linear_ce_frozen_bwd: bad row strides");
+  const hipStream_t st = po::stream_of(stream);
+  const int64_t ld = (D + 3) / 4 * 4;
+  const int grid = (int)std::min<int64_t>((N * (ld / 4) + 255) / 256, 8192);
+  const int wide = (uintptr_t)dh % 16 == 0 && lddh * (dtype == PO_F32 ? 4 : 2) % 16 == 0;
+  hipLaunchKernelGGL((dtype == PO_F32    ? frozen_scale_k<3>
+                      : dtype == PO_F16 ? frozen_scale_k<F16>
+                                        : frozen_scale_k<BF16>),
+                     dim3(grid), dim3(256), 0, st, dhu, ld, (int)N, (int)D, target, ignore_index, grad, reduction == 0,
+                     reduction == 2 ? count : nullptr, dh, lddh, wide);
+  return po::check_launch("po_linear_ce_frozen_bwd");
 }

@@ -1,11 +1,13 @@
 """Softmax cross entropy of a linear head over a large vocabulary (``po_linear_ce_fwd``
-/ ``_bwd``): the logits are never in memory, neither is their gradient beyond a
+/ ``_bwd``, ``po_linear_ce_frozen_fwd`` / ``_bwd``): the logits are never in memory, neither is their gradient beyond a
 piece of the vocabulary.
 
 Beside the cell loss over a detector's few classes (``train_patch.cell_loss``,
 reference train_patch.py:468-503): the class objective of a head whose classes
-are thousands of embeddings.  With a frozen vocabulary only the embeddings'
-gradient is computed.
+are thousands of embeddings.  Against a frozen vocabulary (a weight that requires no
+gradient) the embeddings' gradient is made in the forward pass, a piece's
+exponentials being at hand there: two products where three would be.  A loss that is
+not differentiated belongs under ``torch.no_grad()``.
 """
 import torch
 import torch.nn as nn

@@ -765,6 +765,21 @@ int po_linear_ce_bwd(const void* h, int64_t ldh, const void* w, int64_t ldw, int
  * bytes) are laid out in them, w piece by piece. */
 int po_linear_ce_workspace(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V,
                            int64_t D, int dh, int dw, int64_t* fwd_bytes, int64_t* bwd_bytes);
+/* The same loss against a frozen vocabulary, with the gradient of the embeddings in the
+ * forward pass: two products where po_linear_ce_fwd and _bwd take three.  A piece's
+ * exponentials (16 bits; fp32 inputs: three planes) are multiplied with its rows
+ * at once, as multiples of a power of two for each token and 128 rows.  dhu fp32
+ * [N][D up to a multiple of 4], on 16 bytes: the gradient for an upstream
+ * gradient of 1 (a row's, or the sum's).  The backward pass scales it: dh [N][D] of
+ * dtype, grad as for po_linear_ce_bwd, count of the forward pass for reduction 2. */
+int po_linear_ce_frozen_workspace(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V,
+                                  int64_t D, int64_t* bytes);
+int po_linear_ce_frozen_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V,
+                            int64_t D, const int64_t* target, int64_t ignore_index, float scale, int reduction,
+                            void* workspace, int64_t workspace_bytes, float* loss, float* count, float* dhu,
+                            po_stream_t s);
+int po_linear_ce_frozen_bwd(const float* dhu, int dtype, int64_t N, int64_t D, const int64_t* target, int64_t ignore_index,
+                            int reduction, const float* count, const float* grad, void* dh, int64_t lddh, po_stream_t s);
 
 /* scale[m] = max_k |x[m][k]| / 127; q[m][k] = x[m][k] / scale[m] rounded to the
  * nearest (the exact quotient; ties to even), zeros up to the next multiple of 16

@@ -115,6 +115,80 @@ def test_large_tiles(N, V, D, dtype):
     within(dw, ref["dw"], b["dw"], "dw")
 
 
+def check_frozen(h, w, t, g, scale=1.0):
+    """Loss and gradient against a frozen vocabulary.  Beside the other bounds: blocks of the vocabulary whose
+    exponentials stay below 2^-48 of another's are left out of dh."""
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h = h.detach().requires_grad_()
+    loss = lce(h, w, t, reduction="none", scale=scale)
+    (dh,) = torch.autograd.grad(loss, h, g, retain_graph=True)
+    ref = reference(h.detach(), w, t, g, scale)
+    b = bounds(ref, h.dtype, h.shape[0], w.shape[0], h.shape[1])
+    within(loss.detach(), ref["loss"], b["loss"] + 2.0 ** -23 * ref["loss"].abs(), "loss")
+    within(dh, ref["dh"], b["dh"] + 2.0 ** -48 * ref["gmax"] * ref["wsum"], "dh")
+    (again,) = torch.autograd.grad(loss, h, g)
+    assert torch.equal(dh, again)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", SIZES + [(1100, 9001, 513), (2050, 16001, 640), (300, 20000, 1030), (8192, 12001, 40)])
+def test_frozen_vocabulary(N, V, D, dtype):
+    h, w, t = inputs(N, V, D, dtype)
+    check_frozen(h, w, t, (64.0 if dtype == torch.float16 else 1.0) * (0.5 + torch.arange(N, device=DEV) % 7 / 7))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", [(70, 5000, 40), (300, 3000, 200), (2100, 9000, 1000)])
+@pytest.mark.parametrize("order", ["up", "down", "mixed"])
+def test_frozen_vocabulary_of_wide_logits(N, V, D, dtype, order):
+    """Largest logits that differ by hundreds from one stretch of the vocabulary to the next, targets anywhere."""
+    h, w, t = inputs(N, V, D, dtype)
+    amp = torch.linspace(0.0, 60.0, V // 128 + 1, device=DEV)
+    if order == "down":
+        amp = amp.flip(0)
+    elif order == "mixed":
+        amp = amp[torch.randperm(len(amp), generator=torch.Generator(device=DEV).manual_seed(N), device=DEV)]
+    w = (w.float() * amp[torch.arange(V, device=DEV) // 128][:, None]).to(dtype)
+    check_frozen(h, w, t, torch.full((N,), 64.0 if dtype == torch.float16 else 1.0, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_frozen_vocabulary_fitted(dtype):
+    """Probabilities of the targets next to 1: what is left of them is the gradient."""
+    N, V, D = 260, 2000, 64
+    h, w, t = inputs(N, V, D, dtype)
+    h = (w.float()[t.clamp(min=0)] * torch.linspace(1.0, 40.0, N, device=DEV)[:, None]).to(dtype)
+    check_frozen(h, w, t, torch.full((N,), 1024.0 if dtype == torch.float16 else 1.0, device=DEV))
+
+
+@pytest.mark.parametrize("N,V,D", [(90, 700, 64), (2600, 9000, 768)])        # below and above the size that takes a common base
+def test_frozen_vocabulary_of_infinite_logits(N, V, D):
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w, t = inputs(N, V, D, torch.bfloat16)
+    w[5], w[V - 2] = 0, 0
+    h[:, 0] = 1
+    w[:, 0] = 0
+    w[5, 0] = -float("inf")                                     # probability 0
+    t = torch.where((t == 5) | (t == V - 2), 6, t)
+    t[1], t[2], t[3] = 5, V - 2, IGN
+    h[4, 1] = float("nan")
+    h[4:6, 0] = 1
+    x = h.clone().requires_grad_()
+    loss = lce(x, w, t, reduction="none")
+    plain = lce(h, w, t, reduction="none")
+    assert torch.isnan(loss[4]) and torch.isnan(plain[4]) and float(loss[1]) == float("inf") == float(plain[1])
+    (dh,) = torch.autograd.grad(loss[torch.arange(N, device=DEV) != 1].sum(), x)
+    # 0 * inf in column 0, where the vocabulary is infinite; the rest is the formula's
+    live = torch.isfinite(loss.detach()) & (t != IGN)
+    assert torch.isfinite(dh[live][:, 1:]).all() and torch.isnan(dh[4]).all() and not dh[3].any() and not dh[1].any()
+    w[7, 0] = float("inf")
+    x = h.clone().requires_grad_()
+    loss = lce(x, w, t, reduction="none")
+    assert torch.isnan(loss[t != IGN]).all() and not loss[3].any()
+    (dh,) = torch.autograd.grad(loss.sum(), x)
+    assert torch.isnan(dh[t != IGN]).all() and not dh[3].any()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("reduction", ["sum", "mean"])
 @pytest.mark.parametrize("frozen,N", [("", 150), ("hidden", 150), ("weight", 150), ("", 1), ("", 40), ("weight", 640), ("", 2500)])
@@ -183,6 +257,26 @@ def test_long_rows_of_many_tokens(dtype):
     tol = 6e-6 if dtype == torch.float32 else 2 * torch.finfo(dtype).eps / 2 / 3 ** 0.5
     for got, want in ((dh, ref["dh"]), (dw, ref["dw"])):
         assert float((got.double() - want).norm() / want.norm()) < tol
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", [(70, 300, 64), (4200, 5000, 840)])
+def test_frozen_vocabulary_where_ignored_rows_hold_anything(N, V, D, dtype):
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w, t = inputs(N, V, D, dtype, ignored=0.4)
+    clean = h.clone()
+    bad = (t == IGN).nonzero()[:, 0]
+    h[bad[0::3]] = float("nan")
+    h[bad[1::3]] = float("inf")
+    h[bad[2::3]] = torch.finfo(dtype).min
+    out = []
+    for x in (h, clean):
+        x = x.clone().requires_grad_()
+        loss = lce(x, w, t)
+        out.append((loss.detach(),) + torch.autograd.grad(loss * 256, x))
+    for a, b in zip(*out):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    assert not out[0][1][bad].any()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -384,16 +478,16 @@ def test_gradient_against_differences(N):
         assert tol < 0.2 * max(rows, 1)                   # the check says something
 
 
-def test_forward_and_backward_in_a_replayed_graph():
+@pytest.mark.parametrize("N,V,D,frozen", [(130, 600, 64, False), (130, 600, 64, True), (2600, 9000, 768, True)])
+def test_forward_and_backward_in_a_replayed_graph(N, V, D, frozen):
     lce = pkg_mod("vocab_loss").linear_cross_entropy
-    N, V, D = 130, 600, 64
     h, w, t = inputs(N, V, D, torch.bfloat16)
     h.requires_grad_()
-    w.requires_grad_()
+    w.requires_grad_(not frozen)
 
     def step():
         loss = lce(h, w, t)
-        return (loss,) + torch.autograd.grad(loss, (h, w))
+        return (loss,) + torch.autograd.grad(loss, (h,) if frozen else (h, w))
 
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())

@@ -178,6 +178,26 @@ def test_c_entries_refuse_before_launching():
     refused(bwd(c=0.0), "scale")
     assert bwd(dh=None, dw=None) == 0                     # nothing is asked for
 
+    names = "h ldh w ldw dt N V D t ign c red ws wsb loss count dhu s".split()
+    ffwd = lambda **k: lib.po_linear_ce_frozen_fwd(*[{**dict(h=p, ldh=8, w=p, ldw=8, dt=BF16, N=4, V=5, D=8, t=p, ign=-100, c=1.0,  # noqa: E731
+                                                             red=2, ws=p, wsb=1 << 40, loss=p, count=p, dhu=p, s=None), **k}[n]
+                                                     for n in names])
+    for n in ("h", "w", "t", "ws", "loss", "count", "dhu"):
+        refused(ffwd(**{n: None}), "null")
+    for k in (dict(N=0), dict(V=0), dict(D=0), dict(N=(1 << 21) + 1), dict(V=1 << 31), dict(D=(1 << 20) + 1)):
+        refused(ffwd(**k), "sizes")
+    for k, word in ((dict(ldh=7), "strides"), (dict(ldw=7), "strides"), (dict(dt=3), "dtype"), (dict(red=3), "reduction"),
+                    (dict(c=0.0), "scale"), (dict(c=float("nan")), "scale"), (dict(wsb=0), "workspace"), (dict(dhu=p + 4), "16 bytes")):
+        refused(ffwd(**k), word)
+    names = "dhu dt N D t ign red count g dh lddh s".split()
+    fbwd = lambda **k: lib.po_linear_ce_frozen_bwd(*[{**dict(dhu=p, dt=BF16, N=4, D=8, t=p, ign=-100, red=2, count=p, g=p, dh=p,  # noqa: E731
+                                                             lddh=8, s=None), **k}[n] for n in names])
+    for n in ("dhu", "t", "count", "g", "dh"):
+        refused(fbwd(**{n: None}), "null")
+    for k, word in ((dict(N=0), "sizes"), (dict(D=0), "sizes"), (dict(lddh=7), "strides"), (dict(dt=3), "dtype"),
+                    (dict(red=-1), "reduction"), (dict(dhu=p + 8), "16 bytes")):
+        refused(fbwd(**k), word)
+
     qr = lambda **k: lib.po_quantize_rows(*[{**dict(x=p, ldx=20, dt=F32, M=2, K=20, q=p, ldq=32, sc=p, s=None), **k}[n]  # noqa: E731
                                             for n in "x ldx dt M K q ldq sc s".split()])
     for n in ("x", "q", "sc"):
@@ -219,6 +239,18 @@ def test_workspace_sizes_follow_the_work():
     assert sizes(32, 4096, 256, 2, 256, 1, 1)[1] < 64 << 20
     assert sizes(N, V, D, 2, D + 1, 1, 1)[0] > f
     assert sizes(N, V, D, 0, D, 1, 1)[0] > f
+
+
+def test_frozen_workspace_holds_a_piece():
+    lib = pkg_mod("_native").load()
+    b = ctypes.c_int64()
+    # from small heads to the largest: a piece of 640 MB, its transpose and slabs, never the N x V numbers
+    for N, V, D, dt in ((1, 1, 1, 0), (4096, 32768, 1024, 2), (8192, 131072, 2048, 2), (8192, 131072, 2048, 0), (1 << 21, 300000, 64, 1)):
+        assert lib.po_linear_ce_frozen_workspace(256, D, 256, D, dt, N, V, D, ctypes.byref(b)) == 0
+        slabs = 64 * N * D * 4
+        assert 0 < b.value < (900 << 20) + min(slabs, 40 * N * D) + (N * V // 128 * 13 + 64 * N) + (N + 256) * (D + 512) * 12, (N, V, D, dt, b.value)
+    assert lib.po_linear_ce_frozen_workspace(256, 8, 256, 8, 7, 1, 1, 8, ctypes.byref(b)) != 0
+    assert lib.po_linear_ce_frozen_workspace(256, 8, 256, 8, 2, 1, 1, 8, None) != 0
 
 
 def test_lay_out_pads_rows():
