@@ -301,7 +301,10 @@ CeForward ce_forward(const Tensor& hidden, const Tensor& weight, const Tensor& t
 struct LinearCe : torch::autograd::Function<LinearCe> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& target,
                         int64_t ignore, int64_t reduction, double scale) {
-    CeForward r = ce_forward(hidden, weight, target, ignore, reduction, scale, !weight.requires_grad());
+    // of few rows a second pass over the vocabulary is the quicker one (1 x 65536 x 1024 bf16: 67 us against 126)
+    const int64_t few = hidden.scalar_type() == at::kFloat ? 16 : 8;
+    const bool frozen = !weight.requires_grad() && (target.numel() > few || weight.size(1) > 2048);
+    CeForward r = ce_forward(hidden, weight, target, ignore, reduction, scale, frozen);
     ctx->save_for_backward({hidden, weight, r.target, r.stat, r.dhu});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["reduction"] = reduction;

@@ -784,13 +784,16 @@ __global__ __launch_bounds__(256) void transpose_k(const TransposeJob j0, const 
   store_columns<Pane>(lds, j.out + blockIdx.z * j.oplane, j.ldo, r0, c0, j.Rp, Cc);
 }
 
-// four neighbours in the gradients' type (OUT: BF16, F16, or 3: fp32), those below cols
+// four neighbours in the gradients' type (OUT: BF16, F16, or 3: fp32), those below cols; wide: as one
+// store, which needs no alignment
 template <int OUT>
 __device__ __forceinline__ void put4(void* out, int64_t at, int cols, int wide, f4v v) {
+  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint32_t u2u __attribute__((ext_vector_type(2), aligned(2)));
   if constexpr (OUT == 3) {
     float* o = static_cast<float*>(out) + at;
     if (wide && cols >= 4) {
-      *reinterpret_cast<f4v*>(o) = v;
+      *reinterpret_cast<f4u*>(o) = v;
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -800,7 +803,7 @@ __device__ __forceinline__ void put4(void* out, int64_t at, int cols, int wide, 
     const u2v w = {pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
     uint16_t* o = static_cast<uint16_t*>(out) + at;
     if (wide && cols >= 4) {
-      *reinterpret_cast<u2v*>(o) = w;
+      *reinterpret_cast<u2u*>(o) = w;
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -926,6 +929,279 @@ __global__ __launch_bounds__(256) void frozen_scale_k(const float* __restrict__ 
   }
 }
 
+// ---- few rows ------------------------------------------------------------
+// Up to 8 tokens, of fp32 16: the vocabulary's bytes are the work, and one pass over them in their own type, in
+// 32-bit arithmetic, makes all of a pass: the logits, then (backward) their part of dh and the rows of dw.
+// The products above would read them five times and write two copies (fp32: planes too).
+// 8 waves: CW side by side over the columns, 4 to a lane, 256 to a wave; 8 / CW groups of rows.
+// A wave holds its columns of all tokens and of their gradients, and R vocabulary rows with
+// the next R on their way.  Its R x NB dot products end one to a lane: halves of the values go to
+// halves of the lanes, step by step (141 instructions for 64 sums).  The column waves' parts meet
+// in LDS, every wave adds them up, and the logits' gradients return as scalars.
+// Trained, against the products: 1 x 45459 x 896 fp32 508 -> 98 us (490 MB, 95 us), 1 x 131072 x 2048 bf16
+// 739 -> 332, of 8 tokens 519: then it is arithmetic that bounds it, and with 16 tokens of 16 bits the
+// matrix cores are quicker (32768 x 1024 bf16 100 us, 146 here; fp32 428, 178 here).
+constexpr int kFewRows = 8, kFewRowsF32 = 16, kFewDim = 2048, kFewBlocks = 512;
+
+constexpr int few_batch(int tokens, bool backward) { return tokens <= 8 ? 8 : backward ? 2 : 4; }   // R, as registers allow
+
+template <int M, int STEP>
+__device__ __forceinline__ void scatter_sum(float* x, int lane) {
+  // M values a lane over lanes that differ in bits STEP and below: the halves go to the lanes without and with that bit
+  constexpr int H = M / 2;
+  if constexpr (STEP < 0) {
+    return;
+  } else if constexpr (M == 1) {
+    float o;
+    if constexpr (STEP >= 4) o = __shfl_xor(x[0], 1 << STEP);
+    else if constexpr (STEP == 3) o = __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x[0]), 0x140, 15, 15, true));
+    else if constexpr (STEP == 2) o = __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x[0]), 0x141, 15, 15, true));
+    else if constexpr (STEP == 1) o = __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x[0]), 0x1b, 15, 15, true));
+    else o = __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x[0]), 0xb1, 15, 15, true));
+    x[0] += o;
+    scatter_sum<1, STEP - 1>(x, lane);
+  } else {
+    // partners: lane ^ 32, ^ 16, then the mirrors of 16, 8, 4 and 2 lanes (the bits below are still alike)
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      if constexpr (STEP == 5 || STEP == 4) {
+        const auto r = STEP == 5 ? __builtin_amdgcn_permlane32_swap(__float_as_uint(x[i]), __float_as_uint(x[i + H]), false, false)
+                                 : __builtin_amdgcn_permlane16_swap(__float_as_uint(x[i]), __float_as_uint(x[i + H]), false, false);
+        x[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+      } else {
+        const bool high = lane >> STEP & 1;
+        const float keep = high ? x[i + H] : x[i], send = high ? x[i] : x[i + H];
+        constexpr int ctrl = STEP == 3 ? 0x140 : STEP == 2 ? 0x141 : STEP == 1 ? 0x1b : 0xb1;
+        x[i] = keep + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(send), ctrl, 15, 15, true));
+      }
+    }
+    scatter_sum<H, STEP - 1>(x, lane);
+  }
+}
+
+template <int DT>
+struct Row {
+  using type = uint16_t;
+  static __device__ __forceinline__ float f(uint16_t x) {
+    if constexpr (DT == PO_F16) return (float)__builtin_bit_cast(_Float16, x);
+    else return __uint_as_float((uint32_t)x << 16);
+  }
+};
+template <>
+struct Row<PO_F32> {
+  using type = float;
+  static __device__ __forceinline__ float f(float x) { return x; }
+};
+
+struct FewArgs {
+  const void *h, *w;
+  int64_t ldh, ldw, V;
+  int N, D, cw, batches;        // cw: column waves, 1, 2, 4 or 8
+  const int64_t* target;
+  int64_t ignore;
+  float k;                      // c * log2e
+};
+
+// What the two kernels share: a wave's place, its tokens' columns, its rows, their logits.
+template <int DT, int NB, int R_>
+struct FewWave {
+  using T = typename Row<DT>::type;
+  typedef T v4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  static constexpr int R = R_, M = R * NB, SH = M >= 64 ? 0 : M == 32 ? 1 : M == 16 ? 2 : 3;
+  static_assert(M <= 64 && M >= 8, "one dot product to a lane at most");
+  const FewArgs& a;
+  int lane, wave, cwave, group, groups, col, cols;
+  float h[NB][4];
+  v4 next[R];
+  __device__ __forceinline__ explicit FewWave(const FewArgs& args) : a(args) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    cwave = wave % a.cw;
+    group = blockIdx.x * (8 / a.cw) + wave / a.cw;
+    groups = gridDim.x * (8 / a.cw);
+    col = cwave * 256 + lane * 4;
+    cols = max(0, min(4, a.D - col));
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        h[n][e] = n < a.N && e < cols ? Row<DT>::f(static_cast<const T*>(a.h)[n * a.ldh + col + e]) : 0.f;
+  }
+  // the value of this lane after the sums: vocabulary row and token
+  __device__ __forceinline__ int my_row() const { return (lane >> SH) / NB; }
+  __device__ __forceinline__ int my_token() const { return (lane >> SH) % NB; }
+  __device__ __forceinline__ void load(int batch) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t v = (int64_t)batch * R + r;
+      const T* p = static_cast<const T*>(a.w) + v * a.ldw + col;
+      if (v < a.V && cols == 4) {
+        next[r] = *reinterpret_cast<const v4*>(p);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) next[r][e] = v < a.V && e < cols ? p[e] : (T)0;
+      }
+    }
+  }
+  // this lane's sum over all columns, h . w
+  __device__ __forceinline__ float logit(const float (&w)[R][4], float (*red)[64]) {
+    float x[M];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        float s = w[r][0] * h[n][0];
+#pragma unroll
+        for (int e = 1; e < 4; ++e) s = __builtin_fmaf(w[r][e], h[n][e], s);
+        x[r * NB + n] = s;
+      }
+    scatter_sum<M, 5>(x, lane);
+    red[wave][lane] = x[0];
+    __syncthreads();
+    float l = 0.f;
+    const int first = wave / a.cw * a.cw;
+    for (int c = 0; c < a.cw; ++c) l += red[first + c][lane];
+    return l;
+  }
+};
+
+// partial[block][n] and tlogit as StatsEpi's
+template <int DT, int NB>
+__global__ __launch_bounds__(512, NB > 4 ? 2 : 4) void few_rows_fwd_k(const FewArgs a, float2* __restrict__ partial, uint32_t* arrived,
+                                                         float* __restrict__ tlogit) {
+  __shared__ float red[2][8][64];
+  __shared__ float2 ends[8][64];
+  constexpr int R = few_batch(NB, false);
+  FewWave<DT, NB, R> f(a);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
+  const int n = f.my_token(), r = f.my_row();
+  const int64_t t = n < a.N ? a.target[n] : -1;
+  float m = -INFINITY, s = 0.f;
+  f.load(f.group);
+  const int its = (a.batches + f.groups - 1) / f.groups;
+  for (int i = 0; i < its; ++i) {
+    float w[R][4];
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[q][e] = Row<DT>::f(f.next[q][e]);
+    const int batch = f.group + i * f.groups;
+    f.load(batch + f.groups);
+    const float x = f.logit(w, red[i & 1]);
+    const int64_t v = (int64_t)batch * R + r;
+    if (v < a.V) {
+      if (v == t && f.cwave == 0) tlogit[n] = x;
+      const float y = x * a.k, top = fmaxf(m, y), ref = top == -INFINITY ? 0.f : top;
+      s = s * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(y - ref);
+      m = top;
+    }
+  }
+  ends[f.wave][f.lane] = make_float2(m, s);
+  __syncthreads();
+  for (int x = threadIdx.x; x < a.N; x += 512) {
+    float2 o = make_float2(-INFINITY, 0.f);
+    for (int g = 0; g < 8; g += a.cw)
+      for (int q = 0; q < R; ++q) {
+        const float2 b = ends[g][(q * NB + x) << f.SH];
+        const float top = fmaxf(o.x, b.x), ref = top == -INFINITY ? 0.f : top;
+        o = make_float2(top, o.y * __builtin_amdgcn_exp2f(o.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+      }
+    partial[(int64_t)blockIdx.x * a.N + x] = o;
+  }
+}
+
+// slab[block][n][ld] (if any): this block's part of dh over c and the upstream gradients' factor; dw (if any)
+template <int DT, int NB>
+__global__ __launch_bounds__(512, NB > 2 ? 2 : 4) void few_rows_bwd_k(const FewArgs a, const float2* __restrict__ stat, const GradOf g,
+                                                                      float* __restrict__ slab, int ld, void* __restrict__ dw,
+                                                                      int64_t lddw) {
+  __shared__ float red[2][8][64];
+  __shared__ float sums[8][256];
+  constexpr int R = few_batch(NB, true);
+  FewWave<DT, NB, R> f(a);
+  constexpr int OUT = DT == PO_F32 ? 3 : DT == PO_F16 ? F16 : BF16;
+  const int n = f.my_token(), r = f.my_row();
+  const bool in = n < a.N;
+  const int64_t t = in ? a.target[n] : -1;
+  const float2 st = in ? stat[n] : make_float2(0.f, 0.f);
+  const float ratio = in ? g.of_row(n) : 0.f, ir = ratio * st.y, end = g.end();
+  float dh[NB][4];
+#pragma unroll
+  for (int q = 0; q < NB; ++q) {
+    const bool live = q < a.N && g.live(q);                  // rows that take no part may hold anything, NaN too
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      dh[q][e] = 0.f;
+      if (!live) f.h[q][e] = 0.f;
+    }
+  }
+  f.load(f.group);
+  const int its = (a.batches + f.groups - 1) / f.groups;
+  for (int i = 0; i < its; ++i) {
+    float w[R][4];
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[q][e] = Row<DT>::f(f.next[q][e]);
+    const int batch = f.group + i * f.groups;
+    f.load(batch + f.groups);
+    const float x = f.logit(w, red[i & 1]);
+    const int64_t v = (int64_t)batch * R + r;
+    float dl = __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.k, -st.x)) * ir - (v == t ? ratio : 0.f);
+    if (ratio == 0.f || v >= a.V) dl = 0.f;
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      f4v out = {0, 0, 0, 0};
+#pragma unroll
+      for (int y = 0; y < NB; ++y) {
+        const float b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dl), (q * NB + y) << f.SH));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          dh[y][e] = __builtin_fmaf(b, w[q][e], dh[y][e]);
+          out[e] = __builtin_fmaf(b, f.h[y][e], out[e]);
+        }
+      }
+      const int64_t vq = (int64_t)batch * R + q;
+      if (dw && vq < a.V && f.cols > 0) put4<OUT>(dw, vq * lddw + f.col, f.cols, 1, out * end);
+    }
+  }
+  if (!slab) return;
+#pragma unroll
+  for (int y = 0; y < NB; ++y) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[f.wave][f.lane * 4 + e] = dh[y][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.cw * 256 && y < a.N; c += 512) {
+      float s = 0.f;
+      for (int q = c / 256; q < 8; q += a.cw) s += sums[q][c % 256];
+      if (c < ld) slab[((int64_t)blockIdx.x * a.N + y) * ld + c] = s;
+    }
+  }
+}
+
+// dh[n][m] = g.end() * the blocks' sum: 16 groups of 16 threads, 4 columns to a thread, block after block in
+// each, then the groups' in order
+template <int OUT>
+__global__ __launch_bounds__(256) void few_sum_k(const float* __restrict__ slab, int blocks, int64_t slice, int M, const GradOf g,
+                                                 void* __restrict__ out, int64_t ldo, int64_t ld) {
+  __shared__ f4v part[16][16];
+  const int n = blockIdx.y, m = blockIdx.x * 64 + threadIdx.x % 16 * 4, grp = threadIdx.x / 16;
+  f4v v = {0, 0, 0, 0};
+  if (m < ld) {
+    const float* p = slab + n * ld + m;
+#pragma unroll 8
+    for (int s = grp; s < blocks; s += 16) v += *reinterpret_cast<const f4v*>(p + s * slice);
+  }
+  part[grp][threadIdx.x % 16] = v;
+  __syncthreads();
+  if (grp || m >= M) return;
+  v = part[0][threadIdx.x];
+#pragma unroll
+  for (int q = 1; q < 16; ++q) v += part[q][threadIdx.x];
+  put4<OUT>(out, n * ldo + m, M - m, 1, g.live(n) ? v * g.end() : f4v{0, 0, 0, 0});
+}
+
 // ---- the plan ------------------------------------------------------------
 
 // What a piece of the vocabulary may take of the workspace: 16384 rows of 8192 tokens.  Pieces of
@@ -976,6 +1252,18 @@ inline int64_t piece_rows(int64_t V, int64_t per_row) {
   return std::min(V, (each + 255) / 256 * 256);
 }
 
+// Few rows: whether their kernels take a pass, and their grid.
+inline int few_tokens_of(int64_t N) { return N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : N <= 8 ? 8 : 16; }
+inline int few_columns(int64_t D) { return D <= 256 ? 1 : D <= 512 ? 2 : D <= 1024 ? 4 : 8; }
+inline bool few_rows(const Shape& s) { return s.N <= (s.dtype == PO_F32 ? kFewRowsF32 : kFewRows) && s.D <= kFewDim; }
+// forward: 16-bit rows that serve as they are go through the matrix cores at the same rate (32768 x 1024
+// bf16 13 us)
+inline bool few_rows_forward(const Shape& s) { return few_rows(s) && !s.direct_w; }
+inline int few_batches(const Shape& s, bool backward) { return (int)ceil_div(s.V, few_batch((int)s.N, backward)); }
+inline int few_blocks(const Shape& s, bool backward) {
+  return std::min(kFewBlocks, (int)ceil_div(few_batches(s, backward), 8 / few_columns(s.D)));
+}
+
 struct FwdWs {
   float2* partial;
   double* sums;
@@ -986,6 +1274,17 @@ struct FwdWs {
   int parts;
   FwdWs(const Shape& s, void* b) {
     Layout l(b);
+    if (few_rows_forward(s)) {
+      piece = s.V;
+      parts = few_blocks(s, false);
+      partial = l.take<float2>((int64_t)parts * s.N);
+      tlogit = l.take<float>(s.N);
+      sums = l.take<double>(2 * s.N);
+      arrived = l.take<uint32_t>(1);
+      hp = wp = nullptr;
+      bytes = l.at;
+      return;
+    }
     const int64_t wrow = s.direct_w ? 0 : s.ldp() * 2 * s.planes();
     piece = wrow ? piece_rows(s.V, wrow) : s.V;
     parts = 0;
@@ -1010,6 +1309,15 @@ struct BwdWs {
   bool direct_dh;               // one piece in one slice: dh leaves the product as it is wanted
   BwdWs(const Shape& s, bool dh, bool dw, void* b) {
     Layout l(b);
+    if (few_rows(s)) {
+      ratio = l.take<float>(s.N);
+      factor = l.take<float>(1);
+      slab_ld = (s.D + 3) / 4 * 4;
+      slab_slice = s.N * slab_ld;
+      slab = l.take<float>(dh ? few_blocks(s, true) * slab_slice : 0);
+      bytes = l.at;
+      return;
+    }
     const int P = s.planes();
     const int64_t per = (s.direct_w ? 0 : s.ldp() * 2 * P) + (dh ? (s.N + s.D) * 2 * P : 0) + (dw ? s.Np() * 2 * P : 0);
     piece = piece_rows(s.V, per);
@@ -1162,6 +1470,24 @@ inline void row_stats(const float2* partial, int parts, const Shape& s, const fl
     if (rc_ != PO_OK) return rc_; \
   } while (0)
 
+inline FewArgs few_args(const Shape& s, const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* target, int64_t ignore,
+                        float scale, bool backward) {
+  return FewArgs{h, w, ldh, ldw, s.V, (int)s.N, (int)s.D, few_columns(s.D), few_batches(s, backward), target, ignore, scale * kLog2e};
+}
+template <class Fn>
+inline void few_dispatch(int dtype, int nb, Fn fn) {
+  auto tokens = [&](auto dt) {
+    if (nb == 1) fn(dt, std::integral_constant<int, 1>{});
+    else if (nb == 2) fn(dt, std::integral_constant<int, 2>{});
+    else if (nb == 4) fn(dt, std::integral_constant<int, 4>{});
+    else if (nb == 8) fn(dt, std::integral_constant<int, 8>{});
+    else if constexpr (decltype(dt)::value == PO_F32) fn(dt, std::integral_constant<int, 16>{});
+  };
+  if (dtype == PO_F32) tokens(std::integral_constant<int, PO_F32>{});
+  else if (dtype == PO_F16) tokens(std::integral_constant<int, PO_F16>{});
+  else tokens(std::integral_constant<int, PO_BF16>{});
+}
+
 }  // namespace
 
 extern "C" int po_linear_ce_workspace(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N,
@@ -1186,6 +1512,16 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
   PO_REQUIRE(workspace_bytes >= ws.bytes, "po_linear_ce_fwd: workspace of %lld bytes, %lld needed",
              (long long)workspace_bytes, (long long)ws.bytes);
   const hipStream_t st = po::stream_of(stream);
+  if (few_rows_forward(s)) {
+    const FewArgs f = few_args(s, h, ldh, w, ldw, target, ignore_index, scale, false);
+    few_dispatch(dtype, few_tokens_of(N), [&](auto dt, auto nb) {
+      hipLaunchKernelGGL((few_rows_fwd_k<decltype(dt)::value, decltype(nb)::value>), dim3(ws.parts), dim3(512), 0, st, f, ws.partial,
+                         ws.arrived, ws.tlogit);
+    });
+    row_stats(ws.partial, ws.parts, s, ws.tlogit, target, ignore_index, f.k, reinterpret_cast<float2*>(stat), ws.sums, ws.arrived,
+              reduction, loss, count, st);
+    return po::check_launch("po_linear_ce_fwd");
+  }
   Args a{};
   set_pairs(a, s.planes());
   a.kbytes = s.Dp() * 2;
@@ -1299,10 +1635,24 @@ extern "C" int po_linear_ce_bwd(const void* h, int64_t ldh, const void* w, int64
   PO_REQUIRE(workspace_bytes >= ws.bytes, "po_linear_ce_bwd: workspace of %lld bytes, %lld needed",
              (long long)workspace_bytes, (long long)ws.bytes);
   const hipStream_t st = po::stream_of(stream);
-  const GradOf g{grad, count, target, ignore_index, V, reduction == 0, reduction == 2, dtype == PO_F16 ? kF16Lift : 1.f, scale,
+  const bool few = few_rows(s);                              // their dl stay in 32 bits
+  const GradOf g{grad, count, target, ignore_index, V, reduction == 0, reduction == 2, dtype == PO_F16 && !few ? kF16Lift : 1.f, scale,
                  ws.ratio, ws.factor};
   if (g.each) hipLaunchKernelGGL(grad_rows_k, dim3(1), dim3(1024), 0, st, g, (int)N, ws.ratio, ws.factor);
   const float2* st2 = reinterpret_cast<const float2*>(stat);
+  if (few) {
+    const FewArgs f = few_args(s, h, ldh, w, ldw, target, ignore_index, scale, true);
+    const int blocks = few_blocks(s, true);
+    few_dispatch(dtype, few_tokens_of(N), [&](auto dt, auto nb) {
+      hipLaunchKernelGGL((few_rows_bwd_k<decltype(dt)::value, decltype(nb)::value>), dim3(blocks), dim3(512), 0, st, f, st2, g,
+                         dh ? ws.slab : nullptr, (int)ws.slab_ld, dw, lddw);
+    });
+    if (dh)
+      hipLaunchKernelGGL((dtype == PO_F32 ? few_sum_k<3> : dtype == PO_F16 ? few_sum_k<F16> : few_sum_k<BF16>),
+                         dim3(ceil_div(D, 64), (unsigned)N), dim3(256), 0, st, ws.slab, blocks, ws.slab_slice, (int)D, g, dh, lddh,
+                         ws.slab_ld);
+    return po::check_launch("po_linear_ce_bwd");
+  }
   const Side hs{h, ldh, s.direct_h, ws.hp}, wside{w, ldw, s.direct_w, ws.wp};
   if (dtype == PO_F16) return backward<F16, F16>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
   if (dtype == PO_BF16) return backward<BF16, BF16>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);

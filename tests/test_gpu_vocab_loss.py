@@ -115,6 +115,41 @@ def test_large_tiles(N, V, D, dtype):
     within(dw, ref["dw"], b["dw"], "dw")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", [(1, 9001, 793), (1, 33, 2048), (2, 5000, 2047), (3, 7, 5), (4, 1999, 256), (6, 12345, 300), (8, 4096, 512),
+                                   (9, 2222, 1024), (13, 8191, 1025), (16, 5001, 2000), (16, 100000, 64), (16, 50, 2049), (17, 3000, 640)])
+@pytest.mark.parametrize("frozen", ["", "hidden", "weight"])
+def test_few_rows(N, V, D, frozen, dtype):
+    """One pass over the vocabulary, its ends in rows and columns; rows that take no part hold NaN."""
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w, t = inputs(N, V, D, dtype)
+    if N > 2:
+        t[1] = IGN
+        h[1] = float("nan")
+    if N > 1:
+        t[N - 1] = V - 1
+    h.requires_grad_(frozen != "hidden")
+    w.requires_grad_(frozen != "weight")
+    g = (64.0 if dtype == torch.float16 else 1.0) * (0.5 + torch.arange(N, device=DEV) % 7 / 7)
+    loss = lce(h, w, t, reduction="none")
+    leaves = [x for x in (h, w) if x.requires_grad]
+    grads = torch.autograd.grad(loss, leaves, g, retain_graph=True)
+    ref = reference(h.detach(), w.detach(), t, g)
+    b = bounds(ref, dtype, N, V, D)
+    within(loss.detach(), ref["loss"], b["loss"], "loss")
+    for x, d, got in zip(leaves, ["dh", "dw"] if len(leaves) == 2 else ["dw" if frozen == "hidden" else "dh"], grads):
+        within(got, ref[d], b[d], d)
+        if N <= 8 and D <= 2048 and dtype != torch.float32:
+            # the gradient of the logits stays in 32 bits there: the one rounding to 16 is the gradient's own, at most half a step
+            tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-37
+            own = torch.finfo(dtype).eps / 2 * ref[d].abs() + tiny
+            eL = (D + 4) * 2.0 ** -23 * ref["S"]
+            a, r, n = (ref["ah"], ref["rh"], V) if d == "dh" else (ref["aw"], ref["rw"], N)
+            within(got, ref[d], own + (2 * eL + 1e-4) * a + (n + 4) * 2.0 ** -23 * r, d + ", one rounding")
+    for x, y in zip(grads, torch.autograd.grad(loss, leaves, g)):
+        assert torch.equal(x, y)
+
+
 def check_frozen(h, w, t, g, scale=1.0):
     """Loss and gradient against a frozen vocabulary.  Beside the other bounds: blocks of the vocabulary whose
     exponentials stay below 2^-48 of another's are left out of dh."""
@@ -478,7 +513,7 @@ def test_gradient_against_differences(N):
         assert tol < 0.2 * max(rows, 1)                   # the check says something
 
 
-@pytest.mark.parametrize("N,V,D,frozen", [(130, 600, 64, False), (130, 600, 64, True), (2600, 9000, 768, True)])
+@pytest.mark.parametrize("N,V,D,frozen", [(130, 600, 64, False), (130, 600, 64, True), (2600, 9000, 768, True), (5, 600, 64, False), (1, 600, 64, True)])
 def test_forward_and_backward_in_a_replayed_graph(N, V, D, frozen):
     lce = pkg_mod("vocab_loss").linear_cross_entropy
     h, w, t = inputs(N, V, D, torch.bfloat16)
