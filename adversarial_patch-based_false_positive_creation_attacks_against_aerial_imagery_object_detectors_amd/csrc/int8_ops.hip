@@ -262,7 +262,7 @@ struct ScaledEpi {
     void* y;
     int64_t ld;
     const float *sx, *sw, *bias;
-    int N, M, wide;             // tokens, outputs; wide: rows start on 16 bytes
+    int N, M;                   // tokens, outputs
   };
   template <class C>
   struct Pre {
@@ -295,8 +295,8 @@ struct ScaledEpi {
           const int n = t.col(j);
           if (n < e.N) {
             float* o = static_cast<float*>(e.y) + (int64_t)n * e.ld + m;
-            if (e.wide && m + 4 <= e.M) {
-              *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+            if (m + 4 <= e.M) {
+              *reinterpret_cast<f4u*>(o) = f4u{v[0], v[1], v[2], v[3]};
             } else {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
@@ -311,7 +311,7 @@ struct ScaledEpi {
     }
     if constexpr (DT != PO_F32) {
       __syncthreads();
-      store_rows<C>(lds, static_cast<uint16_t*>(e.y), e.ld, t.tn * C::BN, t.tm * C::BM, e.N, e.M, e.wide != 0);
+      store_rows<C>(lds, static_cast<uint16_t*>(e.y), e.ld, t.tn * C::BN, t.tm * C::BM, e.N, e.M);
     }
   }
 };
@@ -415,10 +415,9 @@ int matmul(const int8_t* q, int64_t ldq, const float* sx, const int8_t* w, int64
   a.B = Operand{reinterpret_cast<const char*>(q), ldq, 0, (int)M};
   a.kbytes = (int)((K + 15) / 16 * 16);
   a.pairs = 1;
-  const int wide = (uintptr_t)y % 16 == 0 && ldy * element_bytes(dtype) % 16 == 0;
-  if (dtype == PO_F32) return product_of<PO_F32>(a, {y, ldy, sx, sw, bias, (int)M, (int)N, wide}, s);
-  if (dtype == PO_F16) return product_of<PO_F16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N, wide}, s);
-  return product_of<PO_BF16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N, wide}, s);
+  if (dtype == PO_F32) return product_of<PO_F32>(a, {y, ldy, sx, sw, bias, (int)M, (int)N}, s);
+  if (dtype == PO_F16) return product_of<PO_F16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N}, s);
+  return product_of<PO_BF16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N}, s);
 }
 
 // Workspace of po_int8_linear: the tokens' 8-bit rows, then their scales.  Rows a power of two

@@ -37,6 +37,7 @@ namespace mm {
 
 typedef int i4v __attribute__((ext_vector_type(4)));
 typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // in memory, wherever it starts
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 
@@ -648,10 +649,12 @@ __device__ __forceinline__ void stage4(const Tile<C>& t, char* lds, int i, int j
   *reinterpret_cast<u2v*>(lds + n * (C::BM * 2) + ((c ^ turn<C>(n)) * 16) + 8 * ((t.lane >> 4) & 1)) = four;
 }
 
-// rows [n][m] of the staged tile to out (16-bit, leading dimension ld), n < rows, m < cols
+// rows [n][m] of the staged tile to out (16-bit, leading dimension ld), n < rows, m < cols; 16 bytes at
+// a time wherever the rows start (the stores need no alignment)
 template <class C>
 __device__ __forceinline__ void store_rows(const char* lds, uint16_t* out, int64_t ld, int n0, int m0, int rows,
-                                           int cols, bool wide) {
+                                           int cols) {
+  typedef int i4u __attribute__((ext_vector_type(4), aligned(2)));
   constexpr int NC = C::BM / 8, STEPS = C::BN * NC / (C::NW * 64), U = STEPS % 8 == 0 ? 8 : STEPS;
   static_assert(STEPS * C::NW * 64 == C::BN * NC, "whole steps");
   // a thread's chunk is the same in every step, its row advances
@@ -668,9 +671,9 @@ __device__ __forceinline__ void store_rows(const char* lds, uint16_t* out, int64
 #pragma unroll
     for (int u = 0; u < U; ++u, o += ROWS * ld) {
       if (n0 + n + (s + u) * ROWS >= rows || m >= cols) continue;
-      if (wide && m + 8 <= cols) {
+      if (m + 8 <= cols) {
         // past the caches' keeping: the next product's operands stay (dh of 4096x32768x1024 233 -> 219 us)
-        __builtin_nontemporal_store(v[u], reinterpret_cast<i4v*>(o));
+        __builtin_nontemporal_store(v[u], reinterpret_cast<i4u*>(o));
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)

@@ -277,7 +277,7 @@ struct DlogitsEpi {
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
       const int n0 = t.tn * C::BN, m0 = t.tm * C::BM;
-      if (e.dl) store_rows<C>(lds, e.dl + p * e.pl, e.ldl, n0, m0, e.N, e.Vp, true);
+      if (e.dl) store_rows<C>(lds, e.dl + p * e.pl, e.ldl, n0, m0, e.N, e.Vp);
       __builtin_amdgcn_sched_barrier(0);
       if (e.dlt) store_columns<C>(lds, e.dlt + p * e.pt, e.ldt, n0, m0, e.Np, e.V);
       __builtin_amdgcn_sched_barrier(0);
@@ -447,7 +447,7 @@ struct KeepEpi {
       }
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
-      store_rows<C>(lds, a.kept + q * a.plane, a.ld, t.tn * C::BN, t.tm * C::BM, e.N, a.Vp, true);
+      store_rows<C>(lds, a.kept + q * a.plane, a.ld, t.tn * C::BN, t.tm * C::BM, e.N, a.Vp);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -541,7 +541,7 @@ struct GradEpi {
     void* out;
     int64_t ld;
     GradOf g;
-    int N, M, wide;             // wide: rows start on 16 bytes
+    int N, M;
   };
   template <class C>
   using Pre = NoPre;
@@ -557,8 +557,8 @@ struct GradEpi {
         for (int i = 0; i < C::TM; ++i) {
           const int m = t.row(i);
           float* o = static_cast<float*>(e.out) + (int64_t)n * e.ld + m;
-          if (e.wide && m + 4 <= e.M) {
-            *reinterpret_cast<f4v*>(o) = t.acc[i][j] * f;
+          if (m + 4 <= e.M) {
+            *reinterpret_cast<f4u*>(o) = t.acc[i][j] * f;
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -577,7 +577,7 @@ struct GradEpi {
                                    pack2<OUT>(t.acc[i][j][2] * f, t.acc[i][j][3] * f)});
       }
       __syncthreads();
-      store_rows<C>(lds, static_cast<uint16_t*>(e.out), e.ld, t.tn * C::BN, t.tm * C::BM, e.N, e.M, e.wide != 0);
+      store_rows<C>(lds, static_cast<uint16_t*>(e.out), e.ld, t.tn * C::BN, t.tm * C::BM, e.N, e.M);
     }
   }
 };
@@ -784,15 +784,14 @@ __global__ __launch_bounds__(256) void transpose_k(const TransposeJob j0, const 
   store_columns<Pane>(lds, j.out + blockIdx.z * j.oplane, j.ldo, r0, c0, j.Rp, Cc);
 }
 
-// four neighbours in the gradients' type (OUT: BF16, F16, or 3: fp32), those below cols; wide: as one
-// store, which needs no alignment
+// four neighbours in the gradients' type (OUT: BF16, F16, or 3: fp32), those below cols; one store, which
+// needs no alignment
 template <int OUT>
-__device__ __forceinline__ void put4(void* out, int64_t at, int cols, int wide, f4v v) {
-  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void put4(void* out, int64_t at, int cols, f4v v) {
   typedef uint32_t u2u __attribute__((ext_vector_type(2), aligned(2)));
   if constexpr (OUT == 3) {
     float* o = static_cast<float*>(out) + at;
-    if (wide && cols >= 4) {
+    if (cols >= 4) {
       *reinterpret_cast<f4u*>(o) = v;
     } else {
 #pragma unroll
@@ -802,7 +801,7 @@ __device__ __forceinline__ void put4(void* out, int64_t at, int cols, int wide, 
   } else {
     const u2v w = {pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
     uint16_t* o = static_cast<uint16_t*>(out) + at;
-    if (wide && cols >= 4) {
+    if (cols >= 4) {
       *reinterpret_cast<u2u*>(o) = w;
     } else {
 #pragma unroll
@@ -815,7 +814,7 @@ __device__ __forceinline__ void put4(void* out, int64_t at, int cols, int wide, 
 // dh[n][m] = g.end() * the slabs' sum, slab after slab; a thread makes 4 columns
 template <int OUT>
 __global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab, int slices, int64_t slice, int64_t ld,
-                                                  int N, int M, const GradOf g, void* __restrict__ out, int64_t ldo, int wide) {
+                                                  int N, int M, const GradOf g, void* __restrict__ out, int64_t ldo) {
   const float f = g.end();
   const int per = (int)(ld / 4);
   const int64_t total = (int64_t)N * per;
@@ -827,7 +826,7 @@ __global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab
 #pragma unroll 4
     for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const f4v*>(p + s * slice);
     v *= f;
-    put4<OUT>(out, n * ldo + m, M - m, wide, v);
+    put4<OUT>(out, n * ldo + m, M - m, v);
   }
 }
 
@@ -915,7 +914,7 @@ template <int OUT>
 __global__ __launch_bounds__(256) void frozen_scale_k(const float* __restrict__ dhu, int64_t ld, int N, int M,
                                                       const int64_t* __restrict__ target, int64_t ignore,
                                                       const float* __restrict__ grad, int each, const float* __restrict__ count,
-                                                      void* __restrict__ out, int64_t ldo, int wide) {
+                                                      void* __restrict__ out, int64_t ldo) {
   const int per = (int)(ld / 4);
   const int64_t total = (int64_t)N * per;
   const float over = count ? fmaxf(*count, 1.f) : 1.f;
@@ -925,7 +924,7 @@ __global__ __launch_bounds__(256) void frozen_scale_k(const float* __restrict__ 
     const float g = grad[each ? n : 0] / over;
     f4v v = *reinterpret_cast<const f4v*>(dhu + n * ld + m) * g;
     if (target[n] == ignore || g == 0.f) v = f4v{0, 0, 0, 0};
-    put4<OUT>(out, n * ldo + m, M - m, wide, v);
+    put4<OUT>(out, n * ldo + m, M - m, v);
   }
 }
 
@@ -1162,7 +1161,7 @@ __global__ __launch_bounds__(512, NB > 2 ? 2 : 4) void few_rows_bwd_k(const FewA
         }
       }
       const int64_t vq = (int64_t)batch * R + q;
-      if (dw && vq < a.V && f.cols > 0) put4<OUT>(dw, vq * lddw + f.col, f.cols, 1, out * end);
+      if (dw && vq < a.V && f.cols > 0) put4<OUT>(dw, vq * lddw + f.col, f.cols, out * end);
     }
   }
   if (!slab) return;
@@ -1199,7 +1198,7 @@ __global__ __launch_bounds__(256) void few_sum_k(const float* __restrict__ slab,
   v = part[0][threadIdx.x];
 #pragma unroll
   for (int q = 1; q < 16; ++q) v += part[q][threadIdx.x];
-  put4<OUT>(out, n * ldo + m, M - m, 1, g.live(n) ? v * g.end() : f4v{0, 0, 0, 0});
+  put4<OUT>(out, n * ldo + m, M - m, g.live(n) ? v * g.end() : f4v{0, 0, 0, 0});
 }
 
 // ---- the plan ------------------------------------------------------------
@@ -1592,7 +1591,7 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
       // the last piece may have fewer steps than slices: the other slabs keep their sums
       const Plan p{ws.dh_plan.tile, std::min(ws.dh_plan.slices, ceil_div(a.kbytes, P == 3 ? 64 : 128)), 0};
       if (ws.direct_dh) {
-        const typename GradEpi<OUT>::Args ge{dh, lddh, g, N, D, (uintptr_t)dh % 16 == 0 && lddh * es % 16 == 0};
+        const typename GradEpi<OUT>::Args ge{dh, lddh, g, N, D};
         PO_TRY((launch_planned<KIND, P, GradEpi<OUT>>(a, ge, p, st, what)));
       } else {
         const SlabEpi::Args se{ws.slab, ws.slab_ld, ws.slab_slice, N, D, v > 0};
@@ -1604,15 +1603,14 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
       a.B = Operand{reinterpret_cast<char*>(ws.dlt), s.ldn() * 2, ws.piece * s.ldn() * 2, rows};
       a.kbytes = (int)s.Np() * 2;
       char* out = static_cast<char*>(dw) + v * lddw * es;
-      const typename GradEpi<OUT>::Args ge{out, lddw, g, rows, D, (uintptr_t)out % 16 == 0 && lddw * es % 16 == 0};
+      const typename GradEpi<OUT>::Args ge{out, lddw, g, rows, D};
       PO_TRY((launch_planned<KIND, P, GradEpi<OUT>>(a, ge, plan_of<GradEpi<OUT>>(a), st, what)));
     }
   }
   if (dh && !ws.direct_dh) {
     const int grid = (int)std::min<int64_t>((N * (ws.slab_ld / 4) + 255) / 256, 8192);
-    const int wide = (uintptr_t)dh % 16 == 0 && lddh * es % 16 == 0;
     hipLaunchKernelGGL((slab_sum_k<OUT>), dim3(grid), dim3(256), 0, st, ws.slab, ws.dh_plan.slices, ws.slab_slice, ws.slab_ld,
-                       N, D, g, dh, lddh, wide);
+                       N, D, g, dh, lddh);
   }
   return po::check_launch(what);
 }
@@ -1774,11 +1772,10 @@ extern "C" int po_linear_ce_frozen_bwd(const float* dhu, int dtype, int64_t N, i
   const hipStream_t st = po::stream_of(stream);
   const int64_t ld = (D + 3) / 4 * 4;
   const int grid = (int)std::min<int64_t>((N * (ld / 4) + 255) / 256, 8192);
-  const int wide = (uintptr_t)dh % 16 == 0 && lddh * (dtype == PO_F32 ? 4 : 2) % 16 == 0;
   hipLaunchKernelGGL((dtype == PO_F32    ? frozen_scale_k<3>
                       : dtype == PO_F16 ? frozen_scale_k<F16>
                                         : frozen_scale_k<BF16>),
                      dim3(grid), dim3(256), 0, st, dhu, ld, (int)N, (int)D, target, ignore_index, grad, reduction == 0,
-                     reduction == 2 ? count : nullptr, dh, lddh, wide);
+                     reduction == 2 ? count : nullptr, dh, lddh);
   return po::check_launch("po_linear_ce_frozen_bwd");
 }
