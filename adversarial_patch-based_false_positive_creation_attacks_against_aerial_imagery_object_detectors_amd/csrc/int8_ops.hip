@@ -414,7 +414,6 @@ int matmul(const int8_t* q, int64_t ldq, const float* sx, const int8_t* w, int64
   a.A = Operand{reinterpret_cast<const char*>(w), ldw, 0, (int)N};
   a.B = Operand{reinterpret_cast<const char*>(q), ldq, 0, (int)M};
   a.kbytes = (int)((K + 15) / 16 * 16);
-  a.pairs = 1;
   if (dtype == PO_F32) return product_of<PO_F32>(a, {y, ldy, sx, sw, bias, (int)M, (int)N}, s);
   if (dtype == PO_F16) return product_of<PO_F16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N}, s);
   return product_of<PO_BF16>(a, {y, ldy, sx, sw, bias, (int)M, (int)N}, s);

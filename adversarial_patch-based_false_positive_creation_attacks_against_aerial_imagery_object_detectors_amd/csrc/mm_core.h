@@ -81,10 +81,10 @@ struct Cfg {
   static constexpr int KIND = KIND_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = KB_, STAGES = STAGES_;
   static constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   static constexpr int RPI = 1024 / KB;                                  // rows one wave's DMA instruction fills
-  static constexpr int NA = (BM / RPI + NW - 1) / NW, NB = BN / RPI / NW;   // instructions per wave and stage
+  static constexpr int NA = (BM / RPI + NW - 1) / NW, NB = (BN / RPI + NW - 1) / NW;   // instructions per wave and stage
   static constexpr int STAGE_BYTES = (BM + BN) * KB * PLANES, LDS = KG * STAGES * STAGE_BYTES;
-  static_assert(KB % 64 == 0 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && BM % RPI == 0 && NB * RPI * NW == BN, "tile");
-  static_assert(PLANES == 3 || NA * RPI * NW == BM, "every wave loads as much");
+  static_assert(KB % 64 == 0 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && BM % RPI == 0 && BN % RPI == 0, "tile");
+  static_assert(PLANES == 3 || (NA * RPI * NW == BM && NB * RPI * NW == BN), "every wave loads as much");
   static_assert((KG - 1) * BM * BN * 4 <= LDS, "the groups' sums pass through LDS");
 };
 
@@ -114,7 +114,7 @@ struct NoRefs {
 template <class C>
 struct Refs {
   static constexpr bool on = true;
-  static constexpr int SLOTS = 4, COLS = C::TN * 16;         // four: blocks of single steps, two steps ahead
+  static constexpr int SLOTS = 2, COLS = C::TN * 16;
   static constexpr int LDS = SLOTS * 1024 + C::NW * COLS * 8;
   static_assert(C::KG == 1 && C::BN <= 256, "one group's sums, a tile's references in one load");
   const char* p;                                             // of block 0 and the tile's first column
@@ -177,15 +177,12 @@ struct Refs {
   }
 };
 
-// acc += the tile's product over the k-steps [ks0, ks1) of the plane pairs.
-// Planes: an operand of wider numbers is stored as `planes` 16-bit matrices, and
-// the step index runs over pairs of them: pair q multiplies plane (pa >> 4q & 15)
-// of A with plane (pb >> 4q & 15) of B; steps [q * nk, (q + 1) * nk) are pair q's.
-// kbytes: length of a row; ends inside a step read as zero.  ks1 > ks0.
+// acc += the tile's product over the k-steps [ks0, ks1).  kbytes: length of a row; ends inside a step
+// read as zero.  ks1 > ks0.
 template <class C, class RefsT>
 __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM][C::TN], const Operand& A,
-                                        const Operand& B, int m0, int n0, int kbytes, int ks0, int ks1, int nk,
-                                        uint32_t pa, uint32_t pb, char* lds, RefsT& refs) {
+                                        const Operand& B, int m0, int n0, int kbytes, int ks0, int ks1, char* lds,
+                                        RefsT& refs) {
   constexpr int KB = C::KB, CPR = KB / 16;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = wid % C::NW, kg = wid / C::NW;
@@ -211,20 +208,17 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
   const uint32_t lch = ((lane % CPR) ^ swz<KB>(wave * C::RPI + lrow)) * 16;
   const char* abase = A.p + (int64_t)m0 * A.stride;
   const char* bbase = B.p + (int64_t)n0 * B.stride;
-  int next = ks0 + kg, q = next / nk, kt = next - q * nk;    // the next stage's step, its plane pair and place in it
-  int place = kt;                                            // of the step that is multiplied (one group)
+  int next = ks0 + kg;                                       // the next stage's step
   constexpr int PER = 256 / KB;                              // steps of a block of references
   if constexpr (RefsT::on) refs.start();
+  const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(abase), 0, 0x7fffffff, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(bbase), 0, 0x7fffffff, 0x00020000);
   auto issue = [&](int buf) {
     if constexpr (RefsT::on)
-      if (kt % PER == 0 || next == ks0) refs.load(kt / PER);  // ahead of the operands: the waits below count them
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char*>(abase + (int64_t)((pa >> (4 * q)) & 15) * A.plane), 0, 0x7fffffff, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char*>(bbase + (int64_t)((pb >> (4 * q)) & 15) * B.plane), 0, 0x7fffffff, 0x00020000);
+      if (next % PER == 0 || next == ks0) refs.load(next / PER);   // ahead of the operands: the waits below count them
     char* la = lds + buf * C::STAGE_BYTES;
     char* lb = la + C::BM * KB;
-    const uint32_t k0 = (uint32_t)kt * KB;
+    const uint32_t k0 = (uint32_t)next * KB;
     // past the row's end: out of range by the sign bit (offsets stay below 2^31)
     const uint32_t past = (int)(k0 + lch) < kbytes && (C::KG == 1 || next < ks1) ? k0 : kOOB;
 #pragma unroll
@@ -234,11 +228,6 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
     for (int i = 0; i < C::NB; ++i)
       Loader<C>::dma(rb, lb + (i * C::NW + wave) * 1024, (ob[i] + (past & 0x7fffffffu)) | (past & kOOB) | (ob[i] & kOOB));
     next += C::KG;
-    kt += C::KG;
-    while (kt >= nk) {
-      kt -= nk;
-      ++q;
-    }
   };
   const int n = (ks1 - ks0 + C::KG - 1) / C::KG;             // of every group: a last step past the end adds zeros
 #pragma unroll
@@ -295,9 +284,8 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
     if constexpr (!first) multiply(fa[1], fb[1]);            // the last group of the step before
     if constexpr (RefsT::on) {
       __builtin_amdgcn_sched_barrier(0);
-      if (first || place % PER == 0) refs.take(acc);
+      if (first || (ks0 + s) % PER == 0) refs.take(acc);
       refs.mask(fb[0]);
-      place = place + 1 == nk ? 0 : place + 1;
     }
 #pragma unroll
     for (int g = 1; g < G; ++g) {
@@ -385,7 +373,8 @@ __device__ __forceinline__ void product3(f4v (&acc)[C::TM][C::TN], const Operand
           Loader<C>::dma(ra, la + p * PA + (i * C::NW + wave) * 1024, (oa[i] + (past & 0x7fffffffu)) | (past & kOOB) | (oa[i] & kOOB));
 #pragma unroll
       for (int i = 0; i < C::NB; ++i)
-        Loader<C>::dma(rb, lb + p * PB + (i * C::NW + wave) * 1024, (ob[i] + (past & 0x7fffffffu)) | (past & kOOB) | (ob[i] & kOOB));
+        if (C::NB * C::NW * C::RPI == C::BN || i * C::NW + wave < C::BN / C::RPI)
+          Loader<C>::dma(rb, lb + p * PB + (i * C::NW + wave) * 1024, (ob[i] + (past & 0x7fffffffu)) | (past & kOOB) | (ob[i] & kOOB));
     }
   };
   const int h = lane >> 4, r16 = lane & 15, turned = (h ^ ((r16 >> 2) & 3)) * 16 + r16 * 64;
@@ -463,8 +452,7 @@ __device__ __forceinline__ void product3(f4v (&acc)[C::TM][C::TN], const Operand
 struct Args {
   Operand A, B;
   int tiles_m, tiles_n;
-  int kbytes, nk, pairs;      // bytes of a row, k-steps, plane pairs
-  uint32_t pa, pb;
+  int kbytes, nk;             // bytes of a row, k-steps
 };
 
 template <class C>
@@ -515,13 +503,12 @@ __global__ __launch_bounds__(C::NW * C::KG * 64, C::LDS > 81920 ? 1 : 2) void pr
     for (int j = 0; j < C::TN; ++j) t.acc[i][j] = typename Acc<C::KIND>::type{0, 0, 0, 0};
   typename Epi::template Pre<C> pre;
   pre.load(t, e);
-  const int total = a.nk * a.pairs;
-  const int ks0 = (int)((int64_t)blockIdx.y * total / gridDim.y), ks1 = (int)((int64_t)(blockIdx.y + 1) * total / gridDim.y);
+  const int ks0 = (int)((int64_t)blockIdx.y * a.nk / gridDim.y), ks1 = (int)((int64_t)(blockIdx.y + 1) * a.nk / gridDim.y);
   auto multiply = [&](auto& refs) {
     if constexpr (C::PLANES == 3)
       product3<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, lds, refs);
     else
-      product<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, a.nk, a.pa, a.pb, lds, refs);
+      product<C>(t.acc, a.A, a.B, t.tm * C::BM, t.tn * C::BN, a.kbytes, ks0, ks1, lds, refs);
   };
   if constexpr (HasRefs<Epi>::value) {
     // tokens of one r in all of these blocks: an ordinary product
@@ -555,8 +542,7 @@ inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipSt
   a.tiles_m = ceil_div(a.A.rows, C::BM);
   a.tiles_n = ceil_div(a.B.rows, C::BN);
   a.nk = ceil_div(a.kbytes, C::KB);
-  if (C::PLANES == 3) a.pairs = 1;                           // six in a step
-  if ((int64_t)a.tiles_m * a.tiles_n >= (1LL << 22) || slices > 65535 || (int64_t)a.nk * a.pairs >= (1LL << 31) || slices > (int64_t)a.nk * a.pairs ||
+  if ((int64_t)a.tiles_m * a.tiles_n >= (1LL << 22) || slices > 65535 || slices > a.nk ||
       a.A.stride * C::BM >= (1LL << 31) || a.B.stride * C::BN >= (1LL << 31) || a.kbytes < 0) {
     set_error("%s: operand too large", what);
     return PO_EINVAL;
@@ -574,10 +560,12 @@ inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipSt
 // taken for long k or cheap epilogues, MID for few tiles and short k: the losses' forward
 // product of 32768 x 2048 x 512 78 against 95 us; the gradient of the logits there 117
 // against 112 us, at k = 128 73 against 63.  slices > 1 cuts k between workgroups, each
-// slice's sums then cost sum_us.  Products of three planes: LARGE 256 x 128, MID 128 x 64, and TALL
+// slice's sums then cost sum_us.  Products of three planes: LARGE 256 x 128, MID 128 x 64, SQUARE
+// 128 x 128 (one to a CU: of up to 128 tokens it loads the vocabulary once; logits and their gradient of
+// 100 x 30000 x 1024 84 and 94 us with MID, 69 and 77), and TALL
 // 192 x 128 for widths that fill 256 badly (the gradients of 20011 x 1000 x 513: 172 and 152 us in
 // 768 rows of LARGE tiles, 157 and 141 in 576 of TALL).
-enum TileId { FEW, MID, LARGE, TALL };
+enum TileId { FEW, MID, LARGE, SQUARE, TALL };
 struct Plan {
   TileId tile;
   int slices;
@@ -589,9 +577,10 @@ struct TileKind {
   double step, ends;            // ends: share of the epilogue's time
 };
 // of products of single planes, and of three (a step: 64 k of one of the six products)
-constexpr TileKind kTiles[2][4] = {
-    {{FEW, 128, 32, 512, 0.45, 0}, {MID, 128, 128, 512, 1.08, 1}, {LARGE, 256, 256, 256, 1.7, 1}, {}},
-    {{FEW, 128, 32, 512, 0.45, 0}, {MID, 128, 64, 512, 0.45, 0.5}, {LARGE, 256, 128, 256, 0.73, 0.5}, {TALL, 192, 128, 256, 0.57, 0.4}}};
+constexpr TileKind kTiles[2][5] = {
+    {{FEW, 128, 32, 512, 0.45, 0}, {MID, 128, 128, 512, 1.08, 1}, {LARGE, 256, 256, 256, 1.7, 1}, {}, {}},
+    {{FEW, 128, 32, 512, 0.35, 0}, {MID, 128, 64, 512, 0.45, 0.5}, {LARGE, 256, 128, 256, 0.73, 0.5},
+     {SQUARE, 128, 128, 256, 0.42, 0.5}, {TALL, 192, 128, 256, 0.57, 0.4}}};
 // What the plan has to know of a product's epilogue: us, and whether its tiles may be TALL
 struct Ends {
   double mid, large;

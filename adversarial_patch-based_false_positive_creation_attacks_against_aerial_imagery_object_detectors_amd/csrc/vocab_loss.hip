@@ -47,14 +47,11 @@ using Large = std::conditional_t<P == 3, Cfg<KIND, 256, 128, 4, 2, 64, 2, 1, 3>,
 template <int KIND, int P>
 using Mid = std::conditional_t<P == 3, Cfg<KIND, 128, 64, 2, 2, 64, 2, 1, 3>, Cfg<KIND, 128, 128, 2, 2, 128, 2>>;
 template <int KIND>
-using Tall = Cfg<KIND, 192, 128, 4, 2, 64, 2, 1, 3>;         // of three planes only
+using Square = Cfg<KIND, 128, 128, 4, 2, 64, 2, 1, 3>;       // of three planes only, as
 template <int KIND>
-using Few = Cfg<KIND, 128, 32, 4, 1, 128, 3>;
-// few of them: two groups of waves take the steps of k in turn (fp32 losses of 81 x 7855 x 1032, 186 tiles
-// of 102 steps: 39 -> 30 us; where tiles fill the chip twice the groups stand in each other's way: 10 -> 14)
-template <int KIND>
-using Fewer = Cfg<KIND, 128, 32, 4, 1, 128, 3, 2>;
-
+using Tall = Cfg<KIND, 192, 128, 4, 2, 64, 2, 1, 3>;
+template <int KIND, int P>
+using Few = std::conditional_t<P == 3, Cfg<KIND, 128, 32, 4, 1, 64, 2, 1, 3>, Cfg<KIND, 128, 32, 4, 1, 128, 3>>;
 // over the four lanes that hold a column
 __device__ __forceinline__ float column_max(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
@@ -1380,13 +1377,6 @@ struct FrozenWs {
   }
 };
 
-// pairs of planes, the largest products first: 00 01 10 11 02 20
-inline void set_pairs(Args& a, int planes) {
-  a.pairs = planes == 3 ? 6 : 1;
-  a.pa = planes == 3 ? 0x201100u : 0u;
-  a.pb = planes == 3 ? 0x021010u : 0u;
-}
-
 // operand rows [r0, r0 + rows) of the caller's matrix, or of buf where they do not serve as they are
 struct Side {
   const void* x;
@@ -1429,14 +1419,9 @@ inline int check_shape(const char* what, int64_t N, int64_t V, int64_t D, int dt
 
 template <int KIND, int P, class Epi>
 inline int launch_planned(const Args& a, const typename Epi::Args& e, Plan p, hipStream_t s, const char* what) {
-  if (p.tile == FEW) {
-    if constexpr (!HasRefs<Epi>::value) {
-      const int64_t tiles = (int64_t)ceil_div(a.A.rows, 128) * ceil_div(a.B.rows, 32) * p.slices;
-      if (tiles <= 256 && (int64_t)ceil_div(a.kbytes, 128) * a.pairs >= 8 * p.slices)
-        return launch_product<Fewer<KIND>, Epi>(a, e, p.slices, s, what);
-    }
-    return launch_product<Few<KIND>, Epi>(a, e, p.slices, s, what);
-  }
+  if (p.tile == FEW) return launch_product<Few<KIND, P>, Epi>(a, e, p.slices, s, what);
+  if constexpr (P == 3)
+    if (p.tile == SQUARE) return launch_product<Square<KIND>, Epi>(a, e, p.slices, s, what);
   if constexpr (P == 3 && Epi::kEnds.tall)
     if (p.tile == TALL) return launch_product<Tall<KIND>, Epi>(a, e, p.slices, s, what);
   if (p.tile == MID) return launch_product<Mid<KIND, P>, Epi>(a, e, p.slices, s, what);
@@ -1444,13 +1429,13 @@ inline int launch_planned(const Args& a, const typename Epi::Args& e, Plan p, hi
 }
 
 template <class Epi>
-inline Plan plan_of(const Args& a) {
-  return plan_product(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs, Epi::kEnds, a.pairs > 1);
+inline Plan plan_of(const Args& a, int planes) {
+  return plan_product(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * (planes == 3 ? 6 : 1), Epi::kEnds, planes == 3);
 }
 
 template <class Epi>
-inline int64_t first_part(const Args& a) {
-  return whole_rounds(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * a.pairs, Epi::kEnds, a.pairs > 1);
+inline int64_t first_part(const Args& a, int planes) {
+  return whole_rounds(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * (planes == 3 ? 6 : 1), Epi::kEnds, planes == 3);
 }
 
 inline void row_stats(const float2* partial, int parts, const Shape& s, const float* tlogit, const int64_t* target, int64_t ignore,
@@ -1522,7 +1507,6 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
     return po::check_launch("po_linear_ce_fwd");
   }
   Args a{};
-  set_pairs(a, s.planes());
   a.kbytes = s.Dp() * 2;
   const Side hs{h, ldh, s.direct_h, ws.hp}, wside{w, ldw, s.direct_w, ws.wp};
   a.B = rows_of(s, hs, 0, N);
@@ -1533,11 +1517,11 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
     const Operand W = rows_of(s, wside, v, rows);
     for (int64_t r = 0, part; r < rows; r += part) {
       a.A = W.from(r);
-      part = first_part<StatsEpi>(a);
+      part = first_part<StatsEpi>(a, s.planes());
       a.A.rows = (int)part;
       e.v0 = v + r;
       e.V = (int)part;
-      const Plan p = plan_of<StatsEpi>(a);
+      const Plan p = plan_of<StatsEpi>(a, s.planes());
       PO_TRY((dtype == PO_F16    ? launch_planned<F16, 1, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
                : dtype == PO_BF16 ? launch_planned<BF16, 1, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
                                   : launch_planned<BF16, 3, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")));
@@ -1564,19 +1548,18 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
     const Operand W = rows_of(s, w, v, rows);
     pack(s, h, v ? 0 : N, w, v, rows, st);
     Args a{};
-    set_pairs(a, P);
     // dl of the piece
     a.B = H;
     a.kbytes = s.Dp() * 2;
     for (int64_t r = 0, part; r < rows; r += part) {
       using E = DlogitsEpi<KIND, P>;
       a.A = W.from(r);
-      part = first_part<E>(a);
+      part = first_part<E>(a, P);
       a.A.rows = (int)part;
       const typename E::Args e{stat, g, v + r, N, (int)s.Np(), (int)part, (int)(r + part < rows ? part : rp - r), scale * kLog2e,
                                dh ? ws.dl + r : nullptr, dw ? ws.dlt + r * s.ldn() : nullptr, ws.ldl, s.ldn(), N * ws.ldl,
                                ws.piece * s.ldn()};
-      PO_TRY((launch_planned<KIND, P, E>(a, e, plan_of<E>(a), st, what)));
+      PO_TRY((launch_planned<KIND, P, E>(a, e, plan_of<E>(a, P), st, what)));
     }
     // the piece's w, and once h, the other way round
     const TransposeJob tw{reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, rp, 0, ws.wt, ws.ldl, D * ws.ldl};
@@ -1604,7 +1587,7 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
       a.kbytes = (int)s.Np() * 2;
       char* out = static_cast<char*>(dw) + v * lddw * es;
       const typename GradEpi<OUT>::Args ge{out, lddw, g, rows, D};
-      PO_TRY((launch_planned<KIND, P, GradEpi<OUT>>(a, ge, plan_of<GradEpi<OUT>>(a), st, what)));
+      PO_TRY((launch_planned<KIND, P, GradEpi<OUT>>(a, ge, plan_of<GradEpi<OUT>>(a, P), st, what)));
     }
   }
   if (dh && !ws.direct_dh) {
@@ -1671,17 +1654,16 @@ int frozen_forward(const Shape& s, const FrozenWs& ws, const Side& h, const Side
     pack(s, h, v ? 0 : N, w, v, rows, st);
     const Operand W = rows_of(s, w, v, rows);
     Args a{};
-    set_pairs(a, P);
     a.B = rows_of(s, h, 0, N);
     a.kbytes = s.Dp() * 2;
     for (int64_t r = 0, part; r < rows; r += part) {
       using E = KeepEpi<KIND, P>;
       a.A = W.from(r);
-      part = first_part<E>(a);
+      part = first_part<E>(a, P);
       a.A.rows = (int)part;
       e.v0 = v + r;
       e.V = (int)part;
-      const Plan p = plan_of<E>(a);
+      const Plan p = plan_of<E>(a, P);
       const typename E::Args ke{e, base, ws.refs + r / 128 * ws.ldr, ws.other + r / 128 * ws.ldo, ws.ldr, ws.ldo,
                                 (int)(r + part < rows ? part : rp - r), ws.kept + r, ws.ldk, N * ws.ldk};
       PO_TRY((launch_planned<KIND, P, E>(a, ke, p, st, what)));
