@@ -689,35 +689,22 @@ __global__ __launch_bounds__(1024) void grad_rows_k(const GradOf g, int N, float
   if (threadIdx.x == 0) *factor = top > 0.f ? top / g.lift * g.c : 0.f;
 }
 
-// Rows laid out for the products, cols padded with zeros to a multiple of 8, rows ldo apart: 16-bit
-// numbers, or fp32 as planes of three bf16.  A thread makes 8 columns.  Two matrices in one launch.
-struct PackJob {
-  const void* x;
-  int64_t ld, rows, plane;
-  uint16_t* out;
-};
+// Eight neighbours of a row as the products take them: 16-bit numbers, or the three bf16 of each fp32.
 template <typename T>
-__global__ __launch_bounds__(256) void pack_k(const PackJob j0, const PackJob j1, int cols, int64_t ldo) {
+struct Eight {
+  static constexpr int P = sizeof(T) == 4 ? 3 : 1;
   typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  const int per = (cols + 7) / 8;
-  const int64_t total = (j0.rows + j1.rows) * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    int64_t r = i / per;
-    const int c = (int)(i - r * per) * 8;
-    const bool second = r >= j0.rows;
-    if (second) r -= j0.rows;
-    const int64_t plane = second ? j1.plane : j0.plane;
-    const T* p = static_cast<const T*>(second ? j1.x : j0.x) + r * (second ? j1.ld : j0.ld) + c;
-    uint16_t* const out = second ? j1.out : j0.out;
+  i4v plane[P];
+  // the first n of p, and zeros
+  __device__ __forceinline__ void load(const T* p, int n) {
     v8 v;
-    if (c + 8 <= cols) {
+    if (n >= 8) {
       v = *reinterpret_cast<const v8*>(p);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? p[k] : (T)0;
+      for (int k = 0; k < 8; ++k) v[k] = k < n ? p[k] : (T)0;
     }
-    uint16_t* o = out + r * ldo + c;
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (P == 3) {
       uint32_t b[3][4] = {};
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -736,49 +723,90 @@ __global__ __launch_bounds__(256) void pack_k(const PackJob j0, const PackJob j1
         }
       }
 #pragma unroll
-      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(o + q * plane) = make_uint4(b[q][0], b[q][1], b[q][2], b[q][3]);
+      for (int q = 0; q < 3; ++q) plane[q] = i4v{(int)b[q][0], (int)b[q][1], (int)b[q][2], (int)b[q][3]};
     } else {
       typedef T w8 __attribute__((ext_vector_type(8)));
-      *reinterpret_cast<w8*>(o) = v;
+      plane[0] = __builtin_bit_cast(i4v, (w8)v);
     }
+  }
+};
+
+// Rows laid out for the products, cols padded with zeros to a multiple of 8, rows ldo apart, planes behind
+// each other.  A thread makes 8 columns.  Two matrices in one launch.
+struct PackJob {
+  const void* x;
+  int64_t ld, rows, plane;
+  uint16_t* out;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void pack_k(const PackJob j0, const PackJob j1, int cols, int64_t ldo) {
+  const int per = (cols + 7) / 8;
+  const int64_t total = (j0.rows + j1.rows) * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    int64_t r = i / per;
+    const int c = (int)(i - r * per) * 8;
+    const bool second = r >= j0.rows;
+    if (second) r -= j0.rows;
+    Eight<T> v;
+    v.load(static_cast<const T*>(second ? j1.x : j0.x) + r * (second ? j1.ld : j0.ld) + c, cols - c);
+    uint16_t* const o = (second ? j1.out : j0.out) + r * ldo + c;
+#pragma unroll
+    for (int q = 0; q < Eight<T>::P; ++q) *reinterpret_cast<i4v*>(o + q * (second ? j1.plane : j0.plane)) = v.plane[q];
   }
 }
 
-// out[c][r] = x[r][c] (16 bits) for r < Rp (a multiple of 8): zero for r >= R and, masked, for rows that take
-// no part (they may hold anything and multiply zeros only).  Two matrices of one width in one launch.  x: rows
-// on 16 bytes, readable to the next multiple of 8 columns.  64 rows x 256 columns to a workgroup, through LDS as a product's outputs; blockIdx.z: plane.
+// Rows laid out both ways, from one reading: as pack_k's (rows, if any), and with rows for columns (cols, if
+// any): cols[c][r] = x[r][c] for r < Rp (a multiple of 8), zero for r >= R and, masked, for rows that take no part
+// (they may hold anything and multiply zeros only).  Two matrices of one width in one launch.  64 rows x 256
+// columns to a workgroup, the transpose through LDS as a product's outputs.  fp32, 20011 x 513: 41 us, a
+// kernel for each way (the second reading the first's planes) 49.
 struct Pane {
   static constexpr int BM = 256, BN = 64, NW = 4;
 };
-struct TransposeJob {
-  const uint16_t* x;
-  int64_t ld, plane;
-  int R, Rp, masked;            // masked: rows that take no part are zero
-  uint16_t* out;
-  int64_t ldo, oplane;
+struct LayJob {
+  const void* x;
+  int64_t ld;
+  int R, Rp, masked;
+  uint16_t* rows;
+  int64_t rplane;
+  uint16_t* cols;
+  int64_t ldc, cplane;
 };
-__global__ __launch_bounds__(256) void transpose_k(const TransposeJob j0, const TransposeJob j1, int blocks0, int Cc,
-                                                   const GradOf g) {
+template <typename T>
+__global__ __launch_bounds__(256) void lay_k(const LayJob j0, const LayJob j1, int blocks0, int D, int64_t ldr, const GradOf g) {
   __shared__ __attribute__((aligned(16))) char lds[Pane::BM * Pane::BN * 2];
+  constexpr int P = Eight<T>::P;
   const bool second = (int)blockIdx.x >= blocks0;
-  const TransposeJob& j = second ? j1 : j0;
+  const LayJob& j = second ? j1 : j0;
   const int r0 = ((int)blockIdx.x - (second ? blocks0 : 0)) * 64, c0 = blockIdx.y * 256;
-  const uint16_t* x = j.x + blockIdx.z * j.plane;
-  const int c = threadIdx.x % 32, cc = c0 + c * 8;
-  i4v v[8];
+  const int chunk = threadIdx.x % 32, c = c0 + chunk * 8;
+  Eight<T> v[8];
 #pragma unroll
   for (int s = 0; s < 8; ++s) {
     const int r = r0 + threadIdx.x / 32 + s * 8;
-    const bool ok = r < j.R && cc < Cc && (!j.masked || g.live(r));
-    v[s] = ok ? *reinterpret_cast<const i4v*>(x + r * j.ld + cc) : i4v{0, 0, 0, 0};
-  }
+    const bool in = r < j.R && c < D;
+    v[s].load(static_cast<const T*>(j.x) + (in ? r * j.ld + c : 0), in ? D - c : 0);
+    if (j.rows && in) {
 #pragma unroll
-  for (int s = 0; s < 8; ++s) {
-    const int n = threadIdx.x / 32 + s * 8;
-    *reinterpret_cast<i4v*>(lds + n * 512 + ((c ^ turn<Pane>(n)) * 16)) = v[s];
+      for (int q = 0; q < P; ++q) *reinterpret_cast<i4v*>(j.rows + q * j.rplane + r * ldr + c) = v[s].plane[q];
+    }
+    if (j.masked && r < j.R && !g.live(r)) {
+#pragma unroll
+      for (int q = 0; q < P; ++q) v[s].plane[q] = i4v{0, 0, 0, 0};
+    }
   }
-  __syncthreads();
-  store_columns<Pane>(lds, j.out + blockIdx.z * j.oplane, j.ldo, r0, c0, j.Rp, Cc);
+  if (!j.cols) return;
+#pragma unroll
+  for (int q = 0; q < P; ++q) {
+    __syncthreads();                                         // the last plane's reads are over
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const int n = threadIdx.x / 32 + s * 8;
+      *reinterpret_cast<i4v*>(lds + n * 512 + ((chunk ^ turn<Pane>(n)) * 16)) = v[s].plane[q];
+    }
+    __syncthreads();
+    store_columns<Pane>(lds, j.cols + q * j.cplane, j.ldc, r0, c0, j.Rp, D);
+  }
 }
 
 // four neighbours in the gradients' type (OUT: BF16, F16, or 3: fp32), those below cols; one store, which
@@ -1405,6 +1433,20 @@ inline void pack(const Shape& s, const Side& h, int64_t hrows, const Side& w, in
     hipLaunchKernelGGL((pack_k<uint16_t>), grid, dim3(256), 0, st, a, b, (int)s.D, s.ldp());
 }
 
+// rows [r0, r0 + rows) of the caller's matrix: laid out where they do not serve as they are, and (cols) transposed,
+// rows ldc apart, planes D rows apart
+inline LayJob lay_job(const Shape& s, const Side& m, int64_t r0, int64_t rows, int64_t rp, int masked, uint16_t* cols, int64_t ldc) {
+  return LayJob{static_cast<const char*>(m.x) + r0 * m.ld * (s.dtype == PO_F32 ? 4 : 2), m.ld, (int)rows, (int)rp, masked,
+                m.direct ? nullptr : m.buf, rows * s.ldp(), cols, ldc, s.D * ldc};
+}
+inline void lay(const Shape& s, const LayJob& a, const LayJob& b, const GradOf& g, hipStream_t st) {
+  auto blocks = [](const LayJob& j) { return j.rows || j.cols ? ceil_div(j.cols ? j.Rp : j.R, 64) : 0; };
+  const int b0 = blocks(a), b1 = blocks(b);
+  if (!(b0 + b1)) return;
+  hipLaunchKernelGGL((s.dtype == PO_F32 ? lay_k<float> : lay_k<uint16_t>), dim3(b0 + b1, ceil_div(s.D, 256)), dim3(256), 0, st, a, b, b0,
+                     (int)s.D, s.ldp(), g);
+}
+
 inline bool serves(const void* x, int64_t ld, int dtype, int64_t D) {
   return dtype != PO_F32 && D % 8 == 0 && ld % 8 == 0 && (uintptr_t)x % 16 == 0;
 }
@@ -1546,7 +1588,10 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
     const int rows = (int)std::min(ws.piece, s.V - v);
     const int rp = (rows + 63) / 64 * 64;
     const Operand W = rows_of(s, w, v, rows);
-    pack(s, h, v ? 0 : N, w, v, rows, st);
+    // the piece's w, and once h, laid out and the other way round
+    LayJob hj{};
+    if (!v) hj = lay_job(s, h, 0, N, s.Np(), 1, dw ? ws.ht : nullptr, s.ldn());
+    lay(s, lay_job(s, w, v, rows, rp, 0, dh ? ws.wt : nullptr, ws.ldl), hj, g, st);
     Args a{};
     // dl of the piece
     a.B = H;
@@ -1561,12 +1606,6 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
                                ws.piece * s.ldn()};
       PO_TRY((launch_planned<KIND, P, E>(a, e, plan_of<E>(a, P), st, what)));
     }
-    // the piece's w, and once h, the other way round
-    const TransposeJob tw{reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, rp, 0, ws.wt, ws.ldl, D * ws.ldl};
-    const TransposeJob th{reinterpret_cast<const uint16_t*>(H.p), H.stride / 2, H.plane / 2, N, (int)s.Np(), 1, ws.ht, s.ldn(), D * s.ldn()};
-    const int bw = dh ? ceil_div(rp, 64) : 0, bh = dw && !v ? ceil_div(s.Np(), 64) : 0;
-    if (bw + bh)
-      hipLaunchKernelGGL(transpose_k, dim3(bw + bh, ceil_div(D, 256), P), dim3(256), 0, st, tw, th, bw, D, g);
     if (dh) {                                                // sums over v of dl[n][v] w[v][d]
       a.A = Operand{reinterpret_cast<char*>(ws.wt), ws.ldl * 2, D * ws.ldl * 2, D};
       a.B = Operand{reinterpret_cast<char*>(ws.dl), ws.ldl * 2, N * ws.ldl * 2, N};
@@ -1651,7 +1690,9 @@ int frozen_forward(const Shape& s, const FrozenWs& ws, const Side& h, const Side
   *pieces = 0;
   for (int64_t v = 0; v < s.V; v += ws.piece, ++*pieces) {
     const int rows = (int)std::min(ws.piece, s.V - v), rp = (rows + 63) / 64 * 64;
-    pack(s, h, v ? 0 : N, w, v, rows, st);
+    LayJob hj{};
+    if (!v) hj = lay_job(s, h, 0, N, N, 0, nullptr, 0);
+    lay(s, lay_job(s, w, v, rows, rp, 0, ws.wt, ws.ldk), hj, GradOf{}, st);
     const Operand W = rows_of(s, w, v, rows);
     Args a{};
     a.B = rows_of(s, h, 0, N);
@@ -1669,9 +1710,6 @@ int frozen_forward(const Shape& s, const FrozenWs& ws, const Side& h, const Side
       PO_TRY((launch_planned<KIND, P, E>(a, ke, p, st, what)));
       e.tile0 += ceil_div(part, p.tile == LARGE ? 256 : 128);
     }
-    const TransposeJob tw{reinterpret_cast<const uint16_t*>(W.p), W.stride / 2, W.plane / 2, rows, rp, 0, ws.wt, ws.ldk, D * ws.ldk};
-    const int blocks = ceil_div(rp, 64);
-    hipLaunchKernelGGL(transpose_k, dim3(blocks, ceil_div(D, 256), P), dim3(256), 0, st, tw, tw, blocks, D, GradOf{});
     a.A = Operand{reinterpret_cast<char*>(ws.wt), ws.ldk * 2, D * ws.ldk * 2, D};
     a.B = Operand{reinterpret_cast<char*>(ws.kept), ws.ldk * 2, N * ws.ldk * 2, N};
     a.kbytes = rp * 2;
