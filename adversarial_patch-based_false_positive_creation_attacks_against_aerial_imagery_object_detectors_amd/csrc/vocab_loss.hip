@@ -696,7 +696,7 @@ struct Eight {
   typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
   i4v plane[P];
   // the first n of p, and zeros
-  __device__ __forceinline__ void load(const T* p, int n) {
+  static __device__ __forceinline__ v8 read(const T* p, int n) {
     v8 v;
     if (n >= 8) {
       v = *reinterpret_cast<const v8*>(p);
@@ -704,6 +704,9 @@ struct Eight {
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = k < n ? p[k] : (T)0;
     }
+    return v;
+  }
+  __device__ __forceinline__ void split(v8 v) {
     if constexpr (P == 3) {
       uint32_t b[3][4] = {};
 #pragma unroll
@@ -748,7 +751,7 @@ __global__ __launch_bounds__(256) void pack_k(const PackJob j0, const PackJob j1
     const bool second = r >= j0.rows;
     if (second) r -= j0.rows;
     Eight<T> v;
-    v.load(static_cast<const T*>(second ? j1.x : j0.x) + r * (second ? j1.ld : j0.ld) + c, cols - c);
+    v.split(v.read(static_cast<const T*>(second ? j1.x : j0.x) + r * (second ? j1.ld : j0.ld) + c, cols - c));
     uint16_t* const o = (second ? j1.out : j0.out) + r * ldo + c;
 #pragma unroll
     for (int q = 0; q < Eight<T>::P; ++q) *reinterpret_cast<i4v*>(o + q * (second ? j1.plane : j0.plane)) = v.plane[q];
@@ -780,12 +783,29 @@ __global__ __launch_bounds__(256) void lay_k(const LayJob j0, const LayJob j1, i
   const LayJob& j = second ? j1 : j0;
   const int r0 = ((int)blockIdx.x - (second ? blocks0 : 0)) * 64, c0 = blockIdx.y * 256;
   const int chunk = threadIdx.x % 32, c = c0 + chunk * 8;
+  // one branch over all eight rows, so that their loads are in flight together; rows past the end read the last
+  typename Eight<T>::v8 raw[8];
+  const T* const x = static_cast<const T*>(j.x) + c;
+  if (c + 8 <= D) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) raw[s] = Eight<T>::read(x + min(r0 + (int)threadIdx.x / 32 + s * 8, j.R - 1) * j.ld, 8);
+  } else {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const int r = r0 + threadIdx.x / 32 + s * 8;
+      raw[s] = Eight<T>::read(x + min(r, j.R - 1) * j.ld, max(0, D - c));
+    }
+  }
   Eight<T> v[8];
 #pragma unroll
   for (int s = 0; s < 8; ++s) {
     const int r = r0 + threadIdx.x / 32 + s * 8;
     const bool in = r < j.R && c < D;
-    v[s].load(static_cast<const T*>(j.x) + (in ? r * j.ld + c : 0), in ? D - c : 0);
+    v[s].split(raw[s]);
+    if (r >= j.R) {
+#pragma unroll
+      for (int q = 0; q < P; ++q) v[s].plane[q] = i4v{0, 0, 0, 0};
+    }
     if (j.rows && in) {
 #pragma unroll
       for (int q = 0; q < P; ++q) *reinterpret_cast<i4v*>(j.rows + q * j.rplane + r * ldr + c) = v[s].plane[q];
