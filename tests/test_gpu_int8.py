@@ -98,7 +98,7 @@ def test_quantize_extreme_rows():
 
 
 SIZES = [(1, 1, 1), (1, 16, 5), (1, 4096, 300), (2, 17, 64), (5, 4001, 130), (16, 64, 100), (17, 1000, 257), (32, 129, 128), (33, 31, 65),
-         (64, 256, 1000), (130, 2000, 257), (1111, 4001, 1000), (1500, 96, 2500), (2500, 160, 5000), (300, 7, 9), (2000, 100, 4000), (1, 70000, 33), (4, 14336, 50), (3, 20000, 17), (31, 3000, 16)]
+         (64, 256, 1000), (130, 2000, 257), (1111, 4001, 1000), (1500, 96, 2500), (2500, 160, 5000), (300, 7, 9), (2000, 100, 4000), (1, 70000, 33), (4, 14336, 50), (3, 20000, 17), (31, 3000, 16), (1100, 300, 1000), (1111, 4001, 500), (2000, 129, 2040)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
