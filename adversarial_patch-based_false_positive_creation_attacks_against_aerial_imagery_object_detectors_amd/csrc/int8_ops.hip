@@ -66,8 +66,25 @@ struct RowScale {
   __device__ __forceinline__ uint2 quotients(const float* v) const {
     uint32_t b[2] = {0, 0};
     if (!bad && s > 1e-30f) {
+      // Where every remainder stays below half of s the rounded products are the quotients (ties, and values next to
+      // one, are looked at one by one); added to 1.5 * 2^23 their low byte is the number.
+      float q[8], far = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) b[j >> 2] |= (uint32_t)(quotient(v[j], s, inv) & 255) << (8 * (j & 3));
+      for (int j = 0; j < 8; ++j) {
+        q[j] = __builtin_rintf(v[j] * inv);
+        far = fmaxf(far, fabsf(__builtin_fmaf(-q[j], s, v[j])));
+      }
+      if (far >= 0.5f * s) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = (float)quotient(v[j], s, inv);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(q[4 * h + j] + 12582912.f);
+        b[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400), __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400), 0x05040100);
+      }
     } else if (!bad && s > 0.f) {                            // 1 / s and half steps of s need normal numbers
 #pragma unroll 1
       for (int h = 0; h < 2; ++h)
