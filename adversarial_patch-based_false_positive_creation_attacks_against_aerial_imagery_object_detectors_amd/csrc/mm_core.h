@@ -41,7 +41,7 @@ typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // in memor
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 
-enum Kind { BF16 = 0, F16 = 1, I8 = 2 };
+enum Kind { BF16 = 0, F16 = 1, I8 = 2, F32 = 3 };
 
 template <int KIND>
 struct Acc {
@@ -58,8 +58,15 @@ __device__ __forceinline__ typename Acc<KIND>::type mfma(i4v a, i4v b, typename 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0, 0);
   else if constexpr (KIND == F16)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
-  else
+  else if constexpr (KIND == I8)
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+  else {
+    // four products of 4 k; which k stands in which place of a chunk is the same in both operands
+    const f4v x = __builtin_bit_cast(f4v, a), y = __builtin_bit_cast(f4v, b);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[k], y[k], c, 0, 0, 0);
+    return c;
+  }
 }
 
 // One operand: rows of k-contiguous elements, stride and length in bytes (both
@@ -259,7 +266,8 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
         acc[i][j] = mfma<C::KIND>(a[i], b[j], acc[i][j]);
       }
     // the next group's reads between these MFMAs
-    constexpr int R = C::TM + C::TN, X = C::TM * C::TN, E = X >= 2 * R ? 2 : 1;
+    constexpr int R = C::TM + C::TN, X = C::TM * C::TN * (C::KIND == F32 ? 4 : 1);
+    constexpr int E = C::KIND == F32 ? X / R : X >= 2 * R ? 2 : 1;
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
@@ -576,19 +584,21 @@ struct TileKind {
   int bm, bn, slots;
   double step, ends;            // ends: share of the epilogue's time
 };
-// of products of single planes, and of three (a step: 64 k of one of the six products)
-constexpr TileKind kTiles[2][5] = {
+// of products of single planes, of three (a step: 64 k of one of the six products), and of fp32 as it is
+enum Form { SINGLE, TRIPLE, WHOLE };
+constexpr TileKind kTiles[3][5] = {
     {{FEW, 128, 32, 512, 0.45, 0}, {MID, 128, 128, 512, 1.08, 1}, {LARGE, 256, 256, 256, 1.7, 1}, {}, {}},
     {{FEW, 128, 32, 512, 0.35, 0}, {MID, 128, 64, 512, 0.45, 0.5}, {LARGE, 256, 128, 256, 0.73, 0.5},
-     {SQUARE, 128, 128, 256, 0.42, 0.5}, {TALL, 192, 128, 256, 0.57, 0.4}}};
+     {SQUARE, 128, 128, 256, 0.42, 0.5}, {TALL, 192, 128, 256, 0.57, 0.4}},
+    {{FEW, 128, 32, 512, 1.2, 0}, {MID, 128, 64, 512, 2.1, 0.5}, {}, {}, {}}};
 // What the plan has to know of a product's epilogue: us, and whether its tiles may be TALL
 struct Ends {
   double mid, large;
   bool tall;
 };
-inline Plan plan_product(int64_t M, int64_t N, int64_t steps, Ends ends, bool triple = false, int max_slices = 1, double sum_us = 0) {
+inline Plan plan_product(int64_t M, int64_t N, int64_t steps, Ends ends, Form form = SINGLE, int max_slices = 1, double sum_us = 0) {
   Plan best{LARGE, 1, 1e300};
-  for (auto& k : kTiles[triple]) {
+  for (auto& k : kTiles[form]) {
     if (k.id == TALL && !ends.tall) continue;
     if (!k.bm) continue;
     const int64_t tiles = ((M + k.bm - 1) / k.bm) * ((N + k.bn - 1) / k.bn);
@@ -609,12 +619,13 @@ inline Plan plan_product(int64_t M, int64_t N, int64_t steps, Ends ends, bool tr
 
 // Rows of A (of M) to take first: those of whole rounds of LARGE tiles, where the rest is quicker
 // with tiles of its own than as one more round (the losses of 50001 x 2047 x 1000: 6.1 rounds).
-inline int64_t whole_rounds(int64_t M, int64_t N, int64_t steps, Ends ends, bool triple = false) {
-  const int bm = kTiles[triple][2].bm, bn = kTiles[triple][2].bn;
+inline int64_t whole_rounds(int64_t M, int64_t N, int64_t steps, Ends ends, Form form = SINGLE) {
+  const int bm = kTiles[form][2].bm, bn = kTiles[form][2].bn;
+  if (!bm) return M;
   const int64_t tn = (N + bn - 1) / bn, full = (M + bm - 1) / bm * tn / 256, first = full * 256 / tn * bm;
   if (first <= 0 || first >= M) return M;
   const double gap = 3;                                      // from one launch to the next
-  auto us = [&](int64_t m) { return plan_product(m, N, steps, ends, triple).us; };
+  auto us = [&](int64_t m) { return plan_product(m, N, steps, ends, form).us; };
   return us(first) + us(M - first) + gap < us(M) ? first : M;
 }
 

@@ -30,7 +30,8 @@
 // is the sum of three bf16 (8 + 8 + 8 bits, nearest), and the six leading of the
 // nine products are summed in 32 bits; what is left out is below 2^-24 of a
 // product.  That is six bf16 products (220 TFLOP/s of fp32 in the loop) where the
-// fp32 matrix instructions end at 157.
+// fp32 matrix instructions end at 157.  Of up to 192 tokens, where reading the vocabulary
+// counts for more, those instructions take the numbers as they are.
 #include "mm_core.h"
 #include <math.h>
 
@@ -45,7 +46,8 @@ constexpr float kF16Lift = 16384.f;
 template <int KIND, int P>
 using Large = std::conditional_t<P == 3, Cfg<KIND, 256, 128, 4, 2, 64, 2, 1, 3>, Cfg<KIND, 256, 256, 2, 4, 128, 2>>;
 template <int KIND, int P>
-using Mid = std::conditional_t<P == 3, Cfg<KIND, 128, 64, 2, 2, 64, 2, 1, 3>, Cfg<KIND, 128, 128, 2, 2, 128, 2>>;
+using Mid = std::conditional_t<P == 3, Cfg<KIND, 128, 64, 2, 2, 64, 2, 1, 3>,
+                               std::conditional_t<KIND == F32, Cfg<KIND, 128, 64, 4, 1, 128, 2>, Cfg<KIND, 128, 128, 2, 2, 128, 2>>>;
 template <int KIND>
 using Square = Cfg<KIND, 128, 128, 4, 2, 64, 2, 1, 3>;       // of three planes only, as
 template <int KIND>
@@ -250,6 +252,22 @@ struct DlogitsEpi {
             for (int j = 0; j < C::TN; ++j) t.acc[i][j][k] = 0.f;
           }
     }
+    if constexpr (KIND == F32) {                             // as it is: small beside the vocabulary
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        const int n = t.col(j);
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) {
+          const int m = t.row(i);
+          if (e.dl && n < e.N && m < e.Vp) *reinterpret_cast<f4v*>(reinterpret_cast<float*>(e.dl) + n * e.ldl + m) = t.acc[i][j];
+          if (e.dlt && n < e.Np) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (m + k < e.V) reinterpret_cast<float*>(e.dlt)[(m + k) * e.ldt + n] = t.acc[i][j][k];
+          }
+        }
+      }
+    } else {
 #pragma unroll
     for (int p = 0; p < PLANES; ++p) {
       __syncthreads();                                       // the loop's (or the last plane's) reads are over
@@ -278,6 +296,7 @@ struct DlogitsEpi {
       __builtin_amdgcn_sched_barrier(0);
       if (e.dlt) store_columns<C>(lds, e.dlt + p * e.pt, e.ldt, n0, m0, e.Np, e.V);
       __builtin_amdgcn_sched_barrier(0);
+    }
     }
   }
 };
@@ -829,6 +848,34 @@ __global__ __launch_bounds__(256) void lay_k(const LayJob j0, const LayJob j1, i
   }
 }
 
+// The same of fp32 rows as they are: 64 x 64 to a workgroup.
+__global__ __launch_bounds__(256) void lay32_k(const LayJob j0, const LayJob j1, int blocks0, int D, int64_t ldr, const GradOf g) {
+  __shared__ float tile[64][65];
+  const bool second = (int)blockIdx.x >= blocks0;
+  const LayJob& j = second ? j1 : j0;
+  const int r0 = ((int)blockIdx.x - (second ? blocks0 : 0)) * 64, c0 = blockIdx.y * 64, lane = threadIdx.x % 64, c = c0 + lane;
+  const int Dp = (D + 7) / 8 * 8;
+  float v[16];
+#pragma unroll
+  for (int s = 0; s < 16; ++s) {
+    const int r = r0 + threadIdx.x / 64 + s * 4;
+    v[s] = r < j.R && c < D ? static_cast<const float*>(j.x)[r * j.ld + c] : 0.f;
+  }
+#pragma unroll
+  for (int s = 0; s < 16; ++s) {
+    const int q = threadIdx.x / 64 + s * 4, r = r0 + q;
+    if (j.rows && r < j.R && c < Dp) reinterpret_cast<float*>(j.rows)[r * ldr + c] = v[s];
+    tile[q][lane] = j.masked && r < j.R && !g.live(r) ? 0.f : v[s];
+  }
+  if (!j.cols) return;
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < 16; ++s) {
+    const int q = threadIdx.x / 64 + s * 4;
+    if (c0 + q < D && r0 + lane < j.Rp) reinterpret_cast<float*>(j.cols)[(c0 + q) * j.ldc + r0 + lane] = tile[lane][q];
+  }
+}
+
 // four neighbours in the gradients' type (OUT: BF16, F16, or 3: fp32), those below cols; one store, which
 // needs no alignment
 template <int OUT>
@@ -1266,7 +1313,10 @@ struct Shape {
   int64_t N, V, D;
   int dtype;
   bool direct_h, direct_w;      // the caller's rows serve as they are
-  int planes() const { return dtype == PO_F32 ? 3 : 1; }
+  Form form;                    // of the products
+  int planes() const { return form == TRIPLE ? 3 : 1; }
+  int es() const { return form == WHOLE ? 4 : 2; }            // bytes of an operand's element
+  int halves() const { return planes() * es() / 2; }          // 16-bit places of a number
   int Dp() const { return (int)((D + 7) / 8 * 8); }     // columns of rows laid out here, zeros past D
   int64_t ldp() const { return padded(Dp()); }
   int64_t Np() const { return (N + 31) / 32 * 32; }
@@ -1302,7 +1352,7 @@ inline int few_columns(int64_t D) { return D <= 256 ? 1 : D <= 512 ? 2 : D <= 10
 inline bool few_rows(const Shape& s) { return s.N <= (s.dtype == PO_F32 ? kFewRowsF32 : kFewRows) && s.D <= kFewDim; }
 // forward: 16-bit rows that serve as they are go through the matrix cores at the same rate (32768 x 1024
 // bf16 13 us)
-inline bool few_rows_forward(const Shape& s) { return few_rows(s) && !s.direct_w; }
+inline bool few_rows_forward(const Shape& s) { return few_rows(s) && (s.dtype == PO_F32 || !s.direct_w); }
 inline int few_batches(const Shape& s, bool backward) { return (int)ceil_div(s.V, few_batch((int)s.N, backward)); }
 inline int few_blocks(const Shape& s, bool backward) {
   return std::min(kFewBlocks, (int)ceil_div(few_batches(s, backward), 8 / few_columns(s.D)));
@@ -1329,7 +1379,7 @@ struct FwdWs {
       bytes = l.at;
       return;
     }
-    const int64_t wrow = s.direct_w ? 0 : s.ldp() * 2 * s.planes();
+    const int64_t wrow = s.direct_w ? 0 : s.ldp() * 2 * s.halves();
     piece = wrow ? piece_rows(s.V, wrow) : s.V;
     parts = 0;
     for (int64_t v = 0; v < s.V; v += piece) parts += ceil_div(std::min(piece, s.V - v), 128);
@@ -1337,7 +1387,7 @@ struct FwdWs {
     tlogit = l.take<float>(s.N);
     sums = l.take<double>(2 * s.N);
     arrived = l.take<uint32_t>(1);
-    hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.ldp() * s.planes());
+    hp = l.take<uint16_t>(s.direct_h ? 0 : s.N * s.ldp() * s.halves());
     wp = l.take<uint16_t>(piece * wrow / 2);
     bytes = l.at;
   }
@@ -1362,7 +1412,7 @@ struct BwdWs {
       bytes = l.at;
       return;
     }
-    const int P = s.planes();
+    const int P = s.halves();
     const int64_t per = (s.direct_w ? 0 : s.ldp() * 2 * P) + (dh ? (s.N + s.D) * 2 * P : 0) + (dw ? s.Np() * 2 * P : 0);
     piece = piece_rows(s.V, per);
     ldl = padded(piece);
@@ -1377,8 +1427,8 @@ struct BwdWs {
     slab_ld = (s.D + 3) / 4 * 4;
     slab_slice = s.N * slab_ld;
     // a slice's sums are written and read once: 8 bytes of each at about 4 TB/s
-    dh_plan = plan_product(s.D, s.N, (int64_t)ceil_div(ldl * 2, 128) * (P == 3 ? 6 : 1),
-                           SlabEpi::kEnds, P == 3, kSlabSlices, slab_slice * 8 / 4e6);
+    dh_plan = plan_product(s.D, s.N, (int64_t)ceil_div(ldl * s.es(), 128) * (s.form == TRIPLE ? 6 : 1),
+                           SlabEpi::kEnds, s.form, kSlabSlices, slab_slice * 8 / 4e6);
     direct_dh = piece >= s.V && dh_plan.slices == 1;
     slab = l.take<float>(dh && !direct_dh ? dh_plan.slices * slab_slice : 0);
     bytes = l.at;
@@ -1417,7 +1467,7 @@ struct FrozenWs {
     kept = l.take<uint16_t>(s.N * ldk * P);
     slab_ld = (s.D + 3) / 4 * 4;
     slab_slice = s.N * slab_ld;
-    plan = plan_product(s.D, s.N, (int64_t)ceil_div(ldk * 2, 128) * (P == 3 ? 6 : 1), RefSlabEpi::kEnds, P == 3, kSlabSlices,
+    plan = plan_product(s.D, s.N, (int64_t)ceil_div(ldk * 2, 128) * (P == 3 ? 6 : 1), RefSlabEpi::kEnds, s.form, kSlabSlices,
                         slab_slice * 8 / 4e6);
     slab_refs = l.take<float>(2 * plan.slices * ldr);
     slab = l.take<float>(plan.slices > 1 ? plan.slices * slab_slice : 0);       // one: the gradient's own place
@@ -1433,8 +1483,8 @@ struct Side {
   uint16_t* buf;
 };
 inline Operand rows_of(const Shape& s, const Side& m, int64_t r0, int64_t rows) {
-  if (m.direct) return Operand{static_cast<const char*>(m.x) + r0 * m.ld * 2, m.ld * 2, 0, (int)rows};
-  return Operand{reinterpret_cast<char*>(m.buf), s.ldp() * 2, rows * s.ldp() * 2, (int)rows};
+  if (m.direct) return Operand{static_cast<const char*>(m.x) + r0 * m.ld * s.es(), m.ld * s.es(), 0, (int)rows};
+  return Operand{reinterpret_cast<char*>(m.buf), s.ldp() * s.es(), rows * s.ldp() * 2, (int)rows};
 }
 // lays them out there, h's rows (0: not this time) and w's in one launch
 inline void pack(const Shape& s, const Side& h, int64_t hrows, const Side& w, int64_t w0, int64_t wrows, hipStream_t st) {
@@ -1463,12 +1513,20 @@ inline void lay(const Shape& s, const LayJob& a, const LayJob& b, const GradOf& 
   auto blocks = [](const LayJob& j) { return j.rows || j.cols ? ceil_div(j.cols ? j.Rp : j.R, 64) : 0; };
   const int b0 = blocks(a), b1 = blocks(b);
   if (!(b0 + b1)) return;
-  hipLaunchKernelGGL((s.dtype == PO_F32 ? lay_k<float> : lay_k<uint16_t>), dim3(b0 + b1, ceil_div(s.D, 256)), dim3(256), 0, st, a, b, b0,
-                     (int)s.D, s.ldp(), g);
+  const bool whole = s.form == WHOLE;
+  hipLaunchKernelGGL((whole ? lay32_k : s.dtype == PO_F32 ? lay_k<float> : lay_k<uint16_t>), dim3(b0 + b1, ceil_div(s.D, whole ? 64 : 256)),
+                     dim3(256), 0, st, a, b, b0, (int)s.D, s.ldp(), g);
 }
 
-inline bool serves(const void* x, int64_t ld, int dtype, int64_t D) {
-  return dtype != PO_F32 && D % 8 == 0 && ld % 8 == 0 && (uintptr_t)x % 16 == 0;
+// fp32 of few tokens goes through the fp32 matrix instructions: at less than half the planes' rate, but without
+// making planes, which is 10 bytes a number and 6 at each reading for 4 (trained, of 30000 x 1024: 40 tokens
+// 406 -> 229 us, 100 506 -> 346, 192 574 -> 485; 256 610 against 582, and 106 both ways of 8000 x 300)
+constexpr int kWholeRows = 192;
+inline Shape shape_of(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V, int64_t D, bool frozen) {
+  const Form form = dtype != PO_F32 ? SINGLE : N <= kWholeRows && !frozen ? WHOLE : TRIPLE;
+  const int chunk = 16 / (dtype == PO_F32 ? 4 : 2);
+  auto serves = [&](const void* x, int64_t ld) { return form != TRIPLE && D % 8 == 0 && ld % chunk == 0 && (uintptr_t)x % 16 == 0; };
+  return Shape{N, V, D, dtype, serves(h, ldh), serves(w, ldw), form};
 }
 
 inline int check_shape(const char* what, int64_t N, int64_t V, int64_t D, int dtype, int64_t ldh, int64_t ldw) {
@@ -1486,18 +1544,19 @@ inline int launch_planned(const Args& a, const typename Epi::Args& e, Plan p, hi
     if (p.tile == SQUARE) return launch_product<Square<KIND>, Epi>(a, e, p.slices, s, what);
   if constexpr (P == 3 && Epi::kEnds.tall)
     if (p.tile == TALL) return launch_product<Tall<KIND>, Epi>(a, e, p.slices, s, what);
-  if (p.tile == MID) return launch_product<Mid<KIND, P>, Epi>(a, e, p.slices, s, what);
-  return launch_product<Large<KIND, P>, Epi>(a, e, p.slices, s, what);
+  if constexpr (KIND != F32)
+    if (p.tile == LARGE) return launch_product<Large<KIND, P>, Epi>(a, e, p.slices, s, what);
+  return launch_product<Mid<KIND, P>, Epi>(a, e, p.slices, s, what);
 }
 
 template <class Epi>
-inline Plan plan_of(const Args& a, int planes) {
-  return plan_product(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * (planes == 3 ? 6 : 1), Epi::kEnds, planes == 3);
+inline Plan plan_of(const Args& a, Form form) {
+  return plan_product(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * (form == TRIPLE ? 6 : 1), Epi::kEnds, form);
 }
 
 template <class Epi>
-inline int64_t first_part(const Args& a, int planes) {
-  return whole_rounds(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * (planes == 3 ? 6 : 1), Epi::kEnds, planes == 3);
+inline int64_t first_part(const Args& a, Form form) {
+  return whole_rounds(a.A.rows, a.B.rows, (int64_t)ceil_div(a.kbytes, 128) * (form == TRIPLE ? 6 : 1), Epi::kEnds, form);
 }
 
 inline void row_stats(const float2* partial, int parts, const Shape& s, const float* tlogit, const int64_t* target, int64_t ignore,
@@ -1539,7 +1598,7 @@ inline void few_dispatch(int dtype, int nb, Fn fn) {
 extern "C" int po_linear_ce_workspace(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N,
                                       int64_t V, int64_t D, int dh, int dw, int64_t* fwd_bytes, int64_t* bwd_bytes) {
   PO_TRY(check_shape("po_linear_ce_workspace", N, V, D, dtype, ldh, ldw));
-  const Shape s{N, V, D, dtype, serves(h, ldh, dtype, D), serves(w, ldw, dtype, D)};
+  const Shape s = shape_of(h, ldh, w, ldw, dtype, N, V, D, false);
   if (fwd_bytes) *fwd_bytes = FwdWs(s, nullptr).bytes;
   if (bwd_bytes) *bwd_bytes = BwdWs(s, dh != 0, dw != 0, nullptr).bytes;
   return PO_OK;
@@ -1553,7 +1612,7 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
   PO_REQUIRE(h && w && target && workspace && stat && loss && (reduction == 0 || count), "po_linear_ce_fwd: null pointer");
   PO_REQUIRE(reduction >= 0 && reduction <= 2, "po_linear_ce_fwd: unknown reduction %d", reduction);
   PO_REQUIRE(scale > 0.f && scale < INFINITY, "po_linear_ce_fwd: the scale must be positive and finite");
-  const Shape s{N, V, D, dtype, serves(h, ldh, dtype, D), serves(w, ldw, dtype, D)};
+  const Shape s = shape_of(h, ldh, w, ldw, dtype, N, V, D, false);
   const FwdWs ws(s, workspace);
   PO_REQUIRE(workspace_bytes >= ws.bytes, "po_linear_ce_fwd: workspace of %lld bytes, %lld needed",
              (long long)workspace_bytes, (long long)ws.bytes);
@@ -1569,24 +1628,31 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
     return po::check_launch("po_linear_ce_fwd");
   }
   Args a{};
-  a.kbytes = s.Dp() * 2;
+  a.kbytes = s.Dp() * s.es();
   const Side hs{h, ldh, s.direct_h, ws.hp}, wside{w, ldw, s.direct_w, ws.wp};
   a.B = rows_of(s, hs, 0, N);
   StatsEpi::Args e{ws.partial, ws.arrived, ws.tlogit, target, 0, 0, (int)N, 0, scale * kLog2e};
   for (int64_t v = 0; v < V; v += ws.piece) {
     const int64_t rows = std::min(ws.piece, V - v);
-    pack(s, hs, v ? 0 : N, wside, v, rows, st);
+    if (s.form == WHOLE) {
+      LayJob hj{};
+      if (!v) hj = lay_job(s, hs, 0, N, N, 0, nullptr, 0);
+      lay(s, lay_job(s, wside, v, rows, rows, 0, nullptr, 0), hj, GradOf{}, st);
+    } else {
+      pack(s, hs, v ? 0 : N, wside, v, rows, st);
+    }
     const Operand W = rows_of(s, wside, v, rows);
     for (int64_t r = 0, part; r < rows; r += part) {
       a.A = W.from(r);
-      part = first_part<StatsEpi>(a, s.planes());
+      part = first_part<StatsEpi>(a, s.form);
       a.A.rows = (int)part;
       e.v0 = v + r;
       e.V = (int)part;
-      const Plan p = plan_of<StatsEpi>(a, s.planes());
+      const Plan p = plan_of<StatsEpi>(a, s.form);
       PO_TRY((dtype == PO_F16    ? launch_planned<F16, 1, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
                : dtype == PO_BF16 ? launch_planned<BF16, 1, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
-                                  : launch_planned<BF16, 3, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")));
+               : s.form == TRIPLE ? launch_planned<BF16, 3, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")
+                                  : launch_planned<F32, 1, StatsEpi>(a, e, p, st, "po_linear_ce_fwd")));
       e.tile0 += ceil_div(part, p.tile == LARGE ? 256 : 128);
     }
   }
@@ -1600,7 +1666,7 @@ namespace {
 template <int KIND, int OUT>
 int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, const GradOf& g, float scale,
              const float2* stat, void* dh, int64_t lddh, void* dw, int64_t lddw, hipStream_t st) {
-  constexpr int P = OUT == 3 ? 3 : 1, es = OUT == 3 ? 4 : 2;
+  constexpr int P = OUT == 3 && KIND != F32 ? 3 : 1, es = OUT == 3 ? 4 : 2, ES = KIND == F32 ? 4 : 2;   // bytes outside and of the operands
   const char* what = "po_linear_ce_bwd";
   const int N = (int)s.N, D = (int)s.D;
   const Operand H = rows_of(s, h, 0, N);
@@ -1615,21 +1681,21 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
     Args a{};
     // dl of the piece
     a.B = H;
-    a.kbytes = s.Dp() * 2;
+    a.kbytes = s.Dp() * ES;
     for (int64_t r = 0, part; r < rows; r += part) {
       using E = DlogitsEpi<KIND, P>;
       a.A = W.from(r);
-      part = first_part<E>(a, P);
+      part = first_part<E>(a, s.form);
       a.A.rows = (int)part;
       const typename E::Args e{stat, g, v + r, N, (int)s.Np(), (int)part, (int)(r + part < rows ? part : rp - r), scale * kLog2e,
-                               dh ? ws.dl + r : nullptr, dw ? ws.dlt + r * s.ldn() : nullptr, ws.ldl, s.ldn(), N * ws.ldl,
+                               dh ? ws.dl + r * (ES / 2) : nullptr, dw ? ws.dlt + r * s.ldn() * (ES / 2) : nullptr, ws.ldl, s.ldn(), N * ws.ldl,
                                ws.piece * s.ldn()};
-      PO_TRY((launch_planned<KIND, P, E>(a, e, plan_of<E>(a, P), st, what)));
+      PO_TRY((launch_planned<KIND, P, E>(a, e, plan_of<E>(a, s.form), st, what)));
     }
     if (dh) {                                                // sums over v of dl[n][v] w[v][d]
-      a.A = Operand{reinterpret_cast<char*>(ws.wt), ws.ldl * 2, D * ws.ldl * 2, D};
-      a.B = Operand{reinterpret_cast<char*>(ws.dl), ws.ldl * 2, N * ws.ldl * 2, N};
-      a.kbytes = rp * 2;
+      a.A = Operand{reinterpret_cast<char*>(ws.wt), ws.ldl * ES, D * ws.ldl * 2, D};
+      a.B = Operand{reinterpret_cast<char*>(ws.dl), ws.ldl * ES, N * ws.ldl * 2, N};
+      a.kbytes = rp * ES;
       // the last piece may have fewer steps than slices: the other slabs keep their sums
       const Plan p{ws.dh_plan.tile, std::min(ws.dh_plan.slices, ceil_div(a.kbytes, P == 3 ? 64 : 128)), 0};
       if (ws.direct_dh) {
@@ -1641,12 +1707,12 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
       }
     }
     if (dw) {                                                // dw[v][d] = sum_n dl[n][v] h[n][d]
-      a.A = Operand{reinterpret_cast<char*>(ws.ht), s.ldn() * 2, D * s.ldn() * 2, D};
-      a.B = Operand{reinterpret_cast<char*>(ws.dlt), s.ldn() * 2, ws.piece * s.ldn() * 2, rows};
-      a.kbytes = (int)s.Np() * 2;
+      a.A = Operand{reinterpret_cast<char*>(ws.ht), s.ldn() * ES, D * s.ldn() * 2, D};
+      a.B = Operand{reinterpret_cast<char*>(ws.dlt), s.ldn() * ES, ws.piece * s.ldn() * 2, rows};
+      a.kbytes = (int)s.Np() * ES;
       char* out = static_cast<char*>(dw) + v * lddw * es;
       const typename GradEpi<OUT>::Args ge{out, lddw, g, rows, D};
-      PO_TRY((launch_planned<KIND, P, GradEpi<OUT>>(a, ge, plan_of<GradEpi<OUT>>(a, P), st, what)));
+      PO_TRY((launch_planned<KIND, P, GradEpi<OUT>>(a, ge, plan_of<GradEpi<OUT>>(a, s.form), st, what)));
     }
   }
   if (dh && !ws.direct_dh) {
@@ -1670,7 +1736,7 @@ extern "C" int po_linear_ce_bwd(const void* h, int64_t ldh, const void* w, int64
   PO_REQUIRE(scale > 0.f && scale < INFINITY, "po_linear_ce_bwd: the scale must be positive and finite");
   PO_REQUIRE((!dh || lddh >= D) && (!dw || lddw >= D), "po_linear_ce_bwd: bad row strides");
   if (!dh && !dw) return PO_OK;
-  const Shape s{N, V, D, dtype, serves(h, ldh, dtype, D), serves(w, ldw, dtype, D)};
+  const Shape s = shape_of(h, ldh, w, ldw, dtype, N, V, D, false);
   const BwdWs ws(s, dh != nullptr, dw != nullptr, workspace);
   PO_REQUIRE(workspace_bytes >= ws.bytes, "po_linear_ce_bwd: workspace of %lld bytes, %lld needed",
              (long long)workspace_bytes, (long long)ws.bytes);
@@ -1696,6 +1762,7 @@ extern "C" int po_linear_ce_bwd(const void* h, int64_t ldh, const void* w, int64
   const Side hs{h, ldh, s.direct_h, ws.hp}, wside{w, ldw, s.direct_w, ws.wp};
   if (dtype == PO_F16) return backward<F16, F16>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
   if (dtype == PO_BF16) return backward<BF16, BF16>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
+  if (s.form == WHOLE) return backward<F32, 3>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
   return backward<BF16, 3>(s, ws, hs, wside, g, scale, st2, dh, lddh, dw, lddw, st);
 }
 
@@ -1720,11 +1787,11 @@ int frozen_forward(const Shape& s, const FrozenWs& ws, const Side& h, const Side
     for (int64_t r = 0, part; r < rows; r += part) {
       using E = KeepEpi<KIND, P>;
       a.A = W.from(r);
-      part = first_part<E>(a, P);
+      part = first_part<E>(a, s.form);
       a.A.rows = (int)part;
       e.v0 = v + r;
       e.V = (int)part;
-      const Plan p = plan_of<E>(a, P);
+      const Plan p = plan_of<E>(a, s.form);
       const typename E::Args ke{e, base, ws.refs + r / 128 * ws.ldr, ws.other + r / 128 * ws.ldo, ws.ldr, ws.ldo,
                                 (int)(r + part < rows ? part : rp - r), ws.kept + r, ws.ldk, N * ws.ldk};
       PO_TRY((launch_planned<KIND, P, E>(a, ke, p, st, what)));
@@ -1750,7 +1817,7 @@ extern "C" int po_linear_ce_frozen_workspace(const void* h, int64_t ldh, const v
                                              int64_t V, int64_t D, int64_t* bytes) {
   PO_TRY(check_shape("po_linear_ce_frozen_workspace", N, V, D, dtype, ldh, ldw));
   PO_REQUIRE(bytes, "po_linear_ce_frozen_workspace: null pointer");
-  *bytes = FrozenWs(Shape{N, V, D, dtype, serves(h, ldh, dtype, D), serves(w, ldw, dtype, D)}, nullptr).bytes;
+  *bytes = FrozenWs(shape_of(h, ldh, w, ldw, dtype, N, V, D, true), nullptr).bytes;
   return PO_OK;
 }
 
@@ -1763,7 +1830,7 @@ extern "C" int po_linear_ce_frozen_fwd(const void* h, int64_t ldh, const void* w
   PO_REQUIRE((uintptr_t)dhu % 16 == 0, "po_linear_ce_frozen_fwd: dhu must start on 16 bytes");
   PO_REQUIRE(reduction >= 0 && reduction <= 2, "po_linear_ce_frozen_fwd: unknown reduction %d", reduction);
   PO_REQUIRE(scale > 0.f && scale < INFINITY, "po_linear_ce_frozen_fwd: the scale must be positive and finite");
-  const Shape s{N, V, D, dtype, serves(h, ldh, dtype, D), serves(w, ldw, dtype, D)};
+  const Shape s = shape_of(h, ldh, w, ldw, dtype, N, V, D, true);
   const FrozenWs ws(s, workspace);
   PO_REQUIRE(workspace_bytes >= ws.bytes, "po_linear_ce_frozen_fwd: workspace of %lld bytes, %lld needed",
              (long long)workspace_bytes, (long long)ws.bytes);

@@ -97,6 +97,29 @@ def test_losses_and_gradients(N, V, D, dtype):
     assert not h.grad[t == IGN].any()
 
 
+@pytest.mark.parametrize("N,V,D", [(17, 300, 2056), (20, 5001, 2100), (24, 150001, 1032), (40, 3001, 1123), (65, 2000, 264), (128, 777, 96), (129, 4000, 3001),
+                                   (192, 2049, 640), (193, 2049, 640), (192, 33, 8)])
+@pytest.mark.parametrize("frozen", ["", "hidden", "weight"])
+def test_fp32_of_few_tokens(N, V, D, frozen):
+    """The fp32 matrix instructions, rows that serve as they are and others, more than one piece, and the next size."""
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w, t = inputs(N, V, D, torch.float32)
+    t[1] = IGN
+    h[1] = float("nan")
+    t[N - 1] = V - 1
+    h.requires_grad_(frozen != "hidden")
+    w.requires_grad_(frozen != "weight")
+    g = 0.5 + torch.arange(N, device=DEV) % 7 / 7
+    loss = lce(h, w, t, reduction="none")
+    leaves = [x for x in (h, w) if x.requires_grad]
+    grads = torch.autograd.grad(loss, leaves, g)
+    ref = reference(h.detach(), w.detach(), t, g)
+    b = bounds(ref, torch.float32, N, V, D)
+    within(loss.detach(), ref["loss"], b["loss"], "loss")
+    for x, got in zip(leaves, grads):
+        within(got, ref["dh" if x is h else "dw"], b["dh" if x is h else "dw"], "gradient")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N,V,D", [(1100, 9001, 513), (2050, 16001, 385), (700, 33001, 520), (300, 20000, 1030)])
 def test_large_tiles(N, V, D, dtype):
