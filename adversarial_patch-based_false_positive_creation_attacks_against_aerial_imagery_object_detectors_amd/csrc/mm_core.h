@@ -1,6 +1,7 @@
 // The matrix-product core of the large-vocabulary head (vocab_loss.hip,
-// int8_linear.hip): C[m][n] = sum_k A[m][k] * B[n][k], both operands with k
-// contiguous, 16-bit floats or 8-bit integers, sums in 32 bits.
+// int8_ops.hip): C[m][n] = sum_k A[m][k] * B[n][k], both operands with k
+// contiguous, 16-bit floats, 8-bit integers or fp32 (as it is, or as three planes of
+// bf16: product3), sums in 32 bits.
 //
 // One form only.  LDS reads with a transpose (ds_read_b64_tr_b16) run at 64 B
 // per clock and CU against 128 B for plain 16-byte reads (measured 41 against
@@ -10,7 +11,7 @@
 // them), and every product runs this loop.
 //
 // A workgroup owns a BM x BN tile, its waves WM x WN rectangles of 16 x 16 MFMA
-// blocks (v_mfma 16x16x32 of 16-bit floats, 16x16x64 of bytes).  k advances in steps
+// blocks (v_mfma 16x16x32 of 16-bit floats, 16x16x64 of bytes, 16x16x4 of fp32).  k advances in steps
 // of KB bytes per row; STAGES LDS buffers are filled ahead by 16-byte LDS-DMA.  Rows
 // are KB bytes, their 16-byte chunks XOR-swizzled by row (by the address each lane
 // loads from: the DMA writes LDS linearly), so 8 neighbouring lanes' fragment reads

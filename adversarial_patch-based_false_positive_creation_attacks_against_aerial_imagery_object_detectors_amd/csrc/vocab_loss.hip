@@ -18,7 +18,7 @@
 // exp(l) w - ...) / sum_n needs the exponentials up to a factor of the row.  So a piece's are
 // stored in 16 bits, as multiples of powers of two, and multiplied with its rows at once
 // (KeepEpi, RefSlabEpi); what is left to the backward pass is a scaling.  Two products instead of
-// three: bf16 4096 x 32768 x 1024 784 -> 592 us, 8192 x 100000 x 2048 8.2 -> 5.7 ms,
+// three: bf16 4096 x 32768 x 1024 784 -> 570 us, 8192 x 100000 x 2048 8.2 -> 5.7 ms,
 // fp32 4096 x 32768 x 1024 3.84 -> 2.80.  With dw this gains nothing: dw's terms need
 // the rows' whole sums first.
 //
@@ -42,18 +42,20 @@ using po::ceil_div;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kF16Lift = 16384.f;
 
-// plan_product's tiles, of one plane and of three
+// plan_product's tiles, of one plane (P = 1) and of three
 template <int KIND, int P>
 using Large = std::conditional_t<P == 3, Cfg<KIND, 256, 128, 4, 2, 64, 2, 1, 3>, Cfg<KIND, 256, 256, 2, 4, 128, 2>>;
 template <int KIND, int P>
 using Mid = std::conditional_t<P == 3, Cfg<KIND, 128, 64, 2, 2, 64, 2, 1, 3>,
                                std::conditional_t<KIND == F32, Cfg<KIND, 128, 64, 4, 1, 128, 2>, Cfg<KIND, 128, 128, 2, 2, 128, 2>>>;
-template <int KIND>
-using Square = Cfg<KIND, 128, 128, 4, 2, 64, 2, 1, 3>;       // of three planes only, as
-template <int KIND>
-using Tall = Cfg<KIND, 192, 128, 4, 2, 64, 2, 1, 3>;
 template <int KIND, int P>
 using Few = std::conditional_t<P == 3, Cfg<KIND, 128, 32, 4, 1, 64, 2, 1, 3>, Cfg<KIND, 128, 32, 4, 1, 128, 3>>;
+// of three only
+template <int KIND>
+using Square = Cfg<KIND, 128, 128, 4, 2, 64, 2, 1, 3>;
+template <int KIND>
+using Tall = Cfg<KIND, 192, 128, 4, 2, 64, 2, 1, 3>;
+
 // over the four lanes that hold a column
 __device__ __forceinline__ float column_max(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
