@@ -257,7 +257,7 @@ Tensor keyed_dropout(const py::object& x_, double p, const py::object& seed_, co
 constexpr int64_t kMostStride = 1 << 21;
 
 struct CeForward {
-  Tensor loss, target, stat;                                  // stat: [N][2] statistics, then the count
+  Tensor loss, target, stat;                                  // stat: [3 N] statistics, then the count
   Tensor dhu;                                                 // frozen: the embeddings' gradient, [N][D up to a multiple of 4]
 };
 
@@ -269,7 +269,7 @@ CeForward ce_forward(const Tensor& hidden, const Tensor& weight, const Tensor& t
   CeForward r;
   r.target = target.reshape({-1}).contiguous();
   r.loss = reduction == 0 ? at::empty(target.sizes(), f32) : at::empty({}, f32);
-  r.stat = at::empty({frozen ? 1 : 2 * h.rows + 1}, f32);
+  r.stat = at::empty({frozen ? 1 : 3 * h.rows + 1}, f32);
   if (frozen) r.dhu = at::empty({h.rows, (h.cols + 3) / 4 * 4}, f32);
   if (h.rows == 0) {
     if (reduction) r.loss.fill_(reduction == 2 ? std::numeric_limits<double>::quiet_NaN() : 0.0);
@@ -293,7 +293,7 @@ CeForward ce_forward(const Tensor& hidden, const Tensor& weight, const Tensor& t
   float* stat = r.stat.data_ptr<float>();
   check(lib.ce_fwd(h.t.data_ptr(), h.ld, w.t.data_ptr(), w.ld, dt, h.rows, w.rows, h.cols, r.target.const_data_ptr<int64_t>(),
                    ignore, (float)scale, (int)reduction, ws.data_ptr(), bytes, stat, r.loss.data_ptr<float>(),
-                   stat + 2 * h.rows, on.stream),
+                   stat + 3 * h.rows, on.stream),
         "po_linear_ce_fwd");
   return r;
 }
@@ -369,7 +369,7 @@ struct LinearCe : torch::autograd::Function<LinearCe> {
     const Tensor ws = at::empty({bytes}, contiguous.dtype(at::kByte));
     float* st = stat.data_ptr<float>();
     check(lib.ce_bwd(h.t.data_ptr(), h.ld, w.t.data_ptr(), w.ld, dt, h.rows, w.rows, h.cols, target.const_data_ptr<int64_t>(),
-                     ignore, (float)scale, (int)reduction, st, st + 2 * h.rows, g.const_data_ptr<float>(), ws.data_ptr(),
+                     ignore, (float)scale, (int)reduction, st, st + 3 * h.rows, g.const_data_ptr<float>(), ws.data_ptr(),
                      bytes, dh ? dh->data_ptr() : nullptr, h.cols, dw ? dw->data_ptr() : nullptr, h.cols, on.stream),
           "po_linear_ce_bwd");
   }

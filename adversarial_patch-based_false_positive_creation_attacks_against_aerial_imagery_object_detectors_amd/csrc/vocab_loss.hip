@@ -617,7 +617,7 @@ __device__ __forceinline__ double wave_sum(double x) {
 template <int R>
 __global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ partial, int parts, int N, int64_t V,
                                                    const float* __restrict__ tlogit, const int64_t* __restrict__ target,
-                                                   int64_t ignore, float k, float2* __restrict__ stat,
+                                                   int64_t ignore, float k, float lift, float2* __restrict__ stat, float* __restrict__ rest,
                                                    float* __restrict__ loss, double* sums, uint32_t* arrived, int mean,
                                                    float* __restrict__ total, float* __restrict__ count) {
   __shared__ float2 red[256];
@@ -654,14 +654,24 @@ __global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ pa
   float l = 0.f;
   bool counts = false;
   if (threadIdx.x < R && n < N) {
-    const float2 r = red[threadIdx.x];
+    float2 r = red[threadIdx.x];
     const int64_t t = target[n];
     counts = t != ignore;
+    // the target's exponent, rounded as it was in its exponential (lift: KeepEpi's): with p next to 1 that rounding
+    // would be all of the loss
+    float mine = __builtin_fmaf(tlogit[n], k, lift - r.x) - lift;
+    if (r.y < 0.5f && r.y > 0.f) {                           // a multiple of a power of two far above the row: nearer to the sum
+      const int e = __builtin_amdgcn_frexp_expf(r.y);
+      r = make_float2(r.x + e, __builtin_amdgcn_ldexpf(r.y, -e));
+      mine -= e;
+    }
     stat[n] = make_float2(r.x, 1.f / r.y);
+    // 1 - p of the target, from the logit that is in the sum
+    rest[n] = counts && t >= 0 && t < V ? 1.f - __builtin_amdgcn_exp2f(mine) * (1.f / r.y) : 0.f;
     // log(sum) - (l_t - max): the maximum leaves before anything is rounded to its size
     l = !counts ? 0.f
         : t < 0 || t >= V ? __uint_as_float(0x7fc00000u)
-                          : kLn2 * (__builtin_log2f(r.y) - __builtin_fmaf(tlogit[n], k, -r.x));
+                          : kLn2 * (__builtin_log2f(r.y) - mine);
     if (loss) loss[n] = l;
   }
   if (!total || threadIdx.x >= 64) return;
@@ -965,8 +975,8 @@ template <typename T, bool HALF>
 __global__ __launch_bounds__(256) void frozen_dh_k(const float* __restrict__ slab, int slices, int last_slices, int64_t slice,
                                                    int64_t ld, int N, int M, const float* __restrict__ refs,
                                                    const float* __restrict__ refs_before, int64_t ldr, float lift,
-                                                   const float2* __restrict__ stat, const float* __restrict__ tlogit,
-                                                   const int64_t* __restrict__ target, int64_t ignore, int64_t V, float k, float c,
+                                                   const float2* __restrict__ stat, const float* __restrict__ rests,
+                                                   const int64_t* __restrict__ target, int64_t ignore, int64_t V, float c,
                                                    const T* __restrict__ w, int64_t ldw, float* dhu) {
   const int per = (int)(ld / 4);
   const int64_t total = (int64_t)N * per;
@@ -986,7 +996,7 @@ __global__ __launch_bounds__(256) void frozen_dh_k(const float* __restrict__ sla
         v += *reinterpret_cast<const f4v*>(p + s * slice) * f;
       }
       const bool in = t >= 0 && t < V;
-      const float rest = in ? 1.f - __builtin_amdgcn_exp2f(__builtin_fmaf(tlogit[n], k, -st.x)) * st.y : __uint_as_float(0x7fc00000u);
+      const float rest = in ? rests[n] : __uint_as_float(0x7fc00000u);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float x = 0.f;
@@ -1205,7 +1215,7 @@ __global__ __launch_bounds__(512, NB > 4 ? 2 : 4) void few_rows_fwd_k(const FewA
 
 // slab[block][n][ld] (if any): this block's part of dh over c and the upstream gradients' factor; dw (if any)
 template <int DT, int NB>
-__global__ __launch_bounds__(512, NB > 2 ? 2 : 4) void few_rows_bwd_k(const FewArgs a, const float2* __restrict__ stat, const GradOf g,
+__global__ __launch_bounds__(512, NB > 2 ? 2 : 4) void few_rows_bwd_k(const FewArgs a, const float2* __restrict__ stat, const float* __restrict__ rest, const GradOf g,
                                                                       float* __restrict__ slab, int ld, void* __restrict__ dw,
                                                                       int64_t lddw) {
   __shared__ float red[2][8][64];
@@ -1218,6 +1228,8 @@ __global__ __launch_bounds__(512, NB > 2 ? 2 : 4) void few_rows_bwd_k(const FewA
   const int64_t t = in ? a.target[n] : -1;
   const float2 st = in ? stat[n] : make_float2(0.f, 0.f);
   const float ratio = in ? g.of_row(n) : 0.f, ir = ratio * st.y, end = g.end();
+  // the target's part as the forward pass has it: with p next to 1 the logits' roundings here would be all of it
+  const float mine = in ? -rest[n] * ratio : 0.f;
   float dh[NB][4];
 #pragma unroll
   for (int q = 0; q < NB; ++q) {
@@ -1240,7 +1252,7 @@ __global__ __launch_bounds__(512, NB > 2 ? 2 : 4) void few_rows_bwd_k(const FewA
     f.load(batch + f.groups);
     const float x = f.logit(w, red[i & 1]);
     const int64_t v = (int64_t)batch * R + r;
-    float dl = __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.k, -st.x)) * ir - (v == t ? ratio : 0.f);
+    float dl = v == t ? mine : __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.k, -st.x)) * ir;
     if (ratio == 0.f || v >= a.V) dl = 0.f;
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -1441,7 +1453,7 @@ struct FrozenWs {
   float2 *partial, *stat;
   double* sums;
   uint32_t* arrived;
-  float *tlogit, *base, *refs, *slab_refs, *slab;
+  float *tlogit, *rest, *base, *refs, *slab_refs, *slab;
   uint8_t* other;
   uint16_t *hp, *wp, *wt, *kept;
   int64_t piece, ldk, ldr, ldo, slab_ld, slab_slice, bytes;
@@ -1459,6 +1471,7 @@ struct FrozenWs {
     tlogit = l.take<float>(s.N);
     sums = l.take<double>(2 * s.N);
     arrived = l.take<uint32_t>(1);
+    rest = l.take<float>(s.N);
     base = l.take<float>(s.N);
     refs = l.take<float>(ceil_div(piece, 256) * 2 * ldr);
     ldo = ceil_div(s.N, 32);
@@ -1562,12 +1575,12 @@ inline int64_t first_part(const Args& a, Form form) {
 }
 
 inline void row_stats(const float2* partial, int parts, const Shape& s, const float* tlogit, const int64_t* target, int64_t ignore,
-                      float k, float2* stat, double* sums, uint32_t* arrived, int reduction, float* loss, float* count,
+                      float k, float lift, float2* stat, float* rest, double* sums, uint32_t* arrived, int reduction, float* loss, float* count,
                       hipStream_t st) {
   // total: few workgroups, since each counts itself in (1000 of them: 20 us, 63: 6)
   const int N = (int)s.N, R = reduction ? (N <= 64 ? 1 : N <= 512 ? 4 : 16) : N <= 256 ? 1 : N <= 2048 ? 4 : 16;
   hipLaunchKernelGGL((R == 1 ? row_stats_k<1> : R == 4 ? row_stats_k<4> : row_stats_k<16>), dim3(ceil_div(N, R)), dim3(256), 0, st,
-                     partial, parts, N, s.V, tlogit, target, ignore, k, stat, reduction ? nullptr : loss, sums, arrived,
+                     partial, parts, N, s.V, tlogit, target, ignore, k, lift, stat, rest, reduction ? nullptr : loss, sums, arrived,
                      reduction == 2, reduction ? loss : nullptr, count);
 }
 
@@ -1625,7 +1638,7 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
       hipLaunchKernelGGL((few_rows_fwd_k<decltype(dt)::value, decltype(nb)::value>), dim3(ws.parts), dim3(512), 0, st, f, ws.partial,
                          ws.arrived, ws.tlogit);
     });
-    row_stats(ws.partial, ws.parts, s, ws.tlogit, target, ignore_index, f.k, reinterpret_cast<float2*>(stat), ws.sums, ws.arrived,
+    row_stats(ws.partial, ws.parts, s, ws.tlogit, target, ignore_index, f.k, 0.f, reinterpret_cast<float2*>(stat), stat + 2 * N, ws.sums, ws.arrived,
               reduction, loss, count, st);
     return po::check_launch("po_linear_ce_fwd");
   }
@@ -1658,7 +1671,7 @@ extern "C" int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64
       e.tile0 += ceil_div(part, p.tile == LARGE ? 256 : 128);
     }
   }
-  row_stats(ws.partial, e.tile0, s, ws.tlogit, target, ignore_index, e.k, reinterpret_cast<float2*>(stat), ws.sums, ws.arrived,
+  row_stats(ws.partial, e.tile0, s, ws.tlogit, target, ignore_index, e.k, 0.f, reinterpret_cast<float2*>(stat), stat + 2 * N, ws.sums, ws.arrived,
             reduction, loss, count, st);
   return po::check_launch("po_linear_ce_fwd");
 }
@@ -1752,7 +1765,7 @@ extern "C" int po_linear_ce_bwd(const void* h, int64_t ldh, const void* w, int64
     const FewArgs f = few_args(s, h, ldh, w, ldw, target, ignore_index, scale, true);
     const int blocks = few_blocks(s, true);
     few_dispatch(dtype, few_tokens_of(N), [&](auto dt, auto nb) {
-      hipLaunchKernelGGL((few_rows_bwd_k<decltype(dt)::value, decltype(nb)::value>), dim3(blocks), dim3(512), 0, st, f, st2, g,
+      hipLaunchKernelGGL((few_rows_bwd_k<decltype(dt)::value, decltype(nb)::value>), dim3(blocks), dim3(512), 0, st, f, st2, stat + 2 * N, g,
                          dh ? ws.slab : nullptr, (int)ws.slab_ld, dw, lddw);
     });
     if (dh)
@@ -1854,14 +1867,14 @@ extern "C" int po_linear_ce_frozen_fwd(const void* h, int64_t ldh, const void* w
   PO_TRY((dtype == PO_F16    ? frozen_forward<F16, 1>(s, ws, hs, wside, target, k, base, slab, &parts, &last, &pieces, st)
           : dtype == PO_BF16 ? frozen_forward<BF16, 1>(s, ws, hs, wside, target, k, base, slab, &parts, &last, &pieces, st)
                              : frozen_forward<BF16, 3>(s, ws, hs, wside, target, k, base, slab, &parts, &last, &pieces, st)));
-  row_stats(ws.partial, parts, s, ws.tlogit, target, ignore_index, k, ws.stat, ws.sums, ws.arrived, reduction, loss, count, st);
+  row_stats(ws.partial, parts, s, ws.tlogit, target, ignore_index, k, dtype == PO_F16 ? KeepEpi<F16, 1>::kLift : 0.f, ws.stat, ws.rest, ws.sums, ws.arrived, reduction, loss, count, st);
   const int64_t half = ws.plan.slices * ws.ldr;
   const float *refs = ws.slab_refs + (pieces - 1) % 2 * half, *before = ws.slab_refs + pieces % 2 * half;
   const int grid = (int)std::min<int64_t>((N * (ws.slab_ld / 4) + 255) / 256, 8192);
   const float lift = dtype == PO_F16 ? 0x1p-15f : 1.f;
 #define PO_DH(T, HALF)                                                                                                     \
   hipLaunchKernelGGL((frozen_dh_k<T, HALF>), dim3(grid), dim3(256), 0, st, slab, ws.plan.slices, last, ws.slab_slice, ws.slab_ld, \
-                     (int)N, (int)D, refs, before, ws.ldr, lift, ws.stat, ws.tlogit, target, ignore_index, V, k, scale,     \
+                     (int)N, (int)D, refs, before, ws.ldr, lift, ws.stat, ws.rest, target, ignore_index, V, scale,     \
                      static_cast<const T*>(w), ldw, dhu)
   if (dtype == PO_F32) PO_DH(float, false);
   else if (dtype == PO_F16) PO_DH(uint16_t, true);

@@ -747,7 +747,7 @@ int po_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, in
  * not ignore_index makes its row's loss, and the gradients, NaN.  scale > 0.
  * reduction 0: loss [N]; 1: their sum; 2: their mean over the rows that take part
  * (NaN if there is none), with count [1] receiving the number of those rows
- * (also for 1; may be NULL for 0).  loss is fp32.  stat [N][2] fp32 is what the
+ * (also for 1; may be NULL for 0).  loss is fp32.  stat [3 N] fp32 is what the
  * backward pass needs of the forward's.  N <= 2^21, D <= 2^20. */
 int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V, int64_t D,
                      const int64_t* target, int64_t ignore_index, float scale, int reduction, void* workspace,

@@ -219,6 +219,31 @@ def test_frozen_vocabulary_fitted(dtype):
     check_frozen(h, w, t, torch.full((N,), 1024.0 if dtype == torch.float16 else 1.0, device=DEV))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", [(5, 900, 64), (200, 900, 64), (3000, 9000, 768)])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_small_losses(N, V, D, frozen, dtype):
+    """With p next to 1 a loss is log(1 + rest): an error of the logits, and of the exponentials, counts as much as the
+    rest does, and what is left are the roundings of log2, of 1 + rest and of the target's exponent (an ulp of 1 each)."""
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w, t = inputs(N, V, D, dtype, ignored=0.0)
+    w = (w.float() / w.float().norm(dim=1, keepdim=True)).to(dtype)
+    h = (w.float()[t] * torch.linspace(14.0, 40.0, N, device=DEV)[:, None]).to(dtype)
+    x = h.clone().requires_grad_(frozen)
+    loss = lce(x, w, t, reduction="none")
+    ref = reference(h, w, t)
+    b = bounds(ref, dtype, N, V, D)["loss"]
+    within(loss.detach(), ref["loss"], -torch.expm1(-ref["loss"]) * b + 3 * 2.0 ** -23, "loss")
+    if frozen:
+        (dh,) = torch.autograd.grad(loss, x, torch.full((N,), 64.0, device=DEV))
+        ref = reference(h, w, t, torch.full((N,), 64.0, device=DEV))
+        rest = -torch.expm1(-ref["loss"])[:, None]
+        # the target's part, 64 (1 - p) w, is as exact as 1 - p; the others' terms are off by their roundings
+        tol = (bounds(ref, dtype, N, V, D)["dh"] - (2 * (b - 4e-5) / 2 + 1e-4) * ref["ah"]).clamp(min=0) + \
+            64 * (2 * b * rest + 4 * 2.0 ** -23) * w[t].double().abs() + (2 * b + 1e-4) * (ref["rh"] + 64 * 2.0 ** -48 * ref["wsum"])
+        within(dh, ref["dh"], tol, "dh")
+
+
 @pytest.mark.parametrize("N,V,D", [(90, 700, 64), (2600, 9000, 768)])        # below and above the size that takes a common base
 def test_frozen_vocabulary_of_infinite_logits(N, V, D):
     lce = pkg_mod("vocab_loss").linear_cross_entropy
