@@ -221,20 +221,20 @@ def test_frozen_vocabulary_fitted(dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N,V,D", [(5, 900, 64), (200, 900, 64), (3000, 9000, 768)])
-@pytest.mark.parametrize("frozen", [False, True])
-def test_small_losses(N, V, D, frozen, dtype):
+@pytest.mark.parametrize("mode", ["plain", "frozen", "both"])
+def test_small_losses(N, V, D, mode, dtype):
     """With p next to 1 a loss is log(1 + rest): an error of the logits, and of the exponentials, counts as much as the
     rest does, and what is left are the roundings of log2, of 1 + rest and of the target's exponent (an ulp of 1 each)."""
     lce = pkg_mod("vocab_loss").linear_cross_entropy
     h, w, t = inputs(N, V, D, dtype, ignored=0.0)
     w = (w.float() / w.float().norm(dim=1, keepdim=True)).to(dtype)
     h = (w.float()[t] * torch.linspace(14.0, 40.0, N, device=DEV)[:, None]).to(dtype)
-    x = h.clone().requires_grad_(frozen)
-    loss = lce(x, w, t, reduction="none")
+    x = h.clone().requires_grad_(mode != "plain")
+    loss = lce(x, w.clone().requires_grad_(mode == "both"), t, reduction="none")
     ref = reference(h, w, t)
     b = bounds(ref, dtype, N, V, D)["loss"]
     within(loss.detach(), ref["loss"], -torch.expm1(-ref["loss"]) * b + 3 * 2.0 ** -23, "loss")
-    if frozen:
+    if mode != "plain":
         (dh,) = torch.autograd.grad(loss, x, torch.full((N,), 64.0, device=DEV))
         ref = reference(h, w, t, torch.full((N,), 64.0, device=DEV))
         rest = -torch.expm1(-ref["loss"])[:, None]
