@@ -372,7 +372,6 @@ int few_tokens(bool fused, const void* x, int64_t ldx, const int8_t* q, int64_t 
   return po::check_launch("po_int8_matmul");
 }
 
-inline int element_bytes(int dtype) { return dtype == PO_F32 ? 4 : 2; }
 inline bool known(int dtype) { return dtype == PO_F32 || dtype == PO_F16 || dtype == PO_BF16; }
 
 }  // namespace

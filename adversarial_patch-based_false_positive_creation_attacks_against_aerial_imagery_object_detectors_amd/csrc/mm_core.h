@@ -407,7 +407,7 @@ __device__ __forceinline__ void product3(f4v (&acc)[C::TM][C::TN], const Operand
         const int j = i & 1 ? C::TN - 1 - jj : jj;
         acc[i][j] = mfma<C::KIND>(a[i], b[j], acc[i][j]);
       }
-    constexpr int R = decltype(reads)::value, X = C::TM * C::TN, E = R ? (X / R > 1 ? X / R / 2 * 2 : 1) : 1;
+    constexpr int R = decltype(reads)::value, X = C::TM * C::TN, each = X / (R ? R : 1), E = each > 1 ? each / 2 * 2 : 1;
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
