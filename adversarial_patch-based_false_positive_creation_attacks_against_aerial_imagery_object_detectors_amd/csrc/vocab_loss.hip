@@ -551,7 +551,8 @@ struct SlabEpi {
   }
 };
 
-// out[n][m] = acc * g.end() in the gradients' type (OUT: BF16, F16, or 3: fp32)
+// out[n][m] = acc * g.end() in the gradients' type (OUT: BF16, F16, or 3: fp32).  tokens: n is a token, and
+// rows that take no part are 0 (their sums of zeros times an infinite weight or factor are NaN)
 template <int OUT>
 struct GradEpi {
   static constexpr Ends kEnds{9, 14, OUT == 3};
@@ -559,7 +560,8 @@ struct GradEpi {
     void* out;
     int64_t ld;
     GradOf g;
-    int N, M;
+    int N, M, tokens;
+    __device__ __forceinline__ bool live(int n) const { return !tokens || (n < N && g.live(n)); }
   };
   template <class C>
   using Pre = NoPre;
@@ -571,16 +573,18 @@ struct GradEpi {
       for (int j = 0; j < C::TN; ++j) {
         const int n = t.col(j);
         if (n >= e.N) continue;
+        const bool live = e.live(n);
 #pragma unroll
         for (int i = 0; i < C::TM; ++i) {
           const int m = t.row(i);
           float* o = static_cast<float*>(e.out) + (int64_t)n * e.ld + m;
+          const f4v v = live ? t.acc[i][j] * f : f4v{0, 0, 0, 0};
           if (m + 4 <= e.M) {
-            *reinterpret_cast<f4u*>(o) = t.acc[i][j] * f;
+            *reinterpret_cast<f4u*>(o) = v;
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (m + k < e.M) o[k] = t.acc[i][j][k] * f;
+              if (m + k < e.M) o[k] = v[k];
           }
         }
       }
@@ -589,10 +593,12 @@ struct GradEpi {
 #pragma unroll
       for (int j = 0; j < C::TN; ++j) {
         __builtin_amdgcn_sched_barrier(0);
+        const bool live = e.live(t.col(j));
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i)
-          stage4(t, lds, i, j, u2v{pack2<OUT>(t.acc[i][j][0] * f, t.acc[i][j][1] * f),
-                                   pack2<OUT>(t.acc[i][j][2] * f, t.acc[i][j][3] * f)});
+        for (int i = 0; i < C::TM; ++i) {
+          const u2v w = {pack2<OUT>(t.acc[i][j][0] * f, t.acc[i][j][1] * f), pack2<OUT>(t.acc[i][j][2] * f, t.acc[i][j][3] * f)};
+          stage4(t, lds, i, j, live ? w : u2v{0, 0});
+        }
       }
       __syncthreads();
       store_rows<C>(lds, static_cast<uint16_t*>(e.out), e.ld, t.tn * C::BN, t.tm * C::BM, e.N, e.M);
@@ -699,12 +705,13 @@ __global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ pa
   }
 }
 
-// ratio[n] and *factor (GradOf) of single losses' gradients: relative to the largest |g|
+// ratio[n] and *factor (GradOf) of single losses' gradients: relative to the largest finite |g|, so that one that
+// is not finite stays its own row's (NaN)
 __global__ __launch_bounds__(1024) void grad_rows_k(const GradOf g, int N, float* __restrict__ ratio, float* __restrict__ factor) {
   __shared__ float red[1024];
   float top = 0.f;
   for (int n = threadIdx.x; n < N; n += 1024)
-    if (g.target[n] != g.ignore) top = fmaxf(top, fabsf(g.grad[n]));
+    if (g.target[n] != g.ignore && fabsf(g.grad[n]) < INFINITY) top = fmaxf(top, fabsf(g.grad[n]));
   red[threadIdx.x] = top;
   __syncthreads();
   for (int w = 512; w; w >>= 1) {
@@ -715,7 +722,8 @@ __global__ __launch_bounds__(1024) void grad_rows_k(const GradOf g, int N, float
   for (int n = threadIdx.x; n < N; n += 1024) {
     const int64_t t = g.target[n];
     const float x = g.grad[n];
-    ratio[n] = t == g.ignore ? 0.f : t < 0 || t >= g.V ? __uint_as_float(0x7fc00000u) : x == 0.f ? 0.f : x / top * g.lift;
+    const bool none = t < 0 || t >= g.V || !(fabsf(x) < INFINITY);
+    ratio[n] = t == g.ignore ? 0.f : none ? __uint_as_float(0x7fc00000u) : x == 0.f ? 0.f : x / top * g.lift;
   }
   if (threadIdx.x == 0) *factor = top > 0.f ? top / g.lift * g.c : 0.f;
 }
@@ -915,7 +923,7 @@ __device__ __forceinline__ void put4(void* out, int64_t at, int cols, f4v v) {
   }
 }
 
-// dh[n][m] = g.end() * the slabs' sum, slab after slab; a thread makes 4 columns
+// dh[n][m] = g.end() * the slabs' sum, slab after slab (rows that take no part: 0, as GradEpi's); a thread makes 4 columns
 template <int OUT>
 __global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab, int slices, int64_t slice, int64_t ld,
                                                   int N, int M, const GradOf g, void* __restrict__ out, int64_t ldo) {
@@ -929,8 +937,7 @@ __global__ __launch_bounds__(256) void slab_sum_k(const float* __restrict__ slab
     f4v v = {0, 0, 0, 0};
 #pragma unroll 4
     for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const f4v*>(p + s * slice);
-    v *= f;
-    put4<OUT>(out, n * ldo + m, M - m, v);
+    put4<OUT>(out, n * ldo + m, M - m, g.live((int)n) ? v * f : f4v{0, 0, 0, 0});
   }
 }
 
@@ -1714,7 +1721,7 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
       // the last piece may have fewer steps than slices: the other slabs keep their sums
       const Plan p{ws.dh_plan.tile, std::min(ws.dh_plan.slices, ceil_div(a.kbytes, P == 3 ? 64 : 128)), 0};
       if (ws.direct_dh) {
-        const typename GradEpi<OUT>::Args ge{dh, lddh, g, N, D};
+        const typename GradEpi<OUT>::Args ge{dh, lddh, g, N, D, 1};
         PO_TRY((launch_planned<KIND, P, GradEpi<OUT>>(a, ge, p, st, what)));
       } else {
         const SlabEpi::Args se{ws.slab, ws.slab_ld, ws.slab_slice, N, D, v > 0};
@@ -1726,7 +1733,7 @@ int backward(const Shape& s, const BwdWs& ws, const Side& h, const Side& w, cons
       a.B = Operand{reinterpret_cast<char*>(ws.dlt), s.ldn() * ES, ws.piece * s.ldn() * 2, rows};
       a.kbytes = (int)s.Np() * ES;
       char* out = static_cast<char*>(dw) + v * lddw * es;
-      const typename GradEpi<OUT>::Args ge{out, lddw, g, rows, D};
+      const typename GradEpi<OUT>::Args ge{out, lddw, g, rows, D, 0};
       PO_TRY((launch_planned<KIND, P, GradEpi<OUT>>(a, ge, plan_of<GradEpi<OUT>>(a, s.form), st, what)));
     }
   }

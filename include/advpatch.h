@@ -754,7 +754,9 @@ int po_linear_ce_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, int
                      int64_t workspace_bytes, float* stat, float* loss, float* count, po_stream_t s);
 /* dh [N][D] and dw [V][D] (either may be NULL) of grad (fp32: [N] for reduction
  * 0, else [1]).  Walks the vocabulary piece by piece: the logits once more, their
- * gradient in 16 bits (fp32 inputs: in three planes of 16), the two products. */
+ * gradient in 16 bits (fp32 inputs: in three planes of 16), the two products.  An
+ * upstream gradient that is not finite leaves its own row's dh (and dw) not finite, no
+ * other row's. */
 int po_linear_ce_bwd(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, int64_t N, int64_t V, int64_t D,
                      const int64_t* target, int64_t ignore_index, float scale, int reduction, const float* stat,
                      const float* count, const float* grad, void* workspace, int64_t workspace_bytes, void* dh,

@@ -1,0 +1,70 @@
+"""The head's operators at values and calls that reach few places: gradients that are not
+finite, targets outside the vocabulary, weights that are infinite.  References and
+bounds of the losses are test_gpu_vocab_loss.py's."""
+import pytest
+import torch
+
+from conftest import pkg_mod
+from test_gpu_vocab_loss import IGN, bounds, inputs, reference, within
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+TYPES = (torch.float32, torch.float16, torch.bfloat16)
+INF, NAN = float("inf"), float("nan")
+
+# few rows' kernels, the smallest tiles (fp32: as it is), one piece in one slice, slices, and a size that
+# takes a common base against a frozen vocabulary
+HEADS = [(5, 900, 64), (20, 777, 56), (200, 900, 72), (300, 9001, 40), (2600, 9000, 768)]
+
+
+def _loss_and_grads(h, w, t, up, frozen, reduction="none"):
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w = h.clone().requires_grad_(), w.clone().requires_grad_(not frozen)
+    loss = lce(h, w, t, reduction=reduction)
+    grads = torch.autograd.grad(loss, [h] if frozen else [h, w], up)
+    return loss.detach(), grads[0], None if frozen else grads[1]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", HEADS)
+@pytest.mark.parametrize("frozen", [False, True])
+@pytest.mark.parametrize("what", [INF, -INF, NAN])
+def test_one_rows_gradient_that_is_not_finite_stays_its_own(N, V, D, frozen, what, dtype):
+    h, w, t = inputs(N, V, D, dtype)
+    t[1], t[2], t[3] = 5, 6, IGN
+    h[3] = NAN
+    up = 0.5 + torch.arange(N, device=DEV) % 7 / 7
+    ref = reference(h, w, t, up)                                # of finite gradients
+    up[2] = what
+    up[3] = what                                                # of a row that takes no part
+    loss, dh, dw = _loss_and_grads(h, w, t, up, frozen)
+    rest = torch.arange(N, device=DEV) != 2
+    b = bounds(ref, dtype, N, V, D)
+    within(dh[rest], ref["dh"][rest], (b["dh"] + 2.0 ** -48 * ref["gmax"] * ref["wsum"])[rest], "dh")
+    assert not torch.isfinite(dh[2]).any() and not dh[t == IGN].any()
+    assert dw is None or not torch.isfinite(dw).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", HEADS)
+@pytest.mark.parametrize("frozen", [False, True])
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+@pytest.mark.parametrize("what", [INF, NAN])
+def test_a_sums_gradient_that_is_not_finite_leaves_ignored_rows(N, V, D, frozen, reduction, what, dtype):
+    h, w, t = inputs(N, V, D, dtype)
+    t[1], t[3] = 5, IGN
+    h[3] = NAN
+    loss, dh, dw = _loss_and_grads(h, w, t, torch.tensor(what, device=DEV), frozen, reduction)
+    assert not dh[t == IGN].any() and not torch.isfinite(dh[t != IGN]).any()
+    assert dw is None or not torch.isfinite(dw).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", HEADS)
+@pytest.mark.parametrize("frozen", [False, True])
+def test_infinite_weights_leave_ignored_rows(N, V, D, frozen, dtype):
+    h, w, t = inputs(N, V, D, dtype)
+    t[1], t[3] = 5, IGN
+    w[7, 0], w[8, 0] = INF, NAN
+    loss, dh, dw = _loss_and_grads(h, w, t, torch.tensor(1.0, device=DEV), frozen, "sum")
+    assert not dh[t == IGN].any() and torch.isnan(dh[t != IGN]).all() and torch.isnan(loss)
