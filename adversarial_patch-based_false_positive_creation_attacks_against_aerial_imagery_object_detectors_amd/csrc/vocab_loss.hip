@@ -723,7 +723,7 @@ __global__ __launch_bounds__(1024) void grad_rows_k(const GradOf g, int N, float
     const int64_t t = g.target[n];
     const float x = g.grad[n];
     const bool none = t < 0 || t >= g.V || !(fabsf(x) < INFINITY);
-    ratio[n] = t == g.ignore ? 0.f : none ? __uint_as_float(0x7fc00000u) : x == 0.f ? 0.f : x / top * g.lift;
+    ratio[n] = t == g.ignore || x == 0.f ? 0.f : none ? __uint_as_float(0x7fc00000u) : x / top * g.lift;
   }
   if (threadIdx.x == 0) *factor = top > 0.f ? top / g.lift * g.c : 0.f;
 }

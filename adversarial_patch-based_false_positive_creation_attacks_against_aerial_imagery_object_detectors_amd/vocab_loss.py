@@ -21,7 +21,8 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     hidden [..., D] and weight [V, D] of one type (float32, float16 or bfloat16),
     target [...] int64.  Rows with ``ignore_index`` have loss and gradient 0,
     whatever hidden holds there; "mean" divides by the others' number (NaN if there is none).  A
-    target outside the vocabulary makes its row's loss (and the gradients) NaN:
+    target outside the vocabulary makes its row's loss NaN, and its row of hidden's
+    gradient and all of weight's, unless that loss's upstream gradient is 0:
     nothing is read back to raise for it.  scale > 0 (an inverse temperature).
     The gradients have the inputs' type; their sums are kept in 32 bits.  In
     float16 use a loss scale, as for any float16 training: gradients below 6e-8 are 0.

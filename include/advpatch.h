@@ -744,7 +744,8 @@ int po_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, in
  *   l[n][v] = scale * h[n] . w[v]; loss[n] = log sum_v exp l[n][v] - l[n][target[n]]
  * h [N][D], w [V][D], target [N]; rows with target == ignore_index take no part
  * (loss 0, gradient 0, whatever h holds there); a target outside [0, V) that is
- * not ignore_index makes its row's loss, and the gradients, NaN.  scale > 0.
+ * not ignore_index makes its row's loss NaN, and where that loss's upstream gradient is
+ * not 0 its row of dh and all of dw.  scale > 0.
  * reduction 0: loss [N]; 1: their sum; 2: their mean over the rows that take part
  * (NaN if there is none), with count [1] receiving the number of those rows
  * (also for 1; may be NULL for 0).  loss is fp32.  stat [3 N] fp32 is what the

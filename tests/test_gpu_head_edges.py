@@ -68,3 +68,37 @@ def test_infinite_weights_leave_ignored_rows(N, V, D, frozen, dtype):
     w[7, 0], w[8, 0] = INF, NAN
     loss, dh, dw = _loss_and_grads(h, w, t, torch.tensor(1.0, device=DEV), frozen, "sum")
     assert not dh[t == IGN].any() and torch.isnan(dh[t != IGN]).all() and torch.isnan(loss)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", [(1, 700, 48)] + HEADS)
+@pytest.mark.parametrize("frozen", [False, True])
+@pytest.mark.parametrize("bad", ["below", "above", "far"])
+def test_a_target_outside_the_vocabulary_is_its_rows_alone(N, V, D, frozen, bad, dtype):
+    """Its loss, its row of dh and, since every row of dw takes its part, all of dw are NaN; with an upstream gradient
+    of 0 it takes no part in the gradients."""
+    h, w, t = inputs(N, V, D, dtype, ignored=0.1 if N > 1 else 0.0)
+    row = N // 2
+    t[row] = IGN                                                # the others' reference
+    up = 0.5 + torch.arange(N, device=DEV) % 7 / 7
+    ref = reference(h, w, t, up)
+    b = bounds(ref, dtype, N, V, D)
+    left_out = 2.0 ** -48 * ref["gmax"] * ref["wsum"]
+    others = torch.arange(N, device=DEV) != row
+    t[row] = {"below": -1, "above": V, "far": 1 << 40}[bad]
+    for zero in (False, True):
+        up[row] = 0.0 if zero else 0.75
+        loss, dh, dw = _loss_and_grads(h, w, t, up, frozen)
+        assert torch.isnan(loss[row])
+        within(loss[others], ref["loss"][others], b["loss"], "loss") if N > 1 else None
+        within(dh[others], ref["dh"][others], (b["dh"] + left_out)[others], "dh") if N > 1 else None
+        if zero:
+            assert not dh[row].any()
+            if not frozen:
+                within(dw, ref["dw"], b["dw"], "dw")
+        else:
+            assert torch.isnan(dh[row]).all() and (frozen or torch.isnan(dw).all())
+    for reduction in ("sum", "mean"):
+        loss, dh, dw = _loss_and_grads(h, w, t, torch.tensor(1.0, device=DEV), frozen, reduction)
+        assert torch.isnan(loss) and torch.isnan(dh[row]).all() and not dh[t == IGN].any()
+        assert torch.isfinite(dh[others]).all() and (frozen or torch.isnan(dw).all())
