@@ -102,3 +102,25 @@ def test_a_target_outside_the_vocabulary_is_its_rows_alone(N, V, D, frozen, bad,
         loss, dh, dw = _loss_and_grads(h, w, t, torch.tensor(1.0, device=DEV), frozen, reduction)
         assert torch.isnan(loss) and torch.isnan(dh[row]).all() and not dh[t == IGN].any()
         assert torch.isfinite(dh[others]).all() and (frozen or torch.isnan(dw).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", HEADS)
+@pytest.mark.parametrize("frozen", [False, True])
+def test_gradients_of_large_logits(N, V, D, frozen, dtype):
+    """Logits of hundreds: exponentials that underflow, targets that are far from the largest."""
+    h, w, t = inputs(N, V, D, dtype)
+    h = (h.float() * 40).to(dtype)
+    up = (16.0 if dtype == torch.float16 else 1.0) * (0.5 + torch.arange(N, device=DEV) % 7 / 7)
+    ref = reference(h, w, t, up)
+    b = bounds(ref, dtype, N, V, D)
+    loss, dh, dw = _loss_and_grads(h, w, t, up, frozen)
+    assert float(ref["loss"].max()) > 100
+    # arguments of hundreds: a loss and its exponents are rounded to a 2^-23 of their size
+    more = 2.0 ** -23 * (ref["loss"].abs() + 2 * ref["S"])
+    within(loss, ref["loss"], b["loss"] + more, "loss")
+    within(dh, ref["dh"], b["dh"] + float(more.max()) * ref["ah"] + 2.0 ** -48 * ref["gmax"] * ref["wsum"], "dh")
+    if not frozen:
+        # an exponential below the smallest normal number, 2^-126, is 0, and so is an operand of the matrix cores: a
+        # term of dl loses up to 2^-126 of its upstream gradient at each, which counts |h| times
+        within(dw, ref["dw"], b["dw"] + float(more.max()) * ref["aw"] + 2 * 2.0 ** -126 * ref["gmax"] * ref["hsum"], "dw")
