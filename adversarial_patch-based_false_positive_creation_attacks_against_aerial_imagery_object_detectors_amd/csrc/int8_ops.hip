@@ -85,7 +85,9 @@ struct RowScale {
         for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(q[4 * h + j] + 12582912.f);
         b[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400), __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400), 0x05040100);
       }
-    } else if (!bad && s > 0.f) {                            // 1 / s and half steps of s need normal numbers
+    } else if (!bad && s > 0.f) {
+      // 1 / s and half steps of s need normal numbers.  A scale of few bits (below 127 * 2^-149) can lie so far below
+      // the largest / 127 that quotients pass 127: those are 127.
 #pragma unroll 1
       for (int h = 0; h < 2; ++h)
 #pragma unroll 1
@@ -93,7 +95,7 @@ struct RowScale {
           float x = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) x = i == h * 4 + j ? v[i] : x;
-          const uint32_t n = (uint32_t)((int)__builtin_rint((double)x / (double)s) & 255);
+          const uint32_t n = (uint32_t)(max(-127, min(127, (int)__builtin_rint((double)x / (double)s))) & 255);
           if (h) b[1] = b[1] << 8 | n;
           else b[0] = b[0] << 8 | n;
         }

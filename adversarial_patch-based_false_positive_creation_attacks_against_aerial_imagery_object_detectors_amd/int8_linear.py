@@ -81,7 +81,8 @@ def lay_out(wq):
 def quantize_rows(x):
     """(q, scale): int8 of x's shape and one float32 scale for each row of its last dimension,
     ``scale = max|row| / 127``, ``q = row / scale`` to the nearest (the exact quotient, ties to
-    even).  A row of zeros gets scale 0, a row that holds NaN or an infinity scale NaN and q 0."""
+    even; at most 127, which quotients pass where the scale itself is rounded at 2^-149).  A row
+    of zeros gets scale 0, a row that holds NaN or an infinity scale NaN and q 0."""
     if not isinstance(x, torch.Tensor) or x.dtype not in nat.DTYPES or x.dim() < 1:
         raise TypeError("quantize_rows: x must be a float32, float16 or bfloat16 tensor of rows")
     _check_inner("quantize_rows", x.shape[-1])

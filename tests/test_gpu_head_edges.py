@@ -124,3 +124,27 @@ def test_gradients_of_large_logits(N, V, D, frozen, dtype):
         # an exponential below the smallest normal number, 2^-126, is 0, and so is an operand of the matrix cores: a
         # term of dl loses up to 2^-126 of its upstream gradient at each, which counts |h| times
         within(dw, ref["dw"], b["dw"] + float(more.max()) * ref["aw"] + 2 * 2.0 ** -126 * ref["gmax"] * ref["hsum"], "dw")
+
+
+@pytest.mark.parametrize("K", [3, 40, 5000, 9000])
+def test_rows_of_the_smallest_numbers_are_quantised_without_wrapping(K):
+    """Row maxima of 1, 2, ... times 2^-149: their scales are whole multiples of 2^-149 as well, up to a third below
+    the largest / 127, and the quotients end at 127."""
+    m = pkg_mod("int8_linear")
+    units = torch.cat([torch.arange(0, 2000), torch.tensor([127 * 127, 127 * 127 + 64, 20000, 65536, 1 << 22, (1 << 23) - 1])])
+    R = len(units)
+    bits = (torch.arange(K)[None, :] * 7919 + torch.arange(R)[:, None]) % (units[:, None] + 1)
+    bits[:, 1] = units                                          # a row's largest
+    bits = bits.int()
+    bits[:, 2::2] |= -1 << 31                                   # every second number is negative
+    bits[0::2, 1] |= -1 << 31                                   # and every second row's largest
+    x = bits.view(torch.float32)
+    s = (units.double() / 127).round() * 2.0 ** -149            # ties (63.5 and the like) go to the even one, torch.round's rule
+    q = torch.where(s[:, None] > 0, torch.round(x.double() / s[:, None]), 0.0).clamp(-127, 127)
+    assert float((units.double() * 2.0 ** -149 / s)[s > 0].max()) == 190 and float(q.abs().max()) == 127
+    got_q, got_s = m.quantize_rows(x.to(DEV))
+    assert torch.equal(got_s.cpu().double(), s) and torch.equal(got_q.cpu().double(), q)
+    y = m.int8_linear(x[:4].to(DEV), torch.ones(2, K, dtype=torch.int8, device=DEV), torch.ones(2, device=DEV))
+    assert torch.equal(y.cpu().double(), (q.sum(1) * s)[:4, None].expand(4, 2))
+    y = m.int8_linear(x[160:162].to(DEV), torch.ones(2, K, dtype=torch.int8, device=DEV), torch.ones(2, device=DEV))
+    assert torch.equal(y.cpu().double(), (q.sum(1) * s)[160:162, None].expand(2, 2))
