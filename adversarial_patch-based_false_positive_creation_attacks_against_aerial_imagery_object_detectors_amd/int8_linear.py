@@ -110,7 +110,9 @@ def int8_matmul(q, scale, wq, wscale, bias=None, dtype=torch.bfloat16):
     with nat.device_of(*(t for t in (q, scale, wq, wscale, bias) if t is not None)):
         m, ld = nat.rows2d(q)
         if K % 16 or ld % 16 or m.data_ptr() % 16 or ld > 1 << 22:
-            m = torch.nn.functional.pad(m, (0, -K % 64))     # what lies behind a row's end must be 0
+            store = torch.zeros(m.shape[0], (K + 63) // 64 * 64, dtype=torch.int8, device=q.device)
+            store[:, :K] = m                                 # what lies behind a row's end must be 0
+            m = store
         elif m.shape[0] == 1:
             m = m.as_strided((1, K), (K, 1))
         y = _matmul(m, scale.reshape(-1).contiguous(), m.shape[0], K, wq, wscale.contiguous(),

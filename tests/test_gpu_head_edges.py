@@ -148,3 +148,21 @@ def test_rows_of_the_smallest_numbers_are_quantised_without_wrapping(K):
     assert torch.equal(y.cpu().double(), (q.sum(1) * s)[:4, None].expand(4, 2))
     y = m.int8_linear(x[160:162].to(DEV), torch.ones(2, K, dtype=torch.int8, device=DEV), torch.ones(2, device=DEV))
     assert torch.equal(y.cpu().double(), (q.sum(1) * s)[160:162, None].expand(2, 2))
+
+
+@pytest.mark.parametrize("K", [16, 64, 50, 128])
+@pytest.mark.parametrize("rows", [1, 2])
+def test_product_of_rows_at_odd_places(K, rows):
+    """One row is a matrix of any stride: a view off 16 bytes is copied, and its copy has a stride of its own."""
+    m = pkg_mod("int8_linear")
+    g = torch.Generator(device=DEV).manual_seed(K)
+    buf = torch.randint(-128, 128, (7, 150), generator=g, device=DEV, dtype=torch.int8)
+    w = torch.randint(-128, 128, (20, K), generator=g, device=DEV, dtype=torch.int8)
+    s, ws = torch.rand(rows, generator=g, device=DEV) + 0.5, torch.ones(20, device=DEV)
+    for r in (0, 3):
+        for c in (0, 3, 16):
+            q = buf[r:r + rows, c:c + K]
+            y = m.int8_matmul(q, s, w, ws, dtype=torch.float32)
+            assert torch.equal(y, (q.double() @ w.double().t()).float() * s[:, None])
+            if rows == 1:
+                assert torch.equal(m.int8_matmul(q[0], s[0], w, ws, dtype=torch.float32), y[0])
