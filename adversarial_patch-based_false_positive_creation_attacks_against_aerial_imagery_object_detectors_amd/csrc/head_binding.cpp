@@ -141,6 +141,12 @@ bool wants_grad(const Tensor& a, const Tensor& b) {
   return at::GradMode::is_enabled() && (a.requires_grad() || (b.defined() && b.requires_grad()));
 }
 
+// A dual tensor of forward-mode differentiation: its tangent would be lost, which counts as zero.
+void check_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what);
+}
+
 // A captured backward pass ends at the leaves' gradient accumulators.  One that an eager graph
 // of the same leaf keeps alive belongs to that graph's stream: the engine makes that stream wait
 // for the captured one, which ends the process where it is the default stream.  Refused here,
@@ -243,6 +249,7 @@ Tensor keyed_dropout(const py::object& x_, double p, const py::object& seed_, co
   TORCH_CHECK_VALUE(row0 <= (1ULL << 32) && row0 + (uint64_t)rows <= (1ULL << 32),
                     "keyed_dropout: rows row0 .. row0 + rows must stay within 2^32");
   k.row0 = (int64_t)row0;
+  check_tangents("keyed_dropout has no forward-mode derivative", {&x, &residual});
   py::gil_scoped_release free;
   if (wants_grad(x, residual)) {
     check_capture("keyed_dropout", {&x, &residual});
@@ -393,6 +400,7 @@ Tensor linear_cross_entropy(const py::object& hidden_, const py::object& weight_
   TORCH_CHECK_VALUE(red >= 0, "linear_cross_entropy: reduction must be one of none, sum, mean");
   TORCH_CHECK_VALUE(scale > 0.0 && std::isfinite(scale), "linear_cross_entropy: scale must be positive and finite, got ", scale);
   const Tensor& target = tensor_of(target_);
+  check_tangents("linear_cross_entropy has no forward-mode derivative", {&hidden, &weight});
   py::gil_scoped_release free;
   if (wants_grad(hidden, weight)) {
     check_capture("linear_cross_entropy", {&hidden, &weight});
@@ -431,6 +439,7 @@ Tensor int8_linear(const py::object& x_, const py::object& wq_, const py::object
   const Tensor bias = bias_.is_none() ? Tensor() : tensor_of(bias_);
   TORCH_CHECK(!wants_grad(x, bias) && !wants_grad(wscale, Tensor()),
               "int8_linear has no gradient: call it under torch.no_grad() or on detached tensors");
+  check_tangents("int8_linear has no gradient, nor a forward-mode derivative: call it on detached tensors", {&x, &wscale, &bias});
   py::gil_scoped_release free;
   On on({&x, &wq, &wscale, &bias});
   const Rows r(x);

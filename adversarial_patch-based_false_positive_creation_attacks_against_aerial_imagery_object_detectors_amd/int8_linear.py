@@ -7,6 +7,7 @@ activations quantised token by token on the way.  Inference only.
 """
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -16,6 +17,8 @@ MAX_INNER = (1 << 17) - 1        # 127 * 128 * MAX_INNER stays below 2^31
 def _no_grad(name, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("%s has no gradient: call it under torch.no_grad() or on detached tensors" % name)
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("%s has no gradient, nor a forward-mode derivative: call it on detached tensors" % name)
 
 
 def _check_inner(name, K):

@@ -22,7 +22,8 @@ def keyed_dropout(x, p, seed, step=0, row0=0, residual=None):
     bits, or an int64 tensor of one element on x's device, read by the kernel
     (a captured graph that adds to it draws a new mask on every replay).
     residual: of x's shape and type.  Dropped elements are exactly 0, whatever x
-    holds there; the sum is formed in 32 bits and rounded once."""
+    holds there; the sum is formed in 32 bits and rounded once.
+    Differentiable any number of times backwards; forward-mode derivatives raise."""
     return nat.head().keyed_dropout(x, p, seed, step, row0, residual)
 
 

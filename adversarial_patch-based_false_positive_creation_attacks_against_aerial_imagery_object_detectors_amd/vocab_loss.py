@@ -26,7 +26,7 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     nothing is read back to raise for it.  scale > 0 (an inverse temperature).
     The gradients have the inputs' type; their sums are kept in 32 bits.  In
     float16 use a loss scale, as for any float16 training: gradients below 6e-8 are 0.
-    Gradients of second order are not available."""
+    Gradients of second order and forward-mode derivatives are not available, and raise."""
     return nat.head().linear_cross_entropy(hidden, weight, target, ignore_index, reduction, scale)
 
 
