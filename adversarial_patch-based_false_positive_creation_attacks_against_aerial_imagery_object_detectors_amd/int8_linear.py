@@ -110,6 +110,7 @@ def int8_matmul(q, scale, wq, wscale, bias=None, dtype=torch.bfloat16):
     if dtype not in nat.DTYPES:
         raise TypeError("int8_matmul: dtype must be float32, float16 or bfloat16")
     _check_weights("int8_matmul", K, wq, wscale, bias)
+    _no_grad("int8_matmul", scale, wscale, bias)
     with nat.device_of(*(t for t in (q, scale, wq, wscale, bias) if t is not None)):
         m, ld = nat.rows2d(q)
         if K % 16 or ld % 16 or m.data_ptr() % 16 or ld > 1 << 22:

@@ -19,10 +19,11 @@ def _calls():
         "linear_cross_entropy": (lambda h, w: vl.linear_cross_entropy(h, w, t), (x, w)),
         "int8_linear": (lambda x, s, b: i8.int8_linear(x, wq, s, b), (x, ws, b)),
         "quantize_rows": (lambda x: i8.quantize_rows(x), (x,)),
+        "int8_matmul": (lambda s, ws, b: i8.int8_matmul(q, s, wq, ws, b), (sx, ws, b)),
     }
 
 
-@pytest.mark.parametrize("name", ["keyed_dropout", "linear_cross_entropy", "int8_linear", "quantize_rows"])
+@pytest.mark.parametrize("name", ["keyed_dropout", "linear_cross_entropy", "int8_linear", "quantize_rows", "int8_matmul"])
 def test_forward_mode_is_refused(name):
     call, args = _calls()[name]
     for k in range(len(args)):
@@ -36,3 +37,14 @@ def test_forward_mode_is_refused(name):
             for free in (args, [forward_ad.unpack_dual(a).primal for a in dual]):
                 with pytest.raises(RuntimeError, match="CUDA"):
                     call(*free)
+
+
+@pytest.mark.parametrize("name", ["int8_linear", "quantize_rows", "int8_matmul"])
+def test_gradients_of_8_bit_products_are_refused(name):
+    call, args = _calls()[name]
+    for k in range(len(args)):
+        grads = [a.clone().requires_grad_() if i == k else a for i, a in enumerate(args)]
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(*grads)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            call(*grads)
