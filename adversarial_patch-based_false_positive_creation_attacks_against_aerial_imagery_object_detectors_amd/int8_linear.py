@@ -5,6 +5,8 @@ Beside the convolutions' operand precisions (``po_conv``: exact float32 and spli
 float16): a linear layer of a deployed detector head, its weights kept in 8 bits and its
 activations quantised token by token on the way.  Inference only.
 """
+import warnings
+
 import torch
 import torch.nn as nn
 from torch.autograd import forward_ad
@@ -132,7 +134,9 @@ def int8_linear(x, wq, wscale, bias=None):
 class Int8Linear(nn.Module):
     """A linear layer whose weights are kept in 8 bits, laid out once.
 
-    weight [out, K] float (quantised row by row with ``quantize_rows``), bias [out] or None."""
+    weight [out, K] float (quantised row by row with ``quantize_rows``), bias [out] or None.
+    A served layer: its output is cut off from the graph of an input that requires a gradient,
+    with a warning where grad mode is on (``int8_linear`` raises)."""
 
     def __init__(self, weight, bias=None):
         super().__init__()
@@ -158,6 +162,9 @@ class Int8Linear(nn.Module):
         return self
 
     def forward(self, x):
+        if torch.is_grad_enabled() and x.requires_grad:
+            warnings.warn("Int8Linear has no gradient: its output is cut off from its input's graph; call it under "
+                          "torch.no_grad() or on detached tensors", stacklevel=2)
         with torch.no_grad():
             return int8_linear(x, self.wq, self.wscale, self.bias)
 

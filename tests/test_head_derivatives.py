@@ -1,5 +1,7 @@
 """CPU tests: the derivatives that the head's operators do not have are refused, and none is dropped
 without a word.  The refusals come before a device is looked at."""
+import warnings
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -48,3 +50,19 @@ def test_gradients_of_8_bit_products_are_refused(name):
             call(*grads)
         with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
             call(*grads)
+
+
+def test_a_served_layer_says_that_it_cuts_the_graph():
+    layer = pkg_mod("int8_linear").Int8Linear.__new__(pkg_mod("int8_linear").Int8Linear)
+    torch.nn.Module.__init__(layer)
+    layer.wq, layer.wscale, layer.bias = torch.ones(5, 16, dtype=torch.int8), torch.ones(5), None
+    x = torch.randn(3, 16, requires_grad=True)
+    with pytest.warns(UserWarning, match="cut off"), pytest.raises(RuntimeError, match="CUDA"):
+        layer(x)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        for y in (x.detach(), x):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+                layer(y)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            layer(x.detach())
