@@ -461,6 +461,7 @@ __device__ __forceinline__ void product3(f4v (&acc)[C::TM][C::TN], const Operand
 struct Args {
   Operand A, B;
   int tiles_m, tiles_n;
+  int first;                  // tile of this launch's first workgroup
   int kbytes, nk;             // bytes of a row, k-steps
 };
 
@@ -493,7 +494,7 @@ struct NoPre {
 template <class C, class Epi>
 __global__ __launch_bounds__(C::NW * C::KG * 64, C::LDS > 81920 ? 1 : 2) void product_k(const Args a, const typename Epi::Args e) {
   __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
-  const int id = xcd_remap();
+  const int id = a.first + xcd_remap();
   constexpr int GM = 8;                                      // 4 and 16: within 0.5 %
   const int grp = id / (GM * a.tiles_n), first = grp * GM, gm = min(GM, a.tiles_m - first);
   const int r = id - grp * GM * a.tiles_n;
@@ -551,12 +552,18 @@ inline int launch_product(Args a, const typename Epi::Args& e, int slices, hipSt
   a.tiles_m = ceil_div(a.A.rows, C::BM);
   a.tiles_n = ceil_div(a.B.rows, C::BN);
   a.nk = ceil_div(a.kbytes, C::KB);
-  if ((int64_t)a.tiles_m * a.tiles_n >= (1LL << 22) || slices > 65535 || slices > a.nk ||
-      a.A.stride * C::BM >= (1LL << 31) || a.B.stride * C::BN >= (1LL << 31) || a.kbytes < 0) {
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+  if (tiles >= (1LL << 31) || slices > 65535 || slices > a.nk || a.A.stride * C::BM >= (1LL << 31) ||
+      a.B.stride * C::BN >= (1LL << 31) || a.kbytes < 0) {
     set_error("%s: operand too large", what);
     return PO_EINVAL;
   }
-  hipLaunchKernelGGL((product_k<C, Epi>), dim3(a.tiles_m * a.tiles_n, slices), dim3(C::NW * C::KG * 64), 0, s, a, e);
+  constexpr int64_t kMost = 1 << 22;                         // of 512 threads: a grid's stay below 2^32
+  static_assert(C::NW * C::KG * 64 <= 512, "workgroup");
+  for (int64_t at = 0; at < tiles; at += kMost) {
+    a.first = (int)at;
+    hipLaunchKernelGGL((product_k<C, Epi>), dim3((unsigned)std::min(kMost, tiles - at), slices), dim3(C::NW * C::KG * 64), 0, s, a, e);
+  }
   return check_launch(what);
 }
 

@@ -3,7 +3,7 @@
 
 Beside the convolutions' operand precisions (``po_conv``: exact float32 and split
 float16): a linear layer of a deployed detector head, its weights kept in 8 bits and its
-activations quantised token by token on the way.  Inference only.
+activations quantised token by token on the way.  Inference only.  Up to 2^21 tokens a call.
 """
 import warnings
 

@@ -787,14 +787,14 @@ int po_linear_ce_frozen_bwd(const float* dhu, int dtype, int64_t N, int64_t D, c
 /* scale[m] = max_k |x[m][k]| / 127; q[m][k] = x[m][k] / scale[m] rounded to the
  * nearest (the exact quotient; ties to even), zeros up to the next multiple of 16
  * columns.  A row of zeros gets scale 0 (so does one whose largest / 127 rounds to
- * 0, q 0); a row that holds NaN or an infinity gets scale NaN (and q 0).  Where the
+ * 0, q 0); a row that holds NaN or an infinity gets scale NaN  * scale NaN (and q 0).  M <= 2^21.  Where the
  * scale is so small a number (below 2^-142) that rounding it down lets quotients pass
  * 127, those are 127.  ldq a multiple of 16, q on 16 bytes; K < 2^17. */
 int po_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scale,
                      po_stream_t s);
 /* y[m][n] = (sum_k q[m][k] * w[n][k]) * sx[m] * sw[n] [+ bias[n]]: whole-number
  * sums in 32 bits, y in dtype.  Rows of q and w start on 16 bytes; q is zero (and
- * w anything) from K up to the next multiple of 16.  K < 2^17. */
+ * w anything) from K up to the next multiple of 16.  M <= 2^21, N <= 2^24, K < 2^17. */
 int po_int8_matmul(const int8_t* q, int64_t ldq, const float* sx, const int8_t* w, int64_t ldw, const float* sw,
                    const float* bias, int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int dtype, po_stream_t s);
 

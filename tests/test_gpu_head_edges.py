@@ -166,3 +166,36 @@ def test_product_of_rows_at_odd_places(K, rows):
             assert torch.equal(y, (q.double() @ w.double().t()).float() * s[:, None])
             if rows == 1:
                 assert torch.equal(m.int8_matmul(q[0], s[0], w, ws, dtype=torch.float32), y[0])
+
+
+def _losses_of_a_few_tokens(h, w, t):
+    """In 64 bits, the vocabulary in pieces; also the largest sum of a logit's products."""
+    m = torch.full((len(h),), -INF, device=DEV, dtype=torch.float64)
+    s, S = torch.zeros_like(m), 0.0
+    for a in range(0, len(w), 1 << 24):
+        x = h.double() @ w[a:a + (1 << 24)].double().t()
+        top = torch.maximum(m, x.amax(1))
+        s = s * torch.exp(m - top) + torch.exp(x - top[:, None]).sum(1)
+        m = top
+        S = max(S, float((h.double().abs() @ w[a:a + (1 << 24)].double().abs().t()).max()))
+    return m + torch.log(s) - (h.double() * w[t].double()).sum(1), S
+
+
+@pytest.mark.parametrize("N,V", [(1 << 18, (1 << 20) + 300), (1, (1 << 29) + 1000)])
+def test_losses_of_more_tiles_than_a_grid_holds(N, V):
+    """More than 2^22 tiles, in a second launch, whose last are ragged: many tokens of few kinds, and one token."""
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    D, kinds = 8, min(N, 8)
+    g = torch.Generator(device=DEV).manual_seed(N)
+    w = torch.empty(V, D, device=DEV, dtype=torch.bfloat16).normal_(generator=g)
+    h = torch.randn(kinds, D, generator=g, device=DEV).bfloat16()
+    t = torch.randint(0, V, (kinds,), generator=g, device=DEV)
+    t[0] = V - 1                                                # in the last tile
+    ref, S = _losses_of_a_few_tokens(h, w, t)
+    which = torch.randint(0, kinds, (N,), generator=g, device=DEV)
+    which[0] = which[-1] = 0
+    with torch.no_grad():
+        loss = lce(h[which], w, t[which], reduction="none")
+    # the sums of exponentials go over up to 2^22 tiles, 2^14 to a lane's chain (2^-23 each)
+    tol = 2 * (D + 4) * 2.0 ** -23 * S + 4e-5 + 2.0 ** -9
+    within(loss, ref[which], tol, "loss")
