@@ -617,9 +617,8 @@ __device__ __forceinline__ double wave_sum(double x) {
 // Rows' statistics and losses from the tiles': R rows to a workgroup, 256 / R lanes to a row
 // (many rows: neighbouring lanes read neighbouring rows; one row: all lanes share its tiles).
 // total: also the sum (mean: over the rows that count) of the losses, and those rows' number.
-// Each workgroup publishes its rows' sum past its XCD's cache (agent-scope stores, drained
-// before it counts itself in); the one that arrives last adds them up in order.  A launch of
-// its own for that took 3 us.
+// Each workgroup publishes its rows' sum past its XCD's cache and counts itself in (a release); the one
+// that arrives last (an acquire) adds them up in order.  A launch of its own for that took 3 us.
 template <int R>
 __global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ partial, int parts, int N, int64_t V,
                                                    const float* __restrict__ tlogit, const int64_t* __restrict__ target,
@@ -687,10 +686,10 @@ __global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ pa
   if (threadIdx.x == 0) {
     __hip_atomic_store(sums + 2 * blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __hip_atomic_store(sums + 2 * blockIdx.x + 1, num, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    order = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    order = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (__builtin_amdgcn_readfirstlane(order) != gridDim.x - 1) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");         // the other lanes' loads are behind the counter too
   double a = 0, c = 0;
 #pragma unroll 4
   for (int b = threadIdx.x; b < gridDim.x; b += 64) {

@@ -199,3 +199,27 @@ def test_losses_of_more_tiles_than_a_grid_holds(N, V):
     # the sums of exponentials go over up to 2^22 tiles, 2^14 to a lane's chain (2^-23 each)
     tol = 2 * (D + 4) * 2.0 ** -23 * S + 4e-5 + 2.0 ** -9
     within(loss, ref[which], tol, "loss")
+
+
+@pytest.mark.parametrize("N", [63, 500, 9000, 200000])
+def test_totals_of_many_workgroups(N):
+    """The last workgroup to arrive adds up what the others left, on whichever XCD they ran: the sum and the mean are the
+    single losses', added in 64 bits and rounded once, on every run, beside another stream's."""
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    sets = [inputs(N, 300, 16, torch.bfloat16, seed=k) for k in range(2)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    with torch.no_grad():
+        each = [lce(*s, reduction="none").double() for s in sets]
+        torch.cuda.synchronize()
+        got = [[], []]
+        for _ in range(20):
+            for k, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[k].append(torch.stack([lce(*sets[k], reduction=r) for r in ("sum", "mean")]))
+        torch.cuda.synchronize()
+    for k, e in enumerate(each):
+        total = e.sum()
+        want = torch.stack([total, total / (sets[k][2] != IGN).sum()])
+        for g in got[k]:
+            # half a step of 32 bits, and the order of a sum in 64
+            assert bool(((g.double() - want).abs() <= want.abs() * (2.0 ** -24 + N * 2.0 ** -53)).all())
