@@ -977,8 +977,9 @@ __global__ __launch_bounds__(256) void frozen_base_k(const T* __restrict__ h, in
 // A frozen vocabulary's gradient of the embeddings, of an upstream gradient of 1, in fp32:
 // dhu[n][m] = c (sum over the slabs of 2^(r - M) / S - (1 - p_t) w[t][m]), with S 2^M the row's
 // sum of exponentials; rows that take no part 0, rows whose target is none NaN.  A thread makes 4 columns.
+// slab may be dhu itself (one slice): a thread reads the elements that it writes, before it writes them.
 template <typename T, bool HALF>
-__global__ __launch_bounds__(256) void frozen_dh_k(const float* __restrict__ slab, int slices, int last_slices, int64_t slice,
+__global__ __launch_bounds__(256) void frozen_dh_k(const float* slab, int slices, int last_slices, int64_t slice,
                                                    int64_t ld, int N, int M, const float* __restrict__ refs,
                                                    const float* __restrict__ refs_before, int64_t ldr, float lift,
                                                    const float2* __restrict__ stat, const float* __restrict__ rests,

@@ -223,3 +223,16 @@ def test_totals_of_many_workgroups(N):
         for g in got[k]:
             # half a step of 32 bits, and the order of a sum in 64
             assert bool(((g.double() - want).abs() <= want.abs() * (2.0 ** -24 + N * 2.0 ** -53)).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_frozen_vocabularys_gradient_made_where_its_sums_are(dtype):
+    """256 of the largest tiles, one round: the sums are in one slice, and the gradient takes their place."""
+    N, V, D = 4096, 5003, 4095
+    h, w, t = inputs(N, V, D, dtype)
+    up = (64.0 if dtype == torch.float16 else 1.0) * (0.5 + torch.arange(N, device=DEV) % 7 / 7)
+    ref = reference(h, w, t, up)
+    b = bounds(ref, dtype, N, V, D)
+    loss, dh, _ = _loss_and_grads(h, w, t, up, True)
+    within(loss, ref["loss"], b["loss"], "loss")
+    within(dh, ref["dh"], b["dh"] + 2.0 ** -48 * ref["gmax"] * ref["wsum"], "dh")
