@@ -11,12 +11,15 @@
 #include <cmath>
 #include <limits>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -147,22 +150,43 @@ void check_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
     TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what);
 }
 
-// A captured backward pass ends at the leaves' gradient accumulators.  One that an eager graph
-// of the same leaf keeps alive belongs to that graph's stream: the engine makes that stream wait
-// for the captured one, which ends the process where it is the default stream.  Refused here,
-// before anything is captured.
-void check_capture(const char* what, std::initializer_list<const Tensor*> leaves) {
-  const Tensor& first = **leaves.begin();
+// A captured backward pass ends at the gradient accumulators of the leaves that its inputs come from.
+// One that an eager graph of the same leaf keeps alive belongs to that graph's stream: the engine
+// makes that stream wait for the captured one, which ends the process where it is the default
+// stream.  Refused here, before anything is captured.
+void check_capture(const char* what, std::initializer_list<const Tensor*> inputs) {
+  const Tensor& first = **inputs.begin();
   if (!first.is_cuda()) return;                               // refused later
   const c10::OptionalDeviceGuard guard(first.device());
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   const auto now = c10::hip::getCurrentHIPStream(first.device().index()).id();
-  for (const Tensor* t : leaves) {
-    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto stream = node ? node->stream() : std::nullopt;
-    TORCH_CHECK(!stream || stream->id() == now, what,
+  auto check = [&](torch::autograd::Node& accumulator) {
+    const auto stream = accumulator.stream();
+    if (!stream || stream->id() == now) return;
+    const c10::Device device(c10::DeviceType::HIP, stream->device_index());
+    const hipStream_t other =
+        c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, c10::Stream(c10::Stream::UNSAFE, device, stream->id())).stream();
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;     // another stream of the capture will do
+    if (other && hipStreamIsCapturing(other, &status) == hipSuccess && status == hipStreamCaptureStatusActive) return;
+    TORCH_CHECK(false, what,
                 ": a graph made outside this capture still holds one of its leaves (free that graph's outputs before capturing)");
+  };
+  std::unordered_set<torch::autograd::Node*> seen;
+  std::vector<torch::autograd::Node*> left;
+  for (const Tensor* t : inputs) {
+    if (!t->defined() || !t->requires_grad()) continue;
+    if (t->is_leaf()) {
+      if (const auto node = torch::autograd::impl::try_get_grad_accumulator(*t)) check(*node);
+    } else if (seen.insert(t->grad_fn().get()).second) {
+      left.push_back(t->grad_fn().get());
+    }
+  }
+  while (!left.empty()) {
+    torch::autograd::Node& node = *left.back();
+    left.pop_back();
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(&node)) check(node);
+    for (const auto& edge : node.next_edges())
+      if (edge.function && seen.insert(edge.function.get()).second) left.push_back(edge.function.get());
   }
 }
 

@@ -236,3 +236,55 @@ def test_a_frozen_vocabularys_gradient_made_where_its_sums_are(dtype):
     loss, dh, _ = _loss_and_grads(h, w, t, up, True)
     within(loss, ref["loss"], b["loss"], "loss")
     within(dh, ref["dh"], b["dh"] + 2.0 ** -48 * ref["gmax"] * ref["wsum"], "dh")
+
+
+def test_a_capture_is_refused_while_an_eager_graph_holds_leaves_further_up():
+    """Inputs that are no leaves themselves: the captured backward pass reaches the leaves they come from."""
+    lce, kd = pkg_mod("vocab_loss").linear_cross_entropy, pkg_mod("keyed_dropout").keyed_dropout
+    h, w, t = inputs(60, 400, 40, torch.float32)
+    h.requires_grad_()
+    w.requires_grad_()
+
+    def step():
+        hidden = kd(h * 2, 0.25, 3, residual=h + 1)
+        return lce(hidden, w * 1.5, t)
+
+    want = torch.autograd.grad(step(), (h, w))
+    eager = (h * 3).sum()
+    for call in (step, lambda: lce(h * 2, w.detach(), t), lambda: kd(h * 2, 0.5, 1), lambda: kd(h.detach(), 0.5, 1, residual=h * 2)):
+        with pytest.raises(RuntimeError, match="outside this capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    late = torch.autograd.grad(eager, h)[0]
+    del eager
+    assert torch.equal(late, torch.full_like(h, 3.0))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(step(), (h, w))
+    for _ in range(3):
+        for g in got:
+            g.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_capture_over_two_streams_is_not_refused():
+    """A leaf first used on another stream of the same capture."""
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w, t = inputs(60, 400, 40, torch.float32)
+    h.requires_grad_()
+    want = [lce(h.detach(), w, t), lce(h.detach(), w, t, reduction="sum")]
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            a = lce(h, w, t)
+        main.wait_stream(side)
+        b = lce(h, w, t, reduction="sum")
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a.detach(), want[0]) and torch.equal(b.detach(), want[1])
