@@ -18,9 +18,11 @@
 // cover all banks.  Rows past the operand's end and k past its length read as zero
 // (out-of-range buffer offsets).
 //
-// What bounds it is the chip's power: an 8192^3 bf16 product takes a quarter less time on
+// What bounds it, of a long k, is the chip's power: an 8192^3 bf16 product takes a quarter less time on
 // zeros than on random numbers (clock 1.9 to 2.1 GHz, matrix cores 55 % busy).  So the
-// form that moves least wins.  At that size, fp32 outputs: 8 waves of 128 x 64 in
+// form that moves least wins.  Of a short k it is the tiles' ends as well, which a LARGE tile, alone on
+// its CU, leaves uncovered: a round of the losses' tiles takes 33.7 us of 16 steps and 52 of 32, so some 15 us
+// of each are the first loads and the epilogue.  At 8192^3, fp32 outputs: 8 waves of 128 x 64 in
 // 32x32x16 blocks 1.07 ms; in 16x16x32 blocks, which read and write accumulators half as
 // often, 0.91; 4 waves of 128 x 128 0.99 and 0.86 (a third less read from LDS), but a wave
 // alone on its SIMD leaves the epilogues uncovered: the losses' forward product of
@@ -338,8 +340,10 @@ __device__ __forceinline__ void product(typename Acc<C::KIND>::type (&acc)[C::TM
 // A step holds 32 k of all six planes: what product() loads and reads for each of the six
 // products is loaded once, and read once into registers (a 64 x 64 wave takes 24 fragments for 96
 // MFMAs where the pairs in turn take 36; fp32 head of 3000 x 5000 x 1500, trained: the four
-// products 1100 -> 980 us, of 512 x 8192 x 256 126 -> 100).  Rows are 64 bytes, four chunks, turned every four rows,
-// so that 8 neighbouring lanes' reads cover all banks.
+// products 1100 -> 980 us, of 512 x 8192 x 256 126 -> 100).  Rows are 64 bytes, four chunks, turned every four rows:
+// of 8 neighbouring lanes' reads every two fall on the same banks (rows 0 and 2, 1 and 3, 4 and 6, 5 and 7), and
+// half of LDS's cycles are those conflicts (SQ_LDS_BANK_CONFLICT 1.0e7 of SQ_LDS_IDX_ACTIVE 2.0e7, the products of
+// 1000 x 20011 x 513).
 template <class C, class RefsT>
 __device__ __forceinline__ void product3(f4v (&acc)[C::TM][C::TN], const Operand& A, const Operand& B, int m0, int n0,
                                          int kbytes, int ks0, int ks1, char* lds, RefsT& refs) {

@@ -24,7 +24,10 @@
 //
 // Types.  16-bit inputs: exact products, sums in 32 bits; dl is rounded to the
 // inputs' type once, as an operand of the matrix cores: half a step against
-// each of a row's terms, below the rounding of the gradients themselves.  fp16 has
+// each of a row's terms, below the rounding of the gradients themselves, but seen beside it: the
+// norm of bf16 gradients is off by 2.0e-3 where 32-bit dl would give 1.7e-3 (8192 x 131072 x 2048), since the target's
+// term is most of a gradient.  dl in two planes would cost those products twice their time.  Against a
+// frozen vocabulary the target's term is made in 32 bits (1.7e-3), and of up to 8 tokens all of dl.  fp16 has
 // too little range for exp(l)/sum: its dl are kept relative to the largest |g_n|,
 // times 2^14 (at most 2^14, and normal down to 2^-28).  fp32 inputs: each number
 // is the sum of three bf16 (8 + 8 + 8 bits, nearest), and the six leading of the
@@ -1316,7 +1319,9 @@ __global__ __launch_bounds__(256) void few_sum_k(const float* __restrict__ slab,
 
 // ---- the plan ------------------------------------------------------------
 
-// What a piece of the vocabulary may take of the workspace: 16384 rows of 8192 tokens.  Pieces of
+// What a piece of the vocabulary may take of the workspace, its rows laid out, dl and dl^T: 16384 rows of 8192
+// tokens.  Beside it stand what does not depend on the piece, h^T and the slabs of dh (8192 x 131072 x 2048 bf16:
+// 683 MiB in all, 65536 tokens 1380).  Pieces of
 // 8192, whose gradients would stay in the last-level cache, cost dh more (twice the sums read and
 // written: 486 against 430 us for 16384 rows) than they save elsewhere.
 constexpr int64_t kPieceBytes = 640LL << 20;

@@ -24,7 +24,9 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     target outside the vocabulary makes its row's loss NaN, and its row of hidden's
     gradient and all of weight's, unless that loss's upstream gradient is 0:
     nothing is read back to raise for it.  scale > 0 (an inverse temperature).
-    The gradients have the inputs' type; their sums are kept in 32 bits.  In
+    The gradients have the inputs' type; their sums are kept in 32 bits.  Of 16-bit
+    inputs the gradient of the logits is rounded to their type before its products, but for the
+    target's part against a frozen weight and for all of it of up to 8 rows (and 2048 columns).  In
     float16 use a loss scale, as for any float16 training: gradients below 6e-8 are 0.
     Gradients of second order and forward-mode derivatives are not available, and raise."""
     return nat.head().linear_cross_entropy(hidden, weight, target, ignore_index, reduction, scale)

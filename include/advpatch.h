@@ -592,8 +592,8 @@ typedef struct po_conv_desc {
  * bit-identical to 68.
  * 71 (exact fp32, ABI 23) is the Winograd F(4x4,3x3) form of tile 70 (needs
  * Wwino6): 32 4x4-tiles x 64 channels per unit, one 512-thread workgroup per
- * CU walking the units; the same requirements as tile 70; since round 6 (no
- * ABI change) also the fused pool (pool_y on a plain full-map forward, even
+ * CU walking the units; the same requirements as tile 70; without a
+ * change of the ABI also the fused pool (pool_y on a plain full-map forward, even
  * map, no split-K: each 4x4 tile's four windows pooled in the epilogue).
  * Not bit-identical to the F(2x2) tiles (a different exact-arithmetic
  * factorisation); its error against float64 is tested per layer.
