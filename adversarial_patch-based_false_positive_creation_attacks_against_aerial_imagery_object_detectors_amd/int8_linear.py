@@ -156,7 +156,7 @@ class Int8Linear(nn.Module):
         return self
 
     def forward(self, x):
-        if torch.is_grad_enabled() and x.requires_grad:
+        if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
             warnings.warn("Int8Linear has no gradient: its output is cut off from its input's graph; call it under "
                           "torch.no_grad() or on detached tensors", stacklevel=2)
         with torch.no_grad():

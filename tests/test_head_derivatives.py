@@ -66,3 +66,5 @@ def test_a_served_layer_says_that_it_cuts_the_graph():
                 layer(y)
         with pytest.raises(RuntimeError, match="CUDA"):
             layer(x.detach())
+        with pytest.raises(TypeError, match="x must"):
+            layer([1.0] * 16)
