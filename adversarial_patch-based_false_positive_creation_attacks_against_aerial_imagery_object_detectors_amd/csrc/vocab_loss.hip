@@ -708,7 +708,8 @@ __global__ __launch_bounds__(256) void row_stats_k(const float2* __restrict__ pa
 }
 
 // ratio[n] and *factor (GradOf) of single losses' gradients: relative to the largest finite |g|, so that one that
-// is not finite stays its own row's (NaN)
+// is not finite stays its own row's (NaN).  One workgroup: 2.6 us of 40 rows, 9 of 8192, 71 of 65536, 283 of 2^18
+// (whose products take 3 ms and more)
 __global__ __launch_bounds__(1024) void grad_rows_k(const GradOf g, int N, float* __restrict__ ratio, float* __restrict__ factor) {
   __shared__ float red[1024];
   float top = 0.f;
