@@ -288,3 +288,49 @@ def test_a_capture_over_two_streams_is_not_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(a.detach(), want[0]) and torch.equal(b.detach(), want[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", [(1, 500, 2049), (3, 700, 4096), (8, 300, 2056), (9, 129, 2049), (5, 40, 70001), (20, 40, 70001), (3000, 1, 40),
+                                   (3000, 2, 8), (4097, 17, 1), (200, 4097, 1)])
+@pytest.mark.parametrize("frozen", [False, True])
+@pytest.mark.parametrize("scale", [1.0, 0.03, 6.0])
+def test_sizes_at_the_ends_of_the_paths(N, V, D, frozen, scale, dtype):
+    """Few tokens of long rows, one class, one column, rows of 2^17 bytes and more; a class that is the one to ignore."""
+    lce = pkg_mod("vocab_loss").linear_cross_entropy
+    h, w, t = inputs(N, V, D, dtype)
+    up = (64.0 if dtype == torch.float16 else 1.0) * (0.5 + torch.arange(N, device=DEV) % 7 / 7)
+    ref = reference(h, w, t, up, scale)
+    b = bounds(ref, dtype, N, V, D)
+    ignore = V // 2 if V > 2 else IGN                           # its rows are ignored, and so are no others
+    if ignore != IGN:
+        t = torch.where(t == ignore, IGN, t)
+        ref = reference(h, w, t, up, scale)
+        b = bounds(ref, dtype, N, V, D)
+        t = torch.where(t == IGN, ignore, t)
+    h.requires_grad_()
+    w.requires_grad_(not frozen)
+    loss = lce(h, w, t, ignore_index=ignore, reduction="none", scale=scale)
+    grads = torch.autograd.grad(loss, [h] if frozen else [h, w], up)
+    within(loss.detach(), ref["loss"], b["loss"] + 2.0 ** -23 * ref["loss"].abs(), "loss")
+    within(grads[0], ref["dh"], b["dh"] + 2.0 ** -48 * ref["gmax"] * ref["wsum"], "dh")
+    if not frozen:
+        # 3000 rows of two classes pass fp16's range.  The rounding to nearest gives the infinity from half a step above
+        # the largest number on (65504 + 16), so it is right where the value, within its bound, reaches that.
+        want = ref["dw"]
+        over = (want.abs() + b["dw"] >= 65520) & (grads[1].double() == torch.copysign(torch.full_like(want, INF), want))
+        assert dtype == torch.float16 or not over.any()
+        if not over.all():
+            within(grads[1][~over], want[~over], b["dw"][~over], "dw")
+
+
+@pytest.mark.parametrize("N", [1, 5, 20, 300])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_batches_that_are_ignored_whole(N, frozen):
+    h, w, t = inputs(N, 600, 48, torch.bfloat16)
+    h[0] = NAN
+    for reduction in ("none", "sum", "mean"):
+        up = torch.ones(N if reduction == "none" else (), device=DEV)
+        loss, dh, dw = _loss_and_grads(h, w, torch.full_like(t, IGN), up, frozen, reduction)
+        assert torch.isnan(loss).all() if reduction == "mean" else not loss.any()
+        assert not dh.any() and (frozen or not dw.any())
