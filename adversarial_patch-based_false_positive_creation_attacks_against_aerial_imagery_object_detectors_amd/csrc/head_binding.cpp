@@ -8,6 +8,7 @@
 // (bind() resolves them there), so that there is one library in a process.
 #include <dlfcn.h>
 
+#include <atomic>
 #include <cmath>
 #include <limits>
 #include <string>
@@ -85,7 +86,7 @@ struct On {
       TORCH_CHECK(t->is_cuda(), "advpatch HIP ops need CUDA (ROCm) tensors; got ", t->device());
       TORCH_CHECK(t->device() == d, "advpatch HIP ops need their tensors on one device; got ", d, " and ", t->device());
     }
-    static bool seen[64];                                     // set under whatever thread: only ever to true
+    static std::atomic<bool> seen[64];                        // set under whatever thread: only ever to true
     guard.reset_device(d);
     if (d.index() >= 64 || !seen[d.index()]) {
       check(lib.device_check(d.index()), "po_device_check");

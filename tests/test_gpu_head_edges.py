@@ -334,3 +334,57 @@ def test_batches_that_are_ignored_whole(N, frozen):
         loss, dh, dw = _loss_and_grads(h, w, torch.full_like(t, IGN), up, frozen, reduction)
         assert torch.isnan(loss).all() if reduction == "mean" else not loss.any()
         assert not dh.any() and (frozen or not dw.any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(4, 11264, 40), (4, 11265, 40), (1, 45056, 33), (1, 45057, 33), (2, 22528, 20), (3, 8192, 1), (3, 8193, 1),
+                                   (1, 131071, 3), (5, 8193, 17), (32, 100, 1), (33, 100, 1), (33, 131071, 2)])
+def test_8_bit_products_at_the_ends_of_their_paths(M, K, N, dtype):
+    """Tokens that just fit into LDS and those that do not, rows that just stay in registers, one output."""
+    from test_gpu_int8 import check_product, quant_ref
+    m = pkg_mod("int8_linear")
+    g = torch.Generator(device=DEV).manual_seed(M + K)
+    x = torch.randn(M, K, generator=g, device=DEV).to(dtype)
+    w = torch.randint(-128, 128, (N, K), generator=g, device=DEV, dtype=torch.int8)
+    ws, bias = torch.rand(N, generator=g, device=DEV) / 100, torch.randn(N, generator=g, device=DEV)
+    y = m.int8_linear(x, w, ws, bias)
+    q, s = quant_ref(x)
+    check_product(y, q, s, w, ws, bias, dtype)
+    assert torch.equal(m.int8_matmul(*m.quantize_rows(x), m.lay_out(w), ws, bias, dtype), y)
+
+
+def test_calls_of_two_threads():
+    """Each on a stream of its own, the calls' workspaces their own."""
+    import threading
+    lce, kd, i8 = pkg_mod("vocab_loss").linear_cross_entropy, pkg_mod("keyed_dropout").keyed_dropout, pkg_mod("int8_linear")
+    sets = [inputs(130, 2500, 96, torch.bfloat16, seed=k) for k in range(2)]
+    wq = torch.randint(-127, 128, (50, 96), dtype=torch.int8, device=DEV)
+    ws = torch.rand(50, device=DEV)
+
+    def go(k):
+        h, w, t = sets[k]
+        h = h.detach().requires_grad_()
+        hidden = kd(h, 0.3, k, residual=h)
+        loss = lce(hidden, w, t)
+        (dh,) = torch.autograd.grad(loss, h)
+        return loss.detach(), dh, i8.int8_linear(hidden.detach(), wq, ws)
+
+    want = [go(0), go(1)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[k].append(go(k))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        assert len(got[k]) == 20
+        for r in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[k]))
